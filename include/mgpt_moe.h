@@ -462,6 +462,93 @@ int  mgpt_moe_op_plan_noalloc(const int32_t* top_idx, int n_rows, int E,
                               int32_t* tile_expert, int32_t* n_tiles, int32_t* map, int32_t* pos,
                               int32_t* row_src, int row_cap, int32_t* status, mgpt_stream_t stream);
 
+/* ---- the rest of a training step --------------------------------------------
+ * Operators that stand beside the layer in a language model's training step.
+ * x, h, y and their gradients are token tensors as above: row-major [n, C],
+ * C a multiple of 8, 16-byte aligned. Nothing here synchronises or allocates
+ * except mgpt_moe_optim_create. n = 0 is a call without work. */
+
+/* Softmax cross entropy of the vocabulary product, its logits never kept
+ * (layers/CrossEntropyLossLayer.cpp, the model's last LinearLayer in front of it).
+ *   z[i,v] = <x[i,:], w[v,:]>,  lse[i] = log sum_v exp z[i,v],  loss[i] = lse[i] - z[i, targets[i]]
+ * x: [n, C] of `io`; w: BF16 [V, C], a row per vocabulary entry (the layout of an
+ * embedding, which may be the same tensor); targets: int32 [n]; loss, lse: FP32 [n].
+ * x is rounded to BF16 where it is FP32; products are exact and summed in FP32.
+ * A token whose target is outside [0, V) takes no part: its loss, lse and dx are 0, its
+ * x is not looked at (it may hold NaN), and it costs no work. Targets >= V also set
+ * bit 32 of *status.
+ * status: int32 on the device, OR-ed into and never cleared here (bits as
+ * mgpt_moe_check_status's). workspace: mgpt_moe_op_head_loss_workspace_bytes,
+ * 256-byte aligned; nothing of it is needed after the call. */
+size_t mgpt_moe_op_head_loss_workspace_bytes(int n, int C, int V);
+int  mgpt_moe_op_head_loss(const void* x, int io, const void* w, const int32_t* targets, int n, int C, int V,
+                           float* loss, float* lse, int32_t* status,
+                           void* workspace, size_t workspace_bytes, mgpt_stream_t stream);
+
+/* Its gradients, from the same x, w, targets and the lse of the forward call:
+ *   dz[i,v] = d_loss[i] * (exp(z[i,v] - lse[i]) - [v == targets[i]]),  dx = dz w,  dw = dz^T x
+ * d_loss: FP32 [n] (1/n for the mean). dx: [n, C] of `io`, written. dw: [V, C],
+ * dw_dtype MGPT_MOE_IO_BF16: written; MGPT_MOE_IO_F32: added to, like the layer's
+ * parameter gradients. dz is rounded to BF16, the operand type of both products; their
+ * sums are FP32. The vocabulary is worked on in pieces whose dz fits the workspace behind
+ * its fixed part: workspace_bytes(.., piece_bytes) is the size for pieces of about
+ * piece_bytes (at least one of 256 vocabulary rows; 256 MiB is a good value: larger pieces
+ * gain little). Results are deterministic; the order of the sums for dx, and with it its last
+ * bits, depends on the size of the pieces. */
+size_t mgpt_moe_op_head_loss_backward_workspace_bytes(int n, int C, int V, size_t piece_bytes);
+int  mgpt_moe_op_head_loss_backward(const void* x, int io, const void* w, const int32_t* targets,
+                                    const float* lse, const float* d_loss, int n, int C, int V,
+                                    void* dx, void* dw, int dw_dtype, int32_t* status,
+                                    void* workspace, size_t workspace_bytes, mgpt_stream_t stream);
+
+/* The norms around a block's output h, its gate and the skip connection from the residual stream x:
+ *   y = alpha*x + gate * (h*r1*post_scale),  r1 = 1/sqrt(mean(h^2) + eps)
+ *   u = y*r2*pre_scale,                      r2 = 1/sqrt(mean(y^2) + eps)
+ * post_scale NULL: h is not normalised; gate NULL: 1; pre_scale and u NULL: y alone. Scales are FP32 [C]; gate is
+ * FP32 [ceil(n / tokens_per_gate), C], row i for tokens i*tokens_per_gate.. (one row for all where tokens_per_gate is 0).
+ * u is formed from y before it is rounded to the tokens' dtype. stats: FP32 [2*n], kept for backward. C up to 16384.
+ * (layers/TransformerBlock.cpp:38-46 has the norm before a block and the plain skip connection.) */
+int  mgpt_moe_op_residual_norm(const void* x, const void* h, int io, const float* post_scale, const float* gate,
+                               int tokens_per_gate, const float* pre_scale, float alpha, float eps, int n, int C,
+                               void* y, void* u, float* stats, mgpt_stream_t stream);
+
+/* Its gradients. dy, du: gradients of y (by its other uses) and of u (NULL where there is no u). dx, dh: written.
+ * d_post_scale, d_gate, d_pre_scale: FP32, added to, each may be NULL (workspace may be NULL where all are).
+ * x, h, the parameters and stats are the forward call's. Sums have a fixed order: results are deterministic. */
+size_t mgpt_moe_op_residual_norm_backward_workspace_bytes(int n, int C, int tokens_per_gate);
+int  mgpt_moe_op_residual_norm_backward(const void* x, const void* h, int io, const float* post_scale, const float* gate,
+                                        int tokens_per_gate, const float* pre_scale, float alpha, int n, int C,
+                                        const float* stats, const void* dy, const void* du, void* dx, void* dh,
+                                        float* d_post_scale, float* d_gate, float* d_pre_scale,
+                                        void* workspace, size_t workspace_bytes, mgpt_stream_t stream);
+
+/* AdamW over many tensors at once (optimisers/AdamWOptimiser.h:24-36 calls Tensor::adamw_step per tensor), for the tensors
+ * of a model that are not a layer's own (those: mgpt_moe_adamw_step).
+ * The moments belong to the caller. Elements are taken in blocks of 256, every tensor starting on a block of its own, and
+ * block i of all (mgpt_moe_optim_blocks of them) has the elements 256*i.. of m and v, 16-byte aligned, zero before step 1:
+ *   state_bits 32: FP32.
+ *   state_bits 8:  one byte each, in units of m_scale[i] / v_scale[i] (FP32, powers of two): m as E4M3, v as the E4M3 of
+ *                  its square root. Rounding is stochastic, a function of the element's place, seed and t alone.
+ * The table of the tensors' addresses is built once, by create (which allocates and synchronises). step: t counts
+ * from 1; grad_scale (device, may be NULL) multiplies every gradient first: a loss scale's inverse, or the factor
+ * that clips a global norm. An element whose new moments would not be finite keeps w, m and v, and sets
+ * *found_nonfinite (device, may be NULL; never cleared here) to 1. w_bf16 (may be NULL) gets the new w in BF16. */
+typedef struct {
+    float*      w;             /* FP32 */
+    const void* grad;
+    void*       w_bf16;
+    int64_t     n;             /* elements */
+    float       weight_decay;
+    int         grad_dtype;    /* MGPT_MOE_IO_F32 | MGPT_MOE_IO_BF16 */
+} mgpt_moe_optim_tensor;
+typedef struct mgpt_moe_optim mgpt_moe_optim;
+int64_t mgpt_moe_optim_blocks(const mgpt_moe_optim_tensor* tensors, int n);
+int  mgpt_moe_optim_create(int device, const mgpt_moe_optim_tensor* tensors, int n, int state_bits, mgpt_moe_optim** out);
+void mgpt_moe_optim_destroy(mgpt_moe_optim* opt);
+int  mgpt_moe_optim_step(mgpt_moe_optim* opt, void* m, void* v, float* m_scale, float* v_scale,
+                         double lr, double beta1, double beta2, double eps, int64_t t,
+                         const float* grad_scale, uint32_t seed, int32_t* found_nonfinite, mgpt_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

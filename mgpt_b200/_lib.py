@@ -29,6 +29,9 @@ SYMBOLS = [
     "mgpt_moe_peer_alloc", "mgpt_moe_peer_open", "mgpt_moe_peer_close", "mgpt_moe_peer_free", "mgpt_moe_peer_copy",
     "mgpt_moe_block_workspace_bytes", "mgpt_moe_block_forward", "mgpt_moe_block_backward",
     "mgpt_moe_set_weight_grad_overwrite", "mgpt_moe_inference_workspace_bytes", "mgpt_moe_forward_inference", "mgpt_moe_experts_backward_rows", "mgpt_moe_experts_backward_params",
+    "mgpt_moe_op_head_loss_workspace_bytes", "mgpt_moe_op_head_loss", "mgpt_moe_op_head_loss_backward_workspace_bytes", "mgpt_moe_op_head_loss_backward",
+    "mgpt_moe_op_residual_norm", "mgpt_moe_op_residual_norm_backward_workspace_bytes", "mgpt_moe_op_residual_norm_backward",
+    "mgpt_moe_optim_blocks", "mgpt_moe_optim_create", "mgpt_moe_optim_destroy", "mgpt_moe_optim_step",
 ]
 PLAN_NOALLOC_MAX_ROWS = 1048576
 PEER_HANDLE_BYTES = 64
@@ -45,6 +48,11 @@ class EpConfig(ct.Structure):
     _fields_ = [("embed_dim", ct.c_int), ("hidden_dim", ct.c_int), ("num_experts", ct.c_int), ("top_k", ct.c_int),
                 ("lb_alpha", ct.c_float), ("mode", ct.c_int), ("device", ct.c_int), ("rank", ct.c_int),
                 ("world", ct.c_int), ("n_chunks", ct.c_int), ("max_tokens", ct.c_int)]
+
+
+class OptimTensor(ct.Structure):
+    _fields_ = [("w", ct.c_void_p), ("grad", ct.c_void_p), ("w_bf16", ct.c_void_p), ("n", ct.c_int64),
+                ("weight_decay", ct.c_float), ("grad_dtype", ct.c_int)]
 
 
 EP_ID_BYTES = 128
@@ -143,6 +151,23 @@ def load() -> ct.CDLL:
     lib.mgpt_moe_block_forward.argtypes = [vp, vp, vp, ct.c_float, vp, i32, i32, vp, sz, vp]
     lib.mgpt_moe_block_backward.argtypes = [vp, vp, vp, vp, vp, vp, i32, vp, sz, vp]
     lib.mgpt_moe_op_plan_noalloc.argtypes = [vp, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, i32, vp, vp]
+    f32, f64, i64 = ct.c_float, ct.c_double, ct.c_int64
+    lib.mgpt_moe_op_head_loss_workspace_bytes.argtypes = [i32, i32, i32]
+    lib.mgpt_moe_op_head_loss_workspace_bytes.restype = sz
+    lib.mgpt_moe_op_head_loss.argtypes = [vp, i32, vp, vp, i32, i32, i32, vp, vp, vp, vp, sz, vp]
+    lib.mgpt_moe_op_head_loss_backward_workspace_bytes.argtypes = [i32, i32, i32, sz]
+    lib.mgpt_moe_op_head_loss_backward_workspace_bytes.restype = sz
+    lib.mgpt_moe_op_head_loss_backward.argtypes = [vp, i32, vp, vp, vp, vp, i32, i32, i32, vp, vp, i32, vp, vp, sz, vp]
+    lib.mgpt_moe_op_residual_norm.argtypes = [vp, vp, i32, vp, vp, i32, vp, f32, f32, i32, i32, vp, vp, vp, vp]
+    lib.mgpt_moe_op_residual_norm_backward_workspace_bytes.argtypes = [i32, i32, i32]
+    lib.mgpt_moe_op_residual_norm_backward_workspace_bytes.restype = sz
+    lib.mgpt_moe_op_residual_norm_backward.argtypes = [vp, vp, i32, vp, vp, i32, vp, f32, i32, i32] + [vp] * 9 + [sz, vp]
+    lib.mgpt_moe_optim_blocks.argtypes = [ct.POINTER(OptimTensor), i32]
+    lib.mgpt_moe_optim_blocks.restype = i64
+    lib.mgpt_moe_optim_create.argtypes = [i32, ct.POINTER(OptimTensor), i32, i32, ct.POINTER(vp)]
+    lib.mgpt_moe_optim_destroy.argtypes = [vp]
+    lib.mgpt_moe_optim_destroy.restype = None
+    lib.mgpt_moe_optim_step.argtypes = [vp, vp, vp, vp, vp, f64, f64, f64, f64, i64, vp, ct.c_uint32, vp, vp]
     _lib = lib
     return lib
 

@@ -1677,6 +1677,21 @@ int make_map_blocks(CUtensorMap* m, const void* base, uint64_t rows, uint64_t co
     return 0;
 }
 
+int make_map_tiles(CUtensorMap* m, const void* base, uint64_t tiles, uint32_t box_rows, uint32_t n_tiles)
+{
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return fail(MGPT_MOE_ECUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    cuuint64_t dims[3] = {64, 128, tiles};
+    cuuint64_t strides[2] = {64 * sizeof(bf16), 64 * 128 * sizeof(bf16)};
+    cuuint32_t box[3] = {64, box_rows, n_tiles};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(MGPT_MOE_ECUDA, "cuTensorMapEncodeTiled failed (code " + std::to_string((int)r) + ")");
+    return 0;
+}
+
 // A tile-major weight copy as {64 columns, 128 rows, n2 blocks at stride2 elements, n3 at stride3}, box {64, rows, b2, b3}.
 static int make_map_weights(CUtensorMap* m, const void* base, uint64_t n2, uint64_t stride2, uint64_t n3, uint64_t stride3,
                             uint32_t rows, uint32_t b2, uint32_t b3)

@@ -1,0 +1,902 @@
+// Softmax cross entropy of a vocabulary product, and its gradients, without keeping the logits.
+//
+//   z[i,v] = <x[i,:], w[v,:]>,  lse[i] = log sum_v exp z[i,v],  loss[i] = lse[i] - z[i, target[i]]
+//   dz[i,v] = d_loss[i] * (exp(z[i,v] - lse[i]) - [v == target[i]]),  dx = dz w,  dw = dz^T x
+//
+// The reference forms all logits in FP32 and passes over them for the loss and again for the gradient
+// (layers/CrossEntropyLossLayer.cpp; utils/cuda_ops.cu:748-876).  Here the loss is an epilogue of the product: each 256 x 256
+// tile of logits leaves a row maximum and a row sum of exponentials.  The gradients take the vocabulary piece by piece: the
+// piece's logits are computed again, the epilogue turns them into dz (BF16, the operand type of the two products that
+// follow; FP32 until then), and one launch forms the piece's rows of dw and adds its share of dx.
+//
+// dz is kept over the largest |d_loss|, which the results are multiplied by in FP32: with the usual d_loss, one number for
+// all tokens, a target's entry is then -(1 - p) and rounds by less than p.  (Rounded with its factor it is off by the factor's own
+// rounding, up to 2^-8, in every token alike: gradients of 1800 tokens were 2.9e-3 off the exact ones, of which 1.7e-3 are the
+// results' own rounding.)
+//
+// Tokens whose target is not in [0, vocabulary) take no part: the others are packed first, so that an ignored token costs
+// nothing and its x, whatever it holds, is not read.
+#include "tc_common.cuh"
+
+namespace mgpt {
+
+namespace {
+
+using namespace tcx;
+
+constexpr int TILE = 256;                            // tokens and vocabulary rows of a pair's tile
+constexpr int BK = 64;
+constexpr uint32_t OPER_BYTES = 128 * BK * 2;        // one operand's share of a stage in one CTA: 16 KiB
+constexpr uint32_t STAGE_BYTES = 2 * OPER_BYTES;
+constexpr uint32_t BOX_BYTES = 64 * BK * 2;
+constexpr int EPI_WARPS = 16;                        // four per TMEM lane quarter, 64 columns each
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr uint32_t TMEM_COLS = 2 * TILE;
+constexpr uint32_t STAGING = 4096;                   // per epilogue warp: 32 rows x 128 B
+constexpr int QUEUE = 4;
+constexpr int CLAIM = 6;                             // the next item is claimed this many k-blocks before the last one's loads end
+constexpr int MAX_PIECES = 1024;
+constexpr int COUNTERS = 2 * MAX_PIECES + 2;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int ST_BAD_TARGET = ST_BAD_EXPERT;         // the status bit of an index outside its range
+
+enum { LOSS = 0, DLOGITS = 1, GRADS = 2 };
+
+struct HeadP {
+    const int32_t* n_valid;
+    int32_t* sched;             // next item; zero before the launch
+    int32_t* status;
+    int C, V;
+    int v0;                     // first vocabulary row of the piece
+    int v_tiles;                // 256-row tiles of the vocabulary in this launch
+    int group;                  // token tiles that share a pass over the vocabulary (LOSS, DLOGITS)
+    int c_tiles;                // GRADS: 256-column tiles of C
+    int k_slices, slice_tiles;  // GRADS, dx: the piece's vocabulary in k_slices of slice_tiles tiles
+    int n_pad;                  // row pitch of part; rows of a slice of acc
+    const int32_t* target;      // packed
+    const float *lse, *d_loss;  // packed; d_loss over *scale
+    const float* scale;
+    float2* part;               // LOSS: [v_tiles][n_pad] maximum and sum
+    float* z_target;
+    bf16* dz;                   // DLOGITS: [token tile of 128][64-column block] of swizzled 128 x 64 tiles
+    float* acc;                 // GRADS: [k_slices][n_pad][C], dx so far
+    int first;                  // acc is written, not added to
+    void* dw;
+    int dw_f32;                 // dw is FP32 and added to
+};
+
+// exp(from - to), 1 where both are the same infinity
+__device__ __forceinline__ float shift(float from, float to) { return from == to ? 1.0f : exp2f((from - to) * LOG2E); }
+
+struct Shared {
+    int item[QUEUE];
+    uint64_t full[6], empty[6], acc_full[2], acc_empty[2], item_full[QUEUE], item_empty[QUEUE], joined[4];
+    uint32_t tmem;
+};
+template <int KIND> constexpr int stages() { return KIND == LOSS ? 6 : 5; }
+template <int KIND> constexpr uint32_t extra_bytes() { return KIND == LOSS ? 4 * 4 * 128 * sizeof(float2) : EPI_WARPS * STAGING; }
+template <int KIND> constexpr uint32_t smem_bytes() { return 1024 + stages<KIND>() * STAGE_BYTES + extra_bytes<KIND>() + sizeof(Shared); }
+static_assert(smem_bytes<LOSS>() <= 232448 && smem_bytes<GRADS>() <= 232448, "shared memory of one CTA");
+
+// What an item is.  LOSS, DLOGITS: m (256 tokens), n (256 vocabulary rows), reduction over C.
+// GRADS: dx (m: 256 tokens, n: 256 channels, reduction over a slice of the vocabulary) or dw (m: 256 vocabulary rows, n: 256
+// channels, reduction over the tokens).
+struct Item {
+    int m, n, k0, nkb, half;
+    bool dw;
+    int slice;
+};
+template <int KIND> __device__ __forceinline__ int item_count(const HeadP& p, int n_valid)
+{
+    const int mt = (n_valid + TILE - 1) / TILE;
+    return KIND == GRADS ? (mt * p.k_slices + p.v_tiles) * p.c_tiles : mt * p.v_tiles;
+}
+template <int KIND> __device__ __forceinline__ Item decode(const HeadP& p, int n_valid, int i)
+{
+    Item w;
+    const int mt = (n_valid + TILE - 1) / TILE;
+    w.dw = false;
+    w.slice = w.k0 = 0;
+    w.half = 128;
+    if (KIND != GRADS) {
+        // group token tiles at a time run through the whole vocabulary, so that x stays in L2
+        const int g = i / (p.group * p.v_tiles), r = i - g * p.group * p.v_tiles, in = min(p.group, mt - g * p.group);
+        w.n = r / in;
+        w.m = g * p.group + r - w.n * in;
+        w.nkb = (p.C + BK - 1) / BK;
+        return w;
+    }
+    const int dx = mt * p.k_slices * p.c_tiles;
+    if (i < dx) {
+        w.slice = i / (mt * p.c_tiles);
+        const int r = i - w.slice * mt * p.c_tiles;
+        w.m = r / p.c_tiles;
+        w.n = r - w.m * p.c_tiles;
+        w.k0 = w.slice * p.slice_tiles * (TILE / BK);
+        w.nkb = min(p.slice_tiles * (TILE / BK), p.v_tiles * (TILE / BK) - w.k0);
+    } else {
+        w.dw = true;
+        w.m = (i - dx) / p.c_tiles;
+        w.n = (i - dx) - w.m * p.c_tiles;
+        w.nkb = (n_valid + BK - 1) / BK;
+    }
+    if (p.C - w.n * TILE <= TILE / 2) w.half = 64;
+    return w;
+}
+
+// tmA: LOSS, DLOGITS x (box 64 x 128 rows); GRADS the dz tiles as {64, 128 rows, tiles} in boxes of {64, 128, 1}
+// tmA2: GRADS the dz tiles in boxes of {64, 64, 2}
+// tmB: LOSS, DLOGITS w (box 64 x 128 rows); GRADS w (box 64 x 64 rows); tmB2: x (box 64 x 64 rows)
+template <int KIND>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmA2,
+            const __grid_constant__ CUtensorMap tmB2, const HeadP p)
+{
+    constexpr int NS = stages<KIND>();
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_ctarank();
+    uint8_t* const tiles = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* const extra = tiles + NS * STAGE_BYTES;
+    Shared& sh = *reinterpret_cast<Shared*>(extra + extra_bytes<KIND>());
+    const uint32_t full = smem_u32(sh.full), empty = smem_u32(sh.empty), acc_full = smem_u32(sh.acc_full), acc_empty = smem_u32(sh.acc_empty);
+    const uint32_t item_full = smem_u32(sh.item_full), item_empty = smem_u32(sh.item_empty);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < NS; ++s) {
+            mbar_init(full + 8 * s, 1);                     // (the leader's; the peer's loads count on it too)
+            mbar_init(empty + 8 * s, 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(acc_full + 8 * b, 1);
+            mbar_init(acc_empty + 8 * b, 2 * EPI_WARPS);
+        }
+        for (int i = 0; i < QUEUE; ++i) {
+            mbar_init(item_full + 8 * i, 1);
+            mbar_init(item_empty + 8 * i, 2 * EPI_WARPS + 2);       // the leader's: all epilogue warps, its MMA thread, the peer's producer
+        }
+        for (int q = 0; q < 4; ++q) mbar_init(smem_u32(&sh.joined[q]), 4);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc_pair(smem_u32(&sh.tmem), TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();                                         // the peer's barriers exist before anything is sent to them
+    tc_fence_after();
+    const uint32_t tmem_base = sh.tmem;
+    pdl_wait();
+    const int n_valid = *p.n_valid;
+    const float scale = KIND == GRADS ? *p.scale : 1.0f;
+
+    const uint32_t lead_item_empty = mapa(item_empty, 0);
+    // the pair's n-th item; false: no more
+    auto consume = [&](uint32_t n, int& item) -> bool {
+        const int slot = n % QUEUE;
+        if (!mbar_wait_cluster(item_full + 8 * slot, (n / QUEUE) & 1, p.status, ERR_SCHED_WAIT)) return false;
+        item = *reinterpret_cast<volatile int*>(&sh.item[slot]);
+        return item >= 0;
+    };
+    auto release = [&](uint32_t n) { mbar_arrive_cluster(lead_item_empty + 8 * (n % QUEUE)); };
+
+    if (warp == 0) {
+        if (elect_one()) {
+            const int total = item_count<KIND>(p, n_valid), grid = gridDim.x >> 1;
+            const uint32_t lead_full = mapa(full, 0), tile0 = smem_u32(tiles);
+            const uint32_t peer_item = mapa(smem_u32(sh.item), 1), peer_item_full = mapa(item_full, 1);
+            int s = 0, item = blockIdx.x >> 1, next = 0;
+            uint32_t free_phase = 1;                        // (the first round finds every stage free)
+            bool ok = true;
+            for (uint32_t n = 0; ok; ++n) {
+                const int slot = n % QUEUE;
+                if (rank == 0) {
+                    if (item >= total) item = -1;
+                    if (!mbar_wait_cluster(item_empty + 8 * slot, ((n / QUEUE) & 1) ^ 1, p.status, ERR_SCHED_WAIT)) break;
+                    *reinterpret_cast<volatile int*>(&sh.item[slot]) = item;
+                    st_cluster_u32(peer_item + 4 * slot, (uint32_t)item);
+                    mbar_arrive(item_full + 8 * slot);
+                    mbar_arrive_cluster(peer_item_full + 8 * slot);         // (release at cluster scope: the item is visible)
+                    if (item < 0) break;
+                } else {
+                    const bool more = consume(n, item);
+                    release(n);
+                    if (!more) break;
+                }
+                const Item w = decode<KIND>(p, n_valid, item);
+                if (rank == 0 && w.nkb <= CLAIM) next = atomicAdd(p.sched, 1);
+                for (int kb = 0; kb < w.nkb; ++kb) {
+                    if (rank == 0 && w.nkb - kb == CLAIM + 1) next = atomicAdd(p.sched, 1);
+                    if (!mbar_wait_cluster(empty + 8 * s, free_phase, p.status, ERR_EMPTY_WAIT)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t a_dst = tile0 + s * STAGE_BYTES, b_dst = a_dst + OPER_BYTES, bar = lead_full + 8 * s;
+                    if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * STAGE_BYTES);       // both CTAs' bytes
+                    if (KIND != GRADS) {
+                        tma_load_2d_pair(a_dst, &tmA, kb * BK, w.m * TILE + rank * 128, bar);
+                        tma_load_2d_pair(b_dst, &tmB, kb * BK, p.v0 + w.n * TILE + rank * 128, bar);
+                    } else {
+                        const int blocks = p.v_tiles * (TILE / 64), col = w.n * TILE + rank * w.half;
+                        const CUtensorMap* mB;
+                        int row;
+                        if (!w.dw) {
+                            tma_load_3d_pair(a_dst, &tmA, 0, 0, (w.m * 2 + rank) * blocks + w.k0 + kb, bar);
+                            mB = &tmB;
+                            row = p.v0 + (w.k0 + kb) * BK;
+                        } else {
+                            tma_load_3d_pair(a_dst, &tmA2, 0, (kb & 1) * 64, (kb >> 1) * blocks + w.m * (TILE / 64) + rank * 2, bar);
+                            mB = &tmB2;
+                            row = kb * BK;
+                        }
+                        tma_load_2d_pair(b_dst, mB, col, row, bar);
+                        tma_load_2d_pair(b_dst + BOX_BYTES, mB, col + 64, row, bar);
+                    }
+                    if (++s == NS) {
+                        s = 0;
+                        free_phase ^= 1;
+                    }
+                }
+                item = grid + next;
+            }
+        }
+    } else if (warp == 1) {
+        if (rank == 0 && elect_one()) {
+            uint32_t t = 0, phase = 0;
+            int s = 0, item;
+            bool ok = true;
+            const uint32_t peer_empty = mapa(empty, 1), peer_acc_full = mapa(acc_full, 1);
+            const uint32_t tile0 = smem_u32(tiles);
+            const uint64_t k_major = make_desc(tile0, 16, 1024), mn_major = make_desc(tile0, BOX_BYTES, 1024);
+            for (uint32_t n = 0; ok && consume(n, item); ++n) {
+                release(n);
+                const Item w = decode<KIND>(p, n_valid, item);
+                if (w.nkb == 0) continue;
+                const bool a_mn = KIND == GRADS && w.dw, b_mn = KIND == GRADS;
+                const uint32_t idesc = make_idesc(TILE, 2 * w.half, a_mn, b_mn), buf = t & 1u;
+                const uint64_t a0 = a_mn ? mn_major : k_major, b0 = (b_mn ? mn_major : k_major) + (OPER_BYTES >> 4);
+                const uint32_t a_step = a_mn ? 2048 >> 4 : 32 >> 4, b_step = b_mn ? 2048 >> 4 : 32 >> 4;     // (the address field: 16-byte units)
+                if (!mbar_wait_cluster(acc_empty + 8 * buf, ((t >> 1) & 1) ^ 1, p.status, ERR_ACC_WAIT)) break;
+                tc_fence_after();
+                const uint32_t d_tmem = tmem_base + buf * TILE;
+                for (int kb = 0; kb < w.nkb; ++kb) {
+                    if (!mbar_wait_cluster(full + 8 * s, phase, p.status, ERR_FULL_WAIT)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t ad = a0 + s * (STAGE_BYTES >> 4), bd = b0 + s * (STAGE_BYTES >> 4);
+#pragma unroll
+                    for (int k = 0; k < BK / 16; ++k)
+                        umma_bf16_pair(d_tmem, ad + k * a_step, bd + k * b_step, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+                    umma_commit_pair(empty + 8 * s);
+                    umma_commit_pair(peer_empty + 8 * s);
+                    if (++s == NS) {
+                        s = 0;
+                        phase ^= 1;
+                    }
+                }
+                if (ok) {
+                    umma_commit_pair(acc_full + 8 * buf);
+                    umma_commit_pair(peer_acc_full + 8 * buf);
+                }
+                ++t;
+            }
+        }
+    } else {
+        // 16 epilogue warps: TMEM lane quarter q, 64 columns each
+        const int q = warp & 3, h = (warp - 2) >> 2;
+        uint8_t* const stage = extra + (warp - 2) * STAGING;
+        const uint32_t acc_free = mapa(acc_empty, 0);
+        uint32_t t = 0;
+        int item = -1;
+        for (uint32_t n = 0; __any_sync(0xffffffffu, consume(n, item)); ++n) {
+            __syncwarp();
+            if (lane == 0) release(n);
+            const Item w = decode<KIND>(p, n_valid, item);
+            const uint32_t buf = t & 1u;
+            const bool empty_sum = w.nkb == 0;              // no token takes part: dw is zero
+            if (!empty_sum) {
+                if (!mbar_wait_cluster(acc_full + 8 * buf, (t >> 1) & 1, p.status, ERR_ACC_WAIT)) break;
+                tc_fence_after();
+                ++t;
+            }
+            const uint32_t t_lane = tmem_base + buf * TILE + ((uint32_t)(q * 32) << 16) + h * 64;
+            auto give_back = [&]() {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(acc_free + 8 * buf);
+            };
+            if (KIND == LOSS) {
+                const int row = w.m * TILE + rank * 128 + q * 32 + lane, v = w.n * TILE + h * 64, valid = p.V - v;
+                const int at = p.target[row] - v;           // (rows beyond the packed ones hold target -1)
+                float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float z[32];
+                    tmem_ld32(t_lane + c * 32, z);
+                    tmem_ld_wait();
+                    if (c == 1) give_back();
+                    if (valid < (c + 1) * 32) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (c * 32 + j >= valid) z[j] = -INFINITY;
+                    }
+                    if (__any_sync(0xffffffffu, (at >> 5) == c)) {          // a target in these columns: 32 rows in every ten tiles or so
+                        float zt = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (at == c * 32 + j) zt = z[j];
+                        if ((at >> 5) == c) p.z_target[row] = zt;
+                    }
+                    float m = z[0];
+#pragma unroll
+                    for (int j = 1; j < 32; ++j) m = fmaxf(m, z[j]);
+                    m = fmaxf(m, top);
+                    const float ref = m == -INFINITY ? 0.0f : m * LOG2E;    // (columns beyond the vocabulary alone)
+                    float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        s0 += exp2f(fmaf(z[j], LOG2E, -ref));
+                        s1 += exp2f(fmaf(z[j + 1], LOG2E, -ref));
+                    }
+                    sum = fmaf(sum, exp2f(fmaf(top, LOG2E, -ref)), s0 + s1);
+                    top = m;
+                }
+                // The four warps of a lane quarter join their columns.  (Four buffers: a warp that writes item n + 4 has met the
+                // accumulator that the joining warp gave back at n + 2, after it had read item n.)
+                float2* const mine = reinterpret_cast<float2*>(extra) + (n & 3) * 512 + q * 32 + lane;
+                mine[h * 128] = make_float2(top, sum);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sh.joined[q]));
+                if (h == 0) {
+                    if (!mbar_wait(smem_u32(&sh.joined[q]), n & 1, p.status, ERR_ACC_WAIT)) break;
+                    float2 o[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[i] = mine[i * 128];
+                    const float m = fmaxf(fmaxf(o[0].x, o[1].x), fmaxf(o[2].x, o[3].x));
+                    float all = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) all += o[i].y * shift(o[i].x, m);
+                    p.part[(size_t)w.n * p.n_pad + row] = make_float2(m, all);
+                }
+            } else if (KIND == DLOGITS) {
+                const int row = w.m * TILE + rank * 128 + q * 32 + lane, v = p.v0 + w.n * TILE + h * 64, valid = p.V - v;
+                const int at = p.target[row] - v;
+                const float up = p.d_loss[row], ref = p.lse[row] * LOG2E;
+                const bool real = row < n_valid;
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the staging tile is free again
+                __syncwarp();
+                const uint32_t line = smem_u32(stage) + lane * 128;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float z[32];
+                    tmem_ld32(t_lane + c * 32, z);
+                    tmem_ld_wait();
+                    if (c == 1) give_back();
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) z[j] = real ? exp2f(fmaf(z[j], LOG2E, -ref)) * up : 0.0f;
+                    if (valid < (c + 1) * 32) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (c * 32 + j >= valid) z[j] = 0.0f;
+                    }
+                    if (__any_sync(0xffffffffu, (at >> 5) == c)) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (at == c * 32 + j) z[j] -= up;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {           // 16-byte pieces in the 128-byte swizzle
+                        uint32_t b[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const __nv_bfloat162 two = __floats2bfloat162_rn(z[8 * j + 2 * i], z[8 * j + 2 * i + 1]);
+                            b[i] = *reinterpret_cast<const uint32_t*>(&two);
+                        }
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(line + (((uint32_t)(c * 4 + j) ^ (lane & 7u)) << 4)),
+                                     "r"(b[0]), "r"(b[1]), "r"(b[2]), "r"(b[3]) : "memory");
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    bf16* dst = p.dz + (((size_t)(w.m * 2 + rank) * (p.v_tiles * (TILE / 64)) + w.n * (TILE / 64) + h) * 128 + q * 32) * 64;
+                    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(stage)), "r"(STAGING) : "memory");
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                }
+            } else {
+                // rows r0.. of the result (tokens, or vocabulary rows), columns c0..; 8 lanes share a 128-byte line of a row
+                const int r0 = w.m * TILE + rank * 128 + q * 32, c0 = w.n * TILE + h * 64;
+                const int rows = w.dw ? p.V - p.v0 - r0 : n_valid - r0;
+                const int sub = lane >> 3, piece = lane & 7;
+                const uint32_t base = smem_u32(stage), line = base + lane * 128;
+                float a[2][32];
+                if (empty_sum) {
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) a[j >> 5][j & 31] = 0.0f;
+                } else {
+                    tmem_ld32(t_lane, a[0]);
+                    tmem_ld32(t_lane + 32, a[1]);
+                    tmem_ld_wait();
+                    give_back();
+                    if (w.dw) {
+#pragma unroll
+                        for (int j = 0; j < 64; ++j) a[j >> 5][j & 31] *= scale;
+                    }
+                }
+                if (c0 >= p.C || (w.half == 64 && h >= 2)) continue;
+                auto put = [&](int j, const uint32_t (&b)[4]) {
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(line + (((uint32_t)j ^ (lane & 7u)) << 4)),
+                                 "r"(b[0]), "r"(b[1]), "r"(b[2]), "r"(b[3]) : "memory");
+                };
+                auto get = [&](int r) {                     // this lane's piece of row r
+                    uint4 u;
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                                 : "r"(base + r * 128 + (((uint32_t)piece ^ (r & 7u)) << 4)) : "memory");
+                    return u;
+                };
+                if (w.dw && !p.dw_f32) {
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        uint32_t b[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const __nv_bfloat162 two = __floats2bfloat162_rn(a[j >> 2][(8 * j + 2 * i) & 31], a[j >> 2][(8 * j + 2 * i + 1) & 31]);
+                            b[i] = *reinterpret_cast<const uint32_t*>(&two);
+                        }
+                        put(j, b);
+                    }
+                    __syncwarp();
+                    bf16* dst = (bf16*)p.dw + (size_t)(p.v0 + r0) * p.C + c0 + piece * 8;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = 4 * i + sub;
+                        if (r < rows && c0 + piece * 8 < p.C) *reinterpret_cast<uint4*>(dst + (size_t)r * p.C) = get(r);
+                    }
+                } else {
+                    float* const out = w.dw ? (float*)p.dw + (size_t)(p.v0 + r0) * p.C : p.acc + ((size_t)w.slice * p.n_pad + r0) * p.C;
+                    const bool add = w.dw || !p.first;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const uint32_t b[4] = {__float_as_uint(a[c][4 * j]), __float_as_uint(a[c][4 * j + 1]), __float_as_uint(a[c][4 * j + 2]),
+                                                   __float_as_uint(a[c][4 * j + 3])};
+                            put(j, b);
+                        }
+                        __syncwarp();
+                        const int col = c0 + c * 32 + piece * 4;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int r = 4 * i + sub;
+                            if (r < rows && col < p.C) {
+                                float4* d = reinterpret_cast<float4*>(out + (size_t)r * p.C + col);
+                                const uint4 u = get(r);
+                                float4 x = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
+                                if (add) {
+                                    const float4 o = *d;
+                                    x.x += o.x; x.y += o.y; x.z += o.z; x.w += o.w;
+                                }
+                                *d = x;
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        if (KIND == DLOGITS && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+    // neither CTA may leave (or give its TMEM back) while the other can still read its shared memory or signal it
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, TMEM_COLS);
+    }
+}
+
+// ---- packing ----------------------------------------------------------------------------------------------------------
+struct PackP {
+    const void* x;
+    const int32_t* targets;
+    int n, C, Cp, V, n_pad, per_block;
+    int32_t* n_valid;           // [0], followed by the counters of the products
+    int32_t *rows, *target;     // packed -> token; its target
+    bf16* xp;                   // [n_pad][Cp]
+    int32_t* status;
+    // the loss
+    float *loss, *lse;          // zero for tokens that take no part
+    // the gradients
+    const float *lse_in, *d_loss_in;
+    float *lse_p, *d_loss_p, *scale;
+    void* dx;                   // zero for tokens that take no part
+};
+
+// The tokens that take part, packed in their order, and zeros up to whole tiles.  Every block counts the targets before its
+// own tokens (and all of them, for the zeros): N * 4 bytes out of L2 for each of at most 296 blocks.
+template <typename TIo, bool GRAD>
+__global__ void __launch_bounds__(256) head_pack_kernel(const PackP p)
+{
+    pdl_wait();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int t0 = blockIdx.x * p.per_block, t1 = min(p.n, t0 + p.per_block);
+    __shared__ int sums[2][8];
+    __shared__ float tops[8];
+    int before = 0, all = 0;
+    float top = 0.0f;
+    bool bad = false;
+    for (int i = tid; i < p.n; i += 256) {
+        const int t = p.targets[i], in = t >= 0 && t < p.V;
+        bad |= t >= p.V;
+        all += in;
+        before += i < t0 ? in : 0;
+        if (GRAD && in) top = fmaxf(top, fabsf(p.d_loss_in[i]));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+        all += __shfl_xor_sync(0xffffffffu, all, o);
+        if (GRAD) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+    if (lane == 0) sums[0][warp] = before, sums[1][warp] = all, tops[warp] = top;
+    __syncthreads();
+    before = all = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) before += sums[0][i], all += sums[1][i], top = fmaxf(top, tops[i]);
+    if (!(top > 0.0f && top < INFINITY)) top = 1.0f;        // (a d_loss that is not finite spoils its own token only)
+    if (blockIdx.x == 0) {
+        for (int i = tid; i < COUNTERS; i += 256) p.n_valid[i] = i == 0 ? all : 0;
+        if (GRAD && tid == 0) *p.scale = top;
+        if (bad && p.status) atomicOr(p.status, ST_BAD_TARGET);
+    }
+    constexpr int PER = 8;
+    auto copy_row = [&](const TIo* from, bf16* to) {        // one warp; columns beyond C (and all without `from`) are zero
+        for (int c = lane * PER; c < p.Cp; c += 32 * PER) {
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (from && c < p.C) {
+                if constexpr (sizeof(TIo) == 2) {
+                    u = *reinterpret_cast<const uint4*>(from + c);
+                } else {
+                    const float4 a = *reinterpret_cast<const float4*>(from + c), b = *reinterpret_cast<const float4*>(from + c + 4);
+                    const __nv_bfloat162 h[4] = {__floats2bfloat162_rn(a.x, a.y), __floats2bfloat162_rn(a.z, a.w),
+                                                 __floats2bfloat162_rn(b.x, b.y), __floats2bfloat162_rn(b.z, b.w)};
+                    u = *reinterpret_cast<const uint4*>(h);
+                }
+            }
+            *reinterpret_cast<uint4*>(to + c) = u;
+        }
+    };
+    // 32 tokens at a time: every warp finds their places, and takes every eighth of them
+    for (int i0 = t0; i0 < t1; i0 += 32) {
+        const int i = i0 + lane, t = i < t1 ? p.targets[i] : -1;
+        const bool in = t >= 0 && t < p.V;
+        const uint32_t mask = __ballot_sync(0xffffffffu, in);
+        const int j = before + __popc(mask & ((1u << lane) - 1u));
+        if (warp == 0 && i < t1) {
+            if (in) {
+                p.rows[j] = i;
+                p.target[j] = t;
+                if (GRAD) {
+                    p.lse_p[j] = p.lse_in[i];
+                    p.d_loss_p[j] = p.d_loss_in[i] / top;
+                }
+            } else if (!GRAD) {
+                p.loss[i] = 0.0f;
+                p.lse[i] = 0.0f;
+            }
+        }
+        for (int r = warp; r < min(32, t1 - i0); r += 8) {
+            const size_t o = (size_t)(i0 + r) * p.C;
+            const int at = __shfl_sync(0xffffffffu, j, r);
+            if (mask >> r & 1) {
+                copy_row((const TIo*)p.x + o, p.xp + (size_t)at * p.Cp);
+            } else if (GRAD) {
+                for (int c = lane * PER; c < p.C; c += 32 * PER)
+#pragma unroll
+                    for (int k = 0; k < (int)sizeof(TIo) / 2; ++k) reinterpret_cast<uint4*>((TIo*)p.dx + o + c)[k] = make_uint4(0, 0, 0, 0);
+            }
+        }
+        before += __popc(mask);
+    }
+    const int end = (all + TILE - 1) / TILE * TILE;
+    for (int j = all + blockIdx.x * 8 + warp; j < end; j += gridDim.x * 8) {
+        copy_row(nullptr, p.xp + (size_t)j * p.Cp);
+        if (lane == 0) {
+            p.target[j] = -1;
+            if (GRAD) p.lse_p[j] = p.d_loss_p[j] = 0.0f;
+        }
+    }
+}
+
+// ---- joining ----------------------------------------------------------------------------------------------------------
+// lse and loss from the tiles' maxima and sums: 32 tokens per block, eight warps with every eighth tile each, joined in order.
+__global__ void __launch_bounds__(256)
+head_join_kernel(const int32_t* n_valid, const float2* part, const float* z_target, const int32_t* rows, int v_tiles, int n_pad, float* loss, float* lse)
+{
+    pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
+    if (blockIdx.x * 32 >= *n_valid) return;
+    const bool real = row < *n_valid;
+    __shared__ float2 sh[8][32];
+    float top = -INFINITY, sum = 0.0f;
+    if (real)
+#pragma unroll 4
+        for (int v = warp; v < v_tiles; v += 8) {
+            const float2 o = part[(size_t)v * n_pad + row];
+            const float m = fmaxf(top, o.x);
+            sum = sum * shift(top, m) + o.y * shift(o.x, m);
+            top = m;
+        }
+    sh[warp][lane] = make_float2(top, sum);
+    __syncthreads();
+    if (warp > 0 || !real) return;
+    float m = -INFINITY, all = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, sh[i][lane].x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < v_tiles) all += sh[i][lane].y * shift(sh[i][lane].x, m);
+    const float l = m + logf(all);
+    const int i = rows[row];
+    lse[i] = l;
+    loss[i] = l - z_target[row];
+}
+
+// dx from the slices of the vocabulary, a warp per token.
+template <typename TIo>
+__global__ void __launch_bounds__(256)
+head_dx_kernel(const int32_t* n_valid, const float* scale, const float* acc, const int32_t* rows, int slices, int n_pad, int C, TIo* dx)
+{
+    pdl_wait();
+    const int lane = threadIdx.x & 31, row = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= *n_valid) return;
+    TIo* out = dx + (size_t)rows[row] * C;
+    const float f = *scale;
+    for (int c = lane * 4; c < C; c += 128) {
+        const float* from = acc + (size_t)row * C + c;
+        float4 s = *reinterpret_cast<const float4*>(from);
+        for (int i = 1; i < slices; ++i) {
+            const float4 o = *reinterpret_cast<const float4*>(from + (size_t)i * n_pad * C);
+            s.x += o.x; s.y += o.y; s.z += o.z; s.w += o.w;
+        }
+        s.x *= f; s.y *= f; s.z *= f; s.w *= f;
+        if constexpr (sizeof(TIo) == 2) {
+            const __nv_bfloat162 a = __floats2bfloat162_rn(s.x, s.y), b = __floats2bfloat162_rn(s.z, s.w);
+            *reinterpret_cast<uint2*>(out + c) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+        } else {
+            *reinterpret_cast<float4*>(out + c) = s;
+        }
+    }
+}
+
+// ---- host side --------------------------------------------------------------------------------------------------------
+size_t up(size_t v, size_t a) { return (v + a - 1) / a * a; }
+
+struct HeadWs {
+    size_t counters, scale, rows, target, lse, d_loss, z_target, xp, part, acc, dz;
+    size_t fixed;               // all of it but dz
+    int n_pad, Cp, v_tiles, c_tiles;
+};
+HeadWs head_ws(int n, int C, int V, bool grad, int slices)
+{
+    HeadWs w = {};
+    w.n_pad = (int)up(n, TILE);
+    w.Cp = (int)up(C, 64);
+    w.v_tiles = (int)(up(V, TILE) / TILE);
+    w.c_tiles = (int)(up(C, TILE) / TILE);
+    size_t off = 0;
+    auto take = [&](size_t bytes) {
+        const size_t o = off;
+        off = up(off + bytes, 1024);
+        return o;
+    };
+    const size_t N = w.n_pad;
+    w.counters = take(COUNTERS * 4);
+    w.scale = take(4);
+    w.rows = take(N * 4);
+    w.target = take(N * 4);
+    w.xp = take(N * w.Cp * 2);
+    if (grad) {
+        w.lse = take(N * 4);
+        w.d_loss = take(N * 4);
+        w.acc = take(N * C * 4 * slices);
+        w.dz = off;
+    } else {
+        w.z_target = take(N * 4);
+        w.part = take(N * w.v_tiles * 8);
+    }
+    w.fixed = off;
+    return w;
+}
+size_t dz_tile_bytes(int n_pad) { return (size_t)n_pad * TILE * 2; }     // of 256 vocabulary rows
+
+int check_shape(int n, int C, int V, int io)
+{
+    if (n < 0 || C <= 0 || V <= 0) return fail(MGPT_MOE_EINVAL, "head loss: sizes must be positive");
+    if (C % 8) return fail(MGPT_MOE_EINVAL, "head loss: embed_dim must be a multiple of 8");
+    if (io != MGPT_MOE_IO_F32 && io != MGPT_MOE_IO_BF16) return fail(MGPT_MOE_EINVAL, "unknown io dtype");
+    if (up(n, TILE) > (1u << 30) || up(V, TILE) > (1u << 30) || (double)(up(n, TILE) / TILE) * (up(V, TILE) / TILE) > 1e9 || C > (1 << 20))
+        return fail(MGPT_MOE_EINVAL, "head loss: sizes out of range");
+    return 0;
+}
+// token tiles whose x (and dz) share the L2 with a vocabulary tile
+int group_of(int n_pad, int Cp)
+{
+    const size_t tile = (size_t)TILE * Cp * 2, most = (size_t)32 << 20;
+    const int mt = n_pad / TILE, g = (int)(most / tile);
+    return g < 1 ? 1 : g > mt ? mt : g;
+}
+// Slices of the vocabulary that dx is summed in: as many as give every pair of SMs an item where the tokens are few.
+int slices_of(int n_pad, int c_tiles, int v_tiles)
+{
+    const int items = n_pad / TILE * c_tiles;
+    int s = (2 * 74 + items - 1) / items;
+    if (s > v_tiles / 4) s = v_tiles / 4;
+    return items >= 74 || s < 1 ? 1 : s;
+}
+
+template <int KIND> int launch_head(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& a2, const CUtensorMap& b2, const HeadP& p, int pairs, cudaStream_t st)
+{
+    static bool done[64] = {};
+    int dev = 0;
+    MGPT_CUDA(cudaGetDevice(&dev));
+    if (dev >= 64 || !done[dev]) {
+        MGPT_CUDA(cudaFuncSetAttribute(head_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<KIND>()));
+        if (dev < 64) done[dev] = true;
+    }
+    MGPT_CUDA(launch_pdl(head_kernel<KIND>, 2 * pairs, THREADS, smem_bytes<KIND>(), st, a, b, a2, b2, p));
+    MGPT_LAUNCHED("head_kernel");
+    return 0;
+}
+int sm_count(int* sms)
+{
+    int dev = 0;
+    MGPT_CUDA(cudaGetDevice(&dev));
+    MGPT_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+    if (*sms < 2) return fail(MGPT_MOE_ECUDA, "head loss: needs two SMs");
+    return 0;
+}
+
+template <bool GRAD> int launch_pack(PackP& p, int io, cudaStream_t st)
+{
+    p.per_block = (p.n + 295) / 296;
+    int blocks = (p.n + p.per_block - 1) / p.per_block;
+    if (blocks < 32) blocks = 32;                       // (the zeros behind the last token)
+    if (io == MGPT_MOE_IO_BF16) MGPT_CUDA(launch_pdl(head_pack_kernel<bf16, GRAD>, blocks, 256, 0, st, p));
+    else MGPT_CUDA(launch_pdl(head_pack_kernel<float, GRAD>, blocks, 256, 0, st, p));
+    MGPT_LAUNCHED("head_pack_kernel");
+    return 0;
+}
+
+}  // namespace
+
+}  // namespace mgpt
+
+using namespace mgpt;
+
+extern "C" {
+
+size_t mgpt_moe_op_head_loss_workspace_bytes(int n, int C, int V)
+{
+    if (check_shape(n, C, V, MGPT_MOE_IO_BF16)) return 0;
+    return head_ws(n, C, V, false, 1).fixed;
+}
+
+size_t mgpt_moe_op_head_loss_backward_workspace_bytes(int n, int C, int V, size_t piece_bytes)
+{
+    if (check_shape(n, C, V, MGPT_MOE_IO_BF16)) return 0;
+    HeadWs w = head_ws(n, C, V, true, 1);
+    w = head_ws(n, C, V, true, slices_of(w.n_pad, w.c_tiles, w.v_tiles));
+    const size_t tile = dz_tile_bytes(w.n_pad);
+    size_t tiles = piece_bytes / tile;
+    const size_t least = ((size_t)w.v_tiles + MAX_PIECES - 1) / MAX_PIECES;
+    tiles = tiles < least ? least : tiles > (size_t)w.v_tiles ? w.v_tiles : tiles;
+    return w.fixed + tiles * tile;
+}
+
+int mgpt_moe_op_head_loss(const void* x, int io, const void* w, const int32_t* targets, int n, int C, int V, float* loss, float* lse,
+                          int32_t* status, void* workspace, size_t ws_bytes, mgpt_stream_t stream)
+{
+    MGPT_TRY(check_shape(n, C, V, io));
+    if (n == 0) return 0;
+    if (!x || !w || !targets || !loss || !lse || !status) return fail(MGPT_MOE_EINVAL, "null argument");
+    MGPT_TRY(check_aligned(x, "x"));
+    MGPT_TRY(check_aligned(w, "w"));
+    if (!workspace || ((uintptr_t)workspace & 255)) return fail(MGPT_MOE_EINVAL, "workspace must be 256-byte aligned");
+    const HeadWs h = head_ws(n, C, V, false, 1);
+    if (ws_bytes < h.fixed) return fail(MGPT_MOE_ENOMEM, "workspace smaller than mgpt_moe_op_head_loss_workspace_bytes()");
+    cudaStream_t st = (cudaStream_t)stream;
+    char* ws = (char*)workspace;
+    int sms;
+    MGPT_TRY(sm_count(&sms));
+    CUtensorMap mx, mw;
+    MGPT_TRY(make_map_kind(&mx, ws + h.xp, h.n_pad, h.Cp, 128, false));
+    MGPT_TRY(make_map_kind(&mw, w, V, C, 128, false));
+    PackP k = {};
+    k.x = x; k.targets = targets; k.n = n; k.C = C; k.Cp = h.Cp; k.V = V; k.n_pad = h.n_pad;
+    k.n_valid = (int32_t*)(ws + h.counters);
+    k.rows = (int32_t*)(ws + h.rows); k.target = (int32_t*)(ws + h.target); k.xp = (bf16*)(ws + h.xp);
+    k.status = status; k.loss = loss; k.lse = lse;
+    MGPT_TRY(launch_pack<false>(k, io, st));
+    HeadP p = {};
+    p.n_valid = k.n_valid; p.sched = k.n_valid + 1; p.status = status; p.C = C; p.V = V; p.v_tiles = h.v_tiles;
+    p.group = group_of(h.n_pad, h.Cp); p.n_pad = h.n_pad; p.target = k.target;
+    p.part = (float2*)(ws + h.part); p.z_target = (float*)(ws + h.z_target);
+    const long items = (long)(h.n_pad / TILE) * h.v_tiles;
+    MGPT_TRY(launch_head<LOSS>(mx, mw, mx, mw, p, (int)(items < sms / 2 ? items : sms / 2), st));
+    MGPT_CUDA(launch_pdl(head_join_kernel, (n + 31) / 32, 256, 0, st, k.n_valid, p.part, p.z_target, k.rows, h.v_tiles, h.n_pad, loss, lse));
+    MGPT_LAUNCHED("head_join_kernel");
+    return 0;
+}
+
+int mgpt_moe_op_head_loss_backward(const void* x, int io, const void* w, const int32_t* targets, const float* lse, const float* d_loss,
+                                   int n, int C, int V, void* dx, void* dw, int dw_dtype, int32_t* status,
+                                   void* workspace, size_t ws_bytes, mgpt_stream_t stream)
+{
+    MGPT_TRY(check_shape(n, C, V, io));
+    if (dw_dtype != MGPT_MOE_IO_F32 && dw_dtype != MGPT_MOE_IO_BF16) return fail(MGPT_MOE_EINVAL, "unknown dtype of dw");
+    cudaStream_t st = (cudaStream_t)stream;
+    if (!dw) return fail(MGPT_MOE_EINVAL, "null argument");
+    MGPT_TRY(check_aligned(dw, "dw"));
+    if (n == 0) {
+        if (dw_dtype == MGPT_MOE_IO_BF16) MGPT_CUDA(cudaMemsetAsync(dw, 0, (size_t)V * C * 2, st));
+        return 0;
+    }
+    if (!x || !w || !targets || !lse || !d_loss || !dx || !status) return fail(MGPT_MOE_EINVAL, "null argument");
+    MGPT_TRY(check_aligned(x, "x"));
+    MGPT_TRY(check_aligned(w, "w"));
+    MGPT_TRY(check_aligned(dx, "dx"));
+    if (!workspace || ((uintptr_t)workspace & 255)) return fail(MGPT_MOE_EINVAL, "workspace must be 256-byte aligned");
+    HeadWs h = head_ws(n, C, V, true, 1);
+    const int slices = slices_of(h.n_pad, h.c_tiles, h.v_tiles);
+    h = head_ws(n, C, V, true, slices);
+    const size_t tile = dz_tile_bytes(h.n_pad);
+    const size_t room = ws_bytes > h.fixed ? (ws_bytes - h.fixed) / tile : 0;
+    if (room < ((size_t)h.v_tiles + MAX_PIECES - 1) / MAX_PIECES)
+        return fail(MGPT_MOE_ENOMEM, "workspace smaller than mgpt_moe_op_head_loss_backward_workspace_bytes()");
+    const int most = room > (size_t)h.v_tiles ? h.v_tiles : (int)room;
+    const int pieces = (h.v_tiles + most - 1) / most, per = (h.v_tiles + pieces - 1) / pieces;
+    char* ws = (char*)workspace;
+    int sms;
+    MGPT_TRY(sm_count(&sms));
+    CUtensorMap mx, mw, mx_t, mw_t, mz, mz_t;
+    MGPT_TRY(make_map_kind(&mx, ws + h.xp, h.n_pad, h.Cp, 128, false));
+    MGPT_TRY(make_map_kind(&mw, w, V, C, 128, false));
+    MGPT_TRY(make_map_kind(&mx_t, ws + h.xp, h.n_pad, h.Cp, 64, false));
+    MGPT_TRY(make_map_kind(&mw_t, w, V, C, 64, false));
+    const uint64_t tiles = (uint64_t)(h.n_pad / 128) * per * (TILE / 64);
+    MGPT_TRY(make_map_tiles(&mz, ws + h.dz, tiles, 128, 1));
+    MGPT_TRY(make_map_tiles(&mz_t, ws + h.dz, tiles, 64, 2));
+    PackP k = {};
+    k.x = x; k.targets = targets; k.n = n; k.C = C; k.Cp = h.Cp; k.V = V; k.n_pad = h.n_pad;
+    k.n_valid = (int32_t*)(ws + h.counters);
+    k.rows = (int32_t*)(ws + h.rows); k.target = (int32_t*)(ws + h.target); k.xp = (bf16*)(ws + h.xp);
+    k.status = status; k.lse_in = lse; k.d_loss_in = d_loss; k.lse_p = (float*)(ws + h.lse); k.d_loss_p = (float*)(ws + h.d_loss); k.scale = (float*)(ws + h.scale); k.dx = dx;
+    MGPT_TRY(launch_pack<true>(k, io, st));
+    HeadP p = {};
+    p.n_valid = k.n_valid; p.status = status; p.C = C; p.V = V; p.group = group_of(h.n_pad, h.Cp); p.n_pad = h.n_pad;
+    p.target = k.target; p.lse = k.lse_p; p.d_loss = k.d_loss_p; p.scale = k.scale; p.dz = (bf16*)(ws + h.dz); p.acc = (float*)(ws + h.acc);
+    p.c_tiles = h.c_tiles; p.dw = dw; p.dw_f32 = dw_dtype == MGPT_MOE_IO_F32;
+    for (int i = 0; i < pieces; ++i) {
+        p.v0 = i * per * TILE;
+        p.v_tiles = h.v_tiles - i * per < per ? h.v_tiles - i * per : per;
+        p.slice_tiles = (per + slices - 1) / slices;            // (of a full piece, whose slices the others keep within)
+        p.k_slices = (p.v_tiles + p.slice_tiles - 1) / p.slice_tiles;
+        p.first = i == 0;
+        const long items = (long)(h.n_pad / TILE) * p.v_tiles;
+        p.sched = k.n_valid + 1 + 2 * i;
+        MGPT_TRY(launch_head<DLOGITS>(mx, mw, mx, mw, p, (int)(items < sms / 2 ? items : sms / 2), st));
+        p.sched = k.n_valid + 2 + 2 * i;
+        const long grads = ((long)(h.n_pad / TILE) * p.k_slices + p.v_tiles) * p.c_tiles;
+        MGPT_TRY(launch_head<GRADS>(mz, mw_t, mz_t, mx_t, p, (int)(grads < sms / 2 ? grads : sms / 2), st));
+    }
+    const int used = (per + (per + slices - 1) / slices - 1) / ((per + slices - 1) / slices);
+    const int blocks = (n + 7) / 8;
+    if (io == MGPT_MOE_IO_BF16) MGPT_CUDA(launch_pdl(head_dx_kernel<bf16>, blocks, 256, 0, st, k.n_valid, p.scale, p.acc, k.rows, used, h.n_pad, C, (bf16*)dx));
+    else MGPT_CUDA(launch_pdl(head_dx_kernel<float>, blocks, 256, 0, st, k.n_valid, p.scale, p.acc, k.rows, used, h.n_pad, C, (float*)dx));
+    MGPT_LAUNCHED("head_dx_kernel");
+    return 0;
+}
+
+}  // extern "C"

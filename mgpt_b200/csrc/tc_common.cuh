@@ -265,5 +265,7 @@ int make_map_kind(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols
 // operand in whose reduction runs over the rows.  With cols no multiple of 64 the last block runs on into the next row (the
 // last row's: past the matrix), so that the product's rows or columns beyond cols hold anything.
 int make_map_blocks(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t n_blocks);
+// Tiles of 128 rows x 64 bf16 that lie one after another, loaded as they lie: box = {64, box_rows, n_tiles}.
+int make_map_tiles(CUtensorMap* m, const void* base, uint64_t tiles, uint32_t box_rows, uint32_t n_tiles);
 
 }  // namespace mgpt

@@ -1,0 +1,250 @@
+"""The rest of a training step around the layer, over the C ABI: the loss of a language model's head, the norms around a
+block with its gate and skip connection, and AdamW over many tensors.
+
+As in :mod:`mgpt_b200.moe_layer`, torch is used for device memory and streams only.  Every call enqueues its work on the
+current stream and returns; wrong arguments raise :class:`MoeError` before anything is enqueued.
+"""
+from __future__ import annotations
+
+import ctypes as ct
+
+import torch
+
+from . import _lib
+from ._lib import IO_BF16, IO_F32, MoeError
+
+PIECE_BYTES = 256 << 20         # of the vocabulary's gradient rows that are worked on at a time
+STATE_BLOCK = 256               # elements that share a scale of the 8-bit moments
+
+_DTYPES = {torch.float32: IO_F32, torch.bfloat16: IO_BF16}
+_status = {}
+
+
+def _need(ok, what):
+    if not ok:
+        raise MoeError(what)
+
+
+def _device(t: torch.Tensor) -> torch.device:
+    _need(t.is_cuda, "mgpt_b200: tensors must be on a CUDA device; there is no CPU path")
+    if t.device.index != torch.cuda.current_device():
+        raise MoeError(f"tensors are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return t.device
+
+
+def _check(t, name, shape, dtypes, device):
+    if not (t.device == device and t.dtype in dtypes and t.is_contiguous() and tuple(t.shape) == tuple(shape)):
+        raise MoeError(f"{name}: expected a contiguous {tuple(shape)} tensor of {' or '.join(str(d) for d in dtypes)} on {device}, "
+                       f"got {tuple(t.shape)} of {t.dtype} on {t.device}" + ("" if t.is_contiguous() else ", not contiguous"))
+    return t.data_ptr()
+
+
+def _optional(t, *args):
+    return None if t is None else _check(t, *args)
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _workspace(nbytes, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def _status_word(device):
+    s = _status.get(device)
+    if s is None:
+        s = _status[device] = torch.zeros(1, dtype=torch.int32, device=device)
+        torch.cuda.current_stream(device).synchronize()     # cleared before any stream writes to it
+    return s
+
+
+def check_status(device=None) -> None:
+    """Raises :class:`MoeError` if a call of :func:`head_loss` or :func:`head_loss_backward` on this device recorded an error
+    since the last check (a target beyond the vocabulary, a bounded wait that ran out).  Synchronises the device."""
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    s = _status.get(device)
+    if s is None:
+        return
+    torch.cuda.synchronize(device)
+    bits = int(s.item())
+    if bits:
+        s.zero_()
+        torch.cuda.synchronize(device)
+        what = []
+        if bits & 32:
+            what.append("a target is beyond the vocabulary (it took no part)")
+        if bits & ~32:
+            what.append("a bounded wait ran out: results are incomplete")
+        raise MoeError(f"head loss status {bits}: " + "; ".join(what))
+
+
+# ---- the loss of a language model's head ------------------------------------------------------------------------------
+def _head_args(x, weight, targets):
+    device = _device(x)
+    _need(x.dim() >= 1 and weight.dim() == 2, "head loss: x is [..., C], weight [V, C]")
+    _need(x.dtype in _DTYPES, f"head loss: unsupported token dtype {x.dtype}")
+    V, C = weight.shape
+    _need(V > 0 and C > 0 and x.shape[-1] == C, f"head loss: x is {tuple(x.shape)}, weight {tuple(weight.shape)}")
+    n = x.numel() // C
+    xp = _check(x, "x", x.shape, (x.dtype,), device)
+    wp = _check(weight, "weight", (V, C), (torch.bfloat16,), device)
+    tp = _check(targets, "targets", x.shape[:-1], (torch.int32,), device)
+    return device, n, C, V, xp, wp, tp
+
+
+def head_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor):
+    """Cross entropy of ``x @ weight.T`` against ``targets``, token by token, without keeping the logits.
+
+    x: ``[..., C]``, FP32 or BF16; weight: BF16 ``[V, C]``; targets: int32 ``[...]``.  Returns ``(loss, lse)``, FP32
+    ``[...]``: ``lse`` is what :func:`head_loss_backward` needs.  Tokens whose target is outside ``[0, V)`` (padding, prompts)
+    take no part: loss and lse 0, and no work; targets ``>= V`` are reported by :func:`check_status`."""
+    lib = _lib.load()
+    device, n, C, V, xp, wp, tp = _head_args(x, weight, targets)
+    loss, lse = torch.empty((2, *targets.shape), dtype=torch.float32, device=device).unbind(0)
+    if n:
+        size = lib.mgpt_moe_op_head_loss_workspace_bytes(n, C, V)
+        ws = _workspace(size, device)
+        _lib.check(lib.mgpt_moe_op_head_loss(xp, _DTYPES[x.dtype], wp, tp, n, C, V, loss.data_ptr(), lse.data_ptr(),
+                                             _status_word(device).data_ptr(), ws.data_ptr(), size, _stream(device)))
+    return loss, lse
+
+
+def head_loss_backward(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor, d_loss: torch.Tensor,
+                       d_weight: torch.Tensor = None, *, piece_bytes: int = PIECE_BYTES):
+    """Gradients of :func:`head_loss`: ``(dx, d_weight)``.  ``d_loss``: FP32 ``[...]``, the gradient of each token's loss
+    (``1 / tokens`` for the mean).  ``d_weight``: an FP32 ``[V, C]`` tensor is added to, a BF16 one (or none: it is made) is
+    written.  ``piece_bytes``: workspace for the piece of the vocabulary that is worked on at a time."""
+    lib = _lib.load()
+    device, n, C, V, xp, wp, tp = _head_args(x, weight, targets)
+    lp = _check(lse, "lse", targets.shape, (torch.float32,), device)
+    gp = _check(d_loss, "d_loss", targets.shape, (torch.float32,), device)
+    if d_weight is None:
+        d_weight = torch.empty_like(weight)
+    dwp = _check(d_weight, "d_weight", (V, C), (torch.float32, torch.bfloat16), device)
+    dx = torch.empty_like(x)
+    size = lib.mgpt_moe_op_head_loss_backward_workspace_bytes(n, C, V, piece_bytes) if n else 0
+    ws = _workspace(size, device)
+    _lib.check(lib.mgpt_moe_op_head_loss_backward(xp, _DTYPES[x.dtype], wp, tp, lp, gp, n, C, V, dx.data_ptr(), dwp, _DTYPES[d_weight.dtype],
+                                                  _status_word(device).data_ptr(), ws.data_ptr(), size, _stream(device)))
+    return dx, d_weight
+
+
+# ---- norms around a block ---------------------------------------------------------------------------------------------
+def _norm_args(x, h, post_scale, gate, pre_scale, tokens_per_gate):
+    device = _device(x)
+    _need(x.dim() >= 1 and x.dtype in _DTYPES, f"residual norm: unsupported tokens {tuple(x.shape)} of {x.dtype}")
+    C = x.shape[-1]
+    n = x.numel() // C if C else 0
+    _need(tokens_per_gate >= 0, "residual norm: tokens_per_gate must not be negative")
+    xp, hp = _check(x, "x", x.shape, (x.dtype,), device), _check(h, "h", x.shape, (x.dtype,), device)
+    f32 = (torch.float32,)
+    rows = -(-n // tokens_per_gate) if tokens_per_gate else 1
+    if gate is not None and gate.dim() == 1 and rows == 1:
+        gate = gate.view(1, C) if gate.numel() == C else gate
+    return (device, n, C, rows, xp, hp, _optional(post_scale, "post_scale", (C,), f32, device), _optional(gate, "gate", (rows, C), f32, device),
+            _optional(pre_scale, "pre_scale", (C,), f32, device))
+
+
+def residual_norm(x: torch.Tensor, h: torch.Tensor, *, post_scale=None, gate=None, pre_scale=None, alpha: float = 1.0, eps: float = 1e-5,
+                  tokens_per_gate: int = 0):
+    """``y = alpha*x + gate * rmsnorm(h)*post_scale`` and ``u = rmsnorm(y)*pre_scale``: what follows a block and precedes the
+    next one, in one pass.  x, h: ``[..., C]``, both FP32 or both BF16.  Without ``post_scale`` h is not normalised, without
+    ``gate`` it is 1, without ``pre_scale`` there is no u (None).  ``gate``: FP32 ``[rows, C]``, a row for every
+    ``tokens_per_gate`` consecutive tokens (0: one row, which may be given as ``[C]``).  Returns ``(y, u, stats)``; ``stats`` is
+    what :func:`residual_norm_backward` needs."""
+    lib = _lib.load()
+    device, n, C, _, xp, hp, post, gp, pre = _norm_args(x, h, post_scale, gate, pre_scale, tokens_per_gate)
+    y = torch.empty_like(x)
+    u = torch.empty_like(x) if pre_scale is not None else None
+    stats = torch.empty((2, n), dtype=torch.float32, device=device)
+    _lib.check(lib.mgpt_moe_op_residual_norm(xp, hp, _DTYPES[x.dtype], post, gp, tokens_per_gate, pre, alpha, eps, n, C, y.data_ptr(),
+                                             None if u is None else u.data_ptr(), stats.data_ptr(), _stream(device)))
+    return y, u, stats
+
+
+def residual_norm_backward(x: torch.Tensor, h: torch.Tensor, stats: torch.Tensor, dy: torch.Tensor, du: torch.Tensor = None, *, post_scale=None,
+                           gate=None, pre_scale=None, alpha: float = 1.0, eps: float = 1e-5, tokens_per_gate: int = 0, d_post_scale=None,
+                           d_gate=None, d_pre_scale=None):
+    """Gradients of :func:`residual_norm`: returns ``(dx, dh)`` and adds to ``d_post_scale``, ``d_gate`` and ``d_pre_scale`` (FP32,
+    of the parameters' shapes) where they are given.  ``dy``: the gradient of y by its other uses; ``du``: that of u.  The other
+    arguments are those of the forward call (``eps`` is in ``stats`` already)."""
+    lib = _lib.load()
+    device, n, C, rows, xp, hp, post, gp, pre = _norm_args(x, h, post_scale, gate, pre_scale, tokens_per_gate)
+    f32 = (torch.float32,)
+    sp = _check(stats, "stats", (2, n), f32, device)
+    dyp, dup = _check(dy, "dy", x.shape, (x.dtype,), device), _optional(du, "du", x.shape, (x.dtype,), device)
+    if d_gate is not None and d_gate.dim() == 1 and rows == 1 and d_gate.numel() == C:
+        d_gate = d_gate.view(1, C)
+    dpost, dgate, dpre = (_optional(d_post_scale, "d_post_scale", (C,), f32, device), _optional(d_gate, "d_gate", (rows, C), f32, device),
+                          _optional(d_pre_scale, "d_pre_scale", (C,), f32, device))
+    dx, dh = torch.empty_like(x), torch.empty_like(x)
+    size = lib.mgpt_moe_op_residual_norm_backward_workspace_bytes(n, C, tokens_per_gate)
+    ws = _workspace(size, device)
+    _lib.check(lib.mgpt_moe_op_residual_norm_backward(xp, hp, _DTYPES[x.dtype], post, gp, tokens_per_gate, pre, alpha, n, C, sp, dyp, dup,
+                                                      dx.data_ptr(), dh.data_ptr(), dpost, dgate, dpre, ws.data_ptr(), size, _stream(device)))
+    return dx, dh
+
+
+# ---- optimiser --------------------------------------------------------------------------------------------------------
+class AdamW:
+    """AdamW over many tensors in one launch.  ``weights``: FP32 tensors; ``grads``: FP32 or BF16 tensors of the same sizes;
+    ``copies`` (optional): BF16 tensors that get the new weights; ``weight_decay``: one number, or one per tensor.
+
+    ``state_bits`` 32 keeps the moments in FP32 (``m``, ``v``); 8 keeps a byte each for m and the root of v (``m``, ``v``:
+    float8_e4m3fn, in units of ``m_scale``, ``v_scale``, one power of two per 256 elements; ``v`` stands for sqrt(v)), rounded
+    stochastically as ``seed`` and the step say.  Every tensor starts on a multiple of 256 elements of the state;
+    ``state`` gives buffers of that form to continue from.  The tensors' addresses are taken once, here: a tensor that
+    moves needs a new object (with the old one's state)."""
+
+    def __init__(self, weights, grads, *, copies=None, state_bits: int = 8, state=None, weight_decay=0.01, seed: int = 0):
+        self.lib = _lib.load()
+        self._h = ct.c_void_p()
+        self.weights, self.grads = list(weights), list(grads)
+        self.copies = list(copies) if copies is not None else [None] * len(self.weights)
+        n = len(self.weights)
+        _need(n > 0 and len(self.grads) == n and len(self.copies) == n, "AdamW: as many gradients (and copies) as weights, at least one")
+        decay = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * n
+        _need(len(decay) == n, "AdamW: one weight decay, or one per tensor")
+        _need(state_bits in (8, 32), "AdamW: state_bits must be 8 or 32")
+        self.device, self.state_bits, self.seed = _device(self.weights[0]), state_bits, int(seed) & 0xFFFFFFFF
+        table = (_lib.OptimTensor * n)()
+        for i, (w, g, c) in enumerate(zip(self.weights, self.grads, self.copies)):
+            wp = _check(w, f"weights[{i}]", w.shape, (torch.float32,), self.device)
+            gp = _check(g, f"grads[{i}]", w.shape, (torch.float32, torch.bfloat16), self.device)
+            cp = _optional(c, f"copies[{i}]", w.shape, (torch.bfloat16,), self.device)
+            table[i] = _lib.OptimTensor(wp, gp, cp, w.numel(), decay[i], _DTYPES[g.dtype])
+        self.blocks = int(self.lib.mgpt_moe_optim_blocks(table, n))
+        total, dtype = self.blocks * STATE_BLOCK, torch.float32 if state_bits == 32 else torch.float8_e4m3fn
+        if state is None:
+            self.m, self.v = torch.zeros(total, dtype=dtype, device=self.device), torch.zeros(total, dtype=dtype, device=self.device)
+            self.m_scale, self.v_scale = (torch.ones(self.blocks, device=self.device), torch.ones(self.blocks, device=self.device)) if state_bits == 8 else (None, None)
+        else:
+            _need(len(state) == (2 if state_bits == 32 else 4), "AdamW: state is (m, v), or (m, v, m_scale, v_scale) for 8 bits")
+            self.m, self.v = state[:2]
+            self.m_scale, self.v_scale = state[2:] if state_bits == 8 else (None, None)
+        self._p = [_check(self.m, "m", (total,), (dtype,), self.device), _check(self.v, "v", (total,), (dtype,), self.device),
+                   _optional(self.m_scale, "m_scale", (self.blocks,), (torch.float32,), self.device),
+                   _optional(self.v_scale, "v_scale", (self.blocks,), (torch.float32,), self.device)]
+        self.found_nonfinite = torch.zeros(1, dtype=torch.int32, device=self.device)
+        _lib.check(self.lib.mgpt_moe_optim_create(self.device.index, table, n, state_bits, ct.byref(self._h)))
+
+    def step(self, t: int, lr: float = 3e-4, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8, grad_scale: torch.Tensor = None) -> None:
+        """One step; ``t`` counts from 1.  ``grad_scale``: an FP32 tensor of one element that multiplies the gradients.  Elements
+        whose gradient is not finite keep their values and set ``found_nonfinite``."""
+        _need(self._h.value, "AdamW: closed")
+        gs = _optional(grad_scale, "grad_scale", () if grad_scale is not None and grad_scale.dim() == 0 else (1,), (torch.float32,), self.device)
+        _lib.check(self.lib.mgpt_moe_optim_step(self._h, *self._p, lr, beta1, beta2, eps, int(t), gs, self.seed,
+                                                self.found_nonfinite.data_ptr(), _stream(self.device)))
+
+    def close(self) -> None:
+        if getattr(self, "_h", None) and self._h.value:
+            torch.cuda.synchronize(self.device)              # a step in flight reads the table
+            self.lib.mgpt_moe_optim_destroy(self._h)
+            self._h = ct.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
