@@ -35,6 +35,7 @@ constexpr uint32_t TMEM_COLS = 2 * TILE;
 constexpr uint32_t STAGING = 4096;                   // per epilogue warp: 32 rows x 128 B
 constexpr int QUEUE = 4;
 constexpr int CLAIM = 6;                             // the next item is claimed this many k-blocks before the last one's loads end
+constexpr int PART = 512 / BK;                       // LOSS: k-blocks summed in one accumulator
 constexpr int MAX_PIECES = 1024;
 constexpr int COUNTERS = 2 * MAX_PIECES + 2;
 constexpr float LOG2E = 1.4426950408889634f;
@@ -67,6 +68,14 @@ struct HeadP {
 
 // exp(from - to), 1 where both are the same infinity
 __device__ __forceinline__ float shift(float from, float to) { return from == to ? 1.0f : exp2f((from - to) * LOG2E); }
+
+// (exponents below -126 give 0: terms that a sum with a 1 in it, or a rounding to 8 bits beside the target's, does not see)
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 struct Shared {
     int item[QUEUE];
@@ -250,34 +259,40 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 const Item w = decode<KIND>(p, n_valid, item);
                 if (w.nkb == 0) continue;
                 const bool a_mn = KIND == GRADS && w.dw, b_mn = KIND == GRADS;
-                const uint32_t idesc = make_idesc(TILE, 2 * w.half, a_mn, b_mn), buf = t & 1u;
+                const uint32_t idesc = make_idesc(TILE, 2 * w.half, a_mn, b_mn);
                 const uint64_t a0 = a_mn ? mn_major : k_major, b0 = (b_mn ? mn_major : k_major) + (OPER_BYTES >> 4);
                 const uint32_t a_step = a_mn ? 2048 >> 4 : 32 >> 4, b_step = b_mn ? 2048 >> 4 : 32 >> 4;     // (the address field: 16-byte units)
-                if (!mbar_wait_cluster(acc_empty + 8 * buf, ((t >> 1) & 1) ^ 1, p.status, ERR_ACC_WAIT)) break;
-                tc_fence_after();
-                const uint32_t d_tmem = tmem_base + buf * TILE;
-                for (int kb = 0; kb < w.nkb; ++kb) {
-                    if (!mbar_wait_cluster(full + 8 * s, phase, p.status, ERR_FULL_WAIT)) {
+                for (int k0 = 0; ok && k0 < w.nkb; ++t) {
+                    const uint32_t buf = t & 1u, d_tmem = tmem_base + buf * TILE;
+                    const int k1 = KIND == LOSS ? min(k0 + PART, w.nkb) : w.nkb;
+                    if (!mbar_wait_cluster(acc_empty + 8 * buf, ((t >> 1) & 1) ^ 1, p.status, ERR_ACC_WAIT)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint64_t ad = a0 + s * (STAGE_BYTES >> 4), bd = b0 + s * (STAGE_BYTES >> 4);
+                    for (int kb = k0; kb < k1; ++kb) {
+                        if (!mbar_wait_cluster(full + 8 * s, phase, p.status, ERR_FULL_WAIT)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint64_t ad = a0 + s * (STAGE_BYTES >> 4), bd = b0 + s * (STAGE_BYTES >> 4);
 #pragma unroll
-                    for (int k = 0; k < BK / 16; ++k)
-                        umma_bf16_pair(d_tmem, ad + k * a_step, bd + k * b_step, idesc, (kb > 0 || k > 0) ? 1u : 0u);
-                    umma_commit_pair(empty + 8 * s);
-                    umma_commit_pair(peer_empty + 8 * s);
-                    if (++s == NS) {
-                        s = 0;
-                        phase ^= 1;
+                        for (int k = 0; k < BK / 16; ++k)
+                            umma_bf16_pair(d_tmem, ad + k * a_step, bd + k * b_step, idesc, (kb > k0 || k > 0) ? 1u : 0u);
+                        umma_commit_pair(empty + 8 * s);
+                        umma_commit_pair(peer_empty + 8 * s);
+                        if (++s == NS) {
+                            s = 0;
+                            phase ^= 1;
+                        }
                     }
+                    if (ok) {
+                        umma_commit_pair(acc_full + 8 * buf);
+                        umma_commit_pair(peer_acc_full + 8 * buf);
+                    }
+                    k0 = k1;
                 }
-                if (ok) {
-                    umma_commit_pair(acc_full + 8 * buf);
-                    umma_commit_pair(peer_acc_full + 8 * buf);
-                }
-                ++t;
             }
         }
     } else {
@@ -291,55 +306,66 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             __syncwarp();
             if (lane == 0) release(n);
             const Item w = decode<KIND>(p, n_valid, item);
-            const uint32_t buf = t & 1u;
             const bool empty_sum = w.nkb == 0;              // no token takes part: dw is zero
-            if (!empty_sum) {
-                if (!mbar_wait_cluster(acc_full + 8 * buf, (t >> 1) & 1, p.status, ERR_ACC_WAIT)) break;
+            uint32_t buf = 0, t_lane = 0;
+            auto next_acc = [&]() {                         // the next accumulator is complete; false: the wait ran out
+                buf = t & 1u;
+                t_lane = tmem_base + buf * TILE + ((uint32_t)(q * 32) << 16) + h * 64;
+                if (!mbar_wait_cluster(acc_full + 8 * buf, (t >> 1) & 1, p.status, ERR_ACC_WAIT)) return false;
                 tc_fence_after();
                 ++t;
-            }
-            const uint32_t t_lane = tmem_base + buf * TILE + ((uint32_t)(q * 32) << 16) + h * 64;
+                return true;
+            };
             auto give_back = [&]() {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(acc_free + 8 * buf);
             };
+            if (!empty_sum && !next_acc()) break;
             if (KIND == LOSS) {
                 const int row = w.m * TILE + rank * 128 + q * 32 + lane, v = w.n * TILE + h * 64, valid = p.V - v;
                 const int at = p.target[row] - v;           // (rows beyond the packed ones hold target -1)
-                float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    float z[32];
-                    tmem_ld32(t_lane + c * 32, z);
-                    tmem_ld_wait();
-                    if (c == 1) give_back();
-                    if (valid < (c + 1) * 32) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (c * 32 + j >= valid) z[j] = -INFINITY;
-                    }
-                    if (__any_sync(0xffffffffu, (at >> 5) == c)) {          // a target in these columns: 32 rows in every ten tiles or so
-                        float zt = 0.0f;
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (at == c * 32 + j) zt = z[j];
-                        if ((at >> 5) == c) p.z_target[row] = zt;
-                    }
-                    float m = z[0];
-#pragma unroll
-                    for (int j = 1; j < 32; ++j) m = fmaxf(m, z[j]);
-                    m = fmaxf(m, top);
-                    const float ref = m == -INFINITY ? 0.0f : m * LOG2E;    // (columns beyond the vocabulary alone)
-                    float s0 = 0.0f, s1 = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        s0 += exp2f(fmaf(z[j], LOG2E, -ref));
-                        s1 += exp2f(fmaf(z[j + 1], LOG2E, -ref));
-                    }
-                    sum = fmaf(sum, exp2f(fmaf(top, LOG2E, -ref)), s0 + s1);
-                    top = m;
+                float z[64];
+                {
+                    float (&z0)[32] = *reinterpret_cast<float (*)[32]>(z), (&z1)[32] = *reinterpret_cast<float (*)[32]>(z + 32);
+                    tmem_ld32(t_lane, z0);
+                    tmem_ld32(t_lane + 32, z1);
                 }
+                tmem_ld_wait();
+                give_back();
+                bool ok = true;
+                for (int kb = PART; kb < w.nkb && (ok = next_acc()); kb += PART) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        float o[16];
+                        tmem_ld16(t_lane + 16 * c, o);
+                        tmem_ld_wait();
+                        if (c == 3) give_back();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) z[16 * c + j] += o[j];
+                    }
+                }
+                if (!ok) break;
+                if (valid < 64) {
+#pragma unroll
+                    for (int j = 0; j < 64; ++j)
+                        if (j >= valid) z[j] = -INFINITY;
+                }
+                if (__any_sync(0xffffffffu, (at >> 6) == 0)) {      // a target in these columns: rare
+                    float zt = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 64; ++j)
+                        if (at == j) zt = z[j];
+                    if ((at >> 6) == 0) p.z_target[row] = zt;
+                }
+                float top = z[0], sum = 0.0f;
+#pragma unroll
+                for (int j = 1; j < 64; ++j) top = fmaxf(top, z[j]);
+                const float ref = top == -INFINITY ? 0.0f : top * LOG2E;    // (columns beyond the vocabulary alone)
+                float s[4] = {};
+#pragma unroll
+                for (int j = 0; j < 64; ++j) s[j & 3] += ex2(fmaf(z[j], LOG2E, -ref));
+                sum = (s[0] + s[1]) + (s[2] + s[3]);
                 // The four warps of a lane quarter join their columns.  (Four buffers: a warp that writes item n + 4 has met the
                 // accumulator that the joining warp gave back at n + 2, after it had read item n.)
                 float2* const mine = reinterpret_cast<float2*>(extra) + (n & 3) * 512 + q * 32 + lane;
@@ -372,7 +398,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     tmem_ld_wait();
                     if (c == 1) give_back();
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) z[j] = real ? exp2f(fmaf(z[j], LOG2E, -ref)) * up : 0.0f;
+                    for (int j = 0; j < 32; ++j) z[j] = real ? ex2(fmaf(z[j], LOG2E, -ref)) * up : 0.0f;
                     if (valid < (c + 1) * 32) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j)

@@ -14,86 +14,96 @@
 // y is computed again from x and h; r1 and r2 are kept by the forward pass.
 //
 // Bound by HBM: every element of x, h (dy, du) is read once into registers and y, u (dx, dh) written once.
-#include "common.cuh"
+#include "pairs.cuh"
 
 namespace mgpt {
 
 namespace {
 
 constexpr int MAX_C = 16384;
-constexpr int UNITS = 592;          // blocks of the backward pass aimed at: four per SM
+constexpr int UNITS = 296;          // blocks of the backward pass aimed at: two per SM
+constexpr int FWD_CTAS = 4;         // of the forward pass, per SM
 
-// Eight consecutive elements as they lie in memory.
-template <typename T> struct Raw;
-template <> struct Raw<bf16> {
-    uint4 a;
-    __device__ __forceinline__ void load(const bf16* p) { a = *reinterpret_cast<const uint4*>(p); }
-    __device__ __forceinline__ float at(int i) const
-    {
-        const uint32_t w = i < 2 ? a.x : i < 4 ? a.y : i < 6 ? a.z : a.w;
-        return i & 1 ? __uint_as_float(w & 0xffff0000u) : __uint_as_float(w << 16);
-    }
-};
-template <> struct Raw<float> {
-    float4 a, b;
-    __device__ __forceinline__ void load(const float* p)
-    {
-        a = *reinterpret_cast<const float4*>(p);
-        b = *reinterpret_cast<const float4*>(p + 4);
-    }
-    __device__ __forceinline__ float at(int i) const
-    {
-        return i == 0 ? a.x : i == 1 ? a.y : i == 2 ? a.z : i == 3 ? a.w : i == 4 ? b.x : i == 5 ? b.y : i == 6 ? b.z : b.w;
-    }
-};
-__device__ __forceinline__ void store8(bf16* p, const float (&v)[8])
+// Eight consecutive elements: a thread copies them to a place of its own in shared memory, some tokens ahead, and takes them from
+// there (pieces of 16 bytes, the block's threads side by side).
+template <typename T> constexpr int pieces() { return sizeof(T) / 2; }
+template <typename T> __device__ __forceinline__ void copy8(uint32_t dst, const T* src)
 {
-    uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int k = 0; k < pieces<T>(); ++k) copy16(dst + k * blockDim.x * 16, (const uint4*)src + k);
 }
-__device__ __forceinline__ void store8(float* p, const float (&v)[8])
+// RING: from there, else from memory (rows too wide for a ring, which the second pass over a token finds in the caches)
+template <typename T, bool RING> __device__ __forceinline__ void take8(uint32_t src, const T* mem, F2 (&v)[4])
 {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    if constexpr (sizeof(T) == 2) {
+        const uint4 u = RING ? taken<uint4>(src) : *reinterpret_cast<const uint4*>(mem);
+        v[0] = widen(u.x); v[1] = widen(u.y); v[2] = widen(u.z); v[3] = widen(u.w);
+    } else {
+        const float4 a = RING ? taken<float4>(src) : *reinterpret_cast<const float4*>(mem);
+        const float4 b = RING ? taken<float4>(src + blockDim.x * 16) : *reinterpret_cast<const float4*>(mem + 4);
+        v[0] = F2(a.x, a.y); v[1] = F2(a.z, a.w); v[2] = F2(b.x, b.y); v[3] = F2(b.z, b.w);
+    }
+}
+__device__ __forceinline__ void store8(bf16* p, const F2 (&v)[4])
+{
+    *reinterpret_cast<uint4*>(p) = make_uint4(narrow(v[0]), narrow(v[1]), narrow(v[2]), narrow(v[3]));
+}
+__device__ __forceinline__ void store8(float* p, const F2 (&v)[4])
+{
+    *reinterpret_cast<float4*>(p) = make_float4(v[0].lo(), v[0].hi(), v[1].lo(), v[1].hi());
+    *reinterpret_cast<float4*>(p + 4) = make_float4(v[2].lo(), v[2].hi(), v[3].lo(), v[3].hi());
 }
 // eight parameters, or ones
-__device__ __forceinline__ void params8(const float* p, int c, float (&v)[8])
+__device__ __forceinline__ void params8(const float* p, int c, F2 (&v)[4])
 {
     if (p) {
         const float4 a = *reinterpret_cast<const float4*>(p + c), b = *reinterpret_cast<const float4*>(p + c + 4);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        v[0] = F2(a.x, a.y); v[1] = F2(a.z, a.w); v[2] = F2(b.x, b.y); v[3] = F2(b.z, b.w);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 1.0f;
+        for (int i = 0; i < 4; ++i) v[i] = F2(1.0f);
     }
 }
 
-// Sums of K values over the `warps` warps of a token's group; every thread of the block calls it.
-template <int K> __device__ __forceinline__ void group_sum(float (&v)[K], int warps, float* sh /* [K][32] */)
+// Sums of K values over the `warps` warps of a token's group; every thread of the group calls it.  Two buffers in turn: who
+// writes one again has met the others at the barrier of the call between, and they had read it by then.
+template <int K> struct Sums {
+    float v[2][16][K][16];                                  // [turn][group][value][warp of the group]; warps that are not there: 0
+};
+template <int K> __device__ __forceinline__ void sums_clear(Sums<K>& sh)
+{
+    for (int i = threadIdx.x; i < (int)(sizeof(sh) / 4); i += blockDim.x) (&sh.v[0][0][0][0])[i] = 0.0f;
+    __syncthreads();
+}
+template <int K> __device__ __forceinline__ void group_sum(float (&v)[K], int warps, Sums<K>& sh, int& turn)
 {
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
     if (warps == 1) return;
-    const int warp = threadIdx.x >> 5, first = warp / warps * warps;
-    __syncthreads();                                        // (the last sums have been read)
+    const int warp = threadIdx.x >> 5, group = warp / warps, w = warp - group * warps;
+    float (&mine)[K][16] = sh.v[turn][group];
+    turn ^= 1;
     if ((threadIdx.x & 31) == 0)
 #pragma unroll
-        for (int k = 0; k < K; ++k) sh[k * 32 + warp] = v[k];
-    __syncthreads();
+        for (int k = 0; k < K; ++k) mine[k][w] = v[k];
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * warps) : "memory");
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         v[k] = 0.0f;
-        for (int i = 0; i < warps; ++i) v[k] += sh[k * 32 + first + i];
+        for (int i = 0; i < warps; i += 4) {
+            const float4 a = *reinterpret_cast<const float4*>(&mine[k][i]);
+            v[k] += (a.x + a.y) + (a.z + a.w);
+        }
     }
 }
-__device__ __forceinline__ float inv_rms(float ss, int C, float eps) { return __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, (float)C) + eps)); }
+// 1 / sqrt(x): the approximation (2 ulp) and a Newton step
+__device__ __forceinline__ float inv_sqrt(float x)
+{
+    const float r = rsqrtf(x);
+    return fmaf(fmaf(-x * r, r, 1.0f) * 0.5f, r, r);
+}
 
 struct NormP {
     const void *x, *h;
@@ -109,71 +119,104 @@ struct NormP {
     int splits, length;             // units per gate row, tokens per unit
 };
 
+// Bytes of a block's ring: `arrays` of NV * 8 elements per thread, STAGES tokens.
+constexpr int STAGES = 2;
+template <typename T> constexpr uint32_t ring_bytes(int arrays, int nv, int threads) { return STAGES * arrays * nv * pieces<T>() * threads * 16; }
+
+// A group of warps per token, the groups of the grid taking tokens in turn.
 template <typename T, int NV>
-__global__ void __launch_bounds__(512) norm_fwd_kernel(const NormP p)
+__global__ void __launch_bounds__(NV == 4 ? 512 : 256) norm_fwd_kernel(const NormP p)
 {
+    constexpr bool RING = NV < 4;
+    extern __shared__ __align__(16) uint8_t ring[];
+    __shared__ __align__(16) Sums<1> sh;
+    const int gt = threadIdx.x % (32 * p.warps), GT = 32 * p.warps, groups = blockDim.x / GT, step = gridDim.x * groups;
+    const uint32_t array = NV * pieces<T>() * blockDim.x * 16, vec = pieces<T>() * blockDim.x * 16;
+    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * 16;
+    const float inv = 1.0f / (float)p.C;
+    int turn = 0;
+    sums_clear(sh);
     pdl_wait();
-    __shared__ float sh[32];
-    const int gt = threadIdx.x % (32 * p.warps), GT = 32 * p.warps, groups = blockDim.x / GT;
-    const int tok = blockIdx.x * groups + threadIdx.x / GT;
-    const bool have = tok < p.n;                            // (the barriers are everyone's)
-    const size_t o = (size_t)tok * p.C;
-    Raw<T> h[NV], x[NV];
+    auto fetch = [&](int tok, int s) {
+        if (RING && tok < p.n) {
+            const size_t o = (size_t)tok * p.C;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (gt + i * GT) * 8;
-        if (have && c < p.C) {
-            h[i].load((const T*)p.h + o + c);
-            x[i].load((const T*)p.x + o + c);
-        }
-    }
-    float r1 = 1.0f, s[1] = {0.0f};
-    if (p.post) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (have && (gt + i * GT) * 8 < p.C)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) s[0] = fmaf(h[i].at(j), h[i].at(j), s[0]);
-        group_sum(s, p.warps, sh);
-        r1 = inv_rms(s[0], p.C, p.eps);
-    }
-    const float* gate = p.gate && p.per_gate ? p.gate + (size_t)(tok / p.per_gate) * p.C : p.gate;
-    float y[NV][8];
-    s[0] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (gt + i * GT) * 8;
-        if (have && c < p.C) {
-            float a[8], g[8];
-            params8(p.post, c, a);
-            params8(gate, c, g);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                y[i][j] = fmaf(p.alpha, x[i].at(j), g[j] * (h[i].at(j) * r1 * a[j]));
-                s[0] = fmaf(y[i][j], y[i][j], s[0]);
+            for (int i = 0; i < NV; ++i) {
+                const int c = (gt + i * GT) * 8;
+                if (c < p.C) {
+                    copy8(mine + s * 2 * array + i * vec, (const T*)p.h + o + c);
+                    copy8(mine + (s * 2 + 1) * array + i * vec, (const T*)p.x + o + c);
+                }
             }
-            store8((T*)p.y + o + c, y[i]);
         }
-    }
-    float r2 = 1.0f;
-    if (p.u) {
-        group_sum(s, p.warps, sh);
-        r2 = inv_rms(s[0], p.C, p.eps);
+        copy_commit();
+    };
+    const int tok0 = blockIdx.x * groups, mine0 = threadIdx.x / GT;
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) fetch(tok0 + mine0 + s * step, s);
+    int slot = 0;
+    for (int base = tok0; base < p.n; base += step, slot = slot + 1 == STAGES ? 0 : slot + 1) {
+        const int tok = base + mine0;
+        const bool have = tok < p.n;                        // (the barriers are everyone's)
+        const size_t o = (size_t)tok * p.C;
+        fetch(tok + (STAGES - 1) * step, slot == 0 ? STAGES - 1 : slot - 1);
+        copy_wait<STAGES - 1>();
+        const uint32_t from = mine + slot * 2 * array;
+        float r1 = 1.0f, s[1] = {0.0f};
+        if (p.post) {
+            F2 t(0.0f);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (const int c = (gt + i * GT) * 8; have && c < p.C) {
+                    F2 h[4];
+                    take8<T, RING>(from + i * vec, (const T*)p.h + o + c, h);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) t = fma2(h[j], h[j], t);
+                }
+            s[0] = t.lo() + t.hi();
+            group_sum(s, p.warps, sh, turn);
+            r1 = inv_sqrt(fmaf(s[0], inv, p.eps));
+        }
+        const float* gate = p.gate && p.per_gate ? p.gate + (size_t)(tok / p.per_gate) * p.C : p.gate;
+        F2 y[NV][4], t(0.0f);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (gt + i * GT) * 8;
             if (have && c < p.C) {
-                float b[8];
-                params8(p.pre, c, b);
+                F2 a[4], g[4], h[4], x[4];
+                params8(p.post, c, a);
+                params8(gate, c, g);
+                take8<T, RING>(from + i * vec, (const T*)p.h + o + c, h);
+                take8<T, RING>(from + array + i * vec, (const T*)p.x + o + c, x);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) y[i][j] = y[i][j] * r2 * b[j];
-                store8((T*)p.u + o + c, y[i]);
+                for (int j = 0; j < 4; ++j) {
+                    y[i][j] = fma2(F2(p.alpha), x[j], g[j] * a[j] * (h[j] * F2(r1)));
+                    t = fma2(y[i][j], y[i][j], t);
+                }
+                store8((T*)p.y + o + c, y[i]);
             }
         }
-    }
-    if (have && gt == 0) {
-        p.stats[tok] = r1;
-        p.stats[p.n + tok] = r2;
+        float r2 = 1.0f;
+        if (p.u) {
+            s[0] = t.lo() + t.hi();
+            group_sum(s, p.warps, sh, turn);
+            r2 = inv_sqrt(fmaf(s[0], inv, p.eps));
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (gt + i * GT) * 8;
+                if (have && c < p.C) {
+                    F2 b[4];
+                    params8(p.pre, c, b);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) y[i][j] = y[i][j] * F2(r2) * b[j];
+                    store8((T*)p.u + o + c, y[i]);
+                }
+            }
+        }
+        if (have && gt == 0) {
+            p.stats[tok] = r1;
+            p.stats[p.n + tok] = r2;
+        }
     }
 }
 
@@ -181,79 +224,138 @@ __global__ void __launch_bounds__(512) norm_fwd_kernel(const NormP p)
 // always the same; the three sums over a token's columns are taken in one round:
 //   mean(D*gp*h_hat) = mean((dy + r2*du*pre)*gp*h_hat) - r2 * mean(du*pre*y_hat) * mean(y_hat*gp*h_hat),   gp = gate*post
 template <typename T, int NV>
-__global__ void __launch_bounds__(512) norm_bwd_kernel(const NormP p)
+__global__ void __launch_bounds__(NV == 4 ? 512 : 256, NV == 4 ? 1 : 2) norm_bwd_kernel(const NormP p)
 {
-    pdl_wait();
-    extern __shared__ __align__(16) float cols[];           // [groups][C]
-    __shared__ float sh[3 * 32];
+    constexpr bool RING = NV < 4;
+    extern __shared__ __align__(16) uint8_t ring[];         // at the end: [groups][C] sums
+    __shared__ __align__(16) Sums<3> sh;
     const int gt = threadIdx.x % (32 * p.warps), GT = 32 * p.warps, groups = blockDim.x / GT, group = threadIdx.x / GT;
+    const uint32_t array = NV * pieces<T>() * blockDim.x * 16, vec = pieces<T>() * blockDim.x * 16;
+    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * 16;
     const int row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits;
     const int per = p.per_gate ? p.per_gate : p.n;
     const int t0 = row * per + split * p.length, t1 = min(min(t0 + p.length, (row + 1) * per), p.n);
     const float* gate = p.gate ? p.gate + (size_t)row * p.C : nullptr;
-    float S1[NV][8] = {}, S2[NV][8] = {};
-    for (int tok0 = t0; tok0 < t1; tok0 += groups) {
+    int turn = 0;
+    sums_clear(sh);
+    pdl_wait();
+    const bool with_u = p.du != nullptr;
+    float nr1 = 0.0f, nr2 = 0.0f;                           // of the token that is copied next
+    auto fetch = [&](int tok, int s) {
+        if (RING && tok < t1) {
+            const size_t o = (size_t)tok * p.C;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (gt + i * GT) * 8;
+                if (c < p.C) {
+                    const uint32_t d = mine + s * 4 * array + i * vec;
+                    copy8(d, (const T*)p.h + o + c);
+                    copy8(d + array, (const T*)p.x + o + c);
+                    copy8(d + 2 * array, (const T*)p.dy + o + c);
+                    if (with_u) copy8(d + 3 * array, (const T*)p.du + o + c);
+                }
+            }
+        }
+        copy_commit();
+    };
+    F2 S1[NV][4], S2[NV][4], gp[NV][4];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (gt + i * GT) * 8;
+        F2 a[4], g[4];
+        if (c < p.C) {
+            params8(p.post, c, a);
+            params8(gate, c, g);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            S1[i][j] = S2[i][j] = F2(0.0f);
+            if (c < p.C) gp[i][j] = g[j] * a[j];
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) fetch(t0 + group + s * groups, s);
+    if (t0 + group < t1) {
+        nr1 = p.stats[t0 + group];
+        nr2 = p.stats[p.n + t0 + group];
+    }
+    const float inv = 1.0f / (float)p.C;
+    int slot = 0;
+    for (int tok0 = t0; tok0 < t1; tok0 += groups, slot = slot + 1 == STAGES ? 0 : slot + 1) {
         const int tok = tok0 + group;
         const bool have = tok < t1;
         const size_t o = (size_t)tok * p.C;
-        const float r1 = have ? p.stats[tok] : 0.0f, r2 = have ? p.stats[p.n + tok] : 0.0f;
-        Raw<T> h[NV], x[NV], dy[NV], du[NV];
-        float s[3] = {};
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (gt + i * GT) * 8;
-            if (have && c < p.C) {
-                h[i].load((const T*)p.h + o + c);
-                x[i].load((const T*)p.x + o + c);
-                dy[i].load((const T*)p.dy + o + c);
-                if (p.du) du[i].load((const T*)p.du + o + c);
-            }
+        const float r1 = nr1, r2 = nr2;
+        fetch(tok + (STAGES - 1) * groups, slot == 0 ? STAGES - 1 : slot - 1);
+        if (tok + groups < t1) {
+            nr1 = p.stats[tok + groups];
+            nr2 = p.stats[p.n + tok + groups];
         }
+        copy_wait<STAGES - 1>();
+        const uint32_t from = mine + slot * 4 * array;
+        F2 s0(0.0f), s1(0.0f), s2(0.0f);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (gt + i * GT) * 8;
             if (have && c < p.C) {
-                float a[8], g[8], b[8];
-                params8(p.post, c, a);
-                params8(gate, c, g);
-                params8(p.pre, c, b);
+                F2 h[4], x[4], dy[4], du[4], b[4];
+                take8<T, RING>(from + i * vec, (const T*)p.h + o + c, h);
+                take8<T, RING>(from + array + i * vec, (const T*)p.x + o + c, x);
+                take8<T, RING>(from + 2 * array + i * vec, (const T*)p.dy + o + c, dy);
+                if (with_u) {
+                    take8<T, RING>(from + 3 * array + i * vec, (const T*)p.du + o + c, du);
+                    params8(p.pre, c, b);
+                }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float hh = h[i].at(j) * r1, gp = g[j] * a[j], q = gp * hh;
-                    const float yh = fmaf(p.alpha, x[i].at(j), g[j] * (hh * a[j])) * r2, d = p.du ? du[i].at(j) * b[j] : 0.0f;
-                    s[0] = fmaf(d, yh, s[0]);
-                    s[1] = fmaf(fmaf(r2, d, dy[i].at(j)), q, s[1]);
-                    s[2] = fmaf(yh, q, s[2]);
+                for (int j = 0; j < 4; ++j) {
+                    const F2 q = gp[i][j] * (h[j] * F2(r1)), yh = fma2(F2(p.alpha), x[j], q) * F2(r2);
+                    if (with_u) {
+                        const F2 d = du[j] * b[j];
+                        s0 = fma2(d, yh, s0);
+                        s1 = fma2(fma2(F2(r2), d, dy[j]), q, s1);
+                    } else {
+                        s1 = fma2(dy[j], q, s1);
+                    }
+                    s2 = fma2(yh, q, s2);
                 }
             }
         }
-        group_sum(s, p.warps, sh);
-        const float inv = 1.0f / (float)p.C, mA = p.du ? s[0] * inv : 0.0f, mB = p.post ? (s[1] - r2 * mA * s[2]) * inv : 0.0f;
+        float s[3] = {s0.lo() + s0.hi(), s1.lo() + s1.hi(), s2.lo() + s2.hi()};
+        group_sum(s, p.warps, sh, turn);
+        const float mA = s[0] * inv, mB = p.post ? (s[1] - r2 * mA * s[2]) * inv : 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (gt + i * GT) * 8;
             if (have && c < p.C) {
-                float a[8], g[8], b[8], dx[8], dh[8];
-                params8(p.post, c, a);
-                params8(gate, c, g);
-                params8(p.pre, c, b);
+                F2 h[4], x[4], D[4], du[4], b[4], dx[4];
+                take8<T, RING>(from + i * vec, (const T*)p.h + o + c, h);
+                take8<T, RING>(from + array + i * vec, (const T*)p.x + o + c, x);
+                take8<T, RING>(from + 2 * array + i * vec, (const T*)p.dy + o + c, D);
+                if (with_u) {
+                    take8<T, RING>(from + 3 * array + i * vec, (const T*)p.du + o + c, du);
+                    params8(p.pre, c, b);
+                }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float hh = h[i].at(j) * r1, gp = g[j] * a[j], w = p.du ? du[i].at(j) : 0.0f;
-                    const float yh = fmaf(p.alpha, x[i].at(j), g[j] * (hh * a[j])) * r2;
-                    const float D = p.du ? fmaf(r2, fmaf(-yh, mA, w * b[j]), dy[i].at(j)) : dy[i].at(j);
-                    dx[j] = p.alpha * D;
-                    dh[j] = r1 * fmaf(-hh, mB, D * gp);
-                    S1[i][j] = fmaf(D, hh, S1[i][j]);
-                    S2[i][j] = fmaf(w, yh, S2[i][j]);
+                for (int j = 0; j < 4; ++j) {
+                    const F2 hh = h[j] * F2(r1);
+                    if (with_u) {
+                        const F2 yh = fma2(F2(p.alpha), x[j], gp[i][j] * hh) * F2(r2);
+                        D[j] = fma2(F2(r2), fma2(yh, F2(-mA), du[j] * b[j]), D[j]);
+                        S2[i][j] = fma2(du[j], yh, S2[i][j]);
+                    }
+                    dx[j] = F2(p.alpha) * D[j];
+                    S1[i][j] = fma2(D[j], hh, S1[i][j]);
+                    h[j] = F2(r1) * fma2(hh, F2(-mB), D[j] * gp[i][j]);
                 }
                 store8((T*)p.dx + o + c, dx);
-                store8((T*)p.dh + o + c, dh);
+                store8((T*)p.dh + o + c, h);
             }
         }
     }
     if (!p.part) return;
     float* out = p.part + (size_t)blockIdx.x * 2 * p.C;
+    float* const cols = reinterpret_cast<float*>(ring);
+    copy_wait<0>();
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         if (groups > 1) {
@@ -360,29 +462,54 @@ int check_params(const float* post, const float* gate, const float* pre)
     return 0;
 }
 
-template <typename T> int run_fwd(NormP& p, cudaStream_t st)
+// The threads of a block: groups of whole tokens, 256 threads or one group.
+int threads_of(int warps, int nv) { return nv == 4 && 32 * warps > 256 ? 32 * warps : 256; }
+
+template <typename K> int opt_in(K kernel, uint32_t bytes, bool (&done)[64])
 {
-    // few tokens: as many threads per token as it has pieces, else four pieces per thread
-    const int nv = p.C > 4096 * 2 ? 4 : p.C > 4096 ? 2 : (size_t)p.n * p.C <= (size_t)148 * 2048 * 4 ? 1 : 4;
-    p.warps = warps_of(p.C, nv);
-    const int threads = 32 * p.warps > 256 ? 32 * p.warps : 256, groups = threads / (32 * p.warps), blocks = (p.n + groups - 1) / groups;
-    if (nv == 1) MGPT_CUDA(launch_pdl(norm_fwd_kernel<T, 1>, blocks, threads, 0, st, p));
-    else if (nv == 2) MGPT_CUDA(launch_pdl(norm_fwd_kernel<T, 2>, blocks, threads, 0, st, p));
-    else MGPT_CUDA(launch_pdl(norm_fwd_kernel<T, 4>, blocks, threads, 0, st, p));
+    int dev = 0;
+    MGPT_CUDA(cudaGetDevice(&dev));
+    if (dev < 64 && done[dev]) return 0;
+    MGPT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    if (dev < 64) done[dev] = true;
+    return 0;
+}
+template <typename T, int NV> int run_fwd(NormP& p, cudaStream_t st)
+{
+    p.warps = warps_of(p.C, NV);
+    const int threads = threads_of(p.warps, NV), groups = threads / (32 * p.warps);
+    const uint32_t smem = NV < 4 ? ring_bytes<T>(2, NV, threads) : 0;
+    const int most = 148 * FWD_CTAS, want = (p.n + groups - 1) / groups;
+    static bool done[64];                                   // (threads and bytes are the same in every call of this form)
+    MGPT_TRY(opt_in(norm_fwd_kernel<T, NV>, smem, done));
+    MGPT_CUDA(launch_pdl(norm_fwd_kernel<T, NV>, want < most ? want : most, threads, smem, st, p));
     MGPT_LAUNCHED("norm_fwd_kernel");
     return 0;
 }
-template <typename T> int run_bwd(NormP& p, int units, cudaStream_t st)
+template <typename T, int NV> int run_bwd(NormP& p, int units, cudaStream_t st)
 {
-    const int nv = p.C > 8192 ? 4 : p.C > 4096 || sizeof(T) == 2 ? 2 : 1;
-    p.warps = warps_of(p.C, nv);
-    const int threads = 32 * p.warps > 256 ? 32 * p.warps : 256, groups = threads / (32 * p.warps);
-    const size_t smem = groups > 1 ? (size_t)groups * p.C * 4 : 0;           // at most 256 threads * 8 * nv floats: 32 KiB
-    if (nv == 1) MGPT_CUDA(launch_pdl(norm_bwd_kernel<T, 1>, units, threads, smem, st, p));
-    else if (nv == 2) MGPT_CUDA(launch_pdl(norm_bwd_kernel<T, 2>, units, threads, smem, st, p));
-    else MGPT_CUDA(launch_pdl(norm_bwd_kernel<T, 4>, units, threads, smem, st, p));
+    p.warps = warps_of(p.C, NV);
+    const int threads = threads_of(p.warps, NV);
+    // (the ring is more than the sums at the end, 32 NV bytes per thread where there are groups)
+    const uint32_t smem = NV < 4 ? ring_bytes<T>(4, NV, threads) : 0;
+    static bool done[64];
+    MGPT_TRY(opt_in(norm_bwd_kernel<T, NV>, smem, done));
+    MGPT_CUDA(launch_pdl(norm_bwd_kernel<T, NV>, units, threads, smem, st, p));
     MGPT_LAUNCHED("norm_bwd_kernel");
     return 0;
+}
+template <typename T> int run_fwd(NormP& p, cudaStream_t st)
+{
+    // pieces of eight elements per thread: as few as 256 threads allow where the tokens are few, else two
+    if (p.C > 4096) return run_fwd<T, 4>(p, st);
+    if (p.C > 2048 || (sizeof(T) == 2 && (size_t)p.n * p.C > (size_t)148 * 2048 * 4)) return run_fwd<T, 2>(p, st);
+    return run_fwd<T, 1>(p, st);
+}
+template <typename T> int run_bwd(NormP& p, int units, cudaStream_t st)
+{
+    if (p.C > 4096) return run_bwd<T, 4>(p, units, st);
+    if (p.C > 2048 || sizeof(T) == 2) return run_bwd<T, 2>(p, units, st);
+    return run_bwd<T, 1>(p, units, st);
 }
 
 }  // namespace
