@@ -44,8 +44,10 @@ constexpr int ST_BAD_TARGET = ST_BAD_EXPERT;         // the status bit of an ind
 enum { LOSS = 0, DLOGITS = 1, GRADS = 2 };
 
 struct HeadP {
-    const int32_t* n_valid;
-    int32_t* sched;             // next item; zero before the launch
+    const int32_t* n_valid;     // null: n tokens, as they lie
+    int n;                      // of the call
+    int direct;                 // x has the operand type: where no token is left out, it is read as it lies
+    int32_t* sched;             // next item; zero before the launch (null: items by stride)
     int32_t* status;
     int C, V;
     int v0;                     // first vocabulary row of the piece
@@ -62,6 +64,10 @@ struct HeadP {
     bf16* dz;                   // DLOGITS: [token tile of 128][64-column block] of swizzled 128 x 64 tiles
     float* acc;                 // GRADS: [k_slices][n_pad][C], dx so far
     int first;                  // acc is written, not added to
+    int last;                   // the sums for dx are complete: they are written there
+    const int32_t* rows;        // packed -> token
+    void* dx;
+    int dx_f32;
     void* dw;
     int dw_f32;                 // dw is FP32 and added to
 };
@@ -75,6 +81,18 @@ __device__ __forceinline__ float ex2(float x)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// four channels of dx
+__device__ __forceinline__ void put_dx(void* dx, int f32, size_t at, float4 x, float scale)
+{
+    x.x *= scale; x.y *= scale; x.z *= scale; x.w *= scale;
+    if (f32) {
+        *reinterpret_cast<float4*>((float*)dx + at) = x;
+    } else {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(x.x, x.y), b = __floats2bfloat162_rn(x.z, x.w);
+        *reinterpret_cast<uint2*>((bf16*)dx + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
 }
 
 struct Shared {
@@ -136,10 +154,11 @@ template <int KIND> __device__ __forceinline__ Item decode(const HeadP& p, int n
 // tmA: LOSS, DLOGITS x (box 64 x 128 rows); GRADS the dz tiles as {64, 128 rows, tiles} in boxes of {64, 128, 1}
 // tmA2: GRADS the dz tiles in boxes of {64, 64, 2}
 // tmB: LOSS, DLOGITS w (box 64 x 128 rows); GRADS w (box 64 x 64 rows); tmB2: x (box 64 x 64 rows)
+// tmX: x as it lies in the caller's memory, in boxes like those of x above, which is the packed copy
 template <int KIND>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmA2,
-            const __grid_constant__ CUtensorMap tmB2, const HeadP p)
+            const __grid_constant__ CUtensorMap tmB2, const __grid_constant__ CUtensorMap tmX, const HeadP p)
 {
     constexpr int NS = stages<KIND>();
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -173,7 +192,8 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     tc_fence_after();
     const uint32_t tmem_base = sh.tmem;
     pdl_wait();
-    const int n_valid = *p.n_valid;
+    const int n_valid = p.n_valid ? *p.n_valid : p.n;
+    const bool as_it_lies = p.direct && n_valid == p.n;
     const float scale = KIND == GRADS ? *p.scale : 1.0f;
 
     const uint32_t lead_item_empty = mapa(item_empty, 0);
@@ -210,9 +230,10 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     if (!more) break;
                 }
                 const Item w = decode<KIND>(p, n_valid, item);
-                if (rank == 0 && w.nkb <= CLAIM) next = atomicAdd(p.sched, 1);
+                auto claim = [&]() { next = p.sched ? atomicAdd(p.sched, 1) : item; };       // (the counter starts behind the grid's first items)
+                if (rank == 0 && w.nkb <= CLAIM) claim();
                 for (int kb = 0; kb < w.nkb; ++kb) {
-                    if (rank == 0 && w.nkb - kb == CLAIM + 1) next = atomicAdd(p.sched, 1);
+                    if (rank == 0 && w.nkb - kb == CLAIM + 1) claim();
                     if (!mbar_wait_cluster(empty + 8 * s, free_phase, p.status, ERR_EMPTY_WAIT)) {
                         ok = false;
                         break;
@@ -220,7 +241,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     const uint32_t a_dst = tile0 + s * STAGE_BYTES, b_dst = a_dst + OPER_BYTES, bar = lead_full + 8 * s;
                     if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * STAGE_BYTES);       // both CTAs' bytes
                     if (KIND != GRADS) {
-                        tma_load_2d_pair(a_dst, &tmA, kb * BK, w.m * TILE + rank * 128, bar);
+                        tma_load_2d_pair(a_dst, as_it_lies ? &tmX : &tmA, kb * BK, w.m * TILE + rank * 128, bar);
                         tma_load_2d_pair(b_dst, &tmB, kb * BK, p.v0 + w.n * TILE + rank * 128, bar);
                     } else {
                         const int blocks = p.v_tiles * (TILE / 64), col = w.n * TILE + rank * w.half;
@@ -232,7 +253,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                             row = p.v0 + (w.k0 + kb) * BK;
                         } else {
                             tma_load_3d_pair(a_dst, &tmA2, 0, (kb & 1) * 64, (kb >> 1) * blocks + w.m * (TILE / 64) + rank * 2, bar);
-                            mB = &tmB2;
+                            mB = as_it_lies ? &tmX : &tmB2;
                             row = kb * BK;
                         }
                         tma_load_2d_pair(b_dst, mB, col, row, bar);
@@ -324,7 +345,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             if (!empty_sum && !next_acc()) break;
             if (KIND == LOSS) {
                 const int row = w.m * TILE + rank * 128 + q * 32 + lane, v = w.n * TILE + h * 64, valid = p.V - v;
-                const int at = p.target[row] - v;           // (rows beyond the packed ones hold target -1)
+                const int at = row < n_valid ? p.target[row] - v : -1;
                 float z[64];
                 {
                     float (&z0)[32] = *reinterpret_cast<float (*)[32]>(z), (&z1)[32] = *reinterpret_cast<float (*)[32]>(z + 32);
@@ -381,13 +402,13 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     float all = 0.0f;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) all += o[i].y * shift(o[i].x, m);
-                    p.part[(size_t)w.n * p.n_pad + row] = make_float2(m, all);
+                    if (row < n_valid) p.part[(size_t)w.n * p.n_pad + row] = make_float2(m, all);
                 }
             } else if (KIND == DLOGITS) {
                 const int row = w.m * TILE + rank * 128 + q * 32 + lane, v = p.v0 + w.n * TILE + h * 64, valid = p.V - v;
-                const int at = p.target[row] - v;
-                const float up = p.d_loss[row], ref = p.lse[row] * LOG2E;
                 const bool real = row < n_valid;
+                const int at = real ? p.target[row] - v : -1;
+                const float up = real ? p.d_loss[row] : 0.0f, ref = real ? p.lse[row] * LOG2E : 0.0f;
                 if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the staging tile is free again
                 __syncwarp();
                 const uint32_t line = smem_u32(stage) + lane * 128;
@@ -480,7 +501,8 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     }
                 } else {
                     float* const out = w.dw ? (float*)p.dw + (size_t)(p.v0 + r0) * p.C : p.acc + ((size_t)w.slice * p.n_pad + r0) * p.C;
-                    const bool add = w.dw || !p.first;
+                    const bool add = w.dw || !p.first, done = !w.dw && p.last;
+                    const int to = done && lane < rows ? p.rows[r0 + lane] : 0;
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         __syncwarp();
@@ -495,6 +517,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             const int r = 4 * i + sub;
+                            const int token = __shfl_sync(0xffffffffu, to, r);
                             if (r < rows && col < p.C) {
                                 float4* d = reinterpret_cast<float4*>(out + (size_t)r * p.C + col);
                                 const uint4 u = get(r);
@@ -503,7 +526,8 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                                     const float4 o = *d;
                                     x.x += o.x; x.y += o.y; x.z += o.z; x.w += o.w;
                                 }
-                                *d = x;
+                                if (done) put_dx(p.dx, p.dx_f32, (size_t)token * p.C + col, x, scale);
+                                else *d = x;
                             }
                         }
                     }
@@ -527,6 +551,7 @@ struct PackP {
     const void* x;
     const int32_t* targets;
     int n, C, Cp, V, n_pad, per_block;
+    int direct;                 // no copy where no token is left out
     int32_t* n_valid;           // [0], followed by the counters of the products
     int32_t *rows, *target;     // packed -> token; its target
     bf16* xp;                   // [n_pad][Cp]
@@ -576,6 +601,7 @@ __global__ void __launch_bounds__(256) head_pack_kernel(const PackP p)
         if (GRAD && tid == 0) *p.scale = top;
         if (bad && p.status) atomicOr(p.status, ST_BAD_TARGET);
     }
+    const bool copy = !(p.direct && all == p.n);
     constexpr int PER = 8;
     auto copy_row = [&](const TIo* from, bf16* to) {        // one warp; columns beyond C (and all without `from`) are zero
         for (int c = lane * PER; c < p.Cp; c += 32 * PER) {
@@ -616,7 +642,7 @@ __global__ void __launch_bounds__(256) head_pack_kernel(const PackP p)
             const size_t o = (size_t)(i0 + r) * p.C;
             const int at = __shfl_sync(0xffffffffu, j, r);
             if (mask >> r & 1) {
-                copy_row((const TIo*)p.x + o, p.xp + (size_t)at * p.Cp);
+                if (copy) copy_row((const TIo*)p.x + o, p.xp + (size_t)at * p.Cp);
             } else if (GRAD) {
                 for (int c = lane * PER; c < p.C; c += 32 * PER)
 #pragma unroll
@@ -626,32 +652,35 @@ __global__ void __launch_bounds__(256) head_pack_kernel(const PackP p)
         before += __popc(mask);
     }
     const int end = (all + TILE - 1) / TILE * TILE;
-    for (int j = all + blockIdx.x * 8 + warp; j < end; j += gridDim.x * 8) {
-        copy_row(nullptr, p.xp + (size_t)j * p.Cp);
-        if (lane == 0) {
-            p.target[j] = -1;
-            if (GRAD) p.lse_p[j] = p.d_loss_p[j] = 0.0f;
-        }
-    }
+    if (copy)
+        for (int j = all + blockIdx.x * 8 + warp; j < end; j += gridDim.x * 8) copy_row(nullptr, p.xp + (size_t)j * p.Cp);
 }
 
 // ---- joining ----------------------------------------------------------------------------------------------------------
-// lse and loss from the tiles' maxima and sums: 32 tokens per block, eight warps with every eighth tile each, joined in order.
-__global__ void __launch_bounds__(256)
-head_join_kernel(const int32_t* n_valid, const float2* part, const float* z_target, const int32_t* rows, int v_tiles, int n_pad, float* loss, float* lse)
+// lse and loss from the tiles' maxima and sums: 32 tokens per block, WARPS warps that take runs of eight tiles in turn, joined in order.
+// targets: of tokens that were not packed (null: packed ones)
+template <int WARPS>
+__global__ void __launch_bounds__(32 * WARPS)
+head_join_kernel(const int32_t* n_valid, const float2* part, const float* z_target, const int32_t* rows, const int32_t* targets, int n, int V, int n_pad, float* loss,
+                 float* lse, int32_t* status)
 {
     pdl_wait();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
-    if (blockIdx.x * 32 >= *n_valid) return;
-    const bool real = row < *n_valid;
-    __shared__ float2 sh[8][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * 32 + lane, all_rows = targets ? n : *n_valid, v_tiles = (V + TILE - 1) / TILE;
+    if (blockIdx.x * 32 >= all_rows) return;
+    const bool real = row < all_rows;
+    __shared__ float2 sh[WARPS][32];
     float top = -INFINITY, sum = 0.0f;
     if (real)
-#pragma unroll 4
-        for (int v = warp; v < v_tiles; v += 8) {
-            const float2 o = part[(size_t)v * n_pad + row];
-            const float m = fmaxf(top, o.x);
-            sum = sum * shift(top, m) + o.y * shift(o.x, m);
+        for (int v0 = warp * 8; v0 < v_tiles; v0 += WARPS * 8) {
+            float2 o[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = v0 + i < v_tiles ? part[(size_t)(v0 + i) * n_pad + row] : make_float2(-INFINITY, 0.0f);
+            float m = top;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = fmaxf(m, o[i].x);
+            sum *= shift(top, m);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum = fmaf(o[i].y, shift(o[i].x, m), sum);
             top = m;
         }
     sh[warp][lane] = make_float2(top, sum);
@@ -659,40 +688,36 @@ head_join_kernel(const int32_t* n_valid, const float2* part, const float* z_targ
     if (warp > 0 || !real) return;
     float m = -INFINITY, all = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, sh[i][lane].x);
+    for (int i = 0; i < WARPS; ++i) m = fmaxf(m, sh[i][lane].x);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (i < v_tiles) all += sh[i][lane].y * shift(sh[i][lane].x, m);
+    for (int i = 0; i < WARPS; ++i)
+        if (i * 8 < v_tiles) all = fmaf(sh[i][lane].y, shift(sh[i][lane].x, m), all);
     const float l = m + logf(all);
-    const int i = rows[row];
-    lse[i] = l;
-    loss[i] = l - z_target[row];
+    const int i = targets ? row : rows[row], t = targets ? targets[row] : 0;
+    const bool in = t >= 0 && t < V;
+    if (t >= V) atomicOr(status, ST_BAD_TARGET);
+    lse[i] = in ? l : 0.0f;
+    loss[i] = in ? l - z_target[row] : 0.0f;
 }
 
-// dx from the slices of the vocabulary, a warp per token.
-template <typename TIo>
+// dx from several slices of the vocabulary, a warp per token.
 __global__ void __launch_bounds__(256)
-head_dx_kernel(const int32_t* n_valid, const float* scale, const float* acc, const int32_t* rows, int slices, int n_pad, int C, TIo* dx)
+head_dx_kernel(const int32_t* n_valid, const float* scale, const float* acc, const int32_t* rows, int slices, int n_pad, int C, void* dx, int f32)
 {
     pdl_wait();
     const int lane = threadIdx.x & 31, row = blockIdx.x * 8 + (threadIdx.x >> 5);
     if (row >= *n_valid) return;
-    TIo* out = dx + (size_t)rows[row] * C;
+    const size_t out = (size_t)rows[row] * C, pitch = (size_t)n_pad * C;
     const float f = *scale;
     for (int c = lane * 4; c < C; c += 128) {
         const float* from = acc + (size_t)row * C + c;
         float4 s = *reinterpret_cast<const float4*>(from);
+#pragma unroll 8
         for (int i = 1; i < slices; ++i) {
-            const float4 o = *reinterpret_cast<const float4*>(from + (size_t)i * n_pad * C);
+            const float4 o = *reinterpret_cast<const float4*>(from + i * pitch);
             s.x += o.x; s.y += o.y; s.z += o.z; s.w += o.w;
         }
-        s.x *= f; s.y *= f; s.z *= f; s.w *= f;
-        if constexpr (sizeof(TIo) == 2) {
-            const __nv_bfloat162 a = __floats2bfloat162_rn(s.x, s.y), b = __floats2bfloat162_rn(s.z, s.w);
-            *reinterpret_cast<uint2*>(out + c) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-        } else {
-            *reinterpret_cast<float4*>(out + c) = s;
-        }
+        put_dx(dx, f32, out + c, s, f);
     }
 }
 
@@ -762,7 +787,8 @@ int slices_of(int n_pad, int c_tiles, int v_tiles)
     return items >= 74 || s < 1 ? 1 : s;
 }
 
-template <int KIND> int launch_head(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& a2, const CUtensorMap& b2, const HeadP& p, int pairs, cudaStream_t st)
+template <int KIND>
+int launch_head(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& a2, const CUtensorMap& b2, const CUtensorMap& x, const HeadP& p, int pairs, cudaStream_t st)
 {
     static bool done[64] = {};
     int dev = 0;
@@ -771,7 +797,7 @@ template <int KIND> int launch_head(const CUtensorMap& a, const CUtensorMap& b, 
         MGPT_CUDA(cudaFuncSetAttribute(head_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<KIND>()));
         if (dev < 64) done[dev] = true;
     }
-    MGPT_CUDA(launch_pdl(head_kernel<KIND>, 2 * pairs, THREADS, smem_bytes<KIND>(), st, a, b, a2, b2, p));
+    MGPT_CUDA(launch_pdl(head_kernel<KIND>, 2 * pairs, THREADS, smem_bytes<KIND>(), st, a, b, a2, b2, x, p));
     MGPT_LAUNCHED("head_kernel");
     return 0;
 }
@@ -836,22 +862,28 @@ int mgpt_moe_op_head_loss(const void* x, int io, const void* w, const int32_t* t
     char* ws = (char*)workspace;
     int sms;
     MGPT_TRY(sm_count(&sms));
-    CUtensorMap mx, mw;
+    CUtensorMap mx, mw, mx0;
+    const bool direct = io == MGPT_MOE_IO_BF16, packed = !direct || n > TILE;
     MGPT_TRY(make_map_kind(&mx, ws + h.xp, h.n_pad, h.Cp, 128, false));
     MGPT_TRY(make_map_kind(&mw, w, V, C, 128, false));
+    if (direct) MGPT_TRY(make_map_kind(&mx0, x, n, C, 128, false));
     PackP k = {};
-    k.x = x; k.targets = targets; k.n = n; k.C = C; k.Cp = h.Cp; k.V = V; k.n_pad = h.n_pad;
+    k.x = x; k.targets = targets; k.n = n; k.C = C; k.Cp = h.Cp; k.V = V; k.n_pad = h.n_pad; k.direct = direct;
     k.n_valid = (int32_t*)(ws + h.counters);
     k.rows = (int32_t*)(ws + h.rows); k.target = (int32_t*)(ws + h.target); k.xp = (bf16*)(ws + h.xp);
     k.status = status; k.loss = loss; k.lse = lse;
-    MGPT_TRY(launch_pack<false>(k, io, st));
+    // one tile of tokens costs the same with or without those that take no part: no need to sort them out
+    if (packed) MGPT_TRY(launch_pack<false>(k, io, st));
     HeadP p = {};
-    p.n_valid = k.n_valid; p.sched = k.n_valid + 1; p.status = status; p.C = C; p.V = V; p.v_tiles = h.v_tiles;
-    p.group = group_of(h.n_pad, h.Cp); p.n_pad = h.n_pad; p.target = k.target;
+    p.n_valid = packed ? k.n_valid : nullptr; p.n = n; p.direct = direct; p.sched = packed ? k.n_valid + 1 : nullptr;
+    p.status = status; p.C = C; p.V = V; p.v_tiles = h.v_tiles;
+    p.group = group_of(h.n_pad, h.Cp); p.n_pad = h.n_pad; p.target = packed ? k.target : targets;
     p.part = (float2*)(ws + h.part); p.z_target = (float*)(ws + h.z_target);
     const long items = (long)(h.n_pad / TILE) * h.v_tiles;
-    MGPT_TRY(launch_head<LOSS>(mx, mw, mx, mw, p, (int)(items < sms / 2 ? items : sms / 2), st));
-    MGPT_CUDA(launch_pdl(head_join_kernel, (n + 31) / 32, 256, 0, st, k.n_valid, p.part, p.z_target, k.rows, h.v_tiles, h.n_pad, loss, lse));
+    MGPT_TRY(launch_head<LOSS>(mx, mw, mx, mw, direct ? mx0 : mx, p, (int)(items < sms / 2 ? items : sms / 2), st));
+    const int32_t* as_given = packed ? nullptr : targets;
+    if (n < 32 * sms) MGPT_CUDA(launch_pdl(head_join_kernel<16>, (n + 31) / 32, 512, 0, st, p.n_valid, p.part, p.z_target, k.rows, as_given, n, V, h.n_pad, loss, lse, status));
+    else MGPT_CUDA(launch_pdl(head_join_kernel<4>, (n + 31) / 32, 128, 0, st, p.n_valid, p.part, p.z_target, k.rows, as_given, n, V, h.n_pad, loss, lse, status));
     MGPT_LAUNCHED("head_join_kernel");
     return 0;
 }
@@ -886,11 +918,17 @@ int mgpt_moe_op_head_loss_backward(const void* x, int io, const void* w, const i
     char* ws = (char*)workspace;
     int sms;
     MGPT_TRY(sm_count(&sms));
-    CUtensorMap mx, mw, mx_t, mw_t, mz, mz_t;
+    CUtensorMap mx, mw, mx_t, mw_t, mz, mz_t, mx0, mx0_t;
+    const bool direct = io == MGPT_MOE_IO_BF16;
     MGPT_TRY(make_map_kind(&mx, ws + h.xp, h.n_pad, h.Cp, 128, false));
     MGPT_TRY(make_map_kind(&mw, w, V, C, 128, false));
     MGPT_TRY(make_map_kind(&mx_t, ws + h.xp, h.n_pad, h.Cp, 64, false));
     MGPT_TRY(make_map_kind(&mw_t, w, V, C, 64, false));
+    mx0 = mx; mx0_t = mx_t;
+    if (direct) {
+        MGPT_TRY(make_map_kind(&mx0, x, n, C, 128, false));
+        MGPT_TRY(make_map_kind(&mx0_t, x, n, C, 64, false));
+    }
     const uint64_t tiles = (uint64_t)(h.n_pad / 128) * per * (TILE / 64);
     MGPT_TRY(make_map_tiles(&mz, ws + h.dz, tiles, 128, 1));
     MGPT_TRY(make_map_tiles(&mz_t, ws + h.dz, tiles, 64, 2));
@@ -898,10 +936,10 @@ int mgpt_moe_op_head_loss_backward(const void* x, int io, const void* w, const i
     k.x = x; k.targets = targets; k.n = n; k.C = C; k.Cp = h.Cp; k.V = V; k.n_pad = h.n_pad;
     k.n_valid = (int32_t*)(ws + h.counters);
     k.rows = (int32_t*)(ws + h.rows); k.target = (int32_t*)(ws + h.target); k.xp = (bf16*)(ws + h.xp);
-    k.status = status; k.lse_in = lse; k.d_loss_in = d_loss; k.lse_p = (float*)(ws + h.lse); k.d_loss_p = (float*)(ws + h.d_loss); k.scale = (float*)(ws + h.scale); k.dx = dx;
+    k.direct = direct; k.status = status; k.lse_in = lse; k.d_loss_in = d_loss; k.lse_p = (float*)(ws + h.lse); k.d_loss_p = (float*)(ws + h.d_loss); k.scale = (float*)(ws + h.scale); k.dx = dx;
     MGPT_TRY(launch_pack<true>(k, io, st));
     HeadP p = {};
-    p.n_valid = k.n_valid; p.status = status; p.C = C; p.V = V; p.group = group_of(h.n_pad, h.Cp); p.n_pad = h.n_pad;
+    p.n_valid = k.n_valid; p.n = n; p.direct = direct; p.rows = k.rows; p.dx = dx; p.dx_f32 = !direct; p.status = status; p.C = C; p.V = V; p.group = group_of(h.n_pad, h.Cp); p.n_pad = h.n_pad;
     p.target = k.target; p.lse = k.lse_p; p.d_loss = k.d_loss_p; p.scale = k.scale; p.dz = (bf16*)(ws + h.dz); p.acc = (float*)(ws + h.acc);
     p.c_tiles = h.c_tiles; p.dw = dw; p.dw_f32 = dw_dtype == MGPT_MOE_IO_F32;
     for (int i = 0; i < pieces; ++i) {
@@ -910,17 +948,17 @@ int mgpt_moe_op_head_loss_backward(const void* x, int io, const void* w, const i
         p.slice_tiles = (per + slices - 1) / slices;            // (of a full piece, whose slices the others keep within)
         p.k_slices = (p.v_tiles + p.slice_tiles - 1) / p.slice_tiles;
         p.first = i == 0;
+        p.last = slices == 1 && i == pieces - 1;
         const long items = (long)(h.n_pad / TILE) * p.v_tiles;
         p.sched = k.n_valid + 1 + 2 * i;
-        MGPT_TRY(launch_head<DLOGITS>(mx, mw, mx, mw, p, (int)(items < sms / 2 ? items : sms / 2), st));
+        MGPT_TRY(launch_head<DLOGITS>(mx, mw, mx, mw, mx0, p, (int)(items < sms / 2 ? items : sms / 2), st));
         p.sched = k.n_valid + 2 + 2 * i;
         const long grads = ((long)(h.n_pad / TILE) * p.k_slices + p.v_tiles) * p.c_tiles;
-        MGPT_TRY(launch_head<GRADS>(mz, mw_t, mz_t, mx_t, p, (int)(grads < sms / 2 ? grads : sms / 2), st));
+        MGPT_TRY(launch_head<GRADS>(mz, mw_t, mz_t, mx_t, mx0_t, p, (int)(grads < sms / 2 ? grads : sms / 2), st));
     }
-    const int used = (per + (per + slices - 1) / slices - 1) / ((per + slices - 1) / slices);
-    const int blocks = (n + 7) / 8;
-    if (io == MGPT_MOE_IO_BF16) MGPT_CUDA(launch_pdl(head_dx_kernel<bf16>, blocks, 256, 0, st, k.n_valid, p.scale, p.acc, k.rows, used, h.n_pad, C, (bf16*)dx));
-    else MGPT_CUDA(launch_pdl(head_dx_kernel<float>, blocks, 256, 0, st, k.n_valid, p.scale, p.acc, k.rows, used, h.n_pad, C, (float*)dx));
+    if (slices == 1) return 0;
+    const int used = (per + p.slice_tiles - 1) / p.slice_tiles;
+    MGPT_CUDA(launch_pdl(head_dx_kernel, (n + 7) / 8, 256, 0, st, k.n_valid, p.scale, p.acc, k.rows, used, h.n_pad, C, dx, p.dx_f32));
     MGPT_LAUNCHED("head_dx_kernel");
     return 0;
 }
