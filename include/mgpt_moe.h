@@ -492,7 +492,7 @@ int  mgpt_moe_op_head_loss(const void* x, int io, const void* w, const int32_t* 
  * parameter gradients. dz is rounded to BF16, the operand type of both products; their
  * sums are FP32. The vocabulary is worked on in pieces whose dz fits the workspace behind
  * its fixed part: workspace_bytes(.., piece_bytes) is the size for pieces of about
- * piece_bytes (at least one of 256 vocabulary rows; 256 MiB is a good value: larger pieces
+ * piece_bytes (at least one of 256 vocabulary rows; 512 MiB is a good value: larger pieces
  * gain little). Results are deterministic; the order of the sums for dx, and with it its last
  * bits, depends on the size of the pieces. */
 size_t mgpt_moe_op_head_loss_backward_workspace_bytes(int n, int C, int V, size_t piece_bytes);

@@ -95,6 +95,10 @@ __device__ __forceinline__ void put_dx(void* dx, int f32, size_t at, float4 x, f
     }
 }
 
+// An arrival that hands over nothing that was written: the accumulator's columns, or a queue entry, have been read.  (With release at
+// cluster scope each one waited for the warp's stores to global memory before it, about 2000 cycles of an item.)
+__device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory"); }
+
 struct Shared {
     int item[QUEUE];
     uint64_t full[6], empty[6], acc_full[2], acc_empty[2], item_full[QUEUE], item_empty[QUEUE], joined[4];
@@ -204,7 +208,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         item = *reinterpret_cast<volatile int*>(&sh.item[slot]);
         return item >= 0;
     };
-    auto release = [&](uint32_t n) { mbar_arrive_cluster(lead_item_empty + 8 * (n % QUEUE)); };
+    auto release = [&](uint32_t n) { arrive_remote(lead_item_empty + 8 * (n % QUEUE)); };
 
     if (warp == 0) {
         if (elect_one()) {
@@ -218,7 +222,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 const int slot = n % QUEUE;
                 if (rank == 0) {
                     if (item >= total) item = -1;
-                    if (!mbar_wait_cluster(item_empty + 8 * slot, ((n / QUEUE) & 1) ^ 1, p.status, ERR_SCHED_WAIT)) break;
+                    if (!mbar_wait(item_empty + 8 * slot, ((n / QUEUE) & 1) ^ 1, p.status, ERR_SCHED_WAIT)) break;
                     *reinterpret_cast<volatile int*>(&sh.item[slot]) = item;
                     st_cluster_u32(peer_item + 4 * slot, (uint32_t)item);
                     mbar_arrive(item_full + 8 * slot);
@@ -234,7 +238,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 if (rank == 0 && w.nkb <= CLAIM) claim();
                 for (int kb = 0; kb < w.nkb; ++kb) {
                     if (rank == 0 && w.nkb - kb == CLAIM + 1) claim();
-                    if (!mbar_wait_cluster(empty + 8 * s, free_phase, p.status, ERR_EMPTY_WAIT)) {
+                    if (!mbar_wait(empty + 8 * s, free_phase, p.status, ERR_EMPTY_WAIT)) {
                         ok = false;
                         break;
                     }
@@ -286,13 +290,13 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 for (int k0 = 0; ok && k0 < w.nkb; ++t) {
                     const uint32_t buf = t & 1u, d_tmem = tmem_base + buf * TILE;
                     const int k1 = KIND == LOSS ? min(k0 + PART, w.nkb) : w.nkb;
-                    if (!mbar_wait_cluster(acc_empty + 8 * buf, ((t >> 1) & 1) ^ 1, p.status, ERR_ACC_WAIT)) {
+                    if (!mbar_wait(acc_empty + 8 * buf, ((t >> 1) & 1) ^ 1, p.status, ERR_ACC_WAIT)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
                     for (int kb = k0; kb < k1; ++kb) {
-                        if (!mbar_wait_cluster(full + 8 * s, phase, p.status, ERR_FULL_WAIT)) {
+                        if (!mbar_wait(full + 8 * s, phase, p.status, ERR_FULL_WAIT)) {
                             ok = false;
                             break;
                         }
@@ -332,7 +336,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             auto next_acc = [&]() {                         // the next accumulator is complete; false: the wait ran out
                 buf = t & 1u;
                 t_lane = tmem_base + buf * TILE + ((uint32_t)(q * 32) << 16) + h * 64;
-                if (!mbar_wait_cluster(acc_full + 8 * buf, (t >> 1) & 1, p.status, ERR_ACC_WAIT)) return false;
+                if (!mbar_wait(acc_full + 8 * buf, (t >> 1) & 1, p.status, ERR_ACC_WAIT)) return false;
                 tc_fence_after();
                 ++t;
                 return true;
@@ -340,7 +344,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             auto give_back = [&]() {
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(acc_free + 8 * buf);
+                if (lane == 0) arrive_remote(acc_free + 8 * buf);
             };
             if (!empty_sum && !next_acc()) break;
             if (KIND == LOSS) {

@@ -13,7 +13,7 @@ import torch
 from . import _lib
 from ._lib import IO_BF16, IO_F32, MoeError
 
-PIECE_BYTES = 256 << 20         # of the vocabulary's gradient rows that are worked on at a time
+PIECE_BYTES = 512 << 20         # of the vocabulary's gradient rows that are worked on at a time
 STATE_BLOCK = 256               # elements that share a scale of the 8-bit moments
 
 _DTYPES = {torch.float32: IO_F32, torch.bfloat16: IO_BF16}
