@@ -16,6 +16,7 @@
 //
 // Tokens whose target is not in [0, vocabulary) take no part: the others are packed first, so that an ignored token costs
 // nothing and its x, whatever it holds, is not read.
+#include "pairs.cuh"
 #include "tc_common.cuh"
 
 namespace mgpt {
@@ -99,8 +100,18 @@ __device__ __forceinline__ void put_dx(void* dx, int f32, size_t at, float4 x, f
 // cluster scope each one waited for the warp's stores to global memory before it, about 2000 cycles of an item.)
 __device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory"); }
 
+// What an item is.  LOSS, DLOGITS: m (256 tokens), n (256 vocabulary rows), reduction over C.
+// GRADS: dx (m: 256 tokens, n: 256 channels, reduction over a slice of the vocabulary) or dw (m: 256 vocabulary rows, n: 256
+// channels, reduction over the tokens).  The leader's producer works an item out and passes it to everyone.
+struct __align__(16) Item {
+    int m, n;               // m < 0: no more
+    int slice;              // GRADS: the vocabulary's slice, -1: dw
+    int nkb;                // 64-element blocks of the reduction
+    __device__ __forceinline__ bool dw() const { return slice < 0; }
+    __device__ __forceinline__ int half(int C) const { return C - n * TILE <= TILE / 2 ? 64 : 128; }     // GRADS: columns per CTA
+};
 struct Shared {
-    int item[QUEUE];
+    Item item[QUEUE];
     uint64_t full[6], empty[6], acc_full[2], acc_empty[2], item_full[QUEUE], item_empty[QUEUE], joined[4];
     uint32_t tmem;
 };
@@ -109,14 +120,6 @@ template <int KIND> constexpr uint32_t extra_bytes() { return KIND == LOSS ? 4 *
 template <int KIND> constexpr uint32_t smem_bytes() { return 1024 + stages<KIND>() * STAGE_BYTES + extra_bytes<KIND>() + sizeof(Shared); }
 static_assert(smem_bytes<LOSS>() <= 232448 && smem_bytes<GRADS>() <= 232448, "shared memory of one CTA");
 
-// What an item is.  LOSS, DLOGITS: m (256 tokens), n (256 vocabulary rows), reduction over C.
-// GRADS: dx (m: 256 tokens, n: 256 channels, reduction over a slice of the vocabulary) or dw (m: 256 vocabulary rows, n: 256
-// channels, reduction over the tokens).
-struct Item {
-    int m, n, k0, nkb, half;
-    bool dw;
-    int slice;
-};
 template <int KIND> __device__ __forceinline__ int item_count(const HeadP& p, int n_valid)
 {
     const int mt = (n_valid + TILE - 1) / TILE;
@@ -126,9 +129,7 @@ template <int KIND> __device__ __forceinline__ Item decode(const HeadP& p, int n
 {
     Item w;
     const int mt = (n_valid + TILE - 1) / TILE;
-    w.dw = false;
-    w.slice = w.k0 = 0;
-    w.half = 128;
+    w.slice = 0;
     if (KIND != GRADS) {
         // group token tiles at a time run through the whole vocabulary, so that x stays in L2
         const int g = i / (p.group * p.v_tiles), r = i - g * p.group * p.v_tiles, in = min(p.group, mt - g * p.group);
@@ -143,15 +144,13 @@ template <int KIND> __device__ __forceinline__ Item decode(const HeadP& p, int n
         const int r = i - w.slice * mt * p.c_tiles;
         w.m = r / p.c_tiles;
         w.n = r - w.m * p.c_tiles;
-        w.k0 = w.slice * p.slice_tiles * (TILE / BK);
-        w.nkb = min(p.slice_tiles * (TILE / BK), p.v_tiles * (TILE / BK) - w.k0);
+        w.nkb = min(p.slice_tiles, p.v_tiles - w.slice * p.slice_tiles) * (TILE / BK);
     } else {
-        w.dw = true;
+        w.slice = -1;
         w.m = (i - dx) / p.c_tiles;
         w.n = (i - dx) - w.m * p.c_tiles;
         w.nkb = (n_valid + BK - 1) / BK;
     }
-    if (p.C - w.n * TILE <= TILE / 2) w.half = 64;
     return w;
 }
 
@@ -202,11 +201,12 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 
     const uint32_t lead_item_empty = mapa(item_empty, 0);
     // the pair's n-th item; false: no more
-    auto consume = [&](uint32_t n, int& item) -> bool {
+    auto consume = [&](uint32_t n, Item& w) -> bool {
         const int slot = n % QUEUE;
         if (!mbar_wait_cluster(item_full + 8 * slot, (n / QUEUE) & 1, p.status, ERR_SCHED_WAIT)) return false;
-        item = *reinterpret_cast<volatile int*>(&sh.item[slot]);
-        return item >= 0;
+        const int4 v = taken<int4>(smem_u32(&sh.item[slot]));
+        w.m = v.x; w.n = v.y; w.slice = v.z; w.nkb = v.w;
+        return w.m >= 0;
     };
     auto release = [&](uint32_t n) { arrive_remote(lead_item_empty + 8 * (n % QUEUE)); };
 
@@ -220,20 +220,21 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             bool ok = true;
             for (uint32_t n = 0; ok; ++n) {
                 const int slot = n % QUEUE;
+                Item w;
                 if (rank == 0) {
-                    if (item >= total) item = -1;
+                    if (item < total) w = decode<KIND>(p, n_valid, item);
+                    else w.m = -1;
                     if (!mbar_wait(item_empty + 8 * slot, ((n / QUEUE) & 1) ^ 1, p.status, ERR_SCHED_WAIT)) break;
-                    *reinterpret_cast<volatile int*>(&sh.item[slot]) = item;
-                    st_cluster_u32(peer_item + 4 * slot, (uint32_t)item);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(&sh.item[slot])), "r"(w.m), "r"(w.n), "r"(w.slice), "r"(w.nkb) : "memory");
+                    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(peer_item + (uint32_t)sizeof(Item) * slot), "r"(w.m), "r"(w.n), "r"(w.slice), "r"(w.nkb) : "memory");
                     mbar_arrive(item_full + 8 * slot);
                     mbar_arrive_cluster(peer_item_full + 8 * slot);         // (release at cluster scope: the item is visible)
-                    if (item < 0) break;
+                    if (w.m < 0) break;
                 } else {
-                    const bool more = consume(n, item);
+                    const bool more = consume(n, w);
                     release(n);
                     if (!more) break;
                 }
-                const Item w = decode<KIND>(p, n_valid, item);
                 auto claim = [&]() { next = p.sched ? atomicAdd(p.sched, 1) : item; };       // (the counter starts behind the grid's first items)
                 if (rank == 0 && w.nkb <= CLAIM) claim();
                 for (int kb = 0; kb < w.nkb; ++kb) {
@@ -248,13 +249,13 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                         tma_load_2d_pair(a_dst, as_it_lies ? &tmX : &tmA, kb * BK, w.m * TILE + rank * 128, bar);
                         tma_load_2d_pair(b_dst, &tmB, kb * BK, p.v0 + w.n * TILE + rank * 128, bar);
                     } else {
-                        const int blocks = p.v_tiles * (TILE / 64), col = w.n * TILE + rank * w.half;
+                        const int blocks = p.v_tiles * (TILE / 64), col = w.n * TILE + rank * w.half(p.C), k0 = w.slice * p.slice_tiles * (TILE / BK);
                         const CUtensorMap* mB;
                         int row;
-                        if (!w.dw) {
-                            tma_load_3d_pair(a_dst, &tmA, 0, 0, (w.m * 2 + rank) * blocks + w.k0 + kb, bar);
+                        if (!w.dw()) {
+                            tma_load_3d_pair(a_dst, &tmA, 0, 0, (w.m * 2 + rank) * blocks + k0 + kb, bar);
                             mB = &tmB;
-                            row = p.v0 + (w.k0 + kb) * BK;
+                            row = p.v0 + (k0 + kb) * BK;
                         } else {
                             tma_load_3d_pair(a_dst, &tmA2, 0, (kb & 1) * 64, (kb >> 1) * blocks + w.m * (TILE / 64) + rank * 2, bar);
                             mB = as_it_lies ? &tmX : &tmB2;
@@ -274,17 +275,17 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     } else if (warp == 1) {
         if (rank == 0 && elect_one()) {
             uint32_t t = 0, phase = 0;
-            int s = 0, item;
+            int s = 0;
             bool ok = true;
+            Item w;
             const uint32_t peer_empty = mapa(empty, 1), peer_acc_full = mapa(acc_full, 1);
             const uint32_t tile0 = smem_u32(tiles);
             const uint64_t k_major = make_desc(tile0, 16, 1024), mn_major = make_desc(tile0, BOX_BYTES, 1024);
-            for (uint32_t n = 0; ok && consume(n, item); ++n) {
+            for (uint32_t n = 0; ok && consume(n, w); ++n) {
                 release(n);
-                const Item w = decode<KIND>(p, n_valid, item);
                 if (w.nkb == 0) continue;
-                const bool a_mn = KIND == GRADS && w.dw, b_mn = KIND == GRADS;
-                const uint32_t idesc = make_idesc(TILE, 2 * w.half, a_mn, b_mn);
+                const bool a_mn = KIND == GRADS && w.dw(), b_mn = KIND == GRADS;
+                const uint32_t idesc = make_idesc(TILE, KIND == GRADS ? 2 * w.half(p.C) : TILE, a_mn, b_mn);
                 const uint64_t a0 = a_mn ? mn_major : k_major, b0 = (b_mn ? mn_major : k_major) + (OPER_BYTES >> 4);
                 const uint32_t a_step = a_mn ? 2048 >> 4 : 32 >> 4, b_step = b_mn ? 2048 >> 4 : 32 >> 4;     // (the address field: 16-byte units)
                 for (int k0 = 0; ok && k0 < w.nkb; ++t) {
@@ -326,11 +327,25 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         uint8_t* const stage = extra + (warp - 2) * STAGING;
         const uint32_t acc_free = mapa(acc_empty, 0);
         uint32_t t = 0;
-        int item = -1;
-        for (uint32_t n = 0; __any_sync(0xffffffffu, consume(n, item)); ++n) {
+        Item w, before = {};
+        uint32_t summed = 0;                                // LOSS: items
+        float2* const sums = reinterpret_cast<float2*>(extra) + q * 32 + lane;
+        auto join = [&](uint32_t n, const Item& of) {
+            if (!mbar_wait(smem_u32(&sh.joined[q]), n & 1, p.status, ERR_ACC_WAIT)) return false;
+            float2 o[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = sums[(n & 3) * 512 + i * 128];
+            const float m = fmaxf(fmaxf(o[0].x, o[1].x), fmaxf(o[2].x, o[3].x));
+            float all = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) all = fmaf(o[i].y, shift(o[i].x, m), all);
+            const int row = of.m * TILE + rank * 128 + q * 32 + lane;
+            if (row < n_valid) p.part[(size_t)of.n * p.n_pad + row] = make_float2(m, all);
+            return true;
+        };
+        for (uint32_t n = 0; __any_sync(0xffffffffu, consume(n, w)); ++n) {
             __syncwarp();
             if (lane == 0) release(n);
-            const Item w = decode<KIND>(p, n_valid, item);
             const bool empty_sum = w.nkb == 0;              // no token takes part: dw is zero
             uint32_t buf = 0, t_lane = 0;
             auto next_acc = [&]() {                         // the next accumulator is complete; false: the wait ran out
@@ -346,10 +361,13 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 __syncwarp();
                 if (lane == 0) arrive_remote(acc_free + 8 * buf);
             };
+            // this thread's token, and where its target lies behind the warp's first column
+            const int row = w.m * TILE + rank * 128 + q * 32 + lane, v = p.v0 + w.n * TILE + h * 64, valid = p.V - v;
+            const bool real = KIND != GRADS && row < n_valid;
+            const int at = real ? p.target[row] - v : -1;
+            const float up = KIND == DLOGITS && real ? p.d_loss[row] : 0.0f, lse = KIND == DLOGITS && real ? p.lse[row] : 0.0f;
             if (!empty_sum && !next_acc()) break;
             if (KIND == LOSS) {
-                const int row = w.m * TILE + rank * 128 + q * 32 + lane, v = w.n * TILE + h * 64, valid = p.V - v;
-                const int at = row < n_valid ? p.target[row] - v : -1;
                 float z[64];
                 {
                     float (&z0)[32] = *reinterpret_cast<float (*)[32]>(z), (&z1)[32] = *reinterpret_cast<float (*)[32]>(z + 32);
@@ -383,36 +401,29 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                         if (at == j) zt = z[j];
                     if ((at >> 6) == 0) p.z_target[row] = zt;
                 }
-                float top = z[0], sum = 0.0f;
+                float t4[4] = {z[0], z[1], z[2], z[3]};
 #pragma unroll
-                for (int j = 1; j < 64; ++j) top = fmaxf(top, z[j]);
-                const float ref = top == -INFINITY ? 0.0f : top * LOG2E;    // (columns beyond the vocabulary alone)
-                float s[4] = {};
+                for (int j = 4; j < 64; ++j) t4[j & 3] = fmaxf(t4[j & 3], z[j]);
+                const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+                const F2 ref(top == -INFINITY ? 0.0f : -top * LOG2E);       // (columns beyond the vocabulary alone)
+                F2 s2[2] = {F2(0.0f), F2(0.0f)};
 #pragma unroll
-                for (int j = 0; j < 64; ++j) s[j & 3] += ex2(fmaf(z[j], LOG2E, -ref));
-                sum = (s[0] + s[1]) + (s[2] + s[3]);
-                // The four warps of a lane quarter join their columns.  (Four buffers: a warp that writes item n + 4 has met the
-                // accumulator that the joining warp gave back at n + 2, after it had read item n.)
-                float2* const mine = reinterpret_cast<float2*>(extra) + (n & 3) * 512 + q * 32 + lane;
-                mine[h * 128] = make_float2(top, sum);
+                for (int j = 0; j < 32; ++j) {
+                    const F2 e = fma2(F2(z[2 * j], z[2 * j + 1]), F2(LOG2E), ref);
+                    s2[j & 1] = s2[j & 1] + F2(ex2(e.lo()), ex2(e.hi()));
+                }
+                const F2 sum = s2[0] + s2[1];
+                // The four warps of a lane quarter join their columns, in turn, an item later, so that none waits for another.  (A warp
+                // joins item n - 1 before it has arrived for n, which therefore is the barrier's phase.  Four buffers: who writes item
+                // n + 3 has met the accumulator that the joining warp gave back at n + 1, after it had read item n - 1.)
+                if (n > 0 && h == (int)((n - 1) & 3) && !join(n - 1, before)) break;
+                before = w;
+                ++summed;
+                sums[(n & 3) * 512 + h * 128] = make_float2(top, sum.lo() + sum.hi());
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&sh.joined[q]));
-                if (h == 0) {
-                    if (!mbar_wait(smem_u32(&sh.joined[q]), n & 1, p.status, ERR_ACC_WAIT)) break;
-                    float2 o[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[i] = mine[i * 128];
-                    const float m = fmaxf(fmaxf(o[0].x, o[1].x), fmaxf(o[2].x, o[3].x));
-                    float all = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) all += o[i].y * shift(o[i].x, m);
-                    if (row < n_valid) p.part[(size_t)w.n * p.n_pad + row] = make_float2(m, all);
-                }
             } else if (KIND == DLOGITS) {
-                const int row = w.m * TILE + rank * 128 + q * 32 + lane, v = p.v0 + w.n * TILE + h * 64, valid = p.V - v;
-                const bool real = row < n_valid;
-                const int at = real ? p.target[row] - v : -1;
-                const float up = real ? p.d_loss[row] : 0.0f, ref = real ? p.lse[row] * LOG2E : 0.0f;
+                const F2 ref(-lse * LOG2E), up2(up);        // (rows behind the last token: logits 0, up 0)
                 if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the staging tile is free again
                 __syncwarp();
                 const uint32_t line = smem_u32(stage) + lane * 128;
@@ -423,7 +434,10 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     tmem_ld_wait();
                     if (c == 1) give_back();
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) z[j] = real ? ex2(fmaf(z[j], LOG2E, -ref)) * up : 0.0f;
+                    for (int j = 0; j < 32; j += 2) {
+                        const F2 e = fma2(F2(z[j], z[j + 1]), F2(LOG2E), ref);
+                        (F2(ex2(e.lo()), ex2(e.hi())) * up2).get(z[j], z[j + 1]);
+                    }
                     if (valid < (c + 1) * 32) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
@@ -456,7 +470,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             } else {
                 // rows r0.. of the result (tokens, or vocabulary rows), columns c0..; 8 lanes share a 128-byte line of a row
                 const int r0 = w.m * TILE + rank * 128 + q * 32, c0 = w.n * TILE + h * 64;
-                const int rows = w.dw ? p.V - p.v0 - r0 : n_valid - r0;
+                const int rows = w.dw() ? p.V - p.v0 - r0 : n_valid - r0;
                 const int sub = lane >> 3, piece = lane & 7;
                 const uint32_t base = smem_u32(stage), line = base + lane * 128;
                 float a[2][32];
@@ -468,12 +482,12 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     tmem_ld32(t_lane + 32, a[1]);
                     tmem_ld_wait();
                     give_back();
-                    if (w.dw) {
+                    if (w.dw()) {
 #pragma unroll
                         for (int j = 0; j < 64; ++j) a[j >> 5][j & 31] *= scale;
                     }
                 }
-                if (c0 >= p.C || (w.half == 64 && h >= 2)) continue;
+                if (c0 >= p.C || (w.half(p.C) == 64 && h >= 2)) continue;
                 auto put = [&](int j, const uint32_t (&b)[4]) {
                     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(line + (((uint32_t)j ^ (lane & 7u)) << 4)),
                                  "r"(b[0]), "r"(b[1]), "r"(b[2]), "r"(b[3]) : "memory");
@@ -484,7 +498,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                                  : "r"(base + r * 128 + (((uint32_t)piece ^ (r & 7u)) << 4)) : "memory");
                     return u;
                 };
-                if (w.dw && !p.dw_f32) {
+                if (w.dw() && !p.dw_f32) {
                     __syncwarp();
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
@@ -504,8 +518,8 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                         if (r < rows && c0 + piece * 8 < p.C) *reinterpret_cast<uint4*>(dst + (size_t)r * p.C) = get(r);
                     }
                 } else {
-                    float* const out = w.dw ? (float*)p.dw + (size_t)(p.v0 + r0) * p.C : p.acc + ((size_t)w.slice * p.n_pad + r0) * p.C;
-                    const bool add = w.dw || !p.first, done = !w.dw && p.last;
+                    float* const out = w.dw() ? (float*)p.dw + (size_t)(p.v0 + r0) * p.C : p.acc + ((size_t)w.slice * p.n_pad + r0) * p.C;
+                    const bool add = w.dw() || !p.first, done = !w.dw() && p.last;
                     const int to = done && lane < rows ? p.rows[r0 + lane] : 0;
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
@@ -538,6 +552,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 }
             }
         }
+        if (KIND == LOSS && summed > 0 && h == (int)((summed - 1) & 3)) join(summed - 1, before);
         if (KIND == DLOGITS && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     // neither CTA may leave (or give its TMEM back) while the other can still read its shared memory or signal it
