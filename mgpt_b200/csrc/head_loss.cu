@@ -158,12 +158,18 @@ template <int KIND> __device__ __forceinline__ Item decode(const HeadP& p, int n
 // tmA2: GRADS the dz tiles in boxes of {64, 64, 2}
 // tmB: LOSS, DLOGITS w (box 64 x 128 rows); GRADS w (box 64 x 64 rows); tmB2: x (box 64 x 64 rows)
 // tmX: x as it lies in the caller's memory, in boxes like those of x above, which is the packed copy
+// The epilogue's 16 warps: all of them on an item, 64 columns each; or two groups of eight that take items in turn, 128 columns
+// each.  What a warp of DLOGITS does for an item is a chain of some 6000 cycles (tcgen05.ld, exponentials, shared memory, the copy that has
+// to have left it), of which an item of C = 512 with 4100 cycles of products hides one only half: 1.3 % of the gradients' time where the
+// power limit sets the clock, 6 % where it does not.  The loss is 2 % slower in groups: it gives the accumulator back at once.
+template <int KIND> constexpr int item_warps() { return KIND == DLOGITS ? EPI_WARPS / 2 : EPI_WARPS; }
+
 template <int KIND>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmA2,
             const __grid_constant__ CUtensorMap tmB2, const __grid_constant__ CUtensorMap tmX, const HeadP p)
 {
-    constexpr int NS = stages<KIND>();
+    constexpr int NS = stages<KIND>(), ITEM_WARPS = item_warps<KIND>(), GROUPS = EPI_WARPS / ITEM_WARPS, UNITS = 16 / ITEM_WARPS;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_ctarank();
@@ -179,11 +185,11 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full + 8 * b, 1);
-            mbar_init(acc_empty + 8 * b, 2 * EPI_WARPS);
+            mbar_init(acc_empty + 8 * b, 2 * ITEM_WARPS);
         }
         for (int i = 0; i < QUEUE; ++i) {
             mbar_init(item_full + 8 * i, 1);
-            mbar_init(item_empty + 8 * i, 2 * EPI_WARPS + 2);       // the leader's: all epilogue warps, its MMA thread, the peer's producer
+            mbar_init(item_empty + 8 * i, 2 * ITEM_WARPS + 2);      // the leader's: the epilogue, its MMA thread, the peer's producer
         }
         for (int q = 0; q < 4; ++q) mbar_init(smem_u32(&sh.joined[q]), 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -217,19 +223,23 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             const uint32_t peer_item = mapa(smem_u32(sh.item), 1), peer_item_full = mapa(item_full, 1);
             int s = 0, item = blockIdx.x >> 1, next = 0;
             uint32_t free_phase = 1;                        // (the first round finds every stage free)
-            bool ok = true;
+            bool ok = true, end = false;
             for (uint32_t n = 0; ok; ++n) {
                 const int slot = n % QUEUE;
                 Item w;
                 if (rank == 0) {
                     if (item < total) w = decode<KIND>(p, n_valid, item);
-                    else w.m = -1;
+                    else w.m = -1, w.n = w.nkb = 0, w.slice = end ? -1 : 0;
                     if (!mbar_wait(item_empty + 8 * slot, ((n / QUEUE) & 1) ^ 1, p.status, ERR_SCHED_WAIT)) break;
                     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(&sh.item[slot])), "r"(w.m), "r"(w.n), "r"(w.slice), "r"(w.nkb) : "memory");
                     asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(peer_item + (uint32_t)sizeof(Item) * slot), "r"(w.m), "r"(w.n), "r"(w.slice), "r"(w.nkb) : "memory");
                     mbar_arrive(item_full + 8 * slot);
                     mbar_arrive_cluster(peer_item_full + 8 * slot);         // (release at cluster scope: the item is visible)
-                    if (w.m < 0) break;
+                    if (w.m < 0) {                              // (twice: either group of the epilogue may be the one to read on)
+                        if (w.slice < 0) break;
+                        end = true;
+                        continue;
+                    }
                 } else {
                     const bool more = consume(n, w);
                     release(n);
@@ -322,19 +332,19 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             }
         }
     } else {
-        // 16 epilogue warps: TMEM lane quarter q, 64 columns each
-        const int q = warp & 3, h = (warp - 2) >> 2;
+        // TMEM lane quarter q, the h-th of the warps that share its columns
+        const int q = warp & 3, group = (warp - 2) / ITEM_WARPS, h = (warp - 2) % ITEM_WARPS >> 2;
         uint8_t* const stage = extra + (warp - 2) * STAGING;
-        const uint32_t acc_free = mapa(acc_empty, 0);
+        const uint32_t acc_free = mapa(acc_empty, 0), joined = smem_u32(&sh.joined[q]);
         uint32_t t = 0;
         Item w, before = {};
-        uint32_t summed = 0;                                // LOSS: items
+        uint32_t k = 0;                                     // items of the group so far
         float2* const sums = reinterpret_cast<float2*>(extra) + q * 32 + lane;
-        auto join = [&](uint32_t n, const Item& of) {
-            if (!mbar_wait(smem_u32(&sh.joined[q]), n & 1, p.status, ERR_ACC_WAIT)) return false;
+        auto join = [&](uint32_t k, const Item& of) {
+            if (!mbar_wait(joined, k & 1, p.status, ERR_ACC_WAIT)) return false;
             float2 o[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = sums[(n & 3) * 512 + i * 128];
+            for (int i = 0; i < 4; ++i) o[i] = sums[(k & 3) * 512 + i * 128];
             const float m = fmaxf(fmaxf(o[0].x, o[1].x), fmaxf(o[2].x, o[3].x));
             float all = 0.0f;
 #pragma unroll
@@ -343,15 +353,15 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             if (row < n_valid) p.part[(size_t)of.n * p.n_pad + row] = make_float2(m, all);
             return true;
         };
-        for (uint32_t n = 0; __any_sync(0xffffffffu, consume(n, w)); ++n) {
+        for (uint32_t n = group; __any_sync(0xffffffffu, consume(n, w)); n += GROUPS, ++k) {
             __syncwarp();
             if (lane == 0) release(n);
             const bool empty_sum = w.nkb == 0;              // no token takes part: dw is zero
             uint32_t buf = 0, t_lane = 0;
             auto next_acc = [&]() {                         // the next accumulator is complete; false: the wait ran out
-                buf = t & 1u;
-                t_lane = tmem_base + buf * TILE + ((uint32_t)(q * 32) << 16) + h * 64;
-                if (!mbar_wait(acc_full + 8 * buf, (t >> 1) & 1, p.status, ERR_ACC_WAIT)) return false;
+                buf = GROUPS == 2 ? group : t & 1u;         // (two groups: an item is one accumulator, theirs)
+                t_lane = tmem_base + buf * TILE + ((uint32_t)(q * 32) << 16) + h * (UNITS * 64);
+                if (!mbar_wait(acc_full + 8 * buf, (GROUPS == 2 ? t : t >> 1) & 1, p.status, ERR_ACC_WAIT)) return false;
                 tc_fence_after();
                 ++t;
                 return true;
@@ -362,7 +372,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 if (lane == 0) arrive_remote(acc_free + 8 * buf);
             };
             // this thread's token, and where its target lies behind the warp's first column
-            const int row = w.m * TILE + rank * 128 + q * 32 + lane, v = p.v0 + w.n * TILE + h * 64, valid = p.V - v;
+            const int row = w.m * TILE + rank * 128 + q * 32 + lane, v = p.v0 + w.n * TILE + h * (UNITS * 64);
             const bool real = KIND != GRADS && row < n_valid;
             const int at = real ? p.target[row] - v : -1;
             const float up = KIND == DLOGITS && real ? p.d_loss[row] : 0.0f, lse = KIND == DLOGITS && real ? p.lse[row] : 0.0f;
@@ -389,6 +399,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     }
                 }
                 if (!ok) break;
+                const int valid = p.V - v;
                 if (valid < 64) {
 #pragma unroll
                     for (int j = 0; j < 64; ++j)
@@ -414,58 +425,59 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 }
                 const F2 sum = s2[0] + s2[1];
                 // The four warps of a lane quarter join their columns, in turn, an item later, so that none waits for another.  (A warp
-                // joins item n - 1 before it has arrived for n, which therefore is the barrier's phase.  Four buffers: who writes item
-                // n + 3 has met the accumulator that the joining warp gave back at n + 1, after it had read item n - 1.)
-                if (n > 0 && h == (int)((n - 1) & 3) && !join(n - 1, before)) break;
+                // joins item k - 1 before it has arrived for k, which therefore is the barrier's phase.  Four buffers: who writes item
+                // k + 3 has met the accumulator that the joining warp gave back at k + 1, after it had read item k - 1.)
+                if (k > 0 && h == (int)((k - 1) & 3) && !join(k - 1, before)) break;
                 before = w;
-                ++summed;
-                sums[(n & 3) * 512 + h * 128] = make_float2(top, sum.lo() + sum.hi());
+                sums[(k & 3) * 512 + h * 128] = make_float2(top, sum.lo() + sum.hi());
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sh.joined[q]));
+                if (lane == 0) mbar_arrive(joined);
             } else if (KIND == DLOGITS) {
                 const F2 ref(-lse * LOG2E), up2(up);        // (rows behind the last token: logits 0, up 0)
-                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the staging tile is free again
-                __syncwarp();
                 const uint32_t line = smem_u32(stage) + lane * 128;
+#pragma unroll 1
+                for (int u = 0; u < UNITS; ++u) {
+                    const int valid = p.V - v - u * 64, a = at - u * 64;
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the staging tile is free again
+                    __syncwarp();
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    float z[32];
-                    tmem_ld32(t_lane + c * 32, z);
-                    tmem_ld_wait();
-                    if (c == 1) give_back();
+                    for (int c = 0; c < 2; ++c) {
+                        float z[32];
+                        tmem_ld32(t_lane + u * 64 + c * 32, z);
+                        tmem_ld_wait();
+                        if (c == 1 && u + 1 == UNITS) give_back();
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        const F2 e = fma2(F2(z[j], z[j + 1]), F2(LOG2E), ref);
-                        (F2(ex2(e.lo()), ex2(e.hi())) * up2).get(z[j], z[j + 1]);
-                    }
-                    if (valid < (c + 1) * 32) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (c * 32 + j >= valid) z[j] = 0.0f;
-                    }
-                    if (__any_sync(0xffffffffu, (at >> 5) == c)) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (at == c * 32 + j) z[j] -= up;
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {           // 16-byte pieces in the 128-byte swizzle
-                        uint32_t b[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const __nv_bfloat162 two = __floats2bfloat162_rn(z[8 * j + 2 * i], z[8 * j + 2 * i + 1]);
-                            b[i] = *reinterpret_cast<const uint32_t*>(&two);
+                        for (int j = 0; j < 32; j += 2) {
+                            const F2 e = fma2(F2(z[j], z[j + 1]), F2(LOG2E), ref);
+                            (F2(ex2(e.lo()), ex2(e.hi())) * up2).get(z[j], z[j + 1]);
                         }
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(line + (((uint32_t)(c * 4 + j) ^ (lane & 7u)) << 4)),
-                                     "r"(b[0]), "r"(b[1]), "r"(b[2]), "r"(b[3]) : "memory");
+                        if (valid < (c + 1) * 32) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (c * 32 + j >= valid) z[j] = 0.0f;
+                        }
+                        if (__any_sync(0xffffffffu, (a >> 5) == c)) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (a == c * 32 + j) z[j] -= up;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {       // 16-byte pieces in the 128-byte swizzle
+                            uint32_t b[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) b[i] = narrow(F2(z[8 * j + 2 * i], z[8 * j + 2 * i + 1]));
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(line + (((uint32_t)(c * 4 + j) ^ (lane & 7u)) << 4)),
+                                         "r"(b[0]), "r"(b[1]), "r"(b[2]), "r"(b[3]) : "memory");
+                        }
                     }
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) {
-                    bf16* dst = p.dz + (((size_t)(w.m * 2 + rank) * (p.v_tiles * (TILE / 64)) + w.n * (TILE / 64) + h) * 128 + q * 32) * 64;
-                    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(stage)), "r"(STAGING) : "memory");
-                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        const size_t block = (size_t)(w.m * 2 + rank) * (p.v_tiles * (TILE / 64)) + w.n * (TILE / 64) + h * UNITS + u;
+                        bf16* dst = p.dz + (block * 128 + q * 32) * 64;
+                        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(stage)), "r"(STAGING) : "memory");
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    }
                 }
             } else {
                 // rows r0.. of the result (tokens, or vocabulary rows), columns c0..; 8 lanes share a 128-byte line of a row
@@ -552,7 +564,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 }
             }
         }
-        if (KIND == LOSS && summed > 0 && h == (int)((summed - 1) & 3)) join(summed - 1, before);
+        if (KIND == LOSS && k > 0 && h == (int)((k - 1) & 3)) join(k - 1, before);
         if (KIND == DLOGITS && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     // neither CTA may leave (or give its TMEM back) while the other can still read its shared memory or signal it

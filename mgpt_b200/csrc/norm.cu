@@ -124,10 +124,9 @@ constexpr int STAGES = 2;
 template <typename T> constexpr uint32_t ring_bytes(int arrays, int nv, int threads) { return STAGES * arrays * nv * pieces<T>() * threads * 16; }
 
 // A group of warps per token, the groups of the grid taking tokens in turn.
-template <typename T, int NV>
-__global__ void __launch_bounds__(NV == 4 ? 512 : 256) norm_fwd_kernel(const NormP p)
+template <typename T, int NV, bool RING>
+__global__ void __launch_bounds__(RING ? 256 : 512, RING ? (NV == 4 ? 3 : 4) : 1) norm_fwd_kernel(const NormP p)
 {
-    constexpr bool RING = NV < 4;
     extern __shared__ __align__(16) uint8_t ring[];
     __shared__ __align__(16) Sums<1> sh;
     const int gt = threadIdx.x % (32 * p.warps), GT = 32 * p.warps, groups = blockDim.x / GT, step = gridDim.x * groups;
@@ -223,10 +222,9 @@ __global__ void __launch_bounds__(NV == 4 ? 512 : 256) norm_fwd_kernel(const Nor
 // One block per unit: tokens of one gate row.  The sums over a unit's tokens stay in registers, a thread's columns being
 // always the same; the three sums over a token's columns are taken in one round:
 //   mean(D*gp*h_hat) = mean((dy + r2*du*pre)*gp*h_hat) - r2 * mean(du*pre*y_hat) * mean(y_hat*gp*h_hat),   gp = gate*post
-template <typename T, int NV>
-__global__ void __launch_bounds__(NV == 4 ? 512 : 256, NV == 4 ? 1 : 2) norm_bwd_kernel(const NormP p)
+template <typename T, int NV, bool RING>
+__global__ void __launch_bounds__(RING ? 256 : 512, RING ? 2 : 1) norm_bwd_kernel(const NormP p)
 {
-    constexpr bool RING = NV < 4;
     extern __shared__ __align__(16) uint8_t ring[];         // at the end: [groups][C] sums
     __shared__ __align__(16) Sums<3> sh;
     const int gt = threadIdx.x % (32 * p.warps), GT = 32 * p.warps, groups = blockDim.x / GT, group = threadIdx.x / GT;
@@ -462,8 +460,8 @@ int check_params(const float* post, const float* gate, const float* pre)
     return 0;
 }
 
-// The threads of a block: groups of whole tokens, 256 threads or one group.
-int threads_of(int warps, int nv) { return nv == 4 && 32 * warps > 256 ? 32 * warps : 256; }
+// The threads of a block: groups of whole tokens, 256 threads, or one group of up to 512.
+int threads_of(int warps) { return 32 * warps > 256 ? 32 * warps : 256; }
 
 template <typename K> int opt_in(K kernel, uint32_t bytes, bool (&done)[64])
 {
@@ -474,42 +472,43 @@ template <typename K> int opt_in(K kernel, uint32_t bytes, bool (&done)[64])
     if (dev < 64) done[dev] = true;
     return 0;
 }
-template <typename T, int NV> int run_fwd(NormP& p, cudaStream_t st)
+template <typename T, int NV, bool RING> int run_fwd(NormP& p, cudaStream_t st)
 {
     p.warps = warps_of(p.C, NV);
-    const int threads = threads_of(p.warps, NV), groups = threads / (32 * p.warps);
-    const uint32_t smem = NV < 4 ? ring_bytes<T>(2, NV, threads) : 0;
+    const int threads = threads_of(p.warps), groups = threads / (32 * p.warps);
+    const uint32_t smem = RING ? ring_bytes<T>(2, NV, threads) : 0;
     const int most = 148 * FWD_CTAS, want = (p.n + groups - 1) / groups;
     static bool done[64];                                   // (threads and bytes are the same in every call of this form)
-    MGPT_TRY(opt_in(norm_fwd_kernel<T, NV>, smem, done));
-    MGPT_CUDA(launch_pdl(norm_fwd_kernel<T, NV>, want < most ? want : most, threads, smem, st, p));
+    MGPT_TRY(opt_in(norm_fwd_kernel<T, NV, RING>, smem, done));
+    MGPT_CUDA(launch_pdl(norm_fwd_kernel<T, NV, RING>, want < most ? want : most, threads, smem, st, p));
     MGPT_LAUNCHED("norm_fwd_kernel");
     return 0;
 }
-template <typename T, int NV> int run_bwd(NormP& p, int units, cudaStream_t st)
+template <typename T, int NV, bool RING> int run_bwd(NormP& p, int units, cudaStream_t st)
 {
     p.warps = warps_of(p.C, NV);
-    const int threads = threads_of(p.warps, NV);
+    const int threads = threads_of(p.warps);
     // (the ring is more than the sums at the end, 32 NV bytes per thread where there are groups)
-    const uint32_t smem = NV < 4 ? ring_bytes<T>(4, NV, threads) : 0;
+    const uint32_t smem = RING ? ring_bytes<T>(4, NV, threads) : 0;
     static bool done[64];
-    MGPT_TRY(opt_in(norm_bwd_kernel<T, NV>, smem, done));
-    MGPT_CUDA(launch_pdl(norm_bwd_kernel<T, NV>, units, threads, smem, st, p));
+    MGPT_TRY(opt_in(norm_bwd_kernel<T, NV, RING>, smem, done));
+    MGPT_CUDA(launch_pdl(norm_bwd_kernel<T, NV, RING>, units, threads, smem, st, p));
     MGPT_LAUNCHED("norm_bwd_kernel");
     return 0;
 }
 template <typename T> int run_fwd(NormP& p, cudaStream_t st)
 {
-    // pieces of eight elements per thread: as few as 256 threads allow where the tokens are few, else two
-    if (p.C > 4096) return run_fwd<T, 4>(p, st);
-    if (p.C > 2048 || (sizeof(T) == 2 && (size_t)p.n * p.C > (size_t)148 * 2048 * 4)) return run_fwd<T, 2>(p, st);
-    return run_fwd<T, 1>(p, st);
+    // pieces of eight elements per thread: one where the tokens are few
+    if (p.C > 4096) return run_fwd<T, 4, false>(p, st);
+    if (p.C > 2048) return run_fwd<T, 2, true>(p, st);
+    if (sizeof(T) == 2 && (size_t)p.n * p.C > (size_t)148 * 2048 * 4) return run_fwd<T, 2, true>(p, st);
+    return run_fwd<T, 1, true>(p, st);
 }
 template <typename T> int run_bwd(NormP& p, int units, cudaStream_t st)
 {
-    if (p.C > 4096) return run_bwd<T, 4>(p, units, st);
-    if (p.C > 2048 || sizeof(T) == 2) return run_bwd<T, 2>(p, units, st);
-    return run_bwd<T, 1>(p, units, st);
+    if (p.C > 4096) return run_bwd<T, 4, false>(p, units, st);
+    if (p.C > 2048 || sizeof(T) == 2) return run_bwd<T, 2, true>(p, units, st);
+    return run_bwd<T, 1, true>(p, units, st);
 }
 
 }  // namespace
