@@ -21,26 +21,27 @@ namespace mgpt {
 namespace {
 
 constexpr int MAX_C = 16384;
+__host__ __device__ constexpr int threads_of(int warps) { return warps > 8 ? 32 * warps : 256; }     // whole groups of warps, one per token
 constexpr int UNITS = 296;          // blocks of the backward pass aimed at: two per SM
 constexpr int FWD_CTAS = 4;         // of the forward pass, per SM
 
 // Eight consecutive elements: a thread copies them to a place of its own in shared memory, some tokens ahead, and takes them from
 // there (pieces of 16 bytes, the block's threads side by side).
 template <typename T> constexpr int pieces() { return sizeof(T) / 2; }
-template <typename T> __device__ __forceinline__ void copy8(uint32_t dst, const T* src)
+template <typename T, int THREADS> __device__ __forceinline__ void copy8(uint32_t dst, const T* src)
 {
 #pragma unroll
-    for (int k = 0; k < pieces<T>(); ++k) copy16(dst + k * blockDim.x * 16, (const uint4*)src + k);
+    for (int k = 0; k < pieces<T>(); ++k) copy16(dst + k * THREADS * 16, (const uint4*)src + k);
 }
 // RING: from there, else from memory (rows too wide for a ring, which the second pass over a token finds in the caches)
-template <typename T, bool RING> __device__ __forceinline__ void take8(uint32_t src, const T* mem, F2 (&v)[4])
+template <typename T, int THREADS, bool RING> __device__ __forceinline__ void take8(uint32_t src, const T* mem, F2 (&v)[4])
 {
     if constexpr (sizeof(T) == 2) {
         const uint4 u = RING ? taken<uint4>(src) : *reinterpret_cast<const uint4*>(mem);
         v[0] = widen(u.x); v[1] = widen(u.y); v[2] = widen(u.z); v[3] = widen(u.w);
     } else {
         const float4 a = RING ? taken<float4>(src) : *reinterpret_cast<const float4*>(mem);
-        const float4 b = RING ? taken<float4>(src + blockDim.x * 16) : *reinterpret_cast<const float4*>(mem + 4);
+        const float4 b = RING ? taken<float4>(src + THREADS * 16) : *reinterpret_cast<const float4*>(mem + 4);
         v[0] = F2(a.x, a.y); v[1] = F2(a.z, a.w); v[2] = F2(b.x, b.y); v[3] = F2(b.z, b.w);
     }
 }
@@ -65,36 +66,38 @@ __device__ __forceinline__ void params8(const float* p, int c, F2 (&v)[4])
     }
 }
 
-// Sums of K values over the `warps` warps of a token's group; every thread of the group calls it.  Two buffers in turn: who
-// writes one again has met the others at the barrier of the call between, and they had read it by then.
-template <int K> struct Sums {
-    float v[2][16][K][16];                                  // [turn][group][value][warp of the group]; warps that are not there: 0
+// Sums of K values over the W warps of a token's group; every thread of the group calls it.  Two buffers in turn: who writes one
+// again has met the others at the barrier of the call between, and they had read it by then.
+template <int K, int W> struct __align__(16) Sums {
+    float v[2][threads_of(W) / 32 / W][K][W < 4 ? 4 : W];   // [turn][group][value][warp of the group]
 };
-template <int K> __device__ __forceinline__ void sums_clear(Sums<K>& sh)
-{
-    for (int i = threadIdx.x; i < (int)(sizeof(sh) / 4); i += blockDim.x) (&sh.v[0][0][0][0])[i] = 0.0f;
-    __syncthreads();
-}
-template <int K> __device__ __forceinline__ void group_sum(float (&v)[K], int warps, Sums<K>& sh, int& turn)
+template <int K, int W> __device__ __forceinline__ void group_sum(float (&v)[K], Sums<K, W>& sh, int& turn)
 {
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
-    if (warps == 1) return;
-    const int warp = threadIdx.x >> 5, group = warp / warps, w = warp - group * warps;
-    float (&mine)[K][16] = sh.v[turn][group];
-    turn ^= 1;
-    if ((threadIdx.x & 31) == 0)
+    if constexpr (W > 1) {
+        const int group = (threadIdx.x >> 5) / W;
+        auto& mine = sh.v[turn][group];
+        turn ^= 1;
+        if ((threadIdx.x & 31) == 0)
 #pragma unroll
-        for (int k = 0; k < K; ++k) mine[k][w] = v[k];
-    asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * warps) : "memory");
+            for (int k = 0; k < K; ++k) mine[k][(threadIdx.x >> 5) % W] = v[k];
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * W) : "memory");
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        v[k] = 0.0f;
-        for (int i = 0; i < warps; i += 4) {
-            const float4 a = *reinterpret_cast<const float4*>(&mine[k][i]);
-            v[k] += (a.x + a.y) + (a.z + a.w);
+        for (int k = 0; k < K; ++k) {
+            if constexpr (W == 2) {
+                const float2 a = *reinterpret_cast<const float2*>(mine[k]);
+                v[k] = a.x + a.y;
+            } else {
+                v[k] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < W; i += 4) {
+                    const float4 a = *reinterpret_cast<const float4*>(&mine[k][i]);
+                    v[k] += (a.x + a.y) + (a.z + a.w);
+                }
+            }
         }
     }
 }
@@ -109,7 +112,7 @@ struct NormP {
     const void *x, *h;
     const float *post, *gate, *pre;
     float alpha, eps;
-    int n, C, per_gate, warps;
+    int n, C, per_gate;
     void *y, *u;
     float* stats;                   // [2][n]: r1, r2
     // backward
@@ -124,17 +127,17 @@ constexpr int STAGES = 2;
 template <typename T> constexpr uint32_t ring_bytes(int arrays, int nv, int threads) { return STAGES * arrays * nv * pieces<T>() * threads * 16; }
 
 // A group of warps per token, the groups of the grid taking tokens in turn.
-template <typename T, int NV, bool RING>
-__global__ void __launch_bounds__(RING ? 256 : 512, RING ? (NV == 4 ? 3 : 4) : 1) norm_fwd_kernel(const NormP p)
+template <typename T, int NV, int W, bool RING>
+__global__ void __launch_bounds__(threads_of(W), RING ? 4 : 1) norm_fwd_kernel(const NormP p)
 {
     extern __shared__ __align__(16) uint8_t ring[];
-    __shared__ __align__(16) Sums<1> sh;
-    const int gt = threadIdx.x % (32 * p.warps), GT = 32 * p.warps, groups = blockDim.x / GT, step = gridDim.x * groups;
-    const uint32_t array = NV * pieces<T>() * blockDim.x * 16, vec = pieces<T>() * blockDim.x * 16;
+    constexpr int THREADS = threads_of(W), GT = 32 * W, GROUPS = THREADS / GT;
+    __shared__ Sums<1, W> sh;
+    const int gt = threadIdx.x % GT, step = gridDim.x * GROUPS;
+    constexpr uint32_t vec = pieces<T>() * THREADS * 16, array = NV * vec;
     const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * 16;
     const float inv = 1.0f / (float)p.C;
     int turn = 0;
-    sums_clear(sh);
     pdl_wait();
     auto fetch = [&](int tok, int s) {
         if (RING && tok < p.n) {
@@ -143,14 +146,14 @@ __global__ void __launch_bounds__(RING ? 256 : 512, RING ? (NV == 4 ? 3 : 4) : 1
             for (int i = 0; i < NV; ++i) {
                 const int c = (gt + i * GT) * 8;
                 if (c < p.C) {
-                    copy8(mine + s * 2 * array + i * vec, (const T*)p.h + o + c);
-                    copy8(mine + (s * 2 + 1) * array + i * vec, (const T*)p.x + o + c);
+                    copy8<T, THREADS>(mine + s * 2 * array + i * vec, (const T*)p.h + o + c);
+                    copy8<T, THREADS>(mine + (s * 2 + 1) * array + i * vec, (const T*)p.x + o + c);
                 }
             }
         }
         copy_commit();
     };
-    const int tok0 = blockIdx.x * groups, mine0 = threadIdx.x / GT;
+    const int tok0 = blockIdx.x * GROUPS, mine0 = threadIdx.x / GT;
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s) fetch(tok0 + mine0 + s * step, s);
     int slot = 0;
@@ -168,12 +171,12 @@ __global__ void __launch_bounds__(RING ? 256 : 512, RING ? (NV == 4 ? 3 : 4) : 1
             for (int i = 0; i < NV; ++i)
                 if (const int c = (gt + i * GT) * 8; have && c < p.C) {
                     F2 h[4];
-                    take8<T, RING>(from + i * vec, (const T*)p.h + o + c, h);
+                    take8<T, THREADS, RING>(from + i * vec, (const T*)p.h + o + c, h);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) t = fma2(h[j], h[j], t);
                 }
             s[0] = t.lo() + t.hi();
-            group_sum(s, p.warps, sh, turn);
+            group_sum<1, W>(s, sh, turn);
             r1 = inv_sqrt(fmaf(s[0], inv, p.eps));
         }
         const float* gate = p.gate && p.per_gate ? p.gate + (size_t)(tok / p.per_gate) * p.C : p.gate;
@@ -185,8 +188,8 @@ __global__ void __launch_bounds__(RING ? 256 : 512, RING ? (NV == 4 ? 3 : 4) : 1
                 F2 a[4], g[4], h[4], x[4];
                 params8(p.post, c, a);
                 params8(gate, c, g);
-                take8<T, RING>(from + i * vec, (const T*)p.h + o + c, h);
-                take8<T, RING>(from + array + i * vec, (const T*)p.x + o + c, x);
+                take8<T, THREADS, RING>(from + i * vec, (const T*)p.h + o + c, h);
+                take8<T, THREADS, RING>(from + array + i * vec, (const T*)p.x + o + c, x);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     y[i][j] = fma2(F2(p.alpha), x[j], g[j] * a[j] * (h[j] * F2(r1)));
@@ -198,7 +201,7 @@ __global__ void __launch_bounds__(RING ? 256 : 512, RING ? (NV == 4 ? 3 : 4) : 1
         float r2 = 1.0f;
         if (p.u) {
             s[0] = t.lo() + t.hi();
-            group_sum(s, p.warps, sh, turn);
+            group_sum<1, W>(s, sh, turn);
             r2 = inv_sqrt(fmaf(s[0], inv, p.eps));
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
@@ -222,20 +225,20 @@ __global__ void __launch_bounds__(RING ? 256 : 512, RING ? (NV == 4 ? 3 : 4) : 1
 // One block per unit: tokens of one gate row.  The sums over a unit's tokens stay in registers, a thread's columns being
 // always the same; the three sums over a token's columns are taken in one round:
 //   mean(D*gp*h_hat) = mean((dy + r2*du*pre)*gp*h_hat) - r2 * mean(du*pre*y_hat) * mean(y_hat*gp*h_hat),   gp = gate*post
-template <typename T, int NV, bool RING>
-__global__ void __launch_bounds__(RING ? 256 : 512, RING ? 2 : 1) norm_bwd_kernel(const NormP p)
+template <typename T, int NV, int W, bool RING>
+__global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(const NormP p)
 {
     extern __shared__ __align__(16) uint8_t ring[];         // at the end: [groups][C] sums
-    __shared__ __align__(16) Sums<3> sh;
-    const int gt = threadIdx.x % (32 * p.warps), GT = 32 * p.warps, groups = blockDim.x / GT, group = threadIdx.x / GT;
-    const uint32_t array = NV * pieces<T>() * blockDim.x * 16, vec = pieces<T>() * blockDim.x * 16;
+    constexpr int THREADS = threads_of(W), GT = 32 * W, GROUPS = THREADS / GT;
+    __shared__ Sums<3, W> sh;
+    const int gt = threadIdx.x % GT, group = threadIdx.x / GT;
+    constexpr uint32_t vec = pieces<T>() * THREADS * 16, array = NV * vec;
     const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * 16;
     const int row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits;
     const int per = p.per_gate ? p.per_gate : p.n;
     const int t0 = row * per + split * p.length, t1 = min(min(t0 + p.length, (row + 1) * per), p.n);
     const float* gate = p.gate ? p.gate + (size_t)row * p.C : nullptr;
     int turn = 0;
-    sums_clear(sh);
     pdl_wait();
     const bool with_u = p.du != nullptr;
     float nr1 = 0.0f, nr2 = 0.0f;                           // of the token that is copied next
@@ -247,10 +250,10 @@ __global__ void __launch_bounds__(RING ? 256 : 512, RING ? 2 : 1) norm_bwd_kerne
                 const int c = (gt + i * GT) * 8;
                 if (c < p.C) {
                     const uint32_t d = mine + s * 4 * array + i * vec;
-                    copy8(d, (const T*)p.h + o + c);
-                    copy8(d + array, (const T*)p.x + o + c);
-                    copy8(d + 2 * array, (const T*)p.dy + o + c);
-                    if (with_u) copy8(d + 3 * array, (const T*)p.du + o + c);
+                    copy8<T, THREADS>(d, (const T*)p.h + o + c);
+                    copy8<T, THREADS>(d + array, (const T*)p.x + o + c);
+                    copy8<T, THREADS>(d + 2 * array, (const T*)p.dy + o + c);
+                    if (with_u) copy8<T, THREADS>(d + 3 * array, (const T*)p.du + o + c);
                 }
             }
         }
@@ -272,22 +275,22 @@ __global__ void __launch_bounds__(RING ? 256 : 512, RING ? 2 : 1) norm_bwd_kerne
         }
     }
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) fetch(t0 + group + s * groups, s);
+    for (int s = 0; s < STAGES - 1; ++s) fetch(t0 + group + s * GROUPS, s);
     if (t0 + group < t1) {
         nr1 = p.stats[t0 + group];
         nr2 = p.stats[p.n + t0 + group];
     }
     const float inv = 1.0f / (float)p.C;
     int slot = 0;
-    for (int tok0 = t0; tok0 < t1; tok0 += groups, slot = slot + 1 == STAGES ? 0 : slot + 1) {
+    for (int tok0 = t0; tok0 < t1; tok0 += GROUPS, slot = slot + 1 == STAGES ? 0 : slot + 1) {
         const int tok = tok0 + group;
         const bool have = tok < t1;
         const size_t o = (size_t)tok * p.C;
         const float r1 = nr1, r2 = nr2;
-        fetch(tok + (STAGES - 1) * groups, slot == 0 ? STAGES - 1 : slot - 1);
-        if (tok + groups < t1) {
-            nr1 = p.stats[tok + groups];
-            nr2 = p.stats[p.n + tok + groups];
+        fetch(tok + (STAGES - 1) * GROUPS, slot == 0 ? STAGES - 1 : slot - 1);
+        if (tok + GROUPS < t1) {
+            nr1 = p.stats[tok + GROUPS];
+            nr2 = p.stats[p.n + tok + GROUPS];
         }
         copy_wait<STAGES - 1>();
         const uint32_t from = mine + slot * 4 * array;
@@ -297,11 +300,11 @@ __global__ void __launch_bounds__(RING ? 256 : 512, RING ? 2 : 1) norm_bwd_kerne
             const int c = (gt + i * GT) * 8;
             if (have && c < p.C) {
                 F2 h[4], x[4], dy[4], du[4], b[4];
-                take8<T, RING>(from + i * vec, (const T*)p.h + o + c, h);
-                take8<T, RING>(from + array + i * vec, (const T*)p.x + o + c, x);
-                take8<T, RING>(from + 2 * array + i * vec, (const T*)p.dy + o + c, dy);
+                take8<T, THREADS, RING>(from + i * vec, (const T*)p.h + o + c, h);
+                take8<T, THREADS, RING>(from + array + i * vec, (const T*)p.x + o + c, x);
+                take8<T, THREADS, RING>(from + 2 * array + i * vec, (const T*)p.dy + o + c, dy);
                 if (with_u) {
-                    take8<T, RING>(from + 3 * array + i * vec, (const T*)p.du + o + c, du);
+                    take8<T, THREADS, RING>(from + 3 * array + i * vec, (const T*)p.du + o + c, du);
                     params8(p.pre, c, b);
                 }
 #pragma unroll
@@ -319,18 +322,18 @@ __global__ void __launch_bounds__(RING ? 256 : 512, RING ? 2 : 1) norm_bwd_kerne
             }
         }
         float s[3] = {s0.lo() + s0.hi(), s1.lo() + s1.hi(), s2.lo() + s2.hi()};
-        group_sum(s, p.warps, sh, turn);
+        group_sum<3, W>(s, sh, turn);
         const float mA = s[0] * inv, mB = p.post ? (s[1] - r2 * mA * s[2]) * inv : 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (gt + i * GT) * 8;
             if (have && c < p.C) {
                 F2 h[4], x[4], D[4], du[4], b[4], dx[4];
-                take8<T, RING>(from + i * vec, (const T*)p.h + o + c, h);
-                take8<T, RING>(from + array + i * vec, (const T*)p.x + o + c, x);
-                take8<T, RING>(from + 2 * array + i * vec, (const T*)p.dy + o + c, D);
+                take8<T, THREADS, RING>(from + i * vec, (const T*)p.h + o + c, h);
+                take8<T, THREADS, RING>(from + array + i * vec, (const T*)p.x + o + c, x);
+                take8<T, THREADS, RING>(from + 2 * array + i * vec, (const T*)p.dy + o + c, D);
                 if (with_u) {
-                    take8<T, RING>(from + 3 * array + i * vec, (const T*)p.du + o + c, du);
+                    take8<T, THREADS, RING>(from + 3 * array + i * vec, (const T*)p.du + o + c, du);
                     params8(p.pre, c, b);
                 }
 #pragma unroll
@@ -356,7 +359,7 @@ __global__ void __launch_bounds__(RING ? 256 : 512, RING ? 2 : 1) norm_bwd_kerne
     copy_wait<0>();
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        if (groups > 1) {
+        if (GROUPS > 1) {
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
@@ -366,7 +369,7 @@ __global__ void __launch_bounds__(RING ? 256 : 512, RING ? 2 : 1) norm_bwd_kerne
             __syncthreads();
             for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
                 float t = 0.0f;
-                for (int g = 0; g < groups; ++g) t += cols[g * p.C + c];
+                for (int g = 0; g < GROUPS; ++g) t += cols[g * p.C + c];
                 out[k * p.C + c] = t;
             }
         } else {
@@ -424,13 +427,6 @@ norm_params_kernel(const float* part, const float* post, const float* gate, int 
 int gate_rows(int n, int per_gate) { return per_gate ? (n + per_gate - 1) / per_gate : 1; }
 int one_row(int n, int per_gate) { return per_gate >= n ? 0 : per_gate; }
 
-// Warps per token with NV pieces of eight elements per thread, a power of two up to 16.
-int warps_of(int C, int nv)
-{
-    int w = 1;
-    while (w < 16 && w * 32 * 8 * nv < C) w *= 2;
-    return w;
-}
 struct Split {
     int splits, length;
 };
@@ -460,9 +456,6 @@ int check_params(const float* post, const float* gate, const float* pre)
     return 0;
 }
 
-// The threads of a block: groups of whole tokens, 256 threads, or one group of up to 512.
-int threads_of(int warps) { return 32 * warps > 256 ? 32 * warps : 256; }
-
 template <typename K> int opt_in(K kernel, uint32_t bytes, bool (&done)[64])
 {
     int dev = 0;
@@ -472,44 +465,48 @@ template <typename K> int opt_in(K kernel, uint32_t bytes, bool (&done)[64])
     if (dev < 64) done[dev] = true;
     return 0;
 }
-template <typename T, int NV, bool RING> int run_fwd(NormP& p, cudaStream_t st)
+template <typename T, int NV, int W, bool RING> int run_fwd(const NormP& p, cudaStream_t st)
 {
-    p.warps = warps_of(p.C, NV);
-    const int threads = threads_of(p.warps), groups = threads / (32 * p.warps);
-    const uint32_t smem = RING ? ring_bytes<T>(2, NV, threads) : 0;
+    constexpr int threads = threads_of(W), groups = threads / (32 * W);
+    constexpr uint32_t smem = RING ? ring_bytes<T>(2, NV, threads) : 0;
     const int most = 148 * FWD_CTAS, want = (p.n + groups - 1) / groups;
-    static bool done[64];                                   // (threads and bytes are the same in every call of this form)
-    MGPT_TRY(opt_in(norm_fwd_kernel<T, NV, RING>, smem, done));
-    MGPT_CUDA(launch_pdl(norm_fwd_kernel<T, NV, RING>, want < most ? want : most, threads, smem, st, p));
+    static bool done[64];
+    MGPT_TRY(opt_in(norm_fwd_kernel<T, NV, W, RING>, smem, done));
+    MGPT_CUDA(launch_pdl(norm_fwd_kernel<T, NV, W, RING>, want < most ? want : most, threads, smem, st, p));
     MGPT_LAUNCHED("norm_fwd_kernel");
     return 0;
 }
-template <typename T, int NV, bool RING> int run_bwd(NormP& p, int units, cudaStream_t st)
+template <typename T, int NV, int W, bool RING> int run_bwd(const NormP& p, int units, cudaStream_t st)
 {
-    p.warps = warps_of(p.C, NV);
-    const int threads = threads_of(p.warps);
     // (the ring is more than the sums at the end, 32 NV bytes per thread where there are groups)
-    const uint32_t smem = RING ? ring_bytes<T>(4, NV, threads) : 0;
+    constexpr uint32_t smem = RING ? ring_bytes<T>(4, NV, threads_of(W)) : 0;
     static bool done[64];
-    MGPT_TRY(opt_in(norm_bwd_kernel<T, NV, RING>, smem, done));
-    MGPT_CUDA(launch_pdl(norm_bwd_kernel<T, NV, RING>, units, threads, smem, st, p));
+    MGPT_TRY(opt_in(norm_bwd_kernel<T, NV, W, RING>, smem, done));
+    MGPT_CUDA(launch_pdl(norm_bwd_kernel<T, NV, W, RING>, units, threads_of(W), smem, st, p));
     MGPT_LAUNCHED("norm_bwd_kernel");
     return 0;
 }
-template <typename T> int run_fwd(NormP& p, cudaStream_t st)
+// NV pieces of eight elements per thread: W, the fewest warps that hold a token, is a power of two
+#define MGPT_BY_WARPS(run, NV, ...)                                            \
+    (p.C <= 256 * NV ? run<T, NV, 1, true>(__VA_ARGS__)                        \
+     : p.C <= 512 * NV ? run<T, NV, 2, true>(__VA_ARGS__)                      \
+     : p.C <= 1024 * NV ? run<T, NV, 4, true>(__VA_ARGS__) : run<T, NV, 8, true>(__VA_ARGS__))
+template <typename T> int run_fwd(const NormP& p, cudaStream_t st)
 {
-    // pieces of eight elements per thread: one where the tokens are few
-    if (p.C > 4096) return run_fwd<T, 4, false>(p, st);
-    if (p.C > 2048) return run_fwd<T, 2, true>(p, st);
-    if (sizeof(T) == 2 && (size_t)p.n * p.C > (size_t)148 * 2048 * 4) return run_fwd<T, 2, true>(p, st);
-    return run_fwd<T, 1, true>(p, st);
+    if (p.C > 8192) return run_fwd<T, 4, 16, false>(p, st);
+    if (p.C > 4096) return run_fwd<T, 4, 8, false>(p, st);
+    // one piece per thread where the tokens are few, and of FP32, whose pieces are twice as long
+    if (p.C > 2048 || (sizeof(T) == 2 && (size_t)p.n * p.C > (size_t)148 * 2048 * 4)) return MGPT_BY_WARPS(run_fwd, 2, p, st);
+    return MGPT_BY_WARPS(run_fwd, 1, p, st);
 }
-template <typename T> int run_bwd(NormP& p, int units, cudaStream_t st)
+template <typename T> int run_bwd(const NormP& p, int units, cudaStream_t st)
 {
-    if (p.C > 4096) return run_bwd<T, 4, false>(p, units, st);
-    if (p.C > 2048 || sizeof(T) == 2) return run_bwd<T, 2, true>(p, units, st);
-    return run_bwd<T, 1, true>(p, units, st);
+    if (p.C > 8192) return run_bwd<T, 4, 16, false>(p, units, st);
+    if (p.C > 4096) return run_bwd<T, 4, 8, false>(p, units, st);
+    if (p.C > 2048 || sizeof(T) == 2) return MGPT_BY_WARPS(run_bwd, 2, p, units, st);
+    return MGPT_BY_WARPS(run_bwd, 1, p, units, st);
 }
+#undef MGPT_BY_WARPS
 
 }  // namespace
 
