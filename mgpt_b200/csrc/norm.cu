@@ -13,7 +13,12 @@
 //   d_pre += sum du*y_hat,   d_post += sum D*gate*h_hat,   d_gate += sum D*h_hat*post  (over the row's tokens)
 // y is computed again from x and h; r1 and r2 are kept by the forward pass.
 //
-// Bound by HBM: every element of x, h (dy, du) is read once into registers and y, u (dx, dh) written once.
+// Bound by HBM: every element of x, h (dy, du) is read once and y, u (dx, dh) written once.  A token is held by the fewest warps
+// (a constant, so that addresses are immediate) and comes through a ring of two tokens per group of warps; sums take one barrier.
+// us and TB/s on a B200: 32768 x 2048 BF16 forward 106 (5.1), backward 155 (5.2), the parameters' sums 9; 16384 x 2048 FP32
+// forward 89 (6.0), backward 140 (5.7).  BF16, with twice the elements per byte, is at 65 % of the issue slots.  Before: loads
+// into registers, four pieces per thread, 193 and 316; the ring with the number of warps at run time 116 and 190; FP32 in two
+// pieces of 32 bytes side by side, half a sector per access, 137 and 227.  A third token in the ring costs more blocks than it hides.
 #include "pairs.cuh"
 
 namespace mgpt {
@@ -25,44 +30,46 @@ __host__ __device__ constexpr int threads_of(int warps) { return warps > 8 ? 32 
 constexpr int UNITS = 296;          // blocks of the backward pass aimed at: two per SM
 constexpr int FWD_CTAS = 4;         // of the forward pass, per SM
 
-// Eight consecutive elements: a thread copies them to a place of its own in shared memory, some tokens ahead, and takes them from
-// there (pieces of 16 bytes, the block's threads side by side).
-template <typename T> constexpr int pieces() { return sizeof(T) / 2; }
-template <typename T, int THREADS> __device__ __forceinline__ void copy8(uint32_t dst, const T* src)
-{
-#pragma unroll
-    for (int k = 0; k < pieces<T>(); ++k) copy16(dst + k * THREADS * 16, (const uint4*)src + k);
-}
+// A piece: 16 bytes of a row, so that a warp's access is one run of memory whatever the type.  A thread copies its pieces to places
+// of their own in shared memory, some tokens ahead, and takes them from there.
+template <typename T> constexpr int piece() { return 16 / sizeof(T); }          // elements
+template <typename T> struct Piece {
+    F2 v[piece<T>() / 2];
+};
 // RING: from there, else from memory (rows too wide for a ring, which the second pass over a token finds in the caches)
-template <typename T, int THREADS, bool RING> __device__ __forceinline__ void take8(uint32_t src, const T* mem, F2 (&v)[4])
+template <typename T, bool RING> __device__ __forceinline__ void take(uint32_t src, const T* mem, Piece<T>& o)
 {
     if constexpr (sizeof(T) == 2) {
         const uint4 u = RING ? taken<uint4>(src) : *reinterpret_cast<const uint4*>(mem);
-        v[0] = widen(u.x); v[1] = widen(u.y); v[2] = widen(u.z); v[3] = widen(u.w);
+        o.v[0] = widen(u.x); o.v[1] = widen(u.y); o.v[2] = widen(u.z); o.v[3] = widen(u.w);
     } else {
         const float4 a = RING ? taken<float4>(src) : *reinterpret_cast<const float4*>(mem);
-        const float4 b = RING ? taken<float4>(src + THREADS * 16) : *reinterpret_cast<const float4*>(mem + 4);
-        v[0] = F2(a.x, a.y); v[1] = F2(a.z, a.w); v[2] = F2(b.x, b.y); v[3] = F2(b.z, b.w);
+        o.v[0] = F2(a.x, a.y); o.v[1] = F2(a.z, a.w);
     }
 }
-__device__ __forceinline__ void store8(bf16* p, const F2 (&v)[4])
+__device__ __forceinline__ void store(bf16* p, const Piece<bf16>& o)
 {
-    *reinterpret_cast<uint4*>(p) = make_uint4(narrow(v[0]), narrow(v[1]), narrow(v[2]), narrow(v[3]));
+    *reinterpret_cast<uint4*>(p) = make_uint4(narrow(o.v[0]), narrow(o.v[1]), narrow(o.v[2]), narrow(o.v[3]));
 }
-__device__ __forceinline__ void store8(float* p, const F2 (&v)[4])
+__device__ __forceinline__ void store(float* p, const Piece<float>& o)
 {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0].lo(), v[0].hi(), v[1].lo(), v[1].hi());
-    *reinterpret_cast<float4*>(p + 4) = make_float4(v[2].lo(), v[2].hi(), v[3].lo(), v[3].hi());
+    *reinterpret_cast<float4*>(p) = make_float4(o.v[0].lo(), o.v[0].hi(), o.v[1].lo(), o.v[1].hi());
 }
-// eight parameters, or ones
-__device__ __forceinline__ void params8(const float* p, int c, F2 (&v)[4])
+// the same columns of FP32 sums
+template <typename T> __device__ __forceinline__ void store_sums(float* p, const Piece<T>& o)
 {
-    if (p) {
-        const float4 a = *reinterpret_cast<const float4*>(p + c), b = *reinterpret_cast<const float4*>(p + c + 4);
-        v[0] = F2(a.x, a.y); v[1] = F2(a.z, a.w); v[2] = F2(b.x, b.y); v[3] = F2(b.z, b.w);
-    } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = F2(1.0f);
+    for (int j = 0; j < piece<T>() / 4; ++j)
+        *reinterpret_cast<float4*>(p + 4 * j) = make_float4(o.v[2 * j].lo(), o.v[2 * j].hi(), o.v[2 * j + 1].lo(), o.v[2 * j + 1].hi());
+}
+// a piece's parameters, or ones
+template <typename T> __device__ __forceinline__ void params(const float* p, int c, Piece<T>& o)
+{
+#pragma unroll
+    for (int j = 0; j < piece<T>() / 4; ++j) {
+        const float4 a = p ? *reinterpret_cast<const float4*>(p + c + 4 * j) : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+        o.v[2 * j] = F2(a.x, a.y);
+        o.v[2 * j + 1] = F2(a.z, a.w);
     }
 }
 
@@ -122,19 +129,19 @@ struct NormP {
     int splits, length;             // units per gate row, tokens per unit
 };
 
-// Bytes of a block's ring: `arrays` of NV * 8 elements per thread, STAGES tokens.
+// Bytes of a block's ring: `arrays` of NV pieces per thread, STAGES tokens.
 constexpr int STAGES = 2;
-template <typename T> constexpr uint32_t ring_bytes(int arrays, int nv, int threads) { return STAGES * arrays * nv * pieces<T>() * threads * 16; }
+constexpr uint32_t ring_bytes(int arrays, int nv, int threads) { return STAGES * arrays * nv * threads * 16; }
 
 // A group of warps per token, the groups of the grid taking tokens in turn.
 template <typename T, int NV, int W, bool RING>
 __global__ void __launch_bounds__(threads_of(W), RING ? 4 : 1) norm_fwd_kernel(const NormP p)
 {
     extern __shared__ __align__(16) uint8_t ring[];
-    constexpr int THREADS = threads_of(W), GT = 32 * W, GROUPS = THREADS / GT;
+    constexpr int THREADS = threads_of(W), GT = 32 * W, GROUPS = THREADS / GT, E = piece<T>(), H = E / 2;
     __shared__ Sums<1, W> sh;
     const int gt = threadIdx.x % GT, step = gridDim.x * GROUPS;
-    constexpr uint32_t vec = pieces<T>() * THREADS * 16, array = NV * vec;
+    constexpr uint32_t vec = THREADS * 16, array = NV * vec;
     const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * 16;
     const float inv = 1.0f / (float)p.C;
     int turn = 0;
@@ -144,10 +151,10 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 4 : 1) norm_fwd_kernel(c
             const size_t o = (size_t)tok * p.C;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int c = (gt + i * GT) * 8;
+                const int c = (gt + i * GT) * E;
                 if (c < p.C) {
-                    copy8<T, THREADS>(mine + s * 2 * array + i * vec, (const T*)p.h + o + c);
-                    copy8<T, THREADS>(mine + (s * 2 + 1) * array + i * vec, (const T*)p.x + o + c);
+                    copy16(mine + s * 2 * array + i * vec, (const T*)p.h + o + c);
+                    copy16(mine + (s * 2 + 1) * array + i * vec, (const T*)p.x + o + c);
                 }
             }
         }
@@ -169,33 +176,34 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 4 : 1) norm_fwd_kernel(c
             F2 t(0.0f);
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if (const int c = (gt + i * GT) * 8; have && c < p.C) {
-                    F2 h[4];
-                    take8<T, THREADS, RING>(from + i * vec, (const T*)p.h + o + c, h);
+                if (const int c = (gt + i * GT) * E; have && c < p.C) {
+                    Piece<T> h;
+                    take<T, RING>(from + i * vec, (const T*)p.h + o + c, h);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) t = fma2(h[j], h[j], t);
+                    for (int j = 0; j < H; ++j) t = fma2(h.v[j], h.v[j], t);
                 }
             s[0] = t.lo() + t.hi();
             group_sum<1, W>(s, sh, turn);
             r1 = inv_sqrt(fmaf(s[0], inv, p.eps));
         }
         const float* gate = p.gate && p.per_gate ? p.gate + (size_t)(tok / p.per_gate) * p.C : p.gate;
-        F2 y[NV][4], t(0.0f);
+        Piece<T> y[NV];
+        F2 t(0.0f);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (gt + i * GT) * 8;
+            const int c = (gt + i * GT) * E;
             if (have && c < p.C) {
-                F2 a[4], g[4], h[4], x[4];
-                params8(p.post, c, a);
-                params8(gate, c, g);
-                take8<T, THREADS, RING>(from + i * vec, (const T*)p.h + o + c, h);
-                take8<T, THREADS, RING>(from + array + i * vec, (const T*)p.x + o + c, x);
+                Piece<T> a, g, h, x;
+                params<T>(p.post, c, a);
+                params<T>(gate, c, g);
+                take<T, RING>(from + i * vec, (const T*)p.h + o + c, h);
+                take<T, RING>(from + array + i * vec, (const T*)p.x + o + c, x);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    y[i][j] = fma2(F2(p.alpha), x[j], g[j] * a[j] * (h[j] * F2(r1)));
-                    t = fma2(y[i][j], y[i][j], t);
+                for (int j = 0; j < H; ++j) {
+                    y[i].v[j] = fma2(F2(p.alpha), x.v[j], g.v[j] * a.v[j] * (h.v[j] * F2(r1)));
+                    t = fma2(y[i].v[j], y[i].v[j], t);
                 }
-                store8((T*)p.y + o + c, y[i]);
+                store((T*)p.y + o + c, y[i]);
             }
         }
         float r2 = 1.0f;
@@ -205,13 +213,13 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 4 : 1) norm_fwd_kernel(c
             r2 = inv_sqrt(fmaf(s[0], inv, p.eps));
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int c = (gt + i * GT) * 8;
+                const int c = (gt + i * GT) * E;
                 if (have && c < p.C) {
-                    F2 b[4];
-                    params8(p.pre, c, b);
+                    Piece<T> b;
+                    params<T>(p.pre, c, b);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) y[i][j] = y[i][j] * F2(r2) * b[j];
-                    store8((T*)p.u + o + c, y[i]);
+                    for (int j = 0; j < H; ++j) y[i].v[j] = y[i].v[j] * F2(r2) * b.v[j];
+                    store((T*)p.u + o + c, y[i]);
                 }
             }
         }
@@ -229,10 +237,10 @@ template <typename T, int NV, int W, bool RING>
 __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(const NormP p)
 {
     extern __shared__ __align__(16) uint8_t ring[];         // at the end: [groups][C] sums
-    constexpr int THREADS = threads_of(W), GT = 32 * W, GROUPS = THREADS / GT;
+    constexpr int THREADS = threads_of(W), GT = 32 * W, GROUPS = THREADS / GT, E = piece<T>(), H = E / 2;
     __shared__ Sums<3, W> sh;
     const int gt = threadIdx.x % GT, group = threadIdx.x / GT;
-    constexpr uint32_t vec = pieces<T>() * THREADS * 16, array = NV * vec;
+    constexpr uint32_t vec = THREADS * 16, array = NV * vec;
     const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * 16;
     const int row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits;
     const int per = p.per_gate ? p.per_gate : p.n;
@@ -247,31 +255,31 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
             const size_t o = (size_t)tok * p.C;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int c = (gt + i * GT) * 8;
+                const int c = (gt + i * GT) * E;
                 if (c < p.C) {
                     const uint32_t d = mine + s * 4 * array + i * vec;
-                    copy8<T, THREADS>(d, (const T*)p.h + o + c);
-                    copy8<T, THREADS>(d + array, (const T*)p.x + o + c);
-                    copy8<T, THREADS>(d + 2 * array, (const T*)p.dy + o + c);
-                    if (with_u) copy8<T, THREADS>(d + 3 * array, (const T*)p.du + o + c);
+                    copy16(d, (const T*)p.h + o + c);
+                    copy16(d + array, (const T*)p.x + o + c);
+                    copy16(d + 2 * array, (const T*)p.dy + o + c);
+                    if (with_u) copy16(d + 3 * array, (const T*)p.du + o + c);
                 }
             }
         }
         copy_commit();
     };
-    F2 S1[NV][4], S2[NV][4], gp[NV][4];
+    Piece<T> S1[NV], S2[NV], gp[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int c = (gt + i * GT) * 8;
-        F2 a[4], g[4];
+        const int c = (gt + i * GT) * E;
+        Piece<T> a, g;
         if (c < p.C) {
-            params8(p.post, c, a);
-            params8(gate, c, g);
+            params<T>(p.post, c, a);
+            params<T>(gate, c, g);
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            S1[i][j] = S2[i][j] = F2(0.0f);
-            if (c < p.C) gp[i][j] = g[j] * a[j];
+        for (int j = 0; j < H; ++j) {
+            S1[i].v[j] = S2[i].v[j] = F2(0.0f);
+            if (c < p.C) gp[i].v[j] = g.v[j] * a.v[j];
         }
     }
 #pragma unroll
@@ -297,25 +305,25 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
         F2 s0(0.0f), s1(0.0f), s2(0.0f);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (gt + i * GT) * 8;
+            const int c = (gt + i * GT) * E;
             if (have && c < p.C) {
-                F2 h[4], x[4], dy[4], du[4], b[4];
-                take8<T, THREADS, RING>(from + i * vec, (const T*)p.h + o + c, h);
-                take8<T, THREADS, RING>(from + array + i * vec, (const T*)p.x + o + c, x);
-                take8<T, THREADS, RING>(from + 2 * array + i * vec, (const T*)p.dy + o + c, dy);
+                Piece<T> h, x, dy, du, b;
+                take<T, RING>(from + i * vec, (const T*)p.h + o + c, h);
+                take<T, RING>(from + array + i * vec, (const T*)p.x + o + c, x);
+                take<T, RING>(from + 2 * array + i * vec, (const T*)p.dy + o + c, dy);
                 if (with_u) {
-                    take8<T, THREADS, RING>(from + 3 * array + i * vec, (const T*)p.du + o + c, du);
-                    params8(p.pre, c, b);
+                    take<T, RING>(from + 3 * array + i * vec, (const T*)p.du + o + c, du);
+                    params<T>(p.pre, c, b);
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const F2 q = gp[i][j] * (h[j] * F2(r1)), yh = fma2(F2(p.alpha), x[j], q) * F2(r2);
+                for (int j = 0; j < H; ++j) {
+                    const F2 q = gp[i].v[j] * (h.v[j] * F2(r1)), yh = fma2(F2(p.alpha), x.v[j], q) * F2(r2);
                     if (with_u) {
-                        const F2 d = du[j] * b[j];
+                        const F2 d = du.v[j] * b.v[j];
                         s0 = fma2(d, yh, s0);
-                        s1 = fma2(fma2(F2(r2), d, dy[j]), q, s1);
+                        s1 = fma2(fma2(F2(r2), d, dy.v[j]), q, s1);
                     } else {
-                        s1 = fma2(dy[j], q, s1);
+                        s1 = fma2(dy.v[j], q, s1);
                     }
                     s2 = fma2(yh, q, s2);
                 }
@@ -326,30 +334,30 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
         const float mA = s[0] * inv, mB = p.post ? (s[1] - r2 * mA * s[2]) * inv : 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (gt + i * GT) * 8;
+            const int c = (gt + i * GT) * E;
             if (have && c < p.C) {
-                F2 h[4], x[4], D[4], du[4], b[4], dx[4];
-                take8<T, THREADS, RING>(from + i * vec, (const T*)p.h + o + c, h);
-                take8<T, THREADS, RING>(from + array + i * vec, (const T*)p.x + o + c, x);
-                take8<T, THREADS, RING>(from + 2 * array + i * vec, (const T*)p.dy + o + c, D);
+                Piece<T> h, x, D, du, b, dx;
+                take<T, RING>(from + i * vec, (const T*)p.h + o + c, h);
+                take<T, RING>(from + array + i * vec, (const T*)p.x + o + c, x);
+                take<T, RING>(from + 2 * array + i * vec, (const T*)p.dy + o + c, D);
                 if (with_u) {
-                    take8<T, THREADS, RING>(from + 3 * array + i * vec, (const T*)p.du + o + c, du);
-                    params8(p.pre, c, b);
+                    take<T, RING>(from + 3 * array + i * vec, (const T*)p.du + o + c, du);
+                    params<T>(p.pre, c, b);
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const F2 hh = h[j] * F2(r1);
+                for (int j = 0; j < H; ++j) {
+                    const F2 hh = h.v[j] * F2(r1);
                     if (with_u) {
-                        const F2 yh = fma2(F2(p.alpha), x[j], gp[i][j] * hh) * F2(r2);
-                        D[j] = fma2(F2(r2), fma2(yh, F2(-mA), du[j] * b[j]), D[j]);
-                        S2[i][j] = fma2(du[j], yh, S2[i][j]);
+                        const F2 yh = fma2(F2(p.alpha), x.v[j], gp[i].v[j] * hh) * F2(r2);
+                        D.v[j] = fma2(F2(r2), fma2(yh, F2(-mA), du.v[j] * b.v[j]), D.v[j]);
+                        S2[i].v[j] = fma2(du.v[j], yh, S2[i].v[j]);
                     }
-                    dx[j] = F2(p.alpha) * D[j];
-                    S1[i][j] = fma2(D[j], hh, S1[i][j]);
-                    h[j] = F2(r1) * fma2(hh, F2(-mB), D[j] * gp[i][j]);
+                    dx.v[j] = F2(p.alpha) * D.v[j];
+                    S1[i].v[j] = fma2(D.v[j], hh, S1[i].v[j]);
+                    h.v[j] = F2(r1) * fma2(hh, F2(-mB), D.v[j] * gp[i].v[j]);
                 }
-                store8((T*)p.dx + o + c, dx);
-                store8((T*)p.dh + o + c, h);
+                store((T*)p.dx + o + c, dx);
+                store((T*)p.dh + o + c, h);
             }
         }
     }
@@ -363,8 +371,8 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int c = (gt + i * GT) * 8;
-                if (c < p.C) store8(cols + group * p.C + c, k ? S2[i] : S1[i]);
+                const int c = (gt + i * GT) * E;
+                if (c < p.C) store_sums<T>(cols + group * p.C + c, k ? S2[i] : S1[i]);
             }
             __syncthreads();
             for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
@@ -375,8 +383,8 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
         } else {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int c = (gt + i * GT) * 8;
-                if (c < p.C) store8(out + k * p.C + c, k ? S2[i] : S1[i]);
+                const int c = (gt + i * GT) * E;
+                if (c < p.C) store_sums<T>(out + k * p.C + c, k ? S2[i] : S1[i]);
             }
         }
     }
@@ -468,7 +476,7 @@ template <typename K> int opt_in(K kernel, uint32_t bytes, bool (&done)[64])
 template <typename T, int NV, int W, bool RING> int run_fwd(const NormP& p, cudaStream_t st)
 {
     constexpr int threads = threads_of(W), groups = threads / (32 * W);
-    constexpr uint32_t smem = RING ? ring_bytes<T>(2, NV, threads) : 0;
+    constexpr uint32_t smem = RING ? ring_bytes(2, NV, threads) : 0;
     const int most = 148 * FWD_CTAS, want = (p.n + groups - 1) / groups;
     static bool done[64];
     MGPT_TRY(opt_in(norm_fwd_kernel<T, NV, W, RING>, smem, done));
@@ -478,33 +486,37 @@ template <typename T, int NV, int W, bool RING> int run_fwd(const NormP& p, cuda
 }
 template <typename T, int NV, int W, bool RING> int run_bwd(const NormP& p, int units, cudaStream_t st)
 {
-    // (the ring is more than the sums at the end, 32 NV bytes per thread where there are groups)
-    constexpr uint32_t smem = RING ? ring_bytes<T>(4, NV, threads_of(W)) : 0;
+    // (the ring is more than the sums at the end, 4 NV piece<T>() bytes per thread where there are groups)
+    constexpr uint32_t smem = RING ? ring_bytes(4, NV, threads_of(W)) : 0;
     static bool done[64];
     MGPT_TRY(opt_in(norm_bwd_kernel<T, NV, W, RING>, smem, done));
     MGPT_CUDA(launch_pdl(norm_bwd_kernel<T, NV, W, RING>, units, threads_of(W), smem, st, p));
     MGPT_LAUNCHED("norm_bwd_kernel");
     return 0;
 }
-// NV pieces of eight elements per thread: W, the fewest warps that hold a token, is a power of two
-#define MGPT_BY_WARPS(run, NV, ...)                                            \
-    (p.C <= 256 * NV ? run<T, NV, 1, true>(__VA_ARGS__)                        \
-     : p.C <= 512 * NV ? run<T, NV, 2, true>(__VA_ARGS__)                      \
-     : p.C <= 1024 * NV ? run<T, NV, 4, true>(__VA_ARGS__) : run<T, NV, 8, true>(__VA_ARGS__))
+// NV pieces per thread: the fewest warps that hold a token, a power of two
+#define MGPT_BY_WARPS(run, NV, ...)                                                               \
+    (p.C <= 32 * piece<T>() * NV ? run<T, NV, 1, true>(__VA_ARGS__)                               \
+     : p.C <= 64 * piece<T>() * NV ? run<T, NV, 2, true>(__VA_ARGS__)                             \
+     : p.C <= 128 * piece<T>() * NV ? run<T, NV, 4, true>(__VA_ARGS__) : run<T, NV, 8, true>(__VA_ARGS__))
 template <typename T> int run_fwd(const NormP& p, cudaStream_t st)
 {
-    if (p.C > 8192) return run_fwd<T, 4, 16, false>(p, st);
-    if (p.C > 4096) return run_fwd<T, 4, 8, false>(p, st);
-    // one piece per thread where the tokens are few, and of FP32, whose pieces are twice as long
-    if (p.C > 2048 || (sizeof(T) == 2 && (size_t)p.n * p.C > (size_t)148 * 2048 * 4)) return MGPT_BY_WARPS(run_fwd, 2, p, st);
-    return MGPT_BY_WARPS(run_fwd, 1, p, st);
+    constexpr int F = sizeof(T) / 2;                        // pieces that hold eight elements
+    if (p.C > 8192) return run_fwd<T, 4 * F, 16, false>(p, st);
+    if (p.C > 4096) return run_fwd<T, 4 * F, 8, false>(p, st);
+    if (p.C > 2048) return MGPT_BY_WARPS(run_fwd, 2 * F, p, st);
+    // Two pieces per thread (4 of FP32: 16384 x 2048 123 us against 89); one of BF16 where the tokens are few and a thread's chain is
+    // what counts (8 x 1024: 3.1 us against 4.3; 32768 x 2048: 150 against 106).
+    if (sizeof(T) == 2 && (size_t)p.n * p.C <= (size_t)148 * 2048 * 4) return MGPT_BY_WARPS(run_fwd, 1, p, st);
+    return MGPT_BY_WARPS(run_fwd, 2, p, st);
 }
 template <typename T> int run_bwd(const NormP& p, int units, cudaStream_t st)
 {
-    if (p.C > 8192) return run_bwd<T, 4, 16, false>(p, units, st);
-    if (p.C > 4096) return run_bwd<T, 4, 8, false>(p, units, st);
-    if (p.C > 2048 || sizeof(T) == 2) return MGPT_BY_WARPS(run_bwd, 2, p, units, st);
-    return MGPT_BY_WARPS(run_bwd, 1, p, units, st);
+    constexpr int F = sizeof(T) / 2;
+    if (p.C > 8192) return run_bwd<T, 4 * F, 16, false>(p, units, st);
+    if (p.C > 4096) return run_bwd<T, 4 * F, 8, false>(p, units, st);
+    if (p.C > 2048) return MGPT_BY_WARPS(run_bwd, 2 * F, p, units, st);
+    return MGPT_BY_WARPS(run_bwd, 2, p, units, st);
 }
 #undef MGPT_BY_WARPS
 
