@@ -731,25 +731,22 @@ head_join_kernel(const int32_t* n_valid, const float2* part, const float* z_targ
     loss[i] = in ? l - z_target[row] : 0.0f;
 }
 
-// dx from several slices of the vocabulary, a warp per token.
-__global__ void __launch_bounds__(256)
+// dx from several slices of the vocabulary: a token per block of x, four channels per thread.
+__global__ void __launch_bounds__(128)
 head_dx_kernel(const int32_t* n_valid, const float* scale, const float* acc, const int32_t* rows, int slices, int n_pad, int C, void* dx, int f32)
 {
     pdl_wait();
-    const int lane = threadIdx.x & 31, row = blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (row >= *n_valid) return;
-    const size_t out = (size_t)rows[row] * C, pitch = (size_t)n_pad * C;
-    const float f = *scale;
-    for (int c = lane * 4; c < C; c += 128) {
-        const float* from = acc + (size_t)row * C + c;
-        float4 s = *reinterpret_cast<const float4*>(from);
+    const int row = blockIdx.x, c = (blockIdx.y * 128 + threadIdx.x) * 4;
+    if (row >= *n_valid || c >= C) return;
+    const float* from = acc + (size_t)row * C + c;
+    const size_t pitch = (size_t)n_pad * C;
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
-        for (int i = 1; i < slices; ++i) {
-            const float4 o = *reinterpret_cast<const float4*>(from + i * pitch);
-            s.x += o.x; s.y += o.y; s.z += o.z; s.w += o.w;
-        }
-        put_dx(dx, f32, out + c, s, f);
+    for (int i = 0; i < slices; ++i) {
+        const float4 o = *reinterpret_cast<const float4*>(from + i * pitch);
+        s.x += o.x; s.y += o.y; s.z += o.z; s.w += o.w;
     }
+    put_dx(dx, f32, (size_t)rows[row] * C + c, s, *scale);
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------
@@ -989,7 +986,7 @@ int mgpt_moe_op_head_loss_backward(const void* x, int io, const void* w, const i
     }
     if (slices == 1) return 0;
     const int used = (per + p.slice_tiles - 1) / p.slice_tiles;
-    MGPT_CUDA(launch_pdl(head_dx_kernel, (n + 7) / 8, 256, 0, st, k.n_valid, p.scale, p.acc, k.rows, used, h.n_pad, C, dx, p.dx_f32));
+    MGPT_CUDA(launch_pdl(head_dx_kernel, dim3(n, (C + 511) / 512), 128, 0, st, k.n_valid, p.scale, p.acc, k.rows, used, h.n_pad, C, dx, p.dx_f32));
     MGPT_LAUNCHED("head_dx_kernel");
     return 0;
 }
