@@ -35,8 +35,8 @@ constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr uint32_t TMEM_COLS = 2 * TILE;
 constexpr uint32_t STAGING = 4096;                   // per epilogue warp: 32 rows x 128 B
 constexpr int QUEUE = 4;
-constexpr int CLAIM = 6;                             // the next item is claimed this many k-blocks before the last one's loads end
 constexpr int PART = 512 / BK;                       // LOSS: k-blocks summed in one accumulator
+constexpr int CLAIM = 6;                             // GRADS: the next item is claimed this many k-blocks before the last one's loads end
 constexpr int MAX_PIECES = 1024;
 constexpr int COUNTERS = 2 * MAX_PIECES + 2;
 constexpr float LOG2E = 1.4426950408889634f;
@@ -221,34 +221,47 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             const int total = item_count<KIND>(p, n_valid), grid = gridDim.x >> 1;
             const uint32_t lead_full = mapa(full, 0), tile0 = smem_u32(tiles);
             const uint32_t peer_item = mapa(smem_u32(sh.item), 1), peer_item_full = mapa(item_full, 1);
-            int s = 0, item = blockIdx.x >> 1, next = 0;
+            // The logits' items, all alike, are passed on one ahead, so that the peer's loads, which share the leader's barriers, do not wait to
+            // hear of one: a pair's first two are its own by number, those that follow are claimed two ahead (8192 x 512 x 32000: 202 -> 190
+            // us).  The gradients' items are of two lengths and claimed as late as hides the counter (7570 x 312 x 7261: 114 us ahead, 93 so).
+            // Behind the last item come two entries that say so: either group of the epilogue may be the one to read on.
+            constexpr bool AHEAD = KIND != GRADS;
+            int s = 0, after = (blockIdx.x >> 1) + grid, claimed = 0;
             uint32_t free_phase = 1;                        // (the first round finds every stage free)
-            bool ok = true, end = false;
-            for (uint32_t n = 0; ok; ++n) {
+            bool ok = true;
+            auto item_of = [&](int i) {
+                Item w = {-1, 0, 0, 0};
+                if (i < total) w = decode<KIND>(p, n_valid, i);
+                return w;
+            };
+            auto publish = [&](uint32_t n, const Item& w) {
                 const int slot = n % QUEUE;
-                Item w;
+                if (!mbar_wait(item_empty + 8 * slot, ((n / QUEUE) & 1) ^ 1, p.status, ERR_SCHED_WAIT)) return false;
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(&sh.item[slot])), "r"(w.m), "r"(w.n), "r"(w.slice), "r"(w.nkb) : "memory");
+                asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(peer_item + (uint32_t)sizeof(Item) * slot), "r"(w.m), "r"(w.n), "r"(w.slice), "r"(w.nkb) : "memory");
+                mbar_arrive(item_full + 8 * slot);
+                mbar_arrive_cluster(peer_item_full + 8 * slot);             // (release at cluster scope: the item is visible)
+                return true;
+            };
+            Item w, following;
+            if (rank == 0) {
+                w = item_of(blockIdx.x >> 1);
+                ok = publish(0, w);
+            }
+            for (uint32_t n = 0; ok; ++n) {
                 if (rank == 0) {
-                    if (item < total) w = decode<KIND>(p, n_valid, item);
-                    else w.m = -1, w.n = w.nkb = 0, w.slice = end ? -1 : 0;
-                    if (!mbar_wait(item_empty + 8 * slot, ((n / QUEUE) & 1) ^ 1, p.status, ERR_SCHED_WAIT)) break;
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(&sh.item[slot])), "r"(w.m), "r"(w.n), "r"(w.slice), "r"(w.nkb) : "memory");
-                    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(peer_item + (uint32_t)sizeof(Item) * slot), "r"(w.m), "r"(w.n), "r"(w.slice), "r"(w.nkb) : "memory");
-                    mbar_arrive(item_full + 8 * slot);
-                    mbar_arrive_cluster(peer_item_full + 8 * slot);         // (release at cluster scope: the item is visible)
-                    if (w.m < 0) {                              // (twice: either group of the epilogue may be the one to read on)
-                        if (w.slice < 0) break;
-                        end = true;
-                        continue;
+                    if (AHEAD || w.m < 0) {
+                        following = item_of(w.m < 0 ? total : after);
+                        if (!publish(n + 1, following) || w.m < 0) break;
                     }
+                    if (AHEAD || w.nkb <= CLAIM) claimed = p.sched ? atomicAdd(p.sched, 1) : 0;      // (looked at when this item's loads are under way)
                 } else {
                     const bool more = consume(n, w);
                     release(n);
                     if (!more) break;
                 }
-                auto claim = [&]() { next = p.sched ? atomicAdd(p.sched, 1) : item; };       // (the counter starts behind the grid's first items)
-                if (rank == 0 && w.nkb <= CLAIM) claim();
                 for (int kb = 0; kb < w.nkb; ++kb) {
-                    if (rank == 0 && w.nkb - kb == CLAIM + 1) claim();
+                    if (!AHEAD && rank == 0 && w.nkb - kb == CLAIM + 1) claimed = atomicAdd(p.sched, 1);
                     if (!mbar_wait(empty + 8 * s, free_phase, p.status, ERR_EMPTY_WAIT)) {
                         ok = false;
                         break;
@@ -279,7 +292,15 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                         free_phase ^= 1;
                     }
                 }
-                item = grid + next;
+                if (rank == 0) {
+                    if (AHEAD) {
+                        after = p.sched ? 2 * grid + claimed : after + grid;
+                    } else {
+                        following = item_of(grid + claimed);
+                        ok = ok && publish(n + 1, following);
+                    }
+                    w = following;
+                }
             }
         }
     } else if (warp == 1) {
