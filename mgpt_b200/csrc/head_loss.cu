@@ -35,6 +35,7 @@ constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr uint32_t TMEM_COLS = 2 * TILE;
 constexpr uint32_t STAGING = 4096;                   // per epilogue warp: 32 rows x 128 B
 constexpr int QUEUE = 4;
+constexpr int NARROW = 512;                          // LOSS_NARROW up to this C
 constexpr int PART = 512 / BK;                       // LOSS: k-blocks summed in one accumulator
 constexpr int CLAIM = 6;                             // GRADS: the next item is claimed this many k-blocks before the last one's loads end
 constexpr int MAX_PIECES = 1024;
@@ -42,7 +43,8 @@ constexpr int COUNTERS = 2 * MAX_PIECES + 2;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int ST_BAD_TARGET = ST_BAD_EXPERT;         // the status bit of an index outside its range
 
-enum { LOSS = 0, DLOGITS = 1, GRADS = 2 };
+enum { LOSS = 0, DLOGITS = 1, GRADS = 2, LOSS_NARROW = 3 };
+constexpr bool is_loss(int kind) { return kind == LOSS || kind == LOSS_NARROW; }
 
 struct HeadP {
     const int32_t* n_valid;     // null: n tokens, as they lie
@@ -112,11 +114,11 @@ struct __align__(16) Item {
 };
 struct Shared {
     Item item[QUEUE];
-    uint64_t full[6], empty[6], acc_full[2], acc_empty[2], item_full[QUEUE], item_empty[QUEUE], joined[4];
+    uint64_t full[6], empty[6], acc_full[2], acc_empty[2], item_full[QUEUE], item_empty[QUEUE], joined[8][4];
     uint32_t tmem;
 };
-template <int KIND> constexpr int stages() { return KIND == LOSS ? 6 : 5; }
-template <int KIND> constexpr uint32_t extra_bytes() { return KIND == LOSS ? 4 * 4 * 128 * sizeof(float2) : EPI_WARPS * STAGING; }
+template <int KIND> constexpr int stages() { return is_loss(KIND) ? 6 : 5; }
+template <int KIND> constexpr uint32_t extra_bytes() { return is_loss(KIND) ? 4 * 4 * 128 * sizeof(float2) : EPI_WARPS * STAGING; }
 template <int KIND> constexpr uint32_t smem_bytes() { return 1024 + stages<KIND>() * STAGE_BYTES + extra_bytes<KIND>() + sizeof(Shared); }
 static_assert(smem_bytes<LOSS>() <= 232448 && smem_bytes<GRADS>() <= 232448, "shared memory of one CTA");
 
@@ -162,7 +164,7 @@ template <int KIND> __device__ __forceinline__ Item decode(const HeadP& p, int n
 // each.  What a warp of DLOGITS does for an item is a chain of some 6000 cycles (tcgen05.ld, exponentials, shared memory, the copy that has
 // to have left it), of which an item of C = 512 with 4100 cycles of products hides one only half: 1.3 % of the gradients' time where the
 // power limit sets the clock, 6 % where it does not.  The loss is 2 % slower in groups: it gives the accumulator back at once.
-template <int KIND> constexpr int item_warps() { return KIND == DLOGITS ? EPI_WARPS / 2 : EPI_WARPS; }
+template <int KIND> constexpr int item_warps() { return KIND == DLOGITS || KIND == LOSS_NARROW ? EPI_WARPS / 2 : EPI_WARPS; }
 
 template <int KIND>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
@@ -191,7 +193,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             mbar_init(item_full + 8 * i, 1);
             mbar_init(item_empty + 8 * i, 2 * ITEM_WARPS + 2);      // the leader's: the epilogue, its MMA thread, the peer's producer
         }
-        for (int q = 0; q < 4; ++q) mbar_init(smem_u32(&sh.joined[q]), 4);
+        for (int q = 0; q < 32; ++q) mbar_init(smem_u32(&sh.joined[q >> 2][q & 3]), ITEM_WARPS / 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) tmem_alloc_pair(smem_u32(&sh.tmem), TMEM_COLS);
@@ -356,20 +358,23 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         // TMEM lane quarter q, the h-th of the warps that share its columns
         const int q = warp & 3, group = (warp - 2) / ITEM_WARPS, h = (warp - 2) % ITEM_WARPS >> 2;
         uint8_t* const stage = extra + (warp - 2) * STAGING;
-        const uint32_t acc_free = mapa(acc_empty, 0), joined = smem_u32(&sh.joined[q]);
+        const uint32_t acc_free = mapa(acc_empty, 0), joined = smem_u32(sh.joined[group * 4 + q]);
         uint32_t t = 0;
         Item w, before = {};
         uint32_t k = 0;                                     // items of the group so far
-        float2* const sums = reinterpret_cast<float2*>(extra) + q * 32 + lane;
+        constexpr int SHARERS = ITEM_WARPS / 4;             // warps of a lane quarter
+        float2* const sums = reinterpret_cast<float2*>(extra) + group * 4 * SHARERS * 128 + q * 32 + lane;      // [4 items][SHARERS][128 rows]
         auto join = [&](uint32_t k, const Item& of) {
-            if (!mbar_wait(joined, k & 1, p.status, ERR_ACC_WAIT)) return false;
-            float2 o[4];
+            if (!mbar_wait(joined + 8 * (k & 3), k >> 2 & 1, p.status, ERR_ACC_WAIT)) return false;
+            float2 o[SHARERS];
+            float m = -INFINITY, all = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = sums[(k & 3) * 512 + i * 128];
-            const float m = fmaxf(fmaxf(o[0].x, o[1].x), fmaxf(o[2].x, o[3].x));
-            float all = 0.0f;
+            for (int i = 0; i < SHARERS; ++i) {
+                o[i] = sums[((k & 3) * SHARERS + i) * 128];
+                m = fmaxf(m, o[i].x);
+            }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) all = fmaf(o[i].y, shift(o[i].x, m), all);
+            for (int i = 0; i < SHARERS; ++i) all = fmaf(o[i].y, shift(o[i].x, m), all);
             const int row = of.m * TILE + rank * 128 + q * 32 + lane;
             if (row < n_valid) p.part[(size_t)of.n * p.n_pad + row] = make_float2(m, all);
             return true;
@@ -398,61 +403,71 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             const int at = real ? p.target[row] - v : -1;
             const float up = KIND == DLOGITS && real ? p.d_loss[row] : 0.0f, lse = KIND == DLOGITS && real ? p.lse[row] : 0.0f;
             if (!empty_sum && !next_acc()) break;
-            if (KIND == LOSS) {
-                float z[64];
-                {
-                    float (&z0)[32] = *reinterpret_cast<float (*)[32]>(z), (&z1)[32] = *reinterpret_cast<float (*)[32]>(z + 32);
-                    tmem_ld32(t_lane, z0);
-                    tmem_ld32(t_lane + 32, z1);
-                }
-                tmem_ld_wait();
-                give_back();
+            if (is_loss(KIND)) {
+                float top = -INFINITY, sum = 0.0f;
                 bool ok = true;
-                for (int kb = PART; kb < w.nkb && (ok = next_acc()); kb += PART) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        float o[16];
-                        tmem_ld16(t_lane + 16 * c, o);
-                        tmem_ld_wait();
-                        if (c == 3) give_back();
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) z[16 * c + j] += o[j];
+                for (int u = 0; u < UNITS; ++u) {
+                    const int valid = p.V - v - u * 64, a = at - u * 64;
+                    float z[64];
+                    {
+                        float (&z0)[32] = *reinterpret_cast<float (*)[32]>(z), (&z1)[32] = *reinterpret_cast<float (*)[32]>(z + 32);
+                        tmem_ld32(t_lane + u * 64, z0);
+                        tmem_ld32(t_lane + u * 64 + 32, z1);
                     }
+                    tmem_ld_wait();
+                    if (u + 1 == UNITS) give_back();
+                    if (KIND == LOSS) {
+                        for (int kb = PART; kb < w.nkb && (ok = next_acc()); kb += PART) {
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                float o[16];
+                                tmem_ld16(t_lane + 16 * c, o);
+                                tmem_ld_wait();
+                                if (c == 3) give_back();
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) z[16 * c + j] += o[j];
+                            }
+                        }
+                        if (!ok) break;
+                    }
+                    if (valid < 64) {
+#pragma unroll
+                        for (int j = 0; j < 64; ++j)
+                            if (j >= valid) z[j] = -INFINITY;
+                    }
+                    if (__any_sync(0xffffffffu, (a >> 6) == 0)) {           // a target in these columns: rare
+                        float zt = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 64; ++j)
+                            if (a == j) zt = z[j];
+                        if ((a >> 6) == 0) p.z_target[row] = zt;
+                    }
+                    float t4[4] = {fmaxf(z[0], top), z[1], z[2], z[3]};
+#pragma unroll
+                    for (int j = 4; j < 64; ++j) t4[j & 3] = fmaxf(t4[j & 3], z[j]);
+                    const float m = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+                    const F2 ref(m == -INFINITY ? 0.0f : -m * LOG2E);               // (columns beyond the vocabulary alone)
+                    F2 s2[2] = {F2(u ? sum * shift(top, m) : 0.0f, 0.0f), F2(0.0f)};
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const F2 e = fma2(F2(z[2 * j], z[2 * j + 1]), F2(LOG2E), ref);
+                        s2[j & 1] = s2[j & 1] + F2(ex2(e.lo()), ex2(e.hi()));
+                    }
+                    const F2 both = s2[0] + s2[1];
+                    sum = both.lo() + both.hi();
+                    top = m;
                 }
                 if (!ok) break;
-                const int valid = p.V - v;
-                if (valid < 64) {
-#pragma unroll
-                    for (int j = 0; j < 64; ++j)
-                        if (j >= valid) z[j] = -INFINITY;
-                }
-                if (__any_sync(0xffffffffu, (at >> 6) == 0)) {      // a target in these columns: rare
-                    float zt = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 64; ++j)
-                        if (at == j) zt = z[j];
-                    if ((at >> 6) == 0) p.z_target[row] = zt;
-                }
-                float t4[4] = {z[0], z[1], z[2], z[3]};
-#pragma unroll
-                for (int j = 4; j < 64; ++j) t4[j & 3] = fmaxf(t4[j & 3], z[j]);
-                const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-                const F2 ref(top == -INFINITY ? 0.0f : -top * LOG2E);       // (columns beyond the vocabulary alone)
-                F2 s2[2] = {F2(0.0f), F2(0.0f)};
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const F2 e = fma2(F2(z[2 * j], z[2 * j + 1]), F2(LOG2E), ref);
-                    s2[j & 1] = s2[j & 1] + F2(ex2(e.lo()), ex2(e.hi()));
-                }
-                const F2 sum = s2[0] + s2[1];
-                // The four warps of a lane quarter join their columns, in turn, an item later, so that none waits for another.  (A warp
-                // joins item k - 1 before it has arrived for k, which therefore is the barrier's phase.  Four buffers: who writes item
-                // k + 3 has met the accumulator that the joining warp gave back at k + 1, after it had read item k - 1.)
-                if (k > 0 && h == (int)((k - 1) & 3) && !join(k - 1, before)) break;
+                // The warps of a lane quarter join their columns, in turn, an item later, so that none waits for another.  Four barriers and
+                // buffers, for items k, k + 1 ..: a warp that arrives for item k + 4 has met an accumulator that every other warp gave back
+                // at item k + 2 (k + 3 in groups) or later, after it had arrived for k + 1 and, if it was the one to join k, had read
+                // it.  (With one barrier a warp that is an item ahead arrives twice where another has not yet.)
+                if (k > 0 && h == (int)((k - 1) & (SHARERS - 1)) && !join(k - 1, before)) break;
                 before = w;
-                sums[(k & 3) * 512 + h * 128] = make_float2(top, sum.lo() + sum.hi());
+                sums[((k & 3) * SHARERS + h) * 128] = make_float2(top, sum);
                 __syncwarp();
-                if (lane == 0) mbar_arrive(joined);
+                if (lane == 0) mbar_arrive(joined + 8 * (k & 3));
             } else if (KIND == DLOGITS) {
                 const F2 ref(-lse * LOG2E), up2(up);        // (rows behind the last token: logits 0, up 0)
                 const uint32_t line = smem_u32(stage) + lane * 128;
@@ -585,7 +600,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 }
             }
         }
-        if (KIND == LOSS && k > 0 && h == (int)((k - 1) & 3)) join(k - 1, before);
+        if (is_loss(KIND) && k > 0 && h == (int)((k - 1) & (SHARERS - 1))) join(k - 1, before);
         if (KIND == DLOGITS && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     // neither CTA may leave (or give its TMEM back) while the other can still read its shared memory or signal it
@@ -912,7 +927,7 @@ int mgpt_moe_op_head_loss(const void* x, int io, const void* w, const int32_t* t
     int sms;
     MGPT_TRY(sm_count(&sms));
     CUtensorMap mx, mw, mx0;
-    const bool direct = io == MGPT_MOE_IO_BF16, packed = !direct || n > TILE;
+    const bool packed = io != MGPT_MOE_IO_BF16 || n > TILE, direct = io == MGPT_MOE_IO_BF16 && (C % 16 == 0 || !packed);
     MGPT_TRY(make_map_kind(&mx, ws + h.xp, h.n_pad, h.Cp, 128, false));
     MGPT_TRY(make_map_kind(&mw, w, V, C, 128, false));
     if (direct) MGPT_TRY(make_map_kind(&mx0, x, n, C, 128, false));
@@ -929,7 +944,9 @@ int mgpt_moe_op_head_loss(const void* x, int io, const void* w, const int32_t* t
     p.group = group_of(h.n_pad, h.Cp); p.n_pad = h.n_pad; p.target = packed ? k.target : targets;
     p.part = (float2*)(ws + h.part); p.z_target = (float*)(ws + h.z_target);
     const long items = (long)(h.n_pad / TILE) * h.v_tiles;
-    MGPT_TRY(launch_head<LOSS>(mx, mw, mx, mw, direct ? mx0 : mx, p, (int)(items < sms / 2 ? items : sms / 2), st));
+    const int pairs = (int)(items < sms / 2 ? items : sms / 2);
+    if (C <= NARROW) MGPT_TRY(launch_head<LOSS_NARROW>(mx, mw, mx, mw, direct ? mx0 : mx, p, pairs, st));
+    else MGPT_TRY(launch_head<LOSS>(mx, mw, mx, mw, direct ? mx0 : mx, p, pairs, st));
     const int32_t* as_given = packed ? nullptr : targets;
     if (n < 32 * sms) MGPT_CUDA(launch_pdl(head_join_kernel<16>, (n + 31) / 32, 512, 0, st, p.n_valid, p.part, p.z_target, k.rows, as_given, n, V, h.n_pad, loss, lse, status));
     else MGPT_CUDA(launch_pdl(head_join_kernel<4>, (n + 31) / 32, 128, 0, st, p.n_valid, p.part, p.z_target, k.rows, as_given, n, V, h.n_pad, loss, lse, status));
@@ -968,7 +985,7 @@ int mgpt_moe_op_head_loss_backward(const void* x, int io, const void* w, const i
     int sms;
     MGPT_TRY(sm_count(&sms));
     CUtensorMap mx, mw, mx_t, mw_t, mz, mz_t, mx0, mx0_t;
-    const bool direct = io == MGPT_MOE_IO_BF16;
+    const bool direct = io == MGPT_MOE_IO_BF16 && C % 16 == 0;
     MGPT_TRY(make_map_kind(&mx, ws + h.xp, h.n_pad, h.Cp, 128, false));
     MGPT_TRY(make_map_kind(&mw, w, V, C, 128, false));
     MGPT_TRY(make_map_kind(&mx_t, ws + h.xp, h.n_pad, h.Cp, 64, false));
@@ -988,7 +1005,7 @@ int mgpt_moe_op_head_loss_backward(const void* x, int io, const void* w, const i
     k.direct = direct; k.status = status; k.lse_in = lse; k.d_loss_in = d_loss; k.lse_p = (float*)(ws + h.lse); k.d_loss_p = (float*)(ws + h.d_loss); k.scale = (float*)(ws + h.scale); k.dx = dx;
     MGPT_TRY(launch_pack<true>(k, io, st));
     HeadP p = {};
-    p.n_valid = k.n_valid; p.n = n; p.direct = direct; p.rows = k.rows; p.dx = dx; p.dx_f32 = !direct; p.status = status; p.C = C; p.V = V; p.group = group_of(h.n_pad, h.Cp); p.n_pad = h.n_pad;
+    p.n_valid = k.n_valid; p.n = n; p.direct = direct; p.rows = k.rows; p.dx = dx; p.dx_f32 = io == MGPT_MOE_IO_F32; p.status = status; p.C = C; p.V = V; p.group = group_of(h.n_pad, h.Cp); p.n_pad = h.n_pad;
     p.target = k.target; p.lse = k.lse_p; p.d_loss = k.d_loss_p; p.scale = k.scale; p.dz = (bf16*)(ws + h.dz); p.acc = (float*)(ws + h.acc);
     p.c_tiles = h.c_tiles; p.dw = dw; p.dw_f32 = dw_dtype == MGPT_MOE_IO_F32;
     for (int i = 0; i < pieces; ++i) {
