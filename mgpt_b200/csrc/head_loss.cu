@@ -49,6 +49,7 @@ constexpr bool is_loss(int kind) { return kind == LOSS || kind == LOSS_NARROW; }
 struct HeadP {
     const int32_t* n_valid;     // null: n tokens, as they lie
     int n;                      // of the call
+    int few[2];                 // without n_valid: rows of x that each CTA of a pair loads, at most 128; the other rows are never looked at
     int direct;                 // x has the operand type: where no token is left out, it is read as it lies
     int32_t* sched;             // next item; zero before the launch (null: items by stride)
     int32_t* status;
@@ -205,6 +206,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     pdl_wait();
     const int n_valid = p.n_valid ? *p.n_valid : p.n;
     const bool as_it_lies = p.direct && n_valid == p.n;
+    const int x_rows0 = p.n_valid ? 128 : p.few[0], x_rows1 = p.n_valid ? 128 : p.few[1];
     const float scale = KIND == GRADS ? *p.scale : 1.0f;
 
     const uint32_t lead_item_empty = mapa(item_empty, 0);
@@ -269,9 +271,11 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                         break;
                     }
                     const uint32_t a_dst = tile0 + s * STAGE_BYTES, b_dst = a_dst + OPER_BYTES, bar = lead_full + 8 * s;
-                    if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * STAGE_BYTES);       // both CTAs' bytes
+                    if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * OPER_BYTES + (x_rows0 + x_rows1) * (BK * 2));       // both CTAs' bytes
                     if (KIND != GRADS) {
-                        tma_load_2d_pair(a_dst, as_it_lies ? &tmX : &tmA, kb * BK, w.m * TILE + rank * 128, bar);
+                        // (one tile of tokens: tmX has the leader's rows, tmA the peer's)
+                        if ((rank == 0 ? x_rows0 : x_rows1) > 0)
+                            tma_load_2d_pair(a_dst, as_it_lies && (p.n_valid || rank == 0) ? &tmX : &tmA, kb * BK, w.m * TILE + rank * 128, bar);
                         tma_load_2d_pair(b_dst, &tmB, kb * BK, p.v0 + w.n * TILE + rank * 128, bar);
                     } else {
                         const int blocks = p.v_tiles * (TILE / 64), col = w.n * TILE + rank * w.half(p.C), k0 = w.slice * p.slice_tiles * (TILE / BK);
@@ -835,6 +839,10 @@ int check_shape(int n, int C, int V, int io)
         return fail(MGPT_MOE_EINVAL, "head loss: sizes out of range");
     return 0;
 }
+// Whether x is read where it lies rather than from a packed copy, if no token is left out.  Rows off 32-byte boundaries cost two sectors
+// for one (4740 x 296 x 65753: 227 us, 168 at C = 288), boxes that reach beyond the last token as much as full ones and more (3 tokens of
+// 1376 channels, gradient of the logits: 45 us, 37 from the copy); a copy of few tokens costs nothing.
+bool as_it_lies(int n, int C, int io) { return io == MGPT_MOE_IO_BF16 && C % 16 == 0 && (n % TILE == 0 || n >= 8 * TILE); }
 // token tiles whose x (and dz) share the L2 with a vocabulary tile
 int group_of(int n_pad, int Cp)
 {
@@ -927,10 +935,14 @@ int mgpt_moe_op_head_loss(const void* x, int io, const void* w, const int32_t* t
     int sms;
     MGPT_TRY(sm_count(&sms));
     CUtensorMap mx, mw, mx0;
-    const bool packed = io != MGPT_MOE_IO_BF16 || n > TILE, direct = io == MGPT_MOE_IO_BF16 && (C % 16 == 0 || !packed);
+    const bool packed = io != MGPT_MOE_IO_BF16 || n > TILE, direct = !packed || as_it_lies(n, C, io);
     MGPT_TRY(make_map_kind(&mx, ws + h.xp, h.n_pad, h.Cp, 128, false));
     MGPT_TRY(make_map_kind(&mw, w, V, C, 128, false));
-    if (direct) MGPT_TRY(make_map_kind(&mx0, x, n, C, 128, false));
+    // One tile of tokens: only the rows that there are (a box that reaches beyond them is slower than one that is full: 3 tokens of
+    // 1376 channels against 208764 vocabulary rows 153 us, 200 tokens 113).
+    const int few[2] = {n < 128 ? (int)up(n, 8) : 128, n <= 128 ? 0 : (int)up(n - 128, 8)};
+    if (direct) MGPT_TRY(make_map_kind(&mx0, x, n, C, packed ? 128 : few[0], false));
+    if (!packed && few[1]) MGPT_TRY(make_map_kind(&mx, x, n, C, few[1], false));
     PackP k = {};
     k.x = x; k.targets = targets; k.n = n; k.C = C; k.Cp = h.Cp; k.V = V; k.n_pad = h.n_pad; k.direct = direct;
     k.n_valid = (int32_t*)(ws + h.counters);
@@ -939,7 +951,7 @@ int mgpt_moe_op_head_loss(const void* x, int io, const void* w, const int32_t* t
     // one tile of tokens costs the same with or without those that take no part: no need to sort them out
     if (packed) MGPT_TRY(launch_pack<false>(k, io, st));
     HeadP p = {};
-    p.n_valid = packed ? k.n_valid : nullptr; p.n = n; p.direct = direct; p.sched = packed ? k.n_valid + 1 : nullptr;
+    p.n_valid = packed ? k.n_valid : nullptr; p.n = n; p.few[0] = few[0]; p.few[1] = few[1]; p.direct = direct; p.sched = packed ? k.n_valid + 1 : nullptr;
     p.status = status; p.C = C; p.V = V; p.v_tiles = h.v_tiles;
     p.group = group_of(h.n_pad, h.Cp); p.n_pad = h.n_pad; p.target = packed ? k.target : targets;
     p.part = (float2*)(ws + h.part); p.z_target = (float*)(ws + h.z_target);
@@ -985,7 +997,7 @@ int mgpt_moe_op_head_loss_backward(const void* x, int io, const void* w, const i
     int sms;
     MGPT_TRY(sm_count(&sms));
     CUtensorMap mx, mw, mx_t, mw_t, mz, mz_t, mx0, mx0_t;
-    const bool direct = io == MGPT_MOE_IO_BF16 && C % 16 == 0;
+    const bool direct = as_it_lies(n, C, io);
     MGPT_TRY(make_map_kind(&mx, ws + h.xp, h.n_pad, h.Cp, 128, false));
     MGPT_TRY(make_map_kind(&mw, w, V, C, 128, false));
     MGPT_TRY(make_map_kind(&mx_t, ws + h.xp, h.n_pad, h.Cp, 64, false));
