@@ -875,9 +875,12 @@ int launch_head(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& a
 }
 int sm_count(int* sms)
 {
+    static int known[64];
     int dev = 0;
     MGPT_CUDA(cudaGetDevice(&dev));
-    MGPT_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+    *sms = dev < 64 ? known[dev] : 0;
+    if (!*sms) MGPT_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+    if (dev < 64) known[dev] = *sms;
     if (*sms < 2) return fail(MGPT_MOE_ECUDA, "head loss: needs two SMs");
     return 0;
 }

@@ -89,16 +89,12 @@ def check_status(device=None) -> None:
 
 # ---- the loss of a language model's head ------------------------------------------------------------------------------
 def _head_args(x, weight, targets):
-    device = _device(x)
-    _need(x.dim() >= 1 and weight.dim() == 2, "head loss: x is [..., C], weight [V, C]")
-    _need(x.dtype in _DTYPES, f"head loss: unsupported token dtype {x.dtype}")
-    V, C = weight.shape
-    _need(V > 0 and C > 0 and x.shape[-1] == C, f"head loss: x is {tuple(x.shape)}, weight {tuple(weight.shape)}")
-    n = x.numel() // C
-    xp = _check(x, "x", x.shape, (x.dtype,), device)
-    wp = _check(weight, "weight", (V, C), _BF16, device)
-    tp = _check(targets, "targets", x.shape[:-1], _I32, device)
-    return device, n, C, V, xp, wp, tp
+    device, dtype, shape, matrix = _device(x), x.dtype, x.shape, weight.shape
+    if dtype not in _DTYPES or not shape or len(matrix) != 2 or not matrix[0] or not matrix[1] or shape[-1] != matrix[1]:
+        raise MoeError(f"head loss: x is [..., C] of FP32 or BF16, weight [V, C]; got {tuple(shape)} of {dtype}, {tuple(matrix)}")
+    V, C = matrix
+    return (device, x.numel() // C, C, V, _check(x, "x", shape, _EITHER, device), _check(weight, "weight", matrix, _BF16, device),
+            _check(targets, "targets", shape[:-1], _I32, device))
 
 
 def head_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor):
@@ -109,7 +105,7 @@ def head_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor):
     take no part: loss and lse 0, and no work; targets ``>= V`` are reported by :func:`check_status`."""
     lib = _lib.load()
     device, n, C, V, xp, wp, tp = _head_args(x, weight, targets)
-    loss, lse = torch.empty(targets.shape, dtype=torch.float32, device=device), torch.empty(targets.shape, dtype=torch.float32, device=device)
+    loss, lse = torch.empty_like(targets, dtype=torch.float32), torch.empty_like(targets, dtype=torch.float32)
     if n:
         size = lib.mgpt_moe_op_head_loss_workspace_bytes(n, C, V)
         ws = _workspace(size, device)
