@@ -16,6 +16,7 @@
 //
 // An element whose new moments are not finite (its gradient is not, or overflows) keeps w, m and v, and sets the caller's flag.
 #include <cmath>
+#include <cstring>
 #include <memory>
 
 #include <cuda_fp8.h>
@@ -161,9 +162,9 @@ __global__ void __launch_bounds__(32 * WARPS, 2) optim_kernel(const OptP p)
             if (in) return i + __ffs(in) - 1;
         }
     };
-    if (b0 + warp < b1) {
-        ahead = here = find(b0 + warp, start);
-        to_fetch(ahead);
+    if (b0 + warp < b1) {                                           // (a run's first block and most of the others: the tensor is known)
+        to_fetch(start);
+        if (b0 + warp >= fend) to_fetch(ahead = here = find(b0 + warp, start + 1));
         to_work(here);
     }
     auto fetch = [&](int b, int s) {
@@ -434,8 +435,10 @@ int mgpt_moe_optim_create(int device, const mgpt_moe_optim_tensor* tensors, int 
         }
         const size_t tb = ts.size() * sizeof(OptTensor), ib = ints.size() * sizeof(int);
         cudaError_t e = cudaMalloc(&o->tables, tb + ib + 16);
-        if (e == cudaSuccess && tb) e = cudaMemcpy(o->tables, ts.data(), tb, cudaMemcpyHostToDevice);
-        if (e == cudaSuccess && ib) e = cudaMemcpy((char*)o->tables + tb, ints.data(), ib, cudaMemcpyHostToDevice);
+        std::vector<char> table(tb + ib);
+        if (tb) memcpy(table.data(), ts.data(), tb);
+        if (ib) memcpy(table.data() + tb, ints.data(), ib);
+        if (e == cudaSuccess && tb + ib) e = cudaMemcpy(o->tables, table.data(), tb + ib, cudaMemcpyHostToDevice);
         if (e == cudaSuccess) e = state_bits == 8 ? cudaFuncSetAttribute(optim_kernel<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<8>())
                                                   : cudaFuncSetAttribute(optim_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<32>());
         if (e != cudaSuccess) {

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as ct
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -18,6 +19,7 @@ STATE_BLOCK = 256               # elements that share a scale of the 8-bit momen
 
 _DTYPES = {torch.float32: IO_F32, torch.bfloat16: IO_BF16}
 _F32, _BF16, _I32, _EITHER = (torch.float32,), (torch.bfloat16,), (torch.int32,), (torch.float32, torch.bfloat16)
+_TENSOR = np.dtype([("w", "u8"), ("grad", "u8"), ("w_bf16", "u8"), ("n", "i8"), ("weight_decay", "f4"), ("grad_dtype", "i4")])      # mgpt_moe_optim_tensor
 _status = {}
 
 
@@ -215,12 +217,16 @@ class AdamW:
         _need(len(decay) == n, "AdamW: one weight decay, or one per tensor")
         _need(state_bits in (8, 32), "AdamW: state_bits must be 8 or 32")
         self.device, self.state_bits, self.seed = _device(self.weights[0]), state_bits, int(seed) & 0xFFFFFFFF
-        table = (_lib.OptimTensor * n)()
+        table = np.zeros(n, dtype=_TENSOR)
+        device, f32, b16 = self.device, torch.float32, torch.bfloat16
         for i, (w, g, c) in enumerate(zip(self.weights, self.grads, self.copies)):
-            wp = _check(w, f"weights[{i}]", w.shape, _F32, self.device)
-            gp = _check(g, f"grads[{i}]", w.shape, _EITHER, self.device)
-            cp = _optional(c, f"copies[{i}]", w.shape, _BF16, self.device)
-            table[i] = _lib.OptimTensor(wp, gp, cp, w.numel(), decay[i], _DTYPES[g.dtype])
+            shape, gd = w.shape, g.dtype
+            if not (w.dtype is f32 and (gd is f32 or gd is b16) and g.shape == shape and w.is_contiguous() and g.is_contiguous() and w.device == device == g.device
+                    and (c is None or (c.dtype is b16 and c.shape == shape and c.is_contiguous() and c.device == device))):
+                for t, name, dtypes in ((w, "weights", _F32), (g, "grads", _EITHER), (c, "copies", _BF16)):
+                    _optional(t, f"{name}[{i}]", shape, dtypes, device)
+            table[i] = (w.data_ptr(), g.data_ptr(), 0 if c is None else c.data_ptr(), w.numel(), decay[i], _DTYPES[gd])
+        table = table.ctypes.data_as(ct.POINTER(_lib.OptimTensor))
         self.blocks = int(self.lib.mgpt_moe_optim_blocks(table, n))
         total, dtype = self.blocks * STATE_BLOCK, torch.float32 if state_bits == 32 else torch.float8_e4m3fn
         if state is None:
