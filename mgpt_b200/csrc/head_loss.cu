@@ -850,13 +850,16 @@ int group_of(int n_pad, int Cp)
     const int mt = n_pad / TILE, g = (int)(most / tile);
     return g < 1 ? 1 : g > mt ? mt : g;
 }
-// Slices of the vocabulary that dx is summed in: as many as give every pair of SMs an item where the tokens are few.
+// Slices of the vocabulary that dx is summed in.  dx and dw are the same work, so of the 74 pairs' shares half is dx: 60 items are
+// enough for none to be more than two thirds of a share, and more only cost sums.  us, both products and the sum of the slices, at
+// 148 / 74 / 37 items: 1 of 3 tokens, 1376 x 52191 83 / 79 / 76; 300 tokens, 488 x 37571 45 / 40 / 40; 8192 tokens, 512 x 32000
+// 390 / 388 / 366 (one slice); 1501 of 3001 tokens, 1024 x 50021, half of whose items turn out not to exist 234 / 224 / 275 (one).
 int slices_of(int n_pad, int c_tiles, int v_tiles)
 {
     const int items = n_pad / TILE * c_tiles;
-    int s = (2 * 74 + items - 1) / items;
+    int s = (60 + items - 1) / items;
     if (s > v_tiles / 4) s = v_tiles / 4;
-    return items >= 74 || s < 1 ? 1 : s;
+    return s < 1 ? 1 : s;
 }
 
 template <int KIND>
