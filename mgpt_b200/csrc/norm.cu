@@ -390,15 +390,16 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
     }
 }
 
-// The units' sums into the parameters' gradients: 32 columns per block, eight warps that share the units of a row, or the
-// rows where there are eight or more.  Sums are taken in a fixed order.
-__global__ void __launch_bounds__(256)
+// The units' sums into the parameters' gradients: 32 columns per block, PW warps that share the units of a row, or the rows where
+// there are as many.  Sums are taken in a fixed order.
+constexpr int PW = 16;
+__global__ void __launch_bounds__(32 * PW)
 norm_params_kernel(const float* part, const float* post, const float* gate, int C, int n_gate, int splits, float* d_post, float* d_gate, float* d_pre)
 {
     pdl_wait();
-    __shared__ float sh[8][32];
+    __shared__ float sh[PW][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
-    const bool in = c < C, by_row = n_gate >= 8;
+    const bool in = c < C, by_row = n_gate >= PW;
     const float a = post && in ? post[c] : 1.0f;
     auto joined = [&](float v) {                            // over the warps; every thread calls it
         __syncthreads();
@@ -406,15 +407,15 @@ norm_params_kernel(const float* part, const float* post, const float* gate, int 
         __syncthreads();
         float t = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) t += sh[i][lane];
+        for (int i = 0; i < PW; ++i) t += sh[i][lane];
         return t;
     };
     float dp = 0.0f, db = 0.0f;
-    for (int row = by_row ? warp : 0; row < n_gate; row += by_row ? 8 : 1) {
+    for (int row = by_row ? warp : 0; row < n_gate; row += by_row ? PW : 1) {
         float s = 0.0f;
         if (in)
-#pragma unroll 4
-            for (int i = by_row ? 0 : warp; i < splits; i += by_row ? 1 : 8) {
+#pragma unroll 8
+            for (int i = by_row ? 0 : warp; i < splits; i += by_row ? 1 : PW) {
                 const float* from = part + (size_t)(row * splits + i) * 2 * C + c;
                 s += from[0];
                 db += from[C];
@@ -581,7 +582,7 @@ int mgpt_moe_op_residual_norm_backward(const void* x, const void* h, int io, con
     cudaStream_t st = (cudaStream_t)stream;
     MGPT_TRY(io == MGPT_MOE_IO_BF16 ? run_bwd<bf16>(p, units, st) : run_bwd<float>(p, units, st));
     if (!sums) return 0;
-    MGPT_CUDA(launch_pdl(norm_params_kernel, (C + 31) / 32, 256, 0, st, p.part, post_scale, gate, C, rows, s.splits, d_post_scale, d_gate, d_pre_scale));
+    MGPT_CUDA(launch_pdl(norm_params_kernel, (C + 31) / 32, 32 * PW, 0, st, p.part, post_scale, gate, C, rows, s.splits, d_post_scale, d_gate, d_pre_scale));
     MGPT_LAUNCHED("norm_params_kernel");
     return 0;
 }
