@@ -47,7 +47,7 @@ struct OptTensor {
     int block0, block1;                 // its first block, and the one after its last
     float decay;
     int g_bf16;
-    int vec;                            // all of them start on a boundary that four elements can be moved at
+    int vec;                            // w and the gradient start on 16-byte boundaries, the copy on one of 8: whole blocks go in pieces
 };
 struct OptP {
     const OptTensor* tensors;           // those with elements, in order
@@ -409,7 +409,7 @@ int mgpt_moe_optim_create(int device, const mgpt_moe_optim_tensor* tensors, int 
             if (!blocks) continue;
             OptTensor t;
             t.w = s.w; t.g = s.grad; t.copy = (bf16*)s.w_bf16; t.n = s.n; t.block0 = (int)block; t.block1 = (int)(block + blocks); t.decay = s.weight_decay; t.g_bf16 = gb;
-            t.vec = !((uintptr_t)s.w & 15) && !((uintptr_t)s.grad & (gb ? 7 : 15)) && !((uintptr_t)s.w_bf16 & 7);
+            t.vec = !((uintptr_t)s.w & 15) && !((uintptr_t)s.grad & 15) && !((uintptr_t)s.w_bf16 & 7);
             ts.push_back(t);
             block += blocks;
             if (block >= (1L << 31) - 65536) return fail(MGPT_MOE_EINVAL, "optimiser: too many elements");

@@ -198,6 +198,28 @@ def test_scaled_gradients_and_same_bits_again():
             assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
 
 
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("offset", [1, 2, 4, 8])
+@pytest.mark.parametrize("which", ["weights", "grads", "copies"])
+def test_boundaries_do_not_matter(bits, offset, which):
+    """One of a tensor's three buffers off its boundary by 1, 2, 4 or 8 elements, the others on theirs: the same bits."""
+    sizes = [2048, 300, 4096]
+
+    def run(shift):
+        t = dict(zip(("weights", "grads", "copies"), _tensors(sizes, torch.bfloat16, seed=11)))
+        if shift:
+            moved = [torch.empty(a.numel() + shift, dtype=a.dtype, device="cuda")[shift:] for a in t[which]]
+            for a, b in zip(moved, t[which]):
+                a.copy_(b)
+            t[which] = moved
+        opt = AdamW(t["weights"], t["grads"], copies=t["copies"], state_bits=bits, seed=3)
+        for step in (1, 2):
+            opt.step(step, **HYPER)
+        return [a.clone() for a in t["weights"] + t["copies"]] + [opt.m.float(), opt.v.float()]
+
+    assert all(torch.equal(a, b) for a, b in zip(run(0), run(offset)))
+
+
 def test_other_seed_other_rounding_and_continued_state():
     def run(seed, steps, state=None, t0=0):
         w, g, _ = _tensors([4096], seed=5)
