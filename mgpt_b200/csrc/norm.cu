@@ -331,7 +331,8 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
         }
         float s[3] = {s0.lo() + s0.hi(), s1.lo() + s1.hi(), s2.lo() + s2.hi()};
         group_sum<3, W>(s, sh, turn);
-        const float mA = s[0] * inv, mB = p.post ? (s[1] - r2 * mA * s[2]) * inv : 0.0f;
+        // (without u the last sum has y itself in it, and may overflow where nothing of it is wanted)
+        const float mA = s[0] * inv, mB = p.post ? (with_u ? s[1] - r2 * mA * s[2] : s[1]) * inv : 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (gt + i * GT) * E;

@@ -109,6 +109,21 @@ def test_rows_of_zeros_and_rows_that_are_not_finite():
     assert dx[3].isfinite().all() and dh[3].isfinite().all() and dx[fine].isfinite().all()
 
 
+def test_large_residuals_without_a_second_norm():
+    """x near the largest number: y is finite, and the gradients, in which x is not, are what they are with a small x."""
+    n, C = 9, 512
+    x, h, dy, _, a = _inputs(n, C, torch.float32, 4, pre=False, seed=8)
+    h.abs_()
+    a["gate"].fill_(1.0)
+    x.fill_(1e38)
+    y, _, stats = mgpt_b200.residual_norm(x, h, **a)
+    assert y.isfinite().all()
+    _, _, g = _reference(x, h, dy, None, a)
+    dx, dh = mgpt_b200.residual_norm_backward(x, h, stats, dy, **a)
+    _near(dx, g["x"], 80, "dx")
+    _near(dh, g["h"], 160, "dh")
+
+
 def test_gradients_against_differences():
     """In 64 bits: the loss <y, dy> + <u, du> at parameters +- s of a direction, against the gradients' products with it."""
     n, C, per = 12, 64, 5
