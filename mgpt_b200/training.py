@@ -240,6 +240,7 @@ class AdamW:
                    _optional(self.m_scale, "m_scale", (self.blocks,), _F32, self.device),
                    _optional(self.v_scale, "v_scale", (self.blocks,), _F32, self.device)]
         self.found_nonfinite = torch.zeros(1, dtype=torch.int32, device=self.device)
+        torch.cuda.current_stream(self.device).synchronize()       # cleared before a step on any stream reads them
         _lib.check(self.lib.mgpt_moe_optim_create(self.device.index, table, n, state_bits, ct.byref(self._h)))
 
     def step(self, t: int, lr: float = 3e-4, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8, grad_scale: torch.Tensor = None) -> None:

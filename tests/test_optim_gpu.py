@@ -236,6 +236,25 @@ def test_other_seed_other_rounding_and_continued_state():
     assert torch.equal(a[0].float(), c[0].float()) and torch.equal(a[1].float(), c[1].float())
 
 
+def test_made_on_one_stream_stepped_on_another():
+    """The moments are cleared on the stream that the object is made on, which is busy; the first step runs on another."""
+    w, g, _ = _tensors([100000], seed=6)
+    want = AdamW([w[0].clone()], g, state_bits=32)
+    want.step(1)
+    side = torch.cuda.Stream()
+    dirty = [torch.full((want.m.numel(),), 7.0, device="cuda") for _ in range(4)]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for a in dirty:
+            a.record_stream(side)
+        del a, dirty
+        torch.cuda._sleep(50_000_000)
+        opt = AdamW(w, g, state_bits=32)
+    opt.step(1)
+    torch.cuda.synchronize()
+    assert torch.equal(opt.weights[0], want.weights[0]) and torch.equal(opt.m, want.m) and torch.equal(opt.v, want.v)
+
+
 def test_refusals():
     w, g, c = _tensors([300, 20])
     for bad in (lambda: AdamW([], []), lambda: AdamW(w, g[:1]), lambda: AdamW(w, g, state_bits=4), lambda: AdamW([a.cpu() for a in w], g),
