@@ -15,7 +15,7 @@
 //
 // Bound by HBM: every element of x, h (dy, du) is read once and y, u (dx, dh) written once.  A token is held by the fewest warps
 // (a constant, so that addresses are immediate) and comes through a ring of two tokens per group of warps; sums take one barrier.
-// us and TB/s on a B200: 32768 x 2048 BF16 forward 106 (5.1), backward 155 (5.2), the parameters' sums 9; 16384 x 2048 FP32
+// us and TB/s on a B200: 32768 x 2048 BF16 forward 106 (5.1), backward 155 (5.2), the parameters' sums 7; 16384 x 2048 FP32
 // forward 89 (6.0), backward 140 (5.7).  BF16, with twice the elements per byte, is at 65 % of the issue slots.  Before: loads
 // into registers, four pieces per thread, 193 and 316; the ring with the number of warps at run time 116 and 190; FP32 in two
 // pieces of 32 bytes side by side, half a sector per access, 137 and 227.  A third token in the ring costs more blocks than it hides.
@@ -506,10 +506,11 @@ template <typename T> int run_fwd(const NormP& p, cudaStream_t st)
     constexpr int F = sizeof(T) / 2;                        // pieces that hold eight elements
     if (p.C > 8192) return run_fwd<T, 4 * F, 16, false>(p, st);
     if (p.C > 4096) return run_fwd<T, 4 * F, 8, false>(p, st);
-    if (p.C > 2048) return MGPT_BY_WARPS(run_fwd, 2 * F, p, st);
+    if (p.C > 2048) return run_fwd<T, 2 * F, 8, true>(p, st);
     // Two pieces per thread (4 of FP32: 16384 x 2048 123 us against 89); one of BF16 where the tokens are few and a thread's chain is
     // what counts (8 x 1024: 3.1 us against 4.3; 32768 x 2048: 150 against 106).
-    if (sizeof(T) == 2 && (size_t)p.n * p.C <= (size_t)148 * 2048 * 4) return MGPT_BY_WARPS(run_fwd, 1, p, st);
+    if constexpr (sizeof(T) == 2)
+        if ((size_t)p.n * p.C <= (size_t)148 * 2048 * 4) return MGPT_BY_WARPS(run_fwd, 1, p, st);
     return MGPT_BY_WARPS(run_fwd, 2, p, st);
 }
 template <typename T> int run_bwd(const NormP& p, int units, cudaStream_t st)
@@ -517,7 +518,7 @@ template <typename T> int run_bwd(const NormP& p, int units, cudaStream_t st)
     constexpr int F = sizeof(T) / 2;
     if (p.C > 8192) return run_bwd<T, 4 * F, 16, false>(p, units, st);
     if (p.C > 4096) return run_bwd<T, 4 * F, 8, false>(p, units, st);
-    if (p.C > 2048) return MGPT_BY_WARPS(run_bwd, 2 * F, p, units, st);
+    if (p.C > 2048) return run_bwd<T, 2 * F, 8, true>(p, units, st);
     return MGPT_BY_WARPS(run_bwd, 2, p, units, st);
 }
 #undef MGPT_BY_WARPS
