@@ -466,7 +466,7 @@ int  mgpt_moe_op_plan_noalloc(const int32_t* top_idx, int n_rows, int E,
  * Operators that stand beside the layer in a language model's training step.
  * x, h, y and their gradients are token tensors as above: row-major [n, C],
  * C a multiple of 8, 16-byte aligned. Nothing here synchronises or allocates
- * except mgpt_moe_optim_create. n = 0 is a call without work. */
+ * except mgpt_moe_optim_create. n = 0 is a call without work, and its workspace has 0 bytes. */
 
 /* Softmax cross entropy of the vocabulary product, its logits never kept
  * (layers/CrossEntropyLossLayer.cpp, the model's last LinearLayer in front of it).

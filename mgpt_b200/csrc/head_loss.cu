@@ -909,13 +909,13 @@ extern "C" {
 
 size_t mgpt_moe_op_head_loss_workspace_bytes(int n, int C, int V)
 {
-    if (check_shape(n, C, V, MGPT_MOE_IO_BF16)) return 0;
+    if (check_shape(n, C, V, MGPT_MOE_IO_BF16) || n == 0) return 0;
     return head_ws(n, C, V, false, 1).fixed;
 }
 
 size_t mgpt_moe_op_head_loss_backward_workspace_bytes(int n, int C, int V, size_t piece_bytes)
 {
-    if (check_shape(n, C, V, MGPT_MOE_IO_BF16)) return 0;
+    if (check_shape(n, C, V, MGPT_MOE_IO_BF16) || n == 0) return 0;
     HeadWs w = head_ws(n, C, V, true, 1);
     w = head_ws(n, C, V, true, slices_of(w.n_pad, w.c_tiles, w.v_tiles));
     const size_t tile = dz_tile_bytes(w.n_pad);

@@ -1,5 +1,8 @@
 """What the head loss, the residual norm and the optimiser refuse, through the C ABI: before any CUDA call, so without a GPU."""
 import ctypes as ct
+import os
+import subprocess
+import sys
 
 import pytest
 
@@ -46,6 +49,15 @@ def test_head_loss_workspaces(lib):  # noqa: F811
 def test_head_loss_without_tokens_is_no_work(lib):  # noqa: F811
     assert _loss(lib, n=0, x=None, targets=None, loss=None, lse=None, ws=None, size=0) == 0
     assert _loss_bwd(lib, n=0, x=None, targets=None, ws=None, size=0, dw_dtype=0) == 0
+
+
+def test_sizes_of_workspaces_without_tokens():
+    """A caller asks for the size before it looks at the number of tokens.  In a process of its own: a division by zero ends it."""
+    code = ("from mgpt_b200 import _lib; lib = _lib.load(); "
+            "print([lib.mgpt_moe_op_head_loss_backward_workspace_bytes(0, C, V, p) for C, V, p in ((1024, 50021, 512 << 20), (8, 1, 0), (264, 300, 1 << 60))], "
+            "lib.mgpt_moe_op_head_loss_workspace_bytes(0, 64, 100), lib.mgpt_moe_op_residual_norm_backward_workspace_bytes(0, 64, 3))")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0 and r.stdout.split() == "[0, 0, 0] 0 0".split(), (r.returncode, r.stdout, r.stderr)
 
 
 def _norm(lib, x=P, h=P, io=1, post=P, gate=P, per=0, pre=P, n=4, C=64, y=P, u=P, stats=P):
