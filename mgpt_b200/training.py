@@ -146,12 +146,13 @@ def _norm_args(x, h, post_scale, gate, pre_scale, tokens_per_gate):
     if tokens_per_gate:
         _need(tokens_per_gate > 0, "residual norm: tokens_per_gate must not be negative")
         rows = -(-n // tokens_per_gate)
+        tokens_per_gate = min(tokens_per_gate, n)       # (C's int does not hold every number that means one row)
     else:
         rows = 1
     if gate is not None and rows == 1 and gate.dim() == 1 and gate.numel() == C:
         gate = gate.view(1, C)
     types, cols = (dtype,), (C,)
-    return (device, n, C, rows, _check(x, "x", shape, types, device), _check(h, "h", shape, types, device), _optional(post_scale, "post_scale", cols, _F32, device),
+    return (device, n, C, rows, tokens_per_gate, _check(x, "x", shape, types, device), _check(h, "h", shape, types, device), _optional(post_scale, "post_scale", cols, _F32, device),
             _optional(gate, "gate", (rows, C), _F32, device), _optional(pre_scale, "pre_scale", cols, _F32, device))
 
 
@@ -163,7 +164,7 @@ def residual_norm(x: torch.Tensor, h: torch.Tensor, *, post_scale=None, gate=Non
     ``tokens_per_gate`` consecutive tokens (0: one row, which may be given as ``[C]``).  Returns ``(y, u, stats)``; ``stats`` is
     what :func:`residual_norm_backward` needs."""
     lib = _lib.load()
-    device, n, C, _, xp, hp, post, gp, pre = _norm_args(x, h, post_scale, gate, pre_scale, tokens_per_gate)
+    device, n, C, _, tokens_per_gate, xp, hp, post, gp, pre = _norm_args(x, h, post_scale, gate, pre_scale, tokens_per_gate)
     y = torch.empty_like(x)
     u = torch.empty_like(x) if pre_scale is not None else None
     stats = torch.empty((2, n), dtype=torch.float32, device=device)
@@ -179,7 +180,7 @@ def residual_norm_backward(x: torch.Tensor, h: torch.Tensor, stats: torch.Tensor
     of the parameters' shapes) where they are given.  ``dy``: the gradient of y by its other uses; ``du``: that of u.  The other
     arguments are those of the forward call (``eps`` is in ``stats`` already)."""
     lib = _lib.load()
-    device, n, C, rows, xp, hp, post, gp, pre = _norm_args(x, h, post_scale, gate, pre_scale, tokens_per_gate)
+    device, n, C, rows, tokens_per_gate, xp, hp, post, gp, pre = _norm_args(x, h, post_scale, gate, pre_scale, tokens_per_gate)
     f32 = _F32
     sp = _check(stats, "stats", (2, n), f32, device)
     dyp, dup = _check(dy, "dy", x.shape, (x.dtype,), device), _optional(du, "du", x.shape, (x.dtype,), device)

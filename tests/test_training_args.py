@@ -5,8 +5,9 @@ import subprocess
 import sys
 
 import pytest
+import torch
 
-from mgpt_b200 import _lib
+from mgpt_b200 import _lib, training
 from tests.test_abi import lib  # noqa: F401
 
 EINVAL, ENOMEM = 1, 4
@@ -103,3 +104,48 @@ def test_optimiser_refuses(lib):  # noqa: F811
     t = (_lib.OptimTensor * 3)(*[_lib.OptimTensor(P, P, None, n, 0.0, 0) for n in (1, 256, 257)])
     assert lib.mgpt_moe_optim_blocks(t, 3) == 1 + 1 + 2
     assert lib.mgpt_moe_optim_step(None, P, P, P, P, 1e-3, 0.9, 0.999, 1e-8, 1, None, 0, None, None) == EINVAL
+
+
+class _OnDevice(torch.Tensor):
+    """A tensor that says it is on a GPU, for calls that end before anything touches its memory."""
+    is_cuda, device = property(lambda s: True), property(lambda s: torch.device("cuda", 0))
+
+
+class _Records:
+    """Stands for the library: keeps what its functions get, as the C types that they take."""
+
+    def __init__(self, lib):
+        self._lib, self.got = lib, {}
+
+    def __getattr__(self, name):
+        types = getattr(self._lib, name).argtypes
+
+        def call(*args):
+            self.got[name] = [t(a).value if t in (ct.c_int, ct.c_size_t) else a for t, a in zip(types, args)]
+            return 0
+        return call
+
+
+@pytest.fixture
+def recorded(lib, monkeypatch):  # noqa: F811
+    r, empty = _Records(lib), torch.empty
+    monkeypatch.setattr(training._lib, "load", lambda: r)
+    monkeypatch.setattr(training.torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(training, "_stream", lambda device: None)
+    monkeypatch.setattr(training.torch, "empty", lambda *a, device=None, **kw: empty(*a, **kw))
+    return r
+
+
+def _on_device(*shape, dtype=torch.float32):
+    return torch.zeros(shape, dtype=dtype).as_subclass(_OnDevice)
+
+
+@pytest.mark.parametrize("per,rows,passed", [(0, 1, 0), (3, 4, 3), (10, 1, 10), (11, 1, None), (2 ** 31 - 1, 1, None), (2 ** 31, 1, None), (2 ** 32 + 3, 1, None), (2 ** 70 + 1, 1, None)])
+def test_tokens_per_gate_that_int_does_not_hold(recorded, per, rows, passed):
+    """Python's numbers are cut to 32 bits on their way into C: a gate of one row would be read as one of four."""
+    x, h, gate = _on_device(10, 16), _on_device(10, 16), _on_device(rows, 16)
+    stats = training.residual_norm(x, h, gate=gate, tokens_per_gate=per)[2]
+    training.residual_norm_backward(x, h, stats.as_subclass(_OnDevice), x, gate=gate, d_gate=_on_device(rows, 16), tokens_per_gate=per)
+    for name, at in (("mgpt_moe_op_residual_norm", 5), ("mgpt_moe_op_residual_norm_backward", 5), ("mgpt_moe_op_residual_norm_backward_workspace_bytes", 2)):
+        got = recorded.got[name][at]
+        assert got == passed if passed is not None else got == 0 or got >= 10, name
