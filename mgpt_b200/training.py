@@ -20,6 +20,7 @@ STATE_BLOCK = 256               # elements that share a scale of the 8-bit momen
 _DTYPES = {torch.float32: IO_F32, torch.bfloat16: IO_BF16}
 _F32, _BF16, _I32, _EITHER = (torch.float32,), (torch.bfloat16,), (torch.int32,), (torch.float32, torch.bfloat16)
 _TENSOR = np.dtype([("w", "u8"), ("grad", "u8"), ("w_bf16", "u8"), ("n", "i8"), ("weight_decay", "f4"), ("grad_dtype", "i4")])      # mgpt_moe_optim_tensor
+_INT_MAX = 2 ** 31 - 1          # ctypes cuts larger numbers to 32 bits without a word
 _status = {}
 
 
@@ -95,7 +96,9 @@ def _head_args(x, weight, targets):
     if dtype not in _DTYPES or not shape or len(matrix) != 2 or not matrix[0] or not matrix[1] or shape[-1] != matrix[1]:
         raise MoeError(f"head loss: x is [..., C] of FP32 or BF16, weight [V, C]; got {tuple(shape)} of {dtype}, {tuple(matrix)}")
     V, C = matrix
-    return (device, x.numel() // C, C, V, _check(x, "x", shape, _EITHER, device), _check(weight, "weight", matrix, _BF16, device),
+    n = x.numel() // C
+    _need(max(n, C, V) <= _INT_MAX, "head loss: sizes out of range")
+    return (device, n, C, V, _check(x, "x", shape, _EITHER, device), _check(weight, "weight", matrix, _BF16, device),
             _check(targets, "targets", shape[:-1], _I32, device))
 
 
@@ -143,6 +146,7 @@ def _norm_args(x, h, post_scale, gate, pre_scale, tokens_per_gate):
         raise MoeError(f"residual norm: unsupported tokens {tuple(shape)} of {dtype}")
     C = shape[-1]
     n = x.numel() // C if C else 0
+    _need(max(n, C) <= _INT_MAX, "residual norm: sizes out of range")
     if tokens_per_gate:
         _need(tokens_per_gate > 0, "residual norm: tokens_per_gate must not be negative")
         rows = -(-n // tokens_per_gate)

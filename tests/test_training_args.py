@@ -7,7 +7,7 @@ import sys
 import pytest
 import torch
 
-from mgpt_b200 import _lib, training
+from mgpt_b200 import MoeError, _lib, training
 from tests.test_abi import lib  # noqa: F401
 
 EINVAL, ENOMEM = 1, 4
@@ -149,3 +149,37 @@ def test_tokens_per_gate_that_int_does_not_hold(recorded, per, rows, passed):
     for name, at in (("mgpt_moe_op_residual_norm", 5), ("mgpt_moe_op_residual_norm_backward", 5), ("mgpt_moe_op_residual_norm_backward_workspace_bytes", 2)):
         got = recorded.got[name][at]
         assert got == passed if passed is not None else got == 0 or got >= 10, name
+
+
+class _Huge:
+    """Only the sizes of a tensor."""
+    dtype, is_cuda, device = torch.bfloat16, True, torch.device("cuda", 0)
+
+    def __init__(self, *shape, dtype=torch.bfloat16):
+        self.shape, self.dtype = torch.Size(shape), dtype
+
+    def numel(self):
+        return self.shape.numel()
+
+    def dim(self):
+        return len(self.shape)
+
+    def is_contiguous(self):
+        return True
+
+    def data_ptr(self):
+        return P
+
+
+@pytest.mark.parametrize("n,V,C", [(2 ** 32 + 4, 100, 8), (2 ** 31, 100, 8), (4, 2 ** 32 + 100, 8), (4, 100, 2 ** 32 + 8)])
+def test_sizes_that_int_does_not_hold(recorded, n, V, C):
+    x, w, t, f = _Huge(n, C), _Huge(V, C), _Huge(n, dtype=torch.int32), _Huge(n, dtype=torch.float32)
+    for call in (lambda: training.head_loss(x, w, t), lambda: training.head_loss_backward(x, w, t, f, f)):
+        with pytest.raises(MoeError, match="out of range"):
+            call()
+    if V == 100:
+        stats = _Huge(2, n, dtype=torch.float32)
+        for call in (lambda: training.residual_norm(x, x), lambda: training.residual_norm_backward(x, x, stats, x)):
+            with pytest.raises(MoeError, match="out of range"):
+                call()
+    assert not recorded.got
