@@ -529,6 +529,10 @@ int  mgpt_moe_op_residual_norm_backward(const void* x, const void* h, int io, co
  *   state_bits 32: FP32.
  *   state_bits 8:  one byte each, in units of m_scale[i] / v_scale[i] (FP32, powers of two): m as E4M3, v as the E4M3 of
  *                  its square root. Rounding is stochastic, a function of the element's place, seed and t alone.
+ *                  A root that is not zero is kept as 2^-9 units at least, 2^-17 to 2^-16 of its block's largest: elements
+ *                  whose gradients are smaller than that beside the block's take smaller steps than with exact moments,
+ *                  none takes steps out of proportion (up to 2.6 lr seen where exact moments take 1.1). Of the others
+ *                  nine in ten have a root within 0.8 to 1.3 of the exact one; v is 4 % too large in the mean.
  * The table of the tensors' addresses is built once, by create (which allocates and synchronises). step: t counts
  * from 1; grad_scale (device, may be NULL) multiplies every gradient first: a loss scale's inverse, or the factor
  * that clips a global norm. An element whose new moments would not be finite keeps w, m and v, and sets

@@ -14,6 +14,15 @@
 // moves v by a thousandth (1-b2), a code by an eighth, and to nearest no code would ever move.  The 16 random bits of a value come from
 // the finaliser of MurmurHash3 (A. Appleby) over the element's place, the seed and the step: the same call has the same result.
 //
+// A root that is not zero never becomes zero: below the smallest code, 2^-9 units, it is kept as that.  m and the root are rounded by bits of
+// their own, so that an element some 2^17 below its block's largest would now and then keep an m of 2^-9 units and a root of zero, and the
+// next update would divide that m by sqrt(1-b2) of its own small gradient: steps of up to 1600 lr where exact moments take 1.1
+// (steady gradients of 1 and 1e-5 side by side), now 2.4.  Elements further down take smaller steps than exact moments would: the
+// root is at least 2^-17 of the block's largest.
+//
+// Elsewhere the root of v is within a factor of 0.8 to 1.3 of the exact one for nine elements in ten, and v, the square of what
+// is rounded without bias, 4 % too large in the mean.
+//
 // An element whose new moments are not finite (its gradient is not, or overflows) keeps w, m and v, and sets the caller's flag.
 #include <cmath>
 #include <cstring>
@@ -91,6 +100,14 @@ __device__ __forceinline__ F2 rounded(F2 a, uint32_t r0, uint32_t r1)
     const uint32_t q0 = (__float_as_uint(b.lo()) + (r0 << 4)) & 0xfff00000u, q1 = (__float_as_uint(b.hi()) + (r1 << 4)) & 0xfff00000u;
     return F2(__uint_as_float(q0), __uint_as_float(q1)) + F2(-l0, -l1);
 }
+
+// The root's smallest code for a root that is not zero.  (2^126: the smallest quotient of a root and its unit is 2^-119.)
+__device__ __forceinline__ F2 least_root(F2 s)
+{
+    const F2 big = s * F2(0x1p126f);
+    return F2(fminf(big.lo(), 0x1p-9f), fminf(big.hi(), 0x1p-9f));
+}
+__device__ __forceinline__ F2 no_less(F2 a, F2 b) { return F2(fmaxf(a.lo(), b.lo()), fmaxf(a.hi(), b.hi())); }
 
 // A thread block takes runs of blocks, its warps every eighth block of a run.  Lane's elements of a block: four from lane * 4, four
 // from 128 + lane * 4, so that every access of the warp is one run of memory.  A warp's blocks are copied to shared memory some
@@ -357,7 +374,8 @@ __global__ void __launch_bounds__(32 * WARPS, 2) optim_kernel(const OptP p)
                 for (int j = 0; j < 4; j += 2) {
                     const F2 x = m1[2 * i + j / 2], sx = x * F2(inv_m, inv_m), sy = root[2 * i + j / 2] * F2(inv_v, inv_v);
                     const uint32_t r0 = mixed_rest(place ^ (uint32_t)(i * 128 + j)), r1 = mixed_rest(place ^ (uint32_t)(i * 128 + j + 1));    // (bits that at + lane * 4 has not)
-                    const F2 a = rounded(F2(fabsf(sx.lo()), fabsf(sx.hi())), r0 & 0xffffu, r1 & 0xffffu), b = rounded(sy, r0 >> 16, r1 >> 16);
+                    const F2 a = rounded(F2(fabsf(sx.lo()), fabsf(sx.hi())), r0 & 0xffffu, r1 & 0xffffu);
+                    const F2 b = no_less(rounded(sy, r0 >> 16, r1 >> 16), least_root(sy));
                     om |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(copysignf(a.lo(), x.lo()), copysignf(a.hi(), x.hi())), __NV_SATFINITE, __NV_E4M3) << (8 * j);
                     ov |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(b.lo(), b.hi()), __NV_SATFINITE, __NV_E4M3) << (8 * j);
                 }

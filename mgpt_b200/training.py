@@ -207,7 +207,8 @@ class AdamW:
 
     ``state_bits`` 32 keeps the moments in FP32 (``m``, ``v``); 8 keeps a byte each for m and the root of v (``m``, ``v``:
     float8_e4m3fn, in units of ``m_scale``, ``v_scale``, one power of two per 256 elements; ``v`` stands for sqrt(v)), rounded
-    stochastically as ``seed`` and the step say.  Every tensor starts on a multiple of 256 elements of the state;
+    stochastically as ``seed`` and the step say.  An element whose gradients are less than about 2^-17 of its block's largest takes
+    smaller steps than it would with exact moments (32 bits keep them).  Every tensor starts on a multiple of 256 elements of the state;
     ``state`` gives buffers of that form to continue from.  The tensors' addresses are taken once, here: a tensor that
     moves needs a new object (with the old one's state)."""
 
