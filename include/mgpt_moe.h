@@ -506,7 +506,7 @@ int  mgpt_moe_op_head_loss_backward(const void* x, int io, const void* w, const 
  *   u = y*r2*pre_scale,                      r2 = 1/sqrt(mean(y^2) + eps)
  * post_scale NULL: h is not normalised; gate NULL: 1; pre_scale and u NULL: y alone. Scales are FP32 [C]; gate is
  * FP32 [ceil(n / tokens_per_gate), C], row i for tokens i*tokens_per_gate.. (one row for all where tokens_per_gate is 0).
- * u is formed from y before it is rounded to the tokens' dtype. stats: FP32 [2*n], kept for backward. C up to 16384.
+ * u is formed from y before it is rounded to the tokens' dtype. Rows whose squares do not fit FP32 have the same accuracy (up to values of 3e38). stats: FP32 [2*n], kept for backward. C up to 16384.
  * (layers/TransformerBlock.cpp:38-46 has the norm before a block and the plain skip connection.) */
 int  mgpt_moe_op_residual_norm(const void* x, const void* h, int io, const float* post_scale, const float* gate,
                                int tokens_per_gate, const float* pre_scale, float alpha, float eps, int n, int C,

@@ -108,12 +108,15 @@ template <int K, int W> __device__ __forceinline__ void group_sum(float (&v)[K],
         }
     }
 }
-// 1 / sqrt(x): the approximation (2 ulp) and a Newton step
+// 1 / sqrt(x): the approximation (2 ulp) and a Newton step; 0 for infinity
 __device__ __forceinline__ float inv_sqrt(float x)
 {
     const float r = rsqrtf(x);
-    return fmaf(fmaf(-x * r, r, 1.0f) * 0.5f, r, r);
+    return x < INFINITY ? fmaf(fmaf(-x * r, r, 1.0f) * 0.5f, r, r) : r;
 }
+// A row whose squares overflow is summed again with its values at this much of their size: the largest number's square times 16384 fits, and
+// the squares of what made the sum overflow are far above the smallest.
+constexpr float SMALL = 0x1p-72f;
 
 struct NormP {
     const void *x, *h;
@@ -185,6 +188,20 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 4 : 1) norm_fwd_kernel(c
             s[0] = t.lo() + t.hi();
             group_sum<1, W>(s, sh, turn);
             r1 = inv_sqrt(fmaf(s[0], inv, p.eps));
+            if (__builtin_expect(s[0] == INFINITY, 0)) {        // (the same for all of the group)
+                t = F2(0.0f);
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (const int c = (gt + i * GT) * E; have && c < p.C) {
+                        Piece<T> h;
+                        take<T, RING>(from + i * vec, (const T*)p.h + o + c, h);
+#pragma unroll
+                        for (int j = 0; j < H; ++j) t = fma2(h.v[j] * F2(SMALL), h.v[j] * F2(SMALL), t);
+                    }
+                s[0] = t.lo() + t.hi();
+                group_sum<1, W>(s, sh, turn);
+                r1 = inv_sqrt(s[0] * inv) * SMALL;
+            }
         }
         const float* gate = p.gate && p.per_gate ? p.gate + (size_t)(tok / p.per_gate) * p.C : p.gate;
         Piece<T> y[NV];
@@ -211,6 +228,17 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 4 : 1) norm_fwd_kernel(c
             s[0] = t.lo() + t.hi();
             group_sum<1, W>(s, sh, turn);
             r2 = inv_sqrt(fmaf(s[0], inv, p.eps));
+            if (__builtin_expect(s[0] == INFINITY, 0)) {
+                t = F2(0.0f);
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if ((gt + i * GT) * E < p.C && have)
+#pragma unroll
+                        for (int j = 0; j < H; ++j) t = fma2(y[i].v[j] * F2(SMALL), y[i].v[j] * F2(SMALL), t);
+                s[0] = t.lo() + t.hi();
+                group_sum<1, W>(s, sh, turn);
+                r2 = inv_sqrt(s[0] * inv) * SMALL;
+            }
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int c = (gt + i * GT) * E;
