@@ -536,7 +536,9 @@ int  mgpt_moe_op_residual_norm_backward(const void* x, const void* h, int io, co
  * The table of the tensors' addresses is built once, by create (which allocates and synchronises). step: t counts
  * from 1; grad_scale (device, may be NULL) multiplies every gradient first: a loss scale's inverse, or the factor
  * that clips a global norm. An element whose new moments would not be finite keeps w, m and v, and sets
- * *found_nonfinite (device, may be NULL; never cleared here) to 1. w_bf16 (may be NULL) gets the new w in BF16. */
+ * *found_nonfinite (device, may be NULL; never cleared here) to 1. w_bf16 (may be NULL) gets the new w in BF16.
+ * t, lr and the random bits belong to the call: step refuses a stream that is being captured, since every replay would
+ * repeat them (the same rounding at every step lets v fall far behind). */
 typedef struct {
     float*      w;             /* FP32 */
     const void* grad;

@@ -489,6 +489,10 @@ int mgpt_moe_optim_step(mgpt_moe_optim* o, void* m, void* v, float* m_scale, flo
     MGPT_TRY(check_aligned(m, "optimiser: m"));
     MGPT_TRY(check_aligned(v, "optimiser: v"));
     MGPT_CUDA(cudaSetDevice(o->device));
+    cudaStreamCaptureStatus capture;
+    MGPT_CUDA(cudaStreamIsCapturing((cudaStream_t)stream, &capture));
+    if (capture != cudaStreamCaptureStatusNone)
+        return fail(MGPT_MOE_EINVAL, "optimiser: a step is not captured in a graph, whose replays would repeat its number, its rates and its random bits");
     OptP p = {};
     p.tensors = (const OptTensor*)o->tables;
     p.n_tensors = o->n_tensors; p.blocks = (int)o->blocks;

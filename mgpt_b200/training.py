@@ -251,7 +251,8 @@ class AdamW:
 
     def step(self, t: int, lr: float = 3e-4, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8, grad_scale: torch.Tensor = None) -> None:
         """One step; ``t`` counts from 1.  ``grad_scale``: an FP32 tensor of one element that multiplies the gradients.  Elements
-        whose gradient is not finite keep their values and set ``found_nonfinite``."""
+        whose gradient is not finite keep their values and set ``found_nonfinite``.  Not for capture in a graph, which would repeat
+        ``t``, ``lr`` and the rounding's random bits: refused."""
         _need(self._h.value, "AdamW: closed")
         gs = _optional(grad_scale, "grad_scale", () if grad_scale is not None and grad_scale.dim() == 0 else (1,), _F32, self.device)
         _lib.check(self.lib.mgpt_moe_optim_step(self._h, *self._p, lr, beta1, beta2, eps, int(t), gs, self.seed,
