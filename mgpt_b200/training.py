@@ -73,7 +73,9 @@ def _status_word(device):
 def check_status(device=None) -> None:
     """Raises :class:`MoeError` if a call of :func:`head_loss` or :func:`head_loss_backward` on this device recorded an error
     since the last check (a target beyond the vocabulary, a bounded wait that ran out).  Synchronises the device."""
-    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    device = torch.device("cuda" if device is None else device)
+    if device.index is None:                                # ("cuda" is no tensor's device: theirs have a number)
+        device = torch.device(device.type, torch.cuda.current_device())
     s = _status.get(device)
     if s is None:
         return
