@@ -65,8 +65,10 @@ def _workspace(nbytes, device):
 def _status_word(device):
     s = _status.get(device)
     if s is None:
-        s = _status[device] = torch.zeros(1, dtype=torch.int32, device=device)
+        _need(not torch.cuda.is_current_stream_capturing(), "head loss: a device's first call, which makes its status word, cannot be captured in a graph")
+        s = torch.zeros(1, dtype=torch.int32, device=device)
         torch.cuda.current_stream(device).synchronize()     # cleared before any stream writes to it
+        _status[device] = s
     return s
 
 

@@ -22,3 +22,22 @@ def test_every_name_of_the_device(name):
     with pytest.raises(MoeError, match="beyond the vocabulary"):
         mgpt_b200.check_status(name)
     mgpt_b200.check_status(name)
+
+
+def test_a_first_call_in_a_graph_is_refused_and_leaves_nothing(monkeypatch):
+    """The status word is made by a device's first call, cleared and waited for: neither can be part of a capture."""
+    from mgpt_b200 import training
+    monkeypatch.setattr(training, "_status", {})
+    x, w, t = _args()
+    torch.cuda.synchronize()
+    with pytest.raises(MoeError, match="captur"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            mgpt_b200.head_loss(x, w, t)
+    assert not training._status
+    want, lse = mgpt_b200.head_loss(x, w, t)                    # this makes it
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, _ = mgpt_b200.head_loss(x, w, t)
+    graph.replay()
+    mgpt_b200.check_status()
+    assert torch.equal(loss, want)
