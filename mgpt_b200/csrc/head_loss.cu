@@ -35,16 +35,17 @@ constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr uint32_t TMEM_COLS = 2 * TILE;
 constexpr uint32_t STAGING = 4096;                   // per epilogue warp: 32 rows x 128 B
 constexpr int QUEUE = 4;
-constexpr int NARROW = 512;                          // LOSS_NARROW up to this C
-constexpr int PART = 512 / BK;                       // LOSS: k-blocks summed in one accumulator
+constexpr int NARROW = 512;                          // LOSS_NARROW, DLOGITS_NARROW up to this C
+constexpr int PART = 512 / BK;                       // LOSS, DLOGITS: k-blocks summed in one accumulator
 constexpr int CLAIM = 6;                             // GRADS: the next item is claimed this many k-blocks before the last one's loads end
 constexpr int MAX_PIECES = 1024;
 constexpr int COUNTERS = 2 * MAX_PIECES + 2;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int ST_BAD_TARGET = ST_BAD_EXPERT;         // the status bit of an index outside its range
 
-enum { LOSS = 0, DLOGITS = 1, GRADS = 2, LOSS_NARROW = 3 };
+enum { LOSS = 0, DLOGITS = 1, GRADS = 2, LOSS_NARROW = 3, DLOGITS_NARROW = 4 };
 constexpr bool is_loss(int kind) { return kind == LOSS || kind == LOSS_NARROW; }
+constexpr bool in_parts(int kind) { return kind == LOSS || kind == DLOGITS; }       // logits: several accumulators, joined in registers
 
 struct HeadP {
     const int32_t* n_valid;     // null: n tokens, as they lie
@@ -162,10 +163,13 @@ template <int KIND> __device__ __forceinline__ Item decode(const HeadP& p, int n
 // tmB: LOSS, DLOGITS w (box 64 x 128 rows); GRADS w (box 64 x 64 rows); tmB2: x (box 64 x 64 rows)
 // tmX: x as it lies in the caller's memory, in boxes like those of x above, which is the packed copy
 // The epilogue's 16 warps: all of them on an item, 64 columns each; or two groups of eight that take items in turn, 128 columns
-// each.  What a warp of DLOGITS does for an item is a chain of some 6000 cycles (tcgen05.ld, exponentials, shared memory, the copy that has
-// to have left it), of which an item of C = 512 with 4100 cycles of products hides one only half: 1.3 % of the gradients' time where the
-// power limit sets the clock, 6 % where it does not.  The loss is 2 % slower in groups: it gives the accumulator back at once.
-template <int KIND> constexpr int item_warps() { return KIND == DLOGITS || KIND == LOSS_NARROW ? EPI_WARPS / 2 : EPI_WARPS; }
+// each.  What a warp of DLOGITS_NARROW does for an item is a chain of some 6000 cycles (tcgen05.ld, exponentials, shared memory, the copy
+// that has to have left it), of which an item of C = 512 with 4100 cycles of products hides one only half: 1.3 % of the gradients' time where
+// the power limit sets the clock, 6 % where it does not.  LOSS and DLOGITS, all sixteen on an item, add its accumulators in registers and
+// give each back at once.  One accumulator over all channels for the gradients' logits, beside the loss's several, was 1 % faster
+// (1501 of 3001 tokens, 1024 x 50021 458 us, now 464; 8192, 2048 x 131072 12.70 ms, now 12.83) and left exp(z - lse) with what the
+// tensor core cuts off such a sum: 2e-3 of d_loss for a token that is certain (logit 400, 2048 channels), now 3e-5.
+template <int KIND> constexpr int item_warps() { return KIND == DLOGITS_NARROW || KIND == LOSS_NARROW ? EPI_WARPS / 2 : EPI_WARPS; }
 
 template <int KIND>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
@@ -327,7 +331,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 const uint32_t a_step = a_mn ? 2048 >> 4 : 32 >> 4, b_step = b_mn ? 2048 >> 4 : 32 >> 4;     // (the address field: 16-byte units)
                 for (int k0 = 0; ok && k0 < w.nkb; ++t) {
                     const uint32_t buf = t & 1u, d_tmem = tmem_base + buf * TILE;
-                    const int k1 = KIND == LOSS ? min(k0 + PART, w.nkb) : w.nkb;
+                    const int k1 = in_parts(KIND) ? min(k0 + PART, w.nkb) : w.nkb;
                     if (!mbar_wait(acc_empty + 8 * buf, ((t >> 1) & 1) ^ 1, p.status, ERR_ACC_WAIT)) {
                         ok = false;
                         break;
@@ -405,8 +409,25 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             const int row = w.m * TILE + rank * 128 + q * 32 + lane, v = p.v0 + w.n * TILE + h * (UNITS * 64);
             const bool real = KIND != GRADS && row < n_valid;
             const int at = real ? p.target[row] - v : -1;
-            const float up = KIND == DLOGITS && real ? p.d_loss[row] : 0.0f, lse = KIND == DLOGITS && real ? p.lse[row] : 0.0f;
+            constexpr bool dlogits = KIND != GRADS && !is_loss(KIND);
+            const float up = dlogits && real ? p.d_loss[row] : 0.0f, lse = dlogits && real ? p.lse[row] : 0.0f;
             if (!empty_sum && !next_acc()) break;
+            // the item's other accumulators, added to what the first one left in z; false: a wait ran out
+            auto add_parts = [&](float (&z)[64]) {
+                for (int kb = PART; kb < w.nkb; kb += PART) {
+                    if (!next_acc()) return false;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        float o[16];
+                        tmem_ld16(t_lane + 16 * c, o);
+                        tmem_ld_wait();
+                        if (c == 3) give_back();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) z[16 * c + j] += o[j];
+                    }
+                }
+                return true;
+            };
             if (is_loss(KIND)) {
                 float top = -INFINITY, sum = 0.0f;
                 bool ok = true;
@@ -421,20 +442,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     }
                     tmem_ld_wait();
                     if (u + 1 == UNITS) give_back();
-                    if (KIND == LOSS) {
-                        for (int kb = PART; kb < w.nkb && (ok = next_acc()); kb += PART) {
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) {
-                                float o[16];
-                                tmem_ld16(t_lane + 16 * c, o);
-                                tmem_ld_wait();
-                                if (c == 3) give_back();
-#pragma unroll
-                                for (int j = 0; j < 16; ++j) z[16 * c + j] += o[j];
-                            }
-                        }
-                        if (!ok) break;
-                    }
+                    if (KIND == LOSS && !(ok = add_parts(z))) break;
                     if (valid < 64) {
 #pragma unroll
                         for (int j = 0; j < 64; ++j)
@@ -472,9 +480,17 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 sums[((k & 3) * SHARERS + h) * 128] = make_float2(top, sum);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(joined + 8 * (k & 3));
-            } else if (KIND == DLOGITS) {
+            } else if (dlogits) {
                 const F2 ref(-lse * LOG2E), up2(up);        // (rows behind the last token: logits 0, up 0)
                 const uint32_t line = smem_u32(stage) + lane * 128;
+                float all[KIND == DLOGITS ? 64 : 1];
+                if constexpr (KIND == DLOGITS) {
+                    tmem_ld32(t_lane, *reinterpret_cast<float (*)[32]>(all));
+                    tmem_ld32(t_lane + 32, *reinterpret_cast<float (*)[32]>(all + 32));
+                    tmem_ld_wait();
+                    give_back();
+                    if (!add_parts(all)) break;
+                }
 #pragma unroll 1
                 for (int u = 0; u < UNITS; ++u) {
                     const int valid = p.V - v - u * 64, a = at - u * 64;
@@ -483,9 +499,14 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         float z[32];
-                        tmem_ld32(t_lane + u * 64 + c * 32, z);
-                        tmem_ld_wait();
-                        if (c == 1 && u + 1 == UNITS) give_back();
+                        if constexpr (KIND == DLOGITS) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) z[j] = all[c * 32 + j];
+                        } else {
+                            tmem_ld32(t_lane + u * 64 + c * 32, z);
+                            tmem_ld_wait();
+                            if (c == 1 && u + 1 == UNITS) give_back();
+                        }
 #pragma unroll
                         for (int j = 0; j < 32; j += 2) {
                             const F2 e = fma2(F2(z[j], z[j + 1]), F2(LOG2E), ref);
@@ -605,7 +626,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             }
         }
         if (is_loss(KIND) && k > 0 && h == (int)((k - 1) & (SHARERS - 1))) join(k - 1, before);
-        if (KIND == DLOGITS && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        if (KIND != GRADS && !is_loss(KIND) && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     // neither CTA may leave (or give its TMEM back) while the other can still read its shared memory or signal it
     tc_fence_before();
@@ -1035,7 +1056,9 @@ int mgpt_moe_op_head_loss_backward(const void* x, int io, const void* w, const i
         p.last = slices == 1 && i == pieces - 1;
         const long items = (long)(h.n_pad / TILE) * p.v_tiles;
         p.sched = k.n_valid + 1 + 2 * i;
-        MGPT_TRY(launch_head<DLOGITS>(mx, mw, mx, mw, mx0, p, (int)(items < sms / 2 ? items : sms / 2), st));
+        const int pairs = (int)(items < sms / 2 ? items : sms / 2);
+        if (C <= NARROW) MGPT_TRY(launch_head<DLOGITS_NARROW>(mx, mw, mx, mw, mx0, p, pairs, st));
+        else MGPT_TRY(launch_head<DLOGITS>(mx, mw, mx, mw, mx0, p, pairs, st));
         p.sched = k.n_valid + 2 + 2 * i;
         const long grads = ((long)(h.n_pad / TILE) * p.k_slices + p.v_tiles) * p.c_tiles;
         MGPT_TRY(launch_head<GRADS>(mz, mw_t, mz_t, mx_t, mx0_t, p, (int)(grads < sms / 2 ? grads : sms / 2), st));
