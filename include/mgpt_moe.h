@@ -474,9 +474,9 @@ int  mgpt_moe_op_plan_noalloc(const int32_t* top_idx, int n_rows, int E,
  * x: [n, C] of `io`; w: BF16 [V, C], a row per vocabulary entry (the layout of an
  * embedding, which may be the same tensor); targets: int32 [n]; loss, lse: FP32 [n].
  * x is rounded to BF16 where it is FP32; products are exact and summed in FP32.
- * A token whose target is outside [0, V) takes no part: its loss, lse and dx are 0, its
- * x is not looked at (it may hold NaN), and it costs no work. Targets >= V also set
- * bit 32 of *status.
+ * A token whose target is outside [0, V) takes no part: its loss, lse and dx are 0, and what
+ * its x holds (NaN, say) reaches no result. It costs no work and its x is not read, except in the
+ * loss of at most 256 BF16 tokens: those are one tile, worked on whole. Targets >= V also set bit 32 of *status.
  * status: int32 on the device, OR-ed into and never cleared here (bits as
  * mgpt_moe_check_status's). workspace: mgpt_moe_op_head_loss_workspace_bytes,
  * 256-byte aligned; nothing of it is needed after the call. */

@@ -15,7 +15,9 @@
 // results' own rounding.)
 //
 // Tokens whose target is not in [0, vocabulary) take no part: the others are packed first, so that an ignored token costs
-// nothing and its x, whatever it holds, is not read.
+// nothing and its x, whatever it holds, is not read.  The loss of at most TILE tokens of the operand type reads them as they lie:
+// leaving some out would not make their one tile of products shorter.  A row of it is one token, so that what an ignored one holds
+// stays there, and is dropped when the columns are joined.
 #include "pairs.cuh"
 #include "tc_common.cuh"
 

@@ -111,7 +111,7 @@ def head_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor):
 
     x: ``[..., C]``, FP32 or BF16; weight: BF16 ``[V, C]``; targets: int32 ``[...]``.  Returns ``(loss, lse)``, FP32
     ``[...]``: ``lse`` is what :func:`head_loss_backward` needs.  Tokens whose target is outside ``[0, V)`` (padding, prompts)
-    take no part: loss and lse 0, and no work; targets ``>= V`` are reported by :func:`check_status`."""
+    take no part: loss and lse 0, whatever their x holds, and no work (beyond one tile of 256 tokens); targets ``>= V`` are reported by :func:`check_status`."""
     lib = _lib.load()
     device, n, C, V, xp, wp, tp = _head_args(x, weight, targets)
     loss, lse = torch.empty_like(targets, dtype=torch.float32), torch.empty_like(targets, dtype=torch.float32)
