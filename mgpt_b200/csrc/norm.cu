@@ -15,8 +15,9 @@
 //
 // Bound by HBM: every element of x, h (dy, du) is read once and y, u (dx, dh) written once.  A token is held by the fewest warps
 // (a constant, so that addresses are immediate) and comes through a ring of two tokens per group of warps; sums take one barrier.
-// us and TB/s on a B200: 32768 x 2048 BF16 forward 106 (5.1), backward 155 (5.2), the parameters' sums 7; 16384 x 2048 FP32
-// forward 89 (6.0), backward 140 (5.7).  BF16, with twice the elements per byte, is at 65 % of the issue slots.  Before: loads
+// us and TB/s on a B200: 32768 x 2048 BF16 forward 108 (5.0), backward with the parameters' sums 151 (5.3); 16384 x 2048 FP32
+// forward 89 (6.0), backward 140 (5.7).  BF16, with twice the elements per byte, is at 56 and 60 % of the
+// issue slots.  Before: loads
 // into registers, four pieces per thread, 193 and 316; the ring with the number of warps at run time 116 and 190; FP32 in two
 // pieces of 32 bytes side by side, half a sector per access, 137 and 227.  A third token in the ring costs more blocks than it hides.
 #include "pairs.cuh"
@@ -27,7 +28,7 @@ namespace {
 
 constexpr int MAX_C = 16384;
 __host__ __device__ constexpr int threads_of(int warps) { return warps > 8 ? 32 * warps : 256; }     // whole groups of warps, one per token
-constexpr int UNITS = 296;          // blocks of the backward pass aimed at: two per SM
+constexpr int UNITS = 296;          // blocks of the backward pass aimed at: two per SM of 148 (not asked of the device: a workspace's size is known without one)
 constexpr int FWD_CTAS = 4;         // of the forward pass, per SM
 
 // A piece: 16 bytes of a row, so that a warp's access is one run of memory whatever the type.  A thread copies its pieces to places

@@ -113,9 +113,9 @@ __device__ __forceinline__ F2 no_less(F2 a, F2 b) { return F2(fmaxf(a.lo(), b.lo
 // from 128 + lane * 4, so that every access of the warp is one run of memory.  A warp's blocks are copied to shared memory some
 // blocks ahead, in pieces of 16 bytes per lane.
 //
-// Bound by HBM: w, m and v are written where they were read, which this memory takes at 5.5 TB/s at most (the 32-bit form's rate).  With loads
+// Bound by HBM: w, m and v are written where they were read, which this memory takes at 5.7 TB/s at most (the 32-bit form's rate).  With loads
 // into registers, one block per warp and two tables to look up before the first load, 24 warps of 66 registers kept 3.2 TB/s going:
-// 562 us for 386 tensors of 100 M elements, now 337 (5.4 TB/s).  Copies of 4 bytes per lane (the codes, the scales) cost as much
+// 562 us for 386 tensors of 100 M elements, now 336 (5.4 TB/s).  Copies of 4 bytes per lane (the codes, the scales) cost as much
 // as those of 16: 368 us without the scales' against 395.  In 8 bits an element is about 70 instructions for the 14 to 18 bytes
 // that it moves, so that moments go two to an instruction, the update takes its root and quotient from the approximating
 // instructions (2 ulp of an update that is itself a small part of w) and elements that are not finite are sorted out in a rare pass
