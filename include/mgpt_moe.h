@@ -279,6 +279,27 @@ int  mgpt_moe_set_weight_grad_overwrite(mgpt_moe_layer* layer, int enabled);
  * them this way; results do not depend on the value. No reference counterpart. */
 int  mgpt_moe_set_sm_budget(mgpt_moe_layer* layer, int n_sms);
 
+/* Routing other than the reference's clamped softmax and top-k: sigmoid or softmax scores, a bias that balances the experts'
+ * load, groups of experts, renormalised weights (what is computed: mgpt_moe_op_route, below). NULL goes back to the reference's.
+ * Every forward and backward of the layer and the routing-side stage calls follow it: the logits are the layer's own router's
+ * (x Wr + br), the gradient goes through the weights to Wr, br and x, and there is no load-balance term (lb_alpha): the
+ * bias balances. `bias` stays the caller's and is read on the device by every call. A saved routing belongs to the setting it was
+ * saved under, and backward cannot follow a forward of before the call. With a routing set, the workspace view "probs" has what
+ * the router left there (its clamped softmax), top_p the weights. Logits of calls beyond n_tokens * embed_dim * num_experts = 4e8 agree with
+ * exact ones to a few 1e-6 (tensor cores), and experts are chosen from them. */
+#define MGPT_MOE_SCORE_SOFTMAX 0
+#define MGPT_MOE_SCORE_SIGMOID 1
+typedef struct {
+    int   score;         /* MGPT_MOE_SCORE_*                                               */
+    int   groups;        /* of consecutive experts, 1 to 32, a divisor of the experts      */
+    int   top_groups;    /* groups whose experts may be chosen (groups: no choice of groups) */
+    int   group_top;     /* 1 or 2: how many of a group's largest scores are its own       */
+    int   renormalise;   /* weights divided by their sum                                   */
+    float scale;         /* of the weights                                                 */
+    const float* bias;   /* device, FP32 [E], or NULL                                      */
+} mgpt_moe_routing;
+int  mgpt_moe_set_routing(mgpt_moe_layer* layer, const mgpt_moe_routing* routing);
+
 /* Number of kernels the library launched since the counter was last reset
  * (host-side count of its own launches; for benchmark bookkeeping). */
 long mgpt_moe_launch_count(int reset);
@@ -292,6 +313,21 @@ int  mgpt_moe_op_router(const void* x, int io_dtype, const float* Wr, const floa
                         int n_tokens, int C, int E, int k,
                         float* logits, float* probs, int32_t* top_idx, float* top_p,
                         mgpt_stream_t stream);
+
+/* Routing from logits [n, E] of `io` (any router's product; the call above writes such logits):
+ *   s = sigmoid(z) or softmax(z),   c = s + bias
+ *   the top_groups groups with the largest sums of their group_top largest c stay; top_idx: the k largest c of theirs in falling
+ *   order, equal ones by index (without a bias: the k largest z);   w = scale * s / (sum of the chosen s + 1e-20), or scale * s
+ * The choice is that of exact arithmetic (comparisons too close for FP32 are made in FP64). An expert whose logit or bias is -inf or NaN
+ * is out: chosen, by index and with weight 0, only where fewer than k others are left. A NaN among a token's logits (softmax: or
+ * +inf) makes its weights NaN. top_idx always holds k different numbers of [0, E), in the form mgpt_moe_op_plan takes.
+ * counts (may be NULL): int32 [E], added to: how many tokens chose an expert (what a bias is adjusted by). E up to 512, k up to 32. */
+int  mgpt_moe_op_route(const void* logits, int io, int n, int E, int k, const mgpt_moe_routing* routing,
+                       int32_t* top_idx, float* weights, int32_t* counts, mgpt_stream_t stream);
+/* The gradient of the logits, of their type, written: through the weights and, for a softmax, through its sum. Same logits and
+ * routing; top_idx as it was written (an entry outside [0, E) has no gradient; one that is repeated counts as often). */
+int  mgpt_moe_op_route_backward(const void* logits, int io, const int32_t* top_idx, const float* d_weights, int n, int E, int k,
+                                const mgpt_moe_routing* routing, void* d_logits, mgpt_stream_t stream);
 
 /* histogram + prefix sum + stable slot assignment in one call, on the device
  * (cuda_ops.h:56-57 moe_histogram / moe_gather's slot claim, MoELayer.cpp:61-80's
@@ -521,6 +557,28 @@ int  mgpt_moe_op_residual_norm_backward(const void* x, const void* h, int io, co
                                         const float* stats, const void* dy, const void* du, void* dx, void* dh,
                                         float* d_post_scale, float* d_gate, float* d_pre_scale,
                                         void* workspace, size_t workspace_bytes, mgpt_stream_t stream);
+
+/* Activations kept for a backward pass in 8 bits: values int8 [n, C], exponents uint8 [n, ceil(C/32)], a byte b for 32 consecutive
+ * channels of a row (the last of a row may be fewer), whose values are in units of 2^(b-127): the least power of two, 2^-126 at
+ * least, in which the largest of them rounds to 127 or less. Rounding is to nearest, ties to even: off by half a unit at most, 1/128
+ * of the group's largest value (b is 248 at most: values from 3.39e38 on are kept as 127 units). b = 255: a value was NaN or infinite, and all of the group come back as NaN. x: [n, C] of `io`, C a
+ * multiple of 8, 16-byte aligned; values 8-byte aligned. restore8 gives values * 2^(b-127), exact in either type. */
+int  mgpt_moe_op_keep8(const void* x, int io, int n, int C, int8_t* values, uint8_t* exponents, mgpt_stream_t stream);
+int  mgpt_moe_op_restore8(const int8_t* values, const uint8_t* exponents, int n, int C, void* x, int io, mgpt_stream_t stream);
+
+/* mgpt_moe_op_residual_norm that also keeps x and h so, in the same pass, and the backward call that takes them in the
+ * tensors' place (`io` is the type of dy, du, dx and dh). The gradients are the formulas' at the kept x and h, with the
+ * r1 and r2 of the forward pass. Everything else, the workspace too, as above. */
+int  mgpt_moe_op_residual_norm_keep(const void* x, const void* h, int io, const float* post_scale, const float* gate,
+                                    int tokens_per_gate, const float* pre_scale, float alpha, float eps, int n, int C,
+                                    void* y, void* u, float* stats, int8_t* x_values, uint8_t* x_exponents,
+                                    int8_t* h_values, uint8_t* h_exponents, mgpt_stream_t stream);
+int  mgpt_moe_op_residual_norm_backward_kept(const int8_t* x_values, const uint8_t* x_exponents, const int8_t* h_values,
+                                             const uint8_t* h_exponents, int io, const float* post_scale, const float* gate,
+                                             int tokens_per_gate, const float* pre_scale, float alpha, int n, int C,
+                                             const float* stats, const void* dy, const void* du, void* dx, void* dh,
+                                             float* d_post_scale, float* d_gate, float* d_pre_scale,
+                                             void* workspace, size_t workspace_bytes, mgpt_stream_t stream);
 
 /* AdamW over many tensors at once (optimisers/AdamWOptimiser.h:24-36 calls Tensor::adamw_step per tensor), for the tensors
  * of a model that are not a layer's own (those: mgpt_moe_adamw_step).

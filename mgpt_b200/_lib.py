@@ -31,6 +31,8 @@ SYMBOLS = [
     "mgpt_moe_set_weight_grad_overwrite", "mgpt_moe_inference_workspace_bytes", "mgpt_moe_forward_inference", "mgpt_moe_experts_backward_rows", "mgpt_moe_experts_backward_params",
     "mgpt_moe_op_head_loss_workspace_bytes", "mgpt_moe_op_head_loss", "mgpt_moe_op_head_loss_backward_workspace_bytes", "mgpt_moe_op_head_loss_backward",
     "mgpt_moe_op_residual_norm", "mgpt_moe_op_residual_norm_backward_workspace_bytes", "mgpt_moe_op_residual_norm_backward",
+    "mgpt_moe_set_routing", "mgpt_moe_op_route", "mgpt_moe_op_route_backward",
+    "mgpt_moe_op_keep8", "mgpt_moe_op_restore8", "mgpt_moe_op_residual_norm_keep", "mgpt_moe_op_residual_norm_backward_kept",
     "mgpt_moe_optim_blocks", "mgpt_moe_optim_create", "mgpt_moe_optim_destroy", "mgpt_moe_optim_step",
 ]
 PLAN_NOALLOC_MAX_ROWS = 1048576
@@ -55,6 +57,12 @@ class OptimTensor(ct.Structure):
                 ("weight_decay", ct.c_float), ("grad_dtype", ct.c_int)]
 
 
+class Routing(ct.Structure):
+    _fields_ = [("score", ct.c_int), ("groups", ct.c_int), ("top_groups", ct.c_int), ("group_top", ct.c_int),
+                ("renormalise", ct.c_int), ("scale", ct.c_float), ("bias", ct.c_void_p)]
+
+
+SCORES = {"softmax": 0, "sigmoid": 1}
 EP_ID_BYTES = 128
 
 
@@ -162,6 +170,13 @@ def load() -> ct.CDLL:
     lib.mgpt_moe_op_residual_norm_backward_workspace_bytes.argtypes = [i32, i32, i32]
     lib.mgpt_moe_op_residual_norm_backward_workspace_bytes.restype = sz
     lib.mgpt_moe_op_residual_norm_backward.argtypes = [vp, vp, i32, vp, vp, i32, vp, f32, i32, i32] + [vp] * 9 + [sz, vp]
+    lib.mgpt_moe_set_routing.argtypes = [vp, ct.POINTER(Routing)]
+    lib.mgpt_moe_op_route.argtypes = [vp, i32, i32, i32, i32, ct.POINTER(Routing), vp, vp, vp, vp]
+    lib.mgpt_moe_op_route_backward.argtypes = [vp, i32, vp, vp, i32, i32, i32, ct.POINTER(Routing), vp, vp]
+    lib.mgpt_moe_op_keep8.argtypes = [vp, i32, i32, i32, vp, vp, vp]
+    lib.mgpt_moe_op_restore8.argtypes = [vp, vp, i32, i32, vp, i32, vp]
+    lib.mgpt_moe_op_residual_norm_keep.argtypes = lib.mgpt_moe_op_residual_norm.argtypes[:-1] + [vp] * 5
+    lib.mgpt_moe_op_residual_norm_backward_kept.argtypes = [vp] * 4 + lib.mgpt_moe_op_residual_norm_backward.argtypes[2:]
     lib.mgpt_moe_optim_blocks.argtypes = [ct.POINTER(OptimTensor), i32]
     lib.mgpt_moe_optim_blocks.restype = i64
     lib.mgpt_moe_optim_create.argtypes = [i32, ct.POINTER(OptimTensor), i32, i32, ct.POINTER(vp)]

@@ -385,7 +385,7 @@ int mgpt_moe_workspace_view(const mgpt_moe_layer* L, int n_tokens, const char* n
     const Dims& d = L->d;
     const size_t N = n_tokens, E = d.E, k = d.k, C = d.C, H = d.H, rc = w.row_cap, ab = w.act_bytes;
     struct { const char* n; size_t o, b; } tab[] = {
-        {"logits", w.logits, N * E * 4}, {"probs", w.probs, N * E * 4}, {"top_idx", w.top_idx, N * k * 4},
+        {"logits", L->routed ? w.probs : w.logits, N * E * 4}, {"probs", L->routed ? w.logits : w.probs, N * E * 4}, {"top_idx", w.top_idx, N * k * 4},
         {"top_p", w.top_p, N * k * 4}, {"counts", w.counts, E * 4}, {"offsets", w.offsets, E * 4},
         {"padded_offsets", w.padded_offsets, (E + 1) * 4}, {"tile_expert", w.tile_expert, (size_t)w.max_tiles * 4},
         {"n_tiles", w.n_tiles, 4}, {"status", w.status, 4}, {"map", w.map, N * k * 4}, {"pos", w.pos, N * k * 4},
@@ -550,7 +550,9 @@ static int forward_impl(mgpt_moe_layer* L, const void* x, void* y, int n_tokens,
         if (n_tokens > 0) {
             L->stage_begin(ST_ROUTER, st);
             const PlanArgs plan = plan_args(d, w, ws, L->d_status);
-            if (tc_router_usable(L, x, io, n_tokens))
+            if (L->routed)
+                MGPT_TRY(launch_routed(L, w, ws, x, io, st));
+            else if (tc_router_usable(L, x, io, n_tokens))
                 MGPT_TRY(tc_router_fwd(L, w, ws, x, st));
             else
                 MGPT_TRY(launch_router_fwd(x, io, L->p_data[0], L->p_data[1], n_tokens, d.C, d.E, d.k,

@@ -247,6 +247,10 @@ struct mgpt_moe_layer {
     void *ext_Xg = nullptr, *ext_Yg = nullptr, *ext_dYg = nullptr, *ext_dXg = nullptr;
     int n_seg = 0;
 
+    // mgpt_moe_set_routing: how experts are chosen, where it is not by clamped softmax and top-k
+    bool routed = false;
+    mgpt_moe_routing routing = {};
+
     // optional per-stage timing
     bool profiling = false;
     cudaEvent_t ev_begin[mgpt::ST_COUNT] = {}, ev_end[mgpt::ST_COUNT] = {};
@@ -286,6 +290,10 @@ int tc_router_fwd(mgpt_moe_layer* L, const Workspace& w, char* ws, const void* x
 int router_tc_ne(int E);
 int launch_router_bwd(mgpt_moe_layer* L, const Workspace& w, char* ws, const void* x, int io,
                       void* dx, cudaStream_t st, const void* dXg_rows = nullptr, const int32_t* pos_rows = nullptr);
+
+// route.cu
+int launch_routed(mgpt_moe_layer* L, const Workspace& w, char* ws, const void* x, int io, cudaStream_t st);
+int launch_routed_bwd(mgpt_moe_layer* L, const Workspace& w, char* ws, bf16* dl16, int E8, float* d_bias, cudaStream_t st);
 
 // plan.cu
 struct PlanArgs plan_args(const Dims& d, const Workspace& w, char* ws, int32_t* sticky);      // plan_block.cuh

@@ -20,7 +20,7 @@
 // issue slots.  Before: loads
 // into registers, four pieces per thread, 193 and 316; the ring with the number of warps at run time 116 and 190; FP32 in two
 // pieces of 32 bytes side by side, half a sector per access, 137 and 227.  A third token in the ring costs more blocks than it hides.
-#include "pairs.cuh"
+#include "kept.cuh"
 
 namespace mgpt {
 
@@ -71,6 +71,31 @@ template <typename T> __device__ __forceinline__ void params(const float* p, int
         const float4 a = p ? *reinterpret_cast<const float4*>(p + c + 4 * j) : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
         o.v[2 * j] = F2(a.x, a.y);
         o.v[2 * j + 1] = F2(a.z, a.w);
+    }
+}
+
+// a piece of what was kept in 8 bits, RING: as above
+template <typename T, bool RING> __device__ __forceinline__ void take_kept(uint32_t src, const int8_t* mem, uint32_t byte, Piece<T>& o)
+{
+    const F2 unit(kept_unit(byte));
+    if constexpr (sizeof(T) == 2) {
+        const uint2 u = RING ? taken<uint2>(src) : *reinterpret_cast<const uint2*>(mem);
+        kept_unpack(u.x, unit, o.v[0], o.v[1]);
+        kept_unpack(u.y, unit, o.v[2], o.v[3]);
+    } else {
+        kept_unpack(RING ? taken<uint32_t>(src) : *reinterpret_cast<const uint32_t*>(mem), unit, o.v[0], o.v[1]);
+    }
+}
+// keeps a piece: every lane of a warp calls it, `in` where there is one
+template <typename T> __device__ __forceinline__ void keep(const Piece<T>& v, bool in, int8_t* mem, uint8_t* byte)
+{
+    constexpr int E = piece<T>();
+    uint32_t w[E / 4];
+    const uint32_t e = kept_pack<E>(v.v, w);
+    if (in) {
+        if constexpr (E == 8) *reinterpret_cast<uint2*>(mem) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t*>(mem) = w[0];
+        if (threadIdx.x % (KEPT_GROUP / E) == 0) *byte = (uint8_t)e;
     }
 }
 
@@ -131,6 +156,9 @@ struct NormP {
     void *dx, *dh;
     float* part;                    // [units][2][C]: sums of D*h_hat and du*y_hat
     int splits, length;             // units per gate row, tokens per unit
+    // x and h in 8 bits: written by the forward pass, read in place of x and h by the backward one
+    int8_t *xv, *hv;
+    uint8_t *xe, *he;
 };
 
 // Bytes of a block's ring: `arrays` of NV pieces per thread, STAGES tokens.
@@ -138,7 +166,7 @@ constexpr int STAGES = 2;
 constexpr uint32_t ring_bytes(int arrays, int nv, int threads) { return STAGES * arrays * nv * threads * 16; }
 
 // A group of warps per token, the groups of the grid taking tokens in turn.
-template <typename T, int NV, int W, bool RING>
+template <typename T, int NV, int W, bool RING, bool KEEP>
 __global__ void __launch_bounds__(threads_of(W), RING ? 4 : 1) norm_fwd_kernel(const NormP p)
 {
     extern __shared__ __align__(16) uint8_t ring[];
@@ -210,8 +238,14 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 4 : 1) norm_fwd_kernel(c
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (gt + i * GT) * E;
-            if (have && c < p.C) {
-                Piece<T> a, g, h, x;
+            const bool in = have && c < p.C;
+            Piece<T> h, x;
+            if constexpr (KEEP) {
+#pragma unroll
+                for (int j = 0; j < H; ++j) h.v[j] = x.v[j] = F2(0.0f);
+            }
+            if (in) {
+                Piece<T> a, g;
                 params<T>(p.post, c, a);
                 params<T>(gate, c, g);
                 take<T, RING>(from + i * vec, (const T*)p.h + o + c, h);
@@ -222,6 +256,11 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 4 : 1) norm_fwd_kernel(c
                     t = fma2(y[i].v[j], y[i].v[j], t);
                 }
                 store((T*)p.y + o + c, y[i]);
+            }
+            if constexpr (KEEP) {
+                const size_t group = (size_t)tok * kept_groups(p.C) + c / KEPT_GROUP;
+                keep<T>(x, in, p.xv + o + c, p.xe + group);
+                keep<T>(h, in, p.hv + o + c, p.he + group);
             }
         }
         float r2 = 1.0f;
@@ -262,7 +301,7 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 4 : 1) norm_fwd_kernel(c
 // One block per unit: tokens of one gate row.  The sums over a unit's tokens stay in registers, a thread's columns being
 // always the same; the three sums over a token's columns are taken in one round:
 //   mean(D*gp*h_hat) = mean((dy + r2*du*pre)*gp*h_hat) - r2 * mean(du*pre*y_hat) * mean(y_hat*gp*h_hat),   gp = gate*post
-template <typename T, int NV, int W, bool RING>
+template <typename T, int NV, int W, bool RING, bool KEPT>
 __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(const NormP p)
 {
     extern __shared__ __align__(16) uint8_t ring[];         // at the end: [groups][C] sums
@@ -279,6 +318,34 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
     pdl_wait();
     const bool with_u = p.du != nullptr;
     float nr1 = 0.0f, nr2 = 0.0f;                           // of the token that is copied next
+    // A token in the ring: pieces of h, x, dy, du; or of dy, du, then of h and x in 8 bits (whose exponents come as nr1 and nr2 do).
+    constexpr uint32_t kvec = THREADS * E, karray = NV * kvec, stage = KEPT ? 2 * array + 2 * karray : 4 * array;
+    constexpr uint32_t dy_at = KEPT ? 0 : 2 * array, du_at = dy_at + array;
+    const uint32_t mine8 = (uint32_t)__cvta_generic_to_shared(ring) + 2 * array + threadIdx.x * E;
+    const int groups_of = kept_groups(p.C);
+    uint32_t nhe[KEPT ? NV : 1], nxe[KEPT ? NV : 1], he[KEPT ? NV : 1], xe[KEPT ? NV : 1];
+    auto exponents = [&](int tok) {
+        if constexpr (KEPT) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (gt + i * GT) * E;
+                if (c < p.C) {
+                    const size_t group = (size_t)tok * groups_of + c / KEPT_GROUP;
+                    nhe[i] = p.he[group];
+                    nxe[i] = p.xe[group];
+                }
+            }
+        }
+    };
+    auto take_hx = [&](int i, int slot, size_t at, Piece<T>& h, Piece<T>& x) {
+        if constexpr (KEPT) {
+            take_kept<T, RING>(mine8 + slot * stage + i * kvec, p.hv + at, he[i], h);
+            take_kept<T, RING>(mine8 + slot * stage + karray + i * kvec, p.xv + at, xe[i], x);
+        } else {
+            take<T, RING>(mine + slot * stage + i * vec, (const T*)p.h + at, h);
+            take<T, RING>(mine + slot * stage + array + i * vec, (const T*)p.x + at, x);
+        }
+    };
     auto fetch = [&](int tok, int s) {
         if (RING && tok < t1) {
             const size_t o = (size_t)tok * p.C;
@@ -286,11 +353,17 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
             for (int i = 0; i < NV; ++i) {
                 const int c = (gt + i * GT) * E;
                 if (c < p.C) {
-                    const uint32_t d = mine + s * 4 * array + i * vec;
-                    copy16(d, (const T*)p.h + o + c);
-                    copy16(d + array, (const T*)p.x + o + c);
-                    copy16(d + 2 * array, (const T*)p.dy + o + c);
-                    if (with_u) copy16(d + 3 * array, (const T*)p.du + o + c);
+                    const uint32_t d = mine + s * stage + i * vec;
+                    if constexpr (KEPT) {
+                        const uint32_t d8 = mine8 + s * stage + i * kvec;
+                        copy_piece8<E>(d8, p.hv + o + c);
+                        copy_piece8<E>(d8 + karray, p.xv + o + c);
+                    } else {
+                        copy16(d, (const T*)p.h + o + c);
+                        copy16(d + array, (const T*)p.x + o + c);
+                    }
+                    copy16(d + dy_at, (const T*)p.dy + o + c);
+                    if (with_u) copy16(d + du_at, (const T*)p.du + o + c);
                 }
             }
         }
@@ -316,6 +389,7 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
     if (t0 + group < t1) {
         nr1 = p.stats[t0 + group];
         nr2 = p.stats[p.n + t0 + group];
+        exponents(t0 + group);
     }
     const float inv = 1.0f / (float)p.C;
     int slot = 0;
@@ -324,24 +398,31 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
         const bool have = tok < t1;
         const size_t o = (size_t)tok * p.C;
         const float r1 = nr1, r2 = nr2;
+        if constexpr (KEPT) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                he[i] = nhe[i];
+                xe[i] = nxe[i];
+            }
+        }
         fetch(tok + (STAGES - 1) * GROUPS, slot == 0 ? STAGES - 1 : slot - 1);
         if (tok + GROUPS < t1) {
             nr1 = p.stats[tok + GROUPS];
             nr2 = p.stats[p.n + tok + GROUPS];
+            exponents(tok + GROUPS);
         }
         copy_wait<STAGES - 1>();
-        const uint32_t from = mine + slot * 4 * array;
+        const uint32_t from = mine + slot * stage;
         F2 s0(0.0f), s1(0.0f), s2(0.0f);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (gt + i * GT) * E;
             if (have && c < p.C) {
                 Piece<T> h, x, dy, du, b;
-                take<T, RING>(from + i * vec, (const T*)p.h + o + c, h);
-                take<T, RING>(from + array + i * vec, (const T*)p.x + o + c, x);
-                take<T, RING>(from + 2 * array + i * vec, (const T*)p.dy + o + c, dy);
+                take_hx(i, slot, o + c, h, x);
+                take<T, RING>(from + dy_at + i * vec, (const T*)p.dy + o + c, dy);
                 if (with_u) {
-                    take<T, RING>(from + 3 * array + i * vec, (const T*)p.du + o + c, du);
+                    take<T, RING>(from + du_at + i * vec, (const T*)p.du + o + c, du);
                     params<T>(p.pre, c, b);
                 }
 #pragma unroll
@@ -367,11 +448,10 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
             const int c = (gt + i * GT) * E;
             if (have && c < p.C) {
                 Piece<T> h, x, D, du, b, dx;
-                take<T, RING>(from + i * vec, (const T*)p.h + o + c, h);
-                take<T, RING>(from + array + i * vec, (const T*)p.x + o + c, x);
-                take<T, RING>(from + 2 * array + i * vec, (const T*)p.dy + o + c, D);
+                take_hx(i, slot, o + c, h, x);
+                take<T, RING>(from + dy_at + i * vec, (const T*)p.dy + o + c, D);
                 if (with_u) {
-                    take<T, RING>(from + 3 * array + i * vec, (const T*)p.du + o + c, du);
+                    take<T, RING>(from + du_at + i * vec, (const T*)p.du + o + c, du);
                     params<T>(p.pre, c, b);
                 }
 #pragma unroll
@@ -504,26 +584,34 @@ template <typename K> int opt_in(K kernel, uint32_t bytes, bool (&done)[64])
     if (dev < 64) done[dev] = true;
     return 0;
 }
-template <typename T, int NV, int W, bool RING> int run_fwd(const NormP& p, cudaStream_t st)
+template <typename T, int NV, int W, bool RING, bool KEEP> int run_fwd(const NormP& p, cudaStream_t st)
 {
     constexpr int threads = threads_of(W), groups = threads / (32 * W);
     constexpr uint32_t smem = RING ? ring_bytes(2, NV, threads) : 0;
     const int most = 148 * FWD_CTAS, want = (p.n + groups - 1) / groups;
     static bool done[64];
-    MGPT_TRY(opt_in(norm_fwd_kernel<T, NV, W, RING>, smem, done));
-    MGPT_CUDA(launch_pdl(norm_fwd_kernel<T, NV, W, RING>, want < most ? want : most, threads, smem, st, p));
+    MGPT_TRY(opt_in(norm_fwd_kernel<T, NV, W, RING, KEEP>, smem, done));
+    MGPT_CUDA(launch_pdl(norm_fwd_kernel<T, NV, W, RING, KEEP>, want < most ? want : most, threads, smem, st, p));
     MGPT_LAUNCHED("norm_fwd_kernel");
+    return 0;
+}
+template <typename T, int NV, int W, bool RING> int run_fwd(const NormP& p, cudaStream_t st)
+{
+    return p.xv ? run_fwd<T, NV, W, RING, true>(p, st) : run_fwd<T, NV, W, RING, false>(p, st);
+}
+template <typename T, int NV, int W, bool RING, bool KEPT> int run_bwd(const NormP& p, int units, cudaStream_t st)
+{
+    // (the ring is more than the sums at the end, 4 NV piece<T>() bytes per thread where there are groups)
+    constexpr uint32_t smem = !RING ? 0 : KEPT ? ring_bytes(2, NV, threads_of(W)) + STAGES * 2 * NV * threads_of(W) * piece<T>() : ring_bytes(4, NV, threads_of(W));
+    static bool done[64];
+    MGPT_TRY(opt_in(norm_bwd_kernel<T, NV, W, RING, KEPT>, smem, done));
+    MGPT_CUDA(launch_pdl(norm_bwd_kernel<T, NV, W, RING, KEPT>, units, threads_of(W), smem, st, p));
+    MGPT_LAUNCHED("norm_bwd_kernel");
     return 0;
 }
 template <typename T, int NV, int W, bool RING> int run_bwd(const NormP& p, int units, cudaStream_t st)
 {
-    // (the ring is more than the sums at the end, 4 NV piece<T>() bytes per thread where there are groups)
-    constexpr uint32_t smem = RING ? ring_bytes(4, NV, threads_of(W)) : 0;
-    static bool done[64];
-    MGPT_TRY(opt_in(norm_bwd_kernel<T, NV, W, RING>, smem, done));
-    MGPT_CUDA(launch_pdl(norm_bwd_kernel<T, NV, W, RING>, units, threads_of(W), smem, st, p));
-    MGPT_LAUNCHED("norm_bwd_kernel");
-    return 0;
+    return p.xv ? run_bwd<T, NV, W, RING, true>(p, units, st) : run_bwd<T, NV, W, RING, false>(p, units, st);
 }
 // NV pieces per thread: the fewest warps that hold a token, a power of two
 #define MGPT_BY_WARPS(run, NV, ...)                                                               \
@@ -552,6 +640,71 @@ template <typename T> int run_bwd(const NormP& p, int units, cudaStream_t st)
 }
 #undef MGPT_BY_WARPS
 
+struct Kept {
+    int8_t *xv, *hv;
+    uint8_t *xe, *he;
+};
+int check_kept(const Kept& k)
+{
+    if (!k.xv || !k.hv || !k.xe || !k.he) return fail(MGPT_MOE_EINVAL, "null argument");
+    MGPT_TRY(check_aligned(k.xv, "x_values", 8));
+    return check_aligned(k.hv, "h_values", 8);
+}
+
+int forward(const void* x, const void* h, int io, const float* post_scale, const float* gate, int tokens_per_gate, const float* pre_scale,
+            float alpha, float eps, int n, int C, void* y, void* u, float* stats, const Kept* kept, mgpt_stream_t stream)
+{
+    MGPT_TRY(check_norm(n, C, tokens_per_gate, io));
+    if (n == 0) return 0;
+    if (!x || !h || !y || !stats) return fail(MGPT_MOE_EINVAL, "null argument");
+    if (!pre_scale != !u) return fail(MGPT_MOE_EINVAL, "residual norm: u and pre_scale go together");
+    const struct { const void* p; const char* what; } io_bufs[] = {{x, "x"}, {h, "h"}, {y, "y"}, {u, "u"}};
+    for (const auto& b : io_bufs) MGPT_TRY(check_aligned(b.p, b.what));
+    MGPT_TRY(check_params(post_scale, gate, pre_scale));
+    if (kept) MGPT_TRY(check_kept(*kept));
+    NormP p = {};
+    p.x = x; p.h = h; p.post = post_scale; p.gate = gate; p.pre = pre_scale; p.alpha = alpha; p.eps = eps; p.n = n; p.C = C;
+    p.per_gate = one_row(n, tokens_per_gate); p.y = y; p.u = u; p.stats = stats;
+    if (kept) p.xv = kept->xv, p.hv = kept->hv, p.xe = kept->xe, p.he = kept->he;
+    return io == MGPT_MOE_IO_BF16 ? run_fwd<bf16>(p, (cudaStream_t)stream) : run_fwd<float>(p, (cudaStream_t)stream);
+}
+
+int backward(const void* x, const void* h, const Kept* kept, int io, const float* post_scale, const float* gate, int tokens_per_gate,
+             const float* pre_scale, float alpha, int n, int C, const float* stats, const void* dy, const void* du, void* dx, void* dh,
+             float* d_post_scale, float* d_gate, float* d_pre_scale, void* workspace, size_t ws_bytes, mgpt_stream_t stream)
+{
+    MGPT_TRY(check_norm(n, C, tokens_per_gate, io));
+    if (n == 0) return 0;
+    if ((!kept && (!x || !h)) || !stats || !dy || !dx || !dh) return fail(MGPT_MOE_EINVAL, "null argument");
+    if (!pre_scale != !du) return fail(MGPT_MOE_EINVAL, "residual norm: du and pre_scale go together");
+    if ((d_post_scale && !post_scale) || (d_gate && !gate) || (d_pre_scale && !pre_scale))
+        return fail(MGPT_MOE_EINVAL, "residual norm: a gradient of a parameter that is absent");
+    const struct { const void* p; const char* what; } io_bufs[] = {{x, "x"}, {h, "h"}, {dy, "dy"}, {du, "du"}, {dx, "dx"}, {dh, "dh"}};
+    for (const auto& b : io_bufs) MGPT_TRY(check_aligned(b.p, b.what));
+    MGPT_TRY(check_params(post_scale, gate, pre_scale));
+    if (kept) MGPT_TRY(check_kept(*kept));
+    tokens_per_gate = one_row(n, tokens_per_gate);
+    const bool sums = d_post_scale || d_gate || d_pre_scale;
+    const Split s = split_of(n, tokens_per_gate);
+    const int rows = gate_rows(n, tokens_per_gate), units = rows * s.splits;
+    if (sums) {
+        if (!workspace || ((uintptr_t)workspace & 255)) return fail(MGPT_MOE_EINVAL, "workspace must be 256-byte aligned");
+        if (ws_bytes < (size_t)units * 2 * C * sizeof(float))
+            return fail(MGPT_MOE_ENOMEM, "workspace smaller than mgpt_moe_op_residual_norm_backward_workspace_bytes()");
+    }
+    NormP p = {};
+    p.x = x; p.h = h; p.post = post_scale; p.gate = gate; p.pre = pre_scale; p.alpha = alpha; p.n = n; p.C = C; p.per_gate = tokens_per_gate;
+    p.stats = (float*)stats; p.dy = dy; p.du = du; p.dx = dx; p.dh = dh; p.part = sums ? (float*)workspace : nullptr;
+    p.splits = s.splits; p.length = s.length;
+    if (kept) p.xv = kept->xv, p.hv = kept->hv, p.xe = kept->xe, p.he = kept->he;
+    cudaStream_t st = (cudaStream_t)stream;
+    MGPT_TRY(io == MGPT_MOE_IO_BF16 ? run_bwd<bf16>(p, units, st) : run_bwd<float>(p, units, st));
+    if (!sums) return 0;
+    MGPT_CUDA(launch_pdl(norm_params_kernel, (C + 31) / 32, 32 * PW, 0, st, p.part, post_scale, gate, C, rows, s.splits, d_post_scale, d_gate, d_pre_scale));
+    MGPT_LAUNCHED("norm_params_kernel");
+    return 0;
+}
+
 }  // namespace
 
 }  // namespace mgpt
@@ -563,17 +716,15 @@ extern "C" {
 int mgpt_moe_op_residual_norm(const void* x, const void* h, int io, const float* post_scale, const float* gate, int tokens_per_gate,
                               const float* pre_scale, float alpha, float eps, int n, int C, void* y, void* u, float* stats, mgpt_stream_t stream)
 {
-    MGPT_TRY(check_norm(n, C, tokens_per_gate, io));
-    if (n == 0) return 0;
-    if (!x || !h || !y || !stats) return fail(MGPT_MOE_EINVAL, "null argument");
-    if (!pre_scale != !u) return fail(MGPT_MOE_EINVAL, "residual norm: u and pre_scale go together");
-    const struct { const void* p; const char* what; } io_bufs[] = {{x, "x"}, {h, "h"}, {y, "y"}, {u, "u"}};
-    for (const auto& b : io_bufs) MGPT_TRY(check_aligned(b.p, b.what));
-    MGPT_TRY(check_params(post_scale, gate, pre_scale));
-    NormP p = {};
-    p.x = x; p.h = h; p.post = post_scale; p.gate = gate; p.pre = pre_scale; p.alpha = alpha; p.eps = eps; p.n = n; p.C = C;
-    p.per_gate = one_row(n, tokens_per_gate); p.y = y; p.u = u; p.stats = stats;
-    return io == MGPT_MOE_IO_BF16 ? run_fwd<bf16>(p, (cudaStream_t)stream) : run_fwd<float>(p, (cudaStream_t)stream);
+    return forward(x, h, io, post_scale, gate, tokens_per_gate, pre_scale, alpha, eps, n, C, y, u, stats, nullptr, stream);
+}
+
+int mgpt_moe_op_residual_norm_keep(const void* x, const void* h, int io, const float* post_scale, const float* gate, int tokens_per_gate,
+                                   const float* pre_scale, float alpha, float eps, int n, int C, void* y, void* u, float* stats,
+                                   int8_t* x_values, uint8_t* x_exponents, int8_t* h_values, uint8_t* h_exponents, mgpt_stream_t stream)
+{
+    const Kept kept = {x_values, h_values, x_exponents, h_exponents};
+    return forward(x, h, io, post_scale, gate, tokens_per_gate, pre_scale, alpha, eps, n, C, y, u, stats, &kept, stream);
 }
 
 size_t mgpt_moe_op_residual_norm_backward_workspace_bytes(int n, int C, int tokens_per_gate)
@@ -588,34 +739,19 @@ int mgpt_moe_op_residual_norm_backward(const void* x, const void* h, int io, con
                                        void* dx, void* dh, float* d_post_scale, float* d_gate, float* d_pre_scale,
                                        void* workspace, size_t ws_bytes, mgpt_stream_t stream)
 {
-    MGPT_TRY(check_norm(n, C, tokens_per_gate, io));
-    if (n == 0) return 0;
-    if (!x || !h || !stats || !dy || !dx || !dh) return fail(MGPT_MOE_EINVAL, "null argument");
-    if (!pre_scale != !du) return fail(MGPT_MOE_EINVAL, "residual norm: du and pre_scale go together");
-    if ((d_post_scale && !post_scale) || (d_gate && !gate) || (d_pre_scale && !pre_scale))
-        return fail(MGPT_MOE_EINVAL, "residual norm: a gradient of a parameter that is absent");
-    const struct { const void* p; const char* what; } io_bufs[] = {{x, "x"}, {h, "h"}, {dy, "dy"}, {du, "du"}, {dx, "dx"}, {dh, "dh"}};
-    for (const auto& b : io_bufs) MGPT_TRY(check_aligned(b.p, b.what));
-    MGPT_TRY(check_params(post_scale, gate, pre_scale));
-    tokens_per_gate = one_row(n, tokens_per_gate);
-    const bool sums = d_post_scale || d_gate || d_pre_scale;
-    const Split s = split_of(n, tokens_per_gate);
-    const int rows = gate_rows(n, tokens_per_gate), units = rows * s.splits;
-    if (sums) {
-        if (!workspace || ((uintptr_t)workspace & 255)) return fail(MGPT_MOE_EINVAL, "workspace must be 256-byte aligned");
-        if (ws_bytes < (size_t)units * 2 * C * sizeof(float))
-            return fail(MGPT_MOE_ENOMEM, "workspace smaller than mgpt_moe_op_residual_norm_backward_workspace_bytes()");
-    }
-    NormP p = {};
-    p.x = x; p.h = h; p.post = post_scale; p.gate = gate; p.pre = pre_scale; p.alpha = alpha; p.n = n; p.C = C; p.per_gate = tokens_per_gate;
-    p.stats = (float*)stats; p.dy = dy; p.du = du; p.dx = dx; p.dh = dh; p.part = sums ? (float*)workspace : nullptr;
-    p.splits = s.splits; p.length = s.length;
-    cudaStream_t st = (cudaStream_t)stream;
-    MGPT_TRY(io == MGPT_MOE_IO_BF16 ? run_bwd<bf16>(p, units, st) : run_bwd<float>(p, units, st));
-    if (!sums) return 0;
-    MGPT_CUDA(launch_pdl(norm_params_kernel, (C + 31) / 32, 32 * PW, 0, st, p.part, post_scale, gate, C, rows, s.splits, d_post_scale, d_gate, d_pre_scale));
-    MGPT_LAUNCHED("norm_params_kernel");
-    return 0;
+    return backward(x, h, nullptr, io, post_scale, gate, tokens_per_gate, pre_scale, alpha, n, C, stats, dy, du, dx, dh, d_post_scale, d_gate,
+                    d_pre_scale, workspace, ws_bytes, stream);
+}
+
+int mgpt_moe_op_residual_norm_backward_kept(const int8_t* x_values, const uint8_t* x_exponents, const int8_t* h_values, const uint8_t* h_exponents,
+                                            int io, const float* post_scale, const float* gate, int tokens_per_gate, const float* pre_scale,
+                                            float alpha, int n, int C, const float* stats, const void* dy, const void* du, void* dx, void* dh,
+                                            float* d_post_scale, float* d_gate, float* d_pre_scale,
+                                            void* workspace, size_t ws_bytes, mgpt_stream_t stream)
+{
+    const Kept kept = {const_cast<int8_t*>(x_values), const_cast<int8_t*>(h_values), const_cast<uint8_t*>(x_exponents), const_cast<uint8_t*>(h_exponents)};
+    return backward(nullptr, nullptr, &kept, io, post_scale, gate, tokens_per_gate, pre_scale, alpha, n, C, stats, dy, du, dx, dh, d_post_scale,
+                    d_gate, d_pre_scale, workspace, ws_bytes, stream);
 }
 
 }  // extern "C"

@@ -29,7 +29,14 @@ __device__ __forceinline__ uint32_t narrow(F2 v)
 
 // Asynchronous copies to shared memory (addresses of the shared space), in groups.
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void copy8(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
+template <int BYTES> __device__ __forceinline__ void copy_piece8(uint32_t dst, const void* src)
+{
+    static_assert(BYTES == 8 || BYTES == 4, "");
+    if constexpr (BYTES == 8) copy8(dst, src);
+    else copy4(dst, src);
+}
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int PENDING> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
 template <typename T> __device__ __forceinline__ T taken(uint32_t src)

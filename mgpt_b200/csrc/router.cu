@@ -1070,10 +1070,12 @@ int launch_router_bwd(mgpt_moe_layer* L, const Workspace& w, char* ws, const voi
     const bool tc = d.mode == MGPT_MOE_BF16 && d.gemm_impl == 0 && io == MGPT_MOE_IO_BF16;
     const bool tc_wgrad = tc && L->has_grad && E % 4 == 0;
     const int E8 = (E + 7) / 8 * 8;
-    {
+    bf16* dl16 = tc ? (bf16*)(ws + w.dl16) : nullptr;
+    float* gbr = tc_wgrad ? L->p_grad[1] : nullptr;
+    if (L->routed) {
+        MGPT_TRY(launch_routed_bwd(L, w, ws, dl16, E8, gbr, st));
+    } else {
         const int grid = min((N + 31) / 32, 592);
-        bf16* dl16 = tc ? (bf16*)(ws + w.dl16) : nullptr;
-        float* gbr = tc_wgrad ? L->p_grad[1] : nullptr;
         if (E <= 32) MGPT_CUDA(launch_pdl(router_dlogits_kernel<1>, grid, 256, 0, st, probs, top_idx, dtp, counts, N, E, k, d.alpha, dl, dl16, E8, gbr));
         else if (E <= 64) MGPT_CUDA(launch_pdl(router_dlogits_kernel<2>, grid, 256, 0, st, probs, top_idx, dtp, counts, N, E, k, d.alpha, dl, dl16, E8, gbr));
         else MGPT_CUDA(launch_pdl(router_dlogits_kernel<4>, grid, 256, 0, st, probs, top_idx, dtp, counts, N, E, k, d.alpha, dl, dl16, E8, gbr));

@@ -1,5 +1,5 @@
 """The rest of a training step around the layer, over the C ABI: the loss of a language model's head, the norms around a
-block with its gate and skip connection, and AdamW over many tensors.
+block with its gate and skip connection, activations kept in 8 bits for the backward pass, and AdamW over many tensors.
 
 As in :mod:`mgpt_b200.moe_layer`, torch is used for device memory and streams only.  Every call enqueues its work on the
 current stream and returns; wrong arguments raise :class:`MoeError` before anything is enqueued.
@@ -19,6 +19,7 @@ STATE_BLOCK = 256               # elements that share a scale of the 8-bit momen
 
 _DTYPES = {torch.float32: IO_F32, torch.bfloat16: IO_BF16}
 _F32, _BF16, _I32, _EITHER = (torch.float32,), (torch.bfloat16,), (torch.int32,), (torch.float32, torch.bfloat16)
+_I8, _U8 = (torch.int8,), (torch.uint8,)
 _TENSOR = np.dtype([("w", "u8"), ("grad", "u8"), ("w_bf16", "u8"), ("n", "i8"), ("weight_decay", "f4"), ("grad_dtype", "i4")])      # mgpt_moe_optim_tensor
 _INT_MAX = 2 ** 31 - 1          # ctypes cuts larger numbers to 32 bits without a word
 _status = {}
@@ -143,13 +144,86 @@ def head_loss_backward(x: torch.Tensor, weight: torch.Tensor, targets: torch.Ten
     return dx, d_weight
 
 
+# ---- activations kept in 8 bits ---------------------------------------------------------------------------------------
+KEPT_GROUP = 32                 # channels that share an exponent
+
+
+class Kept8:
+    """Activations ``[..., C]`` in 8 bits: ``values`` (int8 ``[..., C]``) in units of ``2**(exponents - 127)`` (uint8
+    ``[..., ceil(C/32)]``: one for 32 consecutive channels).  ``dtype`` is that of the tensor that was kept."""
+    __slots__ = ("values", "exponents", "dtype")
+
+    def __init__(self, values: torch.Tensor, exponents: torch.Tensor, dtype: torch.dtype):
+        self.values, self.exponents, self.dtype = values, exponents, dtype
+
+    @property
+    def shape(self):
+        return self.values.shape
+
+    @property
+    def nbytes(self) -> int:
+        return self.values.numel() + self.exponents.numel()
+
+
+def _kept_size(shape, what):
+    C = shape[-1] if shape else 0
+    if C <= 0 or C % 8:
+        raise MoeError(f"{what}: expected [..., C], C a multiple of 8, got {tuple(shape)}")
+    n = shape[:-1].numel()
+    _need(max(n, C) <= _INT_MAX, f"{what}: sizes out of range")
+    return n, C
+
+
+def _kept_empty(x: torch.Tensor) -> Kept8:
+    groups = -(-x.shape[-1] // KEPT_GROUP)
+    return Kept8(torch.empty_like(x, dtype=torch.int8), torch.empty(x.shape[:-1] + (groups,), dtype=torch.uint8, device=x.device), x.dtype)
+
+
+def _check_kept(kept, name, shape, device):
+    if not isinstance(kept, Kept8):
+        raise MoeError(f"{name}: expected a Kept8, got {type(kept).__name__}")
+    groups = -(-shape[-1] // KEPT_GROUP)
+    return (_check(kept.values, f"{name}.values", shape, _I8, device),
+            _check(kept.exponents, f"{name}.exponents", shape[:-1] + (groups,), _U8, device))
+
+
+def keep8(x: torch.Tensor) -> Kept8:
+    """``x`` (``[..., C]``, FP32 or BF16, C a multiple of 8) in 8 bits, for a backward pass: 1 1/32 bytes per value.  32 consecutive
+    channels share a power of two as their unit, the least in which the largest of them rounds to 127 or less: a value is off by
+    half a unit at most, 1/128 of the largest.  A group with a NaN or an infinity comes back as NaN."""
+    lib = _lib.load()
+    device = _device(x)
+    n, C = _kept_size(x.shape, "keep8")
+    xp = _check(x, "x", x.shape, _EITHER, device)
+    kept = _kept_empty(x)
+    _lib.check(lib.mgpt_moe_op_keep8(xp, _DTYPES[x.dtype], n, C, kept.values.data_ptr(), kept.exponents.data_ptr(), _stream(device)))
+    return kept
+
+
+def restore8(kept: Kept8, dtype: torch.dtype = None) -> torch.Tensor:
+    """The tensor that :func:`keep8` kept, in ``dtype`` (its own where none is given): exactly what the 8 bits stand for."""
+    lib = _lib.load()
+    if not isinstance(kept, Kept8):
+        raise MoeError(f"restore8: expected a Kept8, got {type(kept).__name__}")
+    device, dtype = _device(kept.values), kept.dtype if dtype is None else dtype
+    n, C = _kept_size(kept.shape, "restore8")
+    if dtype not in _DTYPES:
+        raise MoeError(f"restore8: unsupported dtype {dtype}")
+    vp, ep = _check_kept(kept, "kept", kept.shape, device)
+    x = torch.empty_like(kept.values, dtype=dtype)
+    _lib.check(lib.mgpt_moe_op_restore8(vp, ep, n, C, x.data_ptr(), _DTYPES[dtype], _stream(device)))
+    return x
+
+
 # ---- norms around a block ---------------------------------------------------------------------------------------------
-def _norm_args(x, h, post_scale, gate, pre_scale, tokens_per_gate):
-    device, dtype, shape = _device(x), x.dtype, x.shape
+def _norm_args(x, h, post_scale, gate, pre_scale, tokens_per_gate, like=None):
+    """like: dy, where x and h are kept in 8 bits."""
+    kept, like = like is not None, x if like is None else like
+    device, dtype, shape = _device(like), like.dtype, like.shape
     if dtype not in _DTYPES or not shape:
         raise MoeError(f"residual norm: unsupported tokens {tuple(shape)} of {dtype}")
     C = shape[-1]
-    n = x.numel() // C if C else 0
+    n = like.numel() // C if C else 0
     _need(max(n, C) <= _INT_MAX, "residual norm: sizes out of range")
     if tokens_per_gate:
         _need(tokens_per_gate > 0, "residual norm: tokens_per_gate must not be negative")
@@ -160,47 +234,60 @@ def _norm_args(x, h, post_scale, gate, pre_scale, tokens_per_gate):
     if gate is not None and rows == 1 and gate.dim() == 1 and gate.numel() == C:
         gate = gate.view(1, C)
     types, cols = (dtype,), (C,)
-    return (device, n, C, rows, tokens_per_gate, _check(x, "x", shape, types, device), _check(h, "h", shape, types, device), _optional(post_scale, "post_scale", cols, _F32, device),
+    if kept:
+        xp, hp = _check_kept(x, "x", shape, device), _check_kept(h, "h", shape, device)
+    else:
+        xp, hp = _check(x, "x", shape, types, device), _check(h, "h", shape, types, device)
+    return (device, n, C, rows, tokens_per_gate, xp, hp, _optional(post_scale, "post_scale", cols, _F32, device),
             _optional(gate, "gate", (rows, C), _F32, device), _optional(pre_scale, "pre_scale", cols, _F32, device))
 
 
 def residual_norm(x: torch.Tensor, h: torch.Tensor, *, post_scale=None, gate=None, pre_scale=None, alpha: float = 1.0, eps: float = 1e-5,
-                  tokens_per_gate: int = 0):
+                  tokens_per_gate: int = 0, keep: bool = False):
     """``y = alpha*x + gate * rmsnorm(h)*post_scale`` and ``u = rmsnorm(y)*pre_scale``: what follows a block and precedes the
     next one, in one pass.  x, h: ``[..., C]``, both FP32 or both BF16.  Without ``post_scale`` h is not normalised, without
     ``gate`` it is 1, without ``pre_scale`` there is no u (None).  ``gate``: FP32 ``[rows, C]``, a row for every
     ``tokens_per_gate`` consecutive tokens (0: one row, which may be given as ``[C]``).  Returns ``(y, u, stats)``; ``stats`` is
-    what :func:`residual_norm_backward` needs."""
+    what :func:`residual_norm_backward` needs.  With ``keep``: ``(y, u, stats, (x8, h8))``, x and h in 8 bits as :func:`keep8` keeps
+    them, from the same pass."""
     lib = _lib.load()
     device, n, C, _, tokens_per_gate, xp, hp, post, gp, pre = _norm_args(x, h, post_scale, gate, pre_scale, tokens_per_gate)
     y = torch.empty_like(x)
     u = torch.empty_like(x) if pre_scale is not None else None
     stats = torch.empty((2, n), dtype=torch.float32, device=device)
-    _lib.check(lib.mgpt_moe_op_residual_norm(xp, hp, _DTYPES[x.dtype], post, gp, tokens_per_gate, pre, alpha, eps, n, C, y.data_ptr(),
-                                             None if u is None else u.data_ptr(), stats.data_ptr(), _stream(device)))
-    return y, u, stats
+    args = (xp, hp, _DTYPES[x.dtype], post, gp, tokens_per_gate, pre, alpha, eps, n, C, y.data_ptr(), None if u is None else u.data_ptr(), stats.data_ptr())
+    if not keep:
+        _lib.check(lib.mgpt_moe_op_residual_norm(*args, _stream(device)))
+        return y, u, stats
+    x8, h8 = _kept_empty(x), _kept_empty(h)
+    _lib.check(lib.mgpt_moe_op_residual_norm_keep(*args, x8.values.data_ptr(), x8.exponents.data_ptr(), h8.values.data_ptr(), h8.exponents.data_ptr(),
+                                                  _stream(device)))
+    return y, u, stats, (x8, h8)
 
 
-def residual_norm_backward(x: torch.Tensor, h: torch.Tensor, stats: torch.Tensor, dy: torch.Tensor, du: torch.Tensor = None, *, post_scale=None,
+def residual_norm_backward(x, h, stats: torch.Tensor, dy: torch.Tensor, du: torch.Tensor = None, *, post_scale=None,
                            gate=None, pre_scale=None, alpha: float = 1.0, eps: float = 1e-5, tokens_per_gate: int = 0, d_post_scale=None,
                            d_gate=None, d_pre_scale=None):
     """Gradients of :func:`residual_norm`: returns ``(dx, dh)`` and adds to ``d_post_scale``, ``d_gate`` and ``d_pre_scale`` (FP32,
     of the parameters' shapes) where they are given.  ``dy``: the gradient of y by its other uses; ``du``: that of u.  The other
-    arguments are those of the forward call (``eps`` is in ``stats`` already)."""
+    arguments are those of the forward call (``eps`` is in ``stats`` already).  x and h: the tensors, or both as the forward call (or
+    :func:`keep8`) kept them: the gradients are then the formulas' at the kept values, with the forward pass's ``stats``."""
     lib = _lib.load()
-    device, n, C, rows, tokens_per_gate, xp, hp, post, gp, pre = _norm_args(x, h, post_scale, gate, pre_scale, tokens_per_gate)
+    kept = isinstance(x, Kept8) or isinstance(h, Kept8)
+    device, n, C, rows, tokens_per_gate, xp, hp, post, gp, pre = _norm_args(x, h, post_scale, gate, pre_scale, tokens_per_gate, dy if kept else None)
     f32 = _F32
     sp = _check(stats, "stats", (2, n), f32, device)
-    dyp, dup = _check(dy, "dy", x.shape, (x.dtype,), device), _optional(du, "du", x.shape, (x.dtype,), device)
+    dyp, dup = _check(dy, "dy", x.shape, (dy.dtype if kept else x.dtype,), device), _optional(du, "du", x.shape, (dy.dtype,), device)
     if d_gate is not None and d_gate.dim() == 1 and rows == 1 and d_gate.numel() == C:
         d_gate = d_gate.view(1, C)
     dpost, dgate, dpre = (_optional(d_post_scale, "d_post_scale", (C,), f32, device), _optional(d_gate, "d_gate", (rows, C), f32, device),
                           _optional(d_pre_scale, "d_pre_scale", (C,), f32, device))
-    dx, dh = torch.empty_like(x), torch.empty_like(x)
+    dx, dh = torch.empty_like(dy), torch.empty_like(dy)
     size = lib.mgpt_moe_op_residual_norm_backward_workspace_bytes(n, C, tokens_per_gate)
     ws = _workspace(size, device)
-    _lib.check(lib.mgpt_moe_op_residual_norm_backward(xp, hp, _DTYPES[x.dtype], post, gp, tokens_per_gate, pre, alpha, n, C, sp, dyp, dup,
-                                                      dx.data_ptr(), dh.data_ptr(), dpost, dgate, dpre, ws.data_ptr(), size, _stream(device)))
+    args = (_DTYPES[dy.dtype], post, gp, tokens_per_gate, pre, alpha, n, C, sp, dyp, dup, dx.data_ptr(), dh.data_ptr(), dpost, dgate, dpre, ws.data_ptr(), size,
+            _stream(device))
+    _lib.check(lib.mgpt_moe_op_residual_norm_backward_kept(*xp, *hp, *args) if kept else lib.mgpt_moe_op_residual_norm_backward(xp, hp, *args))
     return dx, dh
 
 
