@@ -72,8 +72,10 @@ Workspace make_workspace(const Dims& d, int n_tokens, int kind)
     w.seg = take(E * MAX_SOURCES * 2 * 4);
     w.tile_order = take((size_t)w.max_tiles * 4);
     w.Xg = take(rowbuf * rc * C * ab);
-    w.G = take(bwd * big * rc * H * ab);
-    w.U = take(bwd * big * rc * H * ab);
+    // (gate and up themselves where the CUDA cores form Hh from them, in inference too)
+    const size_t gu = bwd || d.mode != MGPT_MOE_BF16 || d.gemm_impl != 0 ? 1 : 0;
+    w.G = take(gu * big * rc * H * ab);
+    w.U = take(gu * big * rc * H * ab);
     w.Hh = take(big * rc * H * ab);
     w.Yg = take(rowbuf * rc * C * ab);
     w.dYg = take(bwd * rowbuf * rc * C * ab);
