@@ -48,27 +48,13 @@ struct RouteP {
 __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(bf16 v) { return __bfloat162float(v); }
 
-// Numbers as unsigned integers of the same order: minus infinity is NONE, and 0 is below every number.  (-0 and 0 are equal.)
-template <typename V> struct Ordered;
-template <> struct Ordered<float> {
-    using U = uint32_t;
-    static __device__ __forceinline__ U key(float v)
-    {
-        const uint32_t u = __float_as_uint(v + 0.0f);
-        return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
-    }
-    static __device__ __forceinline__ float value(U k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
-};
-template <> struct Ordered<double> {
-    using U = unsigned long long;
-    static constexpr U NONE = 0x000fffffffffffffull;
-    static __device__ __forceinline__ U key(double v)
-    {
-        const long long u = __double_as_longlong(v + 0.0);
-        return (U)u ^ ((U)(u >> 63) | 0x8000000000000000ull);
-    }
-};
-
+// Numbers as unsigned integers of the same order, and back.
+__device__ __forceinline__ uint32_t ordered(float v)
+{
+    const uint32_t u = __float_as_uint(v);
+    return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float from_ordered(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 // over the L lanes of a token
 template <int L, typename V> __device__ __forceinline__ V lanes_max(V v)
 {
@@ -81,13 +67,16 @@ template <int L, typename V> __device__ __forceinline__ V lanes_max(V v)
 }
 template <int L, typename V> __device__ __forceinline__ V lanes_min(V v)
 {
-    if constexpr (L == 32 && sizeof(V) == 4 && (V)(-1) > (V)0) return __reduce_min_sync(FULL, v);
+    if constexpr (L == 32 && sizeof(V) == 4 && (V)(-1) > (V)0) {
+        return __reduce_min_sync(FULL, v);
+    } else {
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) {
-        const V other = __shfl_xor_sync(FULL, v, o);
-        v = other < v ? other : v;
+        for (int o = L / 2; o > 0; o >>= 1) {
+            const V other = __shfl_xor_sync(FULL, v, o);
+            v = other < v ? other : v;
+        }
+        return v;
     }
-    return v;
 }
 template <int L, typename V> __device__ __forceinline__ V lanes_sum(V v)
 {
@@ -97,10 +86,13 @@ template <int L, typename V> __device__ __forceinline__ V lanes_sum(V v)
 }
 template <int L> __device__ __forceinline__ uint32_t lanes_or(uint32_t v)
 {
-    if constexpr (L == 32) return __reduce_or_sync(FULL, v);
+    if constexpr (L == 32) {
+        return __reduce_or_sync(FULL, v);
+    } else {
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) v |= __shfl_xor_sync(FULL, v, o);
-    return v;
+        for (int o = L / 2; o > 0; o >>= 1) v |= __shfl_xor_sync(FULL, v, o);
+        return v;
+    }
 }
 __device__ __forceinline__ float max_nan(float a, float b)
 {
@@ -111,10 +103,13 @@ __device__ __forceinline__ float max_nan(float a, float b)
 // the largest, or a NaN where there is one
 template <int L> __device__ __forceinline__ float lanes_max_nan(float v)
 {
-    if constexpr (L == 32) return Ordered<float>::value(__reduce_max_sync(FULL, Ordered<float>::key(v)));      // (max.NaN's NaN is above infinity)
+    if constexpr (L == 32) {
+        return from_ordered(__reduce_max_sync(FULL, ordered(v)));          // (max.NaN's NaN is above infinity)
+    } else {
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(FULL, v, o));
-    return v;
+        for (int o = L / 2; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(FULL, v, o));
+        return v;
+    }
 }
 template <int L> __device__ __forceinline__ uint32_t lanes_of(int t) { return L == 32 ? FULL : ((1u << (L & 31)) - 1) << (t * L); }
 
@@ -206,87 +201,153 @@ template <typename V, int L> __device__ __forceinline__ uint32_t choose_groups(c
     return lanes_or<L>(kept);
 }
 
-// The chosen experts of the warp's tokens into `chosen` [tokens][k], all in FP64.  top: the token's largest logit.
-template <typename T, int L, int P>
-__device__ __noinline__ void choose_again(const RouteP& p, int tok, bool have, float top, double* c, int32_t* chosen)
+// A token's weights from its chosen experts: a lane per chosen expert of the warp's tokens.  sht: top and 1 / sum of exp(z - top), then the factor.
+template <typename T, int L>
+__device__ __forceinline__ void weigh(const RouteP& p, int tok0, const int32_t* chosen, float* weights, float4* sht, int32_t* hist, float top, float inv, bool bad)
 {
-    using O = Ordered<double>;
     const int lane = threadIdx.x & 31, sub = lane % L, mt = lane / L;
-    O::U key[P];
-    double v[P], sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-        const int e = i * L + sub;
-        const float z = have && e < p.E ? as_float(((const T*)p.logits)[(size_t)tok * p.E + e]) : -INFINITY;
-        v[i] = z;
-        if (p.softmax && z > -INFINITY) sum += exp((double)z - (double)top);
+    if (sub == 0) sht[mt] = make_float4(top, inv, 0.0f, 0.0f);
+    __syncwarp();
+    const int slots = min(32 / L, p.n - tok0) * p.k;
+    for (int q = lane; q < slots; q += 32) {
+        const int t = q * p.kdiv >> 16, e = chosen[q];
+        const float v = as_float(((const T*)p.logits)[(size_t)(tok0 + t) * p.E + e]);
+        const float4 of = sht[t];
+        float s = p.softmax ? (v > -INFINITY ? expf(v - of.x) * of.y : 0.0f) : sigmoid(v);
+        if (p.bias && !(p.bias[e] > -INFINITY)) s = 0.0f;
+        weights[q] = s;
+        p.idx[(size_t)tok0 * p.k + q] = e;
+        if (p.counts) atomicAdd(&hist[e], 1);
     }
-    const double inv = 1.0 / lanes_sum<L>(sum);
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-        const int e = i * L + sub;
-        const float b = p.bias && e < p.E ? p.bias[e] : 0.0f;
-        const bool out = !(v[i] > -INFINITY) || !(b > -INFINITY);
-        double s = -INFINITY;
-        if (!out) s = (p.softmax ? exp(v[i] - (double)top) * inv : 1.0 / (1.0 + exp(-v[i]))) + (double)b;
-        if (e < p.E) c[mt * p.E + e] = s;
-        key[i] = e >= p.E ? 0 : out ? O::NONE : O::key(p.bias ? s : v[i]);
+    __syncwarp();
+    float factor = p.scale;
+    if (p.renorm) {
+        float sum = 0.0f;
+#pragma unroll 4
+        for (int j = 0; j < p.k; ++j) sum += weights[mt * p.k + j];
+        factor = p.scale / (sum + TINY);
+    }
+    if (sub == 0) sht[mt].z = bad ? NAN : factor;
+    __syncwarp();
+    for (int q = lane; q < slots; q += 32) p.w[(size_t)tok0 * p.k + q] = weights[q] * sht[q * p.kdiv >> 16].z;
+    __syncwarp();
+}
+
+// The tokens of a warp from their logits, all scores in FP64.  (Loops rather than unrolled code: this is rare, and what is not in the
+// instruction cache costs more than it computes.)  c: [tokens][E] scores, then [tokens][groups].
+template <typename T, int L>
+__device__ __noinline__ void route_again(const RouteP& p, int tok0, double* c, int32_t* chosen, float4* sht, int32_t* hist)
+{
+    const int lane = threadIdx.x & 31, sub = lane % L, mt = lane / L, tok = tok0 + mt;
+    const bool have = tok < p.n;
+    const T* const row = (const T*)p.logits + (size_t)tok * p.E;
+    double* const mine = c + mt * p.E;
+    float top = -INFINITY;
+    uint32_t taken = 0;                         // bits of the lane's experts i * L + sub
+#pragma unroll 4
+    for (int e = sub; e < p.E; e += L) top = max_nan(top, have ? as_float(row[e]) : -INFINITY);
+    top = lanes_max_nan<L>(top);
+    const bool bad = top != top || (p.softmax && top == INFINITY);
+    double inv = 1.0;
+    if (p.softmax) {
+        double sum = 0.0;
+#pragma unroll 2
+        for (int e = sub; e < p.E; e += L) {
+            const float z = have ? as_float(row[e]) : -INFINITY;
+            const double s = z > -INFINITY ? exp((double)z - (double)top) : 0.0;
+            mine[e] = s;
+            sum += s;
+        }
+        sum = lanes_sum<L>(sum);
+        inv = sum > 0.0 ? 1.0 / sum : 0.0;
+    }
+    // (minus infinity: out)
+#pragma unroll 2
+    for (int e = sub; e < p.E; e += L) {
+        const float z = have ? as_float(row[e]) : -INFINITY;
+        double s = p.softmax ? mine[e] * inv : 1.0 / (1.0 + exp(-(double)z));
+        if (p.bias) s = p.bias[e] > -INFINITY ? s + (double)p.bias[e] : -INFINITY;
+        mine[e] = z > -INFINITY && s > -INFINITY ? s : -INFINITY;
     }
     if (p.top_groups < p.groups) {
         __syncwarp();
         bool close;
         const uint32_t kept = choose_groups<double, L>(p, c, sub, mt, 0.0f, &close);
-#pragma unroll
-        for (int i = 0; i < P; ++i)
-            if (!(kept >> ((uint32_t)(i * L + sub) * p.gdiv >> 20) & 1)) key[i] = 0;
+        for (int i = 0, e = sub; e < p.E; ++i, e += L)
+            if (!(kept >> ((uint32_t)e * p.gdiv >> 20) & 1)) taken |= 1u << i;
     }
+    if (!p.bias && have)                        // the logits' own order
+        for (int e = sub; e < p.E; e += L) mine[e] = as_float(row[e]) > -INFINITY ? (double)as_float(row[e]) : -INFINITY;
     for (int j = 0; j < p.k; ++j) {
-        O::U best = key[0];
-#pragma unroll
-        for (int i = 1; i < P; ++i) best = key[i] > best ? key[i] : best;
-        const O::U m = lanes_max<L>(best);
-        int e = 0x7fffffff;
-#pragma unroll
-        for (int i = P - 1; i >= 0; --i) e = key[i] == m ? i * L + sub : e;
-        e = lanes_min<L>(e);
-#pragma unroll
-        for (int i = 0; i < P; ++i)
-            if (e == i * L + sub) key[i] = 0;
+        constexpr int NOBODY = 0x7fffffff;
+        double best = -INFINITY;
+        int at = NOBODY;
+#pragma unroll 4
+        for (int i = 0, e = sub; e < p.E; ++i, e += L) {
+            const double v = mine[e];
+            if (!(taken >> i & 1) && (at == NOBODY || v > best)) {
+                best = v;
+                at = e;
+            }
+        }
+        const double m = lanes_max<L>(best);
+        const int e = lanes_min<L>(best == m ? at : NOBODY);
+        if (e % L == sub) taken |= 1u << (e / L);
         if (sub == 0) chosen[mt * p.k + j] = e;
     }
     __syncwarp();
+    weigh<T, L>(p, tok0, chosen, (float*)c, sht, hist, top, (float)inv, bad);
 }
 
-// L lanes per token, P neighbouring experts each; 32 / L tokens per warp.  ORDERED: there is a bias or a choice of groups, else z alone decides.
+// exp(-z) and 1 / x to 2^-22 of themselves and the argument's rounding (of scores that only have to be near enough)
+__device__ __forceinline__ float near_exp(float v)
+{
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * 1.4426950409f));
+    return e;
+}
+__device__ __forceinline__ float near_over(float v)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// L lanes per token, P experts each; 32 / L tokens per warp.
 //
 // The rounds of the choice: a score becomes the number of steps of R / 2^23 that it is below a bound on all of them (23 bits; further
-// than R: the last step), and with 511 - e in the bits below, keys are unlike each other, equal scores go by index, and a round is the
-// largest key below the last round's: a subtraction and a minimum per expert, one reduction, nothing to cross out.  Two
-// keys in a row that are further apart than the scores may be wrong are in the right order.  Closer ones are looked at
-// when the rounds are over: those of equal inputs are, any others send the token to choose_again.
-template <typename T, int L, int P, bool ORDERED>
-__global__ void __launch_bounds__(32 * WARPS, P > 8 ? 4 : 8) route_kernel(const RouteP p)
+// than R: the last step, and so is what is out), with e + 1 added below: keys are unlike each other, equal scores go by index, and a round
+// is the least key above the last round's: an addition and a minimum per expert, one reduction, nothing to cross out.  Two
+// keys in a row that are further apart than the scores may be wrong are in the right order.  Where some are not, what was chosen and
+// what is not far enough behind it are put in order by their exact values (FP64; the logits themselves where they decide).  Groups
+// whose scores are too close send the token to route_again.
+enum { BY_LOGIT, BY_SCORE, BY_GROUP };          // no bias and no choice of groups; a bias; groups
+template <typename T, int L, int P, int HOW>
+__global__ void __launch_bounds__(32 * WARPS, P > 8 ? 5 : 8) route_kernel(const RouteP p)
 {
-    constexpr int TOKENS = 32 / L, SLOTS = TOKENS * (8 * L < ROUTE_MAX_K ? 8 * L : ROUTE_MAX_K);
-    constexpr int SCORES = 32 * (TOKENS < P ? TOKENS : P);              // [tokens][groups]
-    constexpr uint32_t LAST = (1u << 23) - 3, OUT = 1u << 9;            // the last step; the keys of experts that are out (0: there is none)
-    __shared__ double shc[WARPS][32 * P + SCORES];
-    __shared__ int32_t shi[WARPS][SLOTS];
-    __shared__ float shw[WARPS][SLOTS];
+    constexpr int TOKENS = 32 / L, KM = P * L < ROUTE_MAX_K ? P * L : ROUTE_MAX_K, EXTRA = 4;
+    constexpr int FOR_GROUPS = 32 * P + 32 * (TOKENS < P ? TOKENS : P), FOR_ORDER = TOKENS * (KM + EXTRA + EXTRA / 2 + KM / 2);
+    constexpr uint32_t LAST = 0x4b000000u + (1u << 23) - 3, NONE = 0xffffffffu;     // the last step, as a number of 2^23 and more; no expert
+    __shared__ double shc[WARPS][FOR_GROUPS > FOR_ORDER ? FOR_GROUPS : FOR_ORDER];
+    __shared__ int32_t shi[WARPS][TOKENS * KM];
     __shared__ float4 sht[WARPS][TOKENS];
     __shared__ int32_t hist[ROUTE_MAX_E];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % L, mt = lane / L, e0 = sub * P;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % L, mt = lane / L;
+    // The lane's experts: neighbours, so that a group is a run of lanes; else four and four (a warp's loads are runs of memory).
+    const int e0 = HOW == BY_GROUP ? sub * P : sub * 4;
+    auto expert = [&](int i) { return e0 + (HOW == BY_GROUP ? i : i / 4 * (4 * L) + i % 4); };
+    double* const scratch = shc[warp];
     pdl_wait();
     if (p.counts) {
         for (int e = threadIdx.x; e < p.E; e += 32 * WARPS) hist[e] = 0;
         __syncthreads();
     }
-    const bool by_score = ORDERED && p.bias;
+    const bool by_score = HOW == BY_SCORE || (HOW == BY_GROUP && p.bias);
     float b[P], bhi = -INFINITY, blo = INFINITY;                        // (out by the bias: minus infinity)
-    if constexpr (ORDERED) {
+    if constexpr (HOW != BY_LOGIT) {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            b[i] = p.bias && e0 + i < p.E ? p.bias[e0 + i] : 0.0f;
+            b[i] = p.bias && expert(i) < p.E ? p.bias[expert(i)] : 0.0f;
             if (b[i] > -INFINITY) {
                 bhi = fmaxf(bhi, b[i]);
                 blo = fminf(blo, b[i]);
@@ -300,172 +361,208 @@ __global__ void __launch_bounds__(32 * WARPS, P > 8 ? 4 : 8) route_kernel(const 
     }
     const float bmax = fmaxf(fabsf(bhi), fabsf(blo)), rounding = 6e-8f * (1.0f + bmax);       // (of a score with its bias)
     int32_t* const chosen = shi[warp];
-    for (int tok0 = (blockIdx.x * WARPS + warp) * TOKENS; tok0 < p.n; tok0 += gridDim.x * WARPS * TOKENS) {
-        const int tok = tok0 + mt;
-        const bool have = tok < p.n;
+    const int stride = gridDim.x * WARPS * TOKENS;
+    float z[P];
+    auto load = [&](int tok) {
         const T* const row = (const T*)p.logits + (size_t)tok * p.E;
-        float z[P], top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < P; i += 4) {
             float v[4];
-            load_four(row, have ? e0 + i : p.E, p.E, p.vec, -INFINITY, v);
+            load_four(row, tok < p.n ? expert(i) : p.E, p.E, p.vec, -INFINITY, v);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                z[i + c] = v[c];
-                top = max_nan(top, v[c]);
-            }
+            for (int c = 0; c < 4; ++c) z[i + c] = v[c];
         }
-        // a NaN (softmax: or infinity) among the logits
-        const bool bad = __ballot_sync(FULL, top != top || (p.softmax && top == INFINITY)) & lanes_of<L>(mt);
-        if (!by_score || p.softmax) top = lanes_max_nan<L>(top);
-        float inv = 1.0f;                       // (what the weights are divided by has exp(0) in it, where they are all there is)
-        uint32_t key[P], apart = 1;
-        bool unsure = false;
-        if constexpr (ORDERED) {
-            float c[P];
-            if (p.softmax) {
-                float sum = 0.0f;
+    };
+    int begin = (blockIdx.x * WARPS + warp) * TOKENS;
+    load(begin + mt);
+    for (; begin < p.n; begin += 32 * stride) {
+        uint32_t again = 0;                     // of 32 rounds of the loop, those with tokens that need route_again
+        for (int round = 0, tok0 = begin; round < 32 && tok0 < p.n; ++round, tok0 += stride) {
+            const int tok = tok0 + mt;
+            const bool have = tok < p.n;
+            float top = z[0];
 #pragma unroll
-                for (int i = 0; i < P; ++i) {
-                    c[i] = z[i] > -INFINITY ? __expf(z[i] - top) : 0.0f;
-                    sum += c[i];
-                }
-                sum = lanes_sum<L>(sum);
-                inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-#pragma unroll
-                for (int i = 0; i < P; ++i) c[i] = z[i] > -INFINITY ? fmaf(c[i], inv, b[i]) : -INFINITY;
-            } else {
-#pragma unroll
-                for (int i = 0; i < P; ++i) c[i] = z[i] > -INFINITY ? __fdividef(1.0f, 1.0f + __expf(-z[i])) + b[i] : -INFINITY;
-            }
-            // How far a score may be off.  exp: (|argument| + 2) 2^-23 of itself.  A softmax's term: that, 0.37 * 2^-23 at most, and its
-            // share of the sum's error: as much in the mean (6.3 + 2) and 21 roundings; a sigmoid: (0.23 + 0.5) 2^-23, and
-            // 2^-24 and 2^-22 for the sum and the quotient.
-            const float most = p.softmax ? inv : 1.0f, base = p.softmax ? fmaf(2.6e-6f, inv, 8e-8f) : 4e-7f;
-            uint32_t outside = 0;               // bit i: not in a group that stays
-            if (p.top_groups < p.groups) {
-                // (a group's score: twice that, and three roundings of twice the size)
-                const float margin = 4.0f * base + 9.0f * rounding;
-                if (p.group_lanes) {
-                    float m1 = -INFINITY, m2 = -INFINITY;
+            for (int i = 1; i < P; ++i) top = max_nan(top, z[i]);
+            // a NaN (softmax: or infinity) among the logits
+            const bool bad = __ballot_sync(FULL, top != top || (p.softmax && top == INFINITY)) & lanes_of<L>(mt);
+            bool unsure = HOW != BY_LOGIT && top == INFINITY;
+            if (!by_score || p.softmax) top = lanes_max_nan<L>(top);
+            float inv = 1.0f;                   // (what the weights are divided by has exp(0) in it, where they are all there is)
+            uint32_t key[P], apart = 1;
+            if constexpr (HOW != BY_LOGIT) {
+                float c[P];                     // (NaN: out.  A logit of infinity has been seen to above)
+                if (p.softmax) {
+                    float sum = 0.0f;
 #pragma unroll
                     for (int i = 0; i < P; ++i) {
-                        m2 = fmaxf(m2, fminf(m1, c[i]));
-                        m1 = fmaxf(m1, c[i]);
+                        c[i] = z[i] > -INFINITY ? near_exp(z[i] - top) : 0.0f;
+                        sum += c[i];
                     }
-                    for (int o = p.group_lanes / 2; o > 0; o >>= 1) {
-                        const float n1 = __shfl_xor_sync(FULL, m1, o), n2 = __shfl_xor_sync(FULL, m2, o);
-                        m2 = fmaxf(fmaxf(m2, n2), fminf(m1, n1));
-                        m1 = fmaxf(m1, n1);
-                    }
-                    if (p.group_top == 2 && m2 > -INFINITY) m1 += m2;
-                    // the groups that may be ahead of this one (it is among them), and those that are
-                    int may = -1, are = 0;
-                    for (int g = 0; g < p.groups; ++g) {
-                        const float d = __shfl_sync(FULL, m1, mt * L + g * p.group_lanes) - m1;
-                        may += !(d <= -margin);
-                        are += d > margin;
-                    }
-                    if (may >= p.top_groups) {
-                        outside = FULL;
-                        unsure = e0 < p.E && are < p.top_groups;
-                    }
+                    sum = lanes_sum<L>(sum);
+                    inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < P; ++i) c[i] = fmaf(c[i], inv, fmaf(z[i], 0.0f, b[i]));
                 } else {
-                    float* const cs = (float*)shc[warp];
-                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < P; ++i) c[i] = near_over(1.0f + near_exp(-z[i])) + fmaf(z[i], 0.0f, b[i]);
+                }
+                // How far a score may be off.  exp: (|argument| + 2) 2^-23 of itself.  A softmax's term: that, 0.37 * 2^-23 at most, and its
+                // share of the sum's error: as much in the mean (6.3 + 2) and 21 roundings; a sigmoid: (0.23 + 0.5) 2^-23, and
+                // 2^-24 and 2^-22 for the sum and the quotient.
+                const float most = p.softmax ? inv : 1.0f, base = p.softmax ? fmaf(2.6e-6f, inv, 8e-8f) : 4e-7f;
+                uint32_t outside = 0;           // bit i: not in a group that stays
+                if constexpr (HOW == BY_GROUP) {
+                    // (a group's score: twice that, and three roundings of twice the size)
+                    const float margin = 4.0f * base + 9.0f * rounding;
+                    if (p.group_lanes) {
+                        float m1 = -INFINITY, m2 = -INFINITY;
+#pragma unroll
+                        for (int i = 0; i < P; ++i) {
+                            const float v = c[i] > -INFINITY ? c[i] : -INFINITY;
+                            m2 = fmaxf(m2, fminf(m1, v));
+                            m1 = fmaxf(m1, v);
+                        }
+                        for (int o = p.group_lanes / 2; o > 0; o >>= 1) {
+                            const float n1 = __shfl_xor_sync(FULL, m1, o), n2 = __shfl_xor_sync(FULL, m2, o);
+                            m2 = fmaxf(fmaxf(m2, n2), fminf(m1, n1));
+                            m1 = fmaxf(m1, n1);
+                        }
+                        if (p.group_top == 2 && m2 > -INFINITY) m1 += m2;
+                        // the groups that may be ahead of this one (it is among them), and those that are
+                        int may = -1, are = 0;
+                        for (int g = 0; g < p.groups; ++g) {
+                            const float d = __shfl_sync(FULL, m1, mt * L + g * p.group_lanes) - m1;
+                            may += !(d <= -margin);
+                            are += d > margin;
+                        }
+                        if (may >= p.top_groups) {
+                            outside = FULL;
+                            unsure |= e0 < p.E && are < p.top_groups;
+                        }
+                    } else {
+                        float* const cs = (float*)scratch;
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < P; ++i)
+                            if (expert(i) < p.E) cs[mt * p.E + expert(i)] = c[i];
+                        __syncwarp();
+                        bool near;
+                        const uint32_t kept = choose_groups<float, L>(p, cs, sub, mt, margin, &near);
+                        unsure |= near;
+#pragma unroll
+                        for (int i = 0; i < P; ++i) outside |= (~kept >> ((uint32_t)expert(i) * p.gdiv >> 20) & 1) << i;
+                    }
+                }
+                if (by_score) {
+                    const float bound = most + bhi + 4.0f * (base + rounding), R = fminf(bound - blo, 4.0f), S = 8388600.0f / R;
+                    apart = (uint32_t)fminf(2.0f * S * (base + rounding) + 4.0f, 4e6f);      // (and two roundings to steps)
+#pragma unroll
+                    for (int i = 0; i < P; ++i) key[i] = (min(__float_as_uint(fmaf(bound - c[i], S, 8388608.0f)), LAST) << 9) + (expert(i) + 1);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < P; ++i) key[i] = (min(__float_as_uint(fmaf(top - z[i], 524288.0f, 8388608.0f)), LAST) << 9) + (expert(i) + 1);
+                }
+                if (HOW == BY_GROUP) {
 #pragma unroll
                     for (int i = 0; i < P; ++i)
-                        if (e0 + i < p.E) cs[mt * p.E + e0 + i] = c[i];
-                    __syncwarp();
-                    const uint32_t kept = choose_groups<float, L>(p, cs, sub, mt, margin, &unsure);
-#pragma unroll
-                    for (int i = 0; i < P; ++i) outside |= (~kept >> ((uint32_t)(e0 + i) * p.gdiv >> 20) & 1) << i;
+                        if (outside >> i & 1) key[i] = NONE;
                 }
-            }
-            if (by_score) {
-                const float bound = most + bhi + 4.0f * (base + rounding), R = fminf(bound - blo, 4.0f), S = 8388600.0f / R;
-                apart = (uint32_t)fminf(2.0f * S * (base + rounding) + 4.0f, 4e6f);      // (and two roundings to steps)
-#pragma unroll
-                for (int i = 0; i < P; ++i) {
-                    const uint32_t q = min(__float_as_uint(fmaf(bound - c[i], S, 8388608.0f)) - 0x4b000000u, LAST);
-                    key[i] = c[i] > -INFINITY ? (0xffffffffu - e0 - i) - (q << 9) : OUT + 511 - e0 - i;
-                }
+                unsure = __ballot_sync(FULL, unsure) & lanes_of<L>(mt);         // (of all the token's lanes: there may be fewer than k keys then)
             } else {
+                // (the steps order logits: R = 16, and what is in another step is further up or down)
 #pragma unroll
-                for (int i = 0; i < P; ++i) {
-                    const uint32_t q = min(__float_as_uint(fmaf(top - z[i], 524288.0f, 8388608.0f)) - 0x4b000000u, LAST);
-                    key[i] = z[i] > -INFINITY ? (0xffffffffu - e0 - i) - (q << 9) : OUT + 511 - e0 - i;
+                for (int i = 0; i < P; ++i) key[i] = (min(__float_as_uint(fmaf(top - z[i], 524288.0f, 8388608.0f)), LAST) << 9) + (expert(i) + 1);
+                if (p.softmax && !p.renorm) {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < P; ++i) sum += z[i] > -INFINITY ? expf(z[i] - top) : 0.0f;
+                    sum = lanes_sum<L>(sum);
+                    inv = sum > 0.0f ? 1.0f / sum : 0.0f;
                 }
             }
+            if (p.E != L * P) {
 #pragma unroll
-            for (int i = 0; i < P; ++i)
-                if (e0 + i >= p.E || outside >> i & 1) key[i] = 0;
-        } else {
-            // (the steps order logits: R = 16, and what is in another step is further up or down)
-#pragma unroll
-            for (int i = 0; i < P; ++i) {
-                const uint32_t q = min(__float_as_uint(fmaf(top - z[i], 524288.0f, 8388608.0f)) - 0x4b000000u, LAST);
-                key[i] = e0 + i >= p.E ? 0 : z[i] > -INFINITY ? (0xffffffffu - e0 - i) - (q << 9) : OUT + 511 - e0 - i;
+                for (int i = 0; i < P; ++i)
+                    if (expert(i) >= p.E) key[i] = NONE;
             }
-            if (p.softmax && !p.renorm) {
-                float sum = 0.0f;
+            load(tok + stride);                 // (what the next round needs, on its way meanwhile)
+            apart <<= 9;
+            // the least key above `last` (a key that was taken is further, modulo 2^32, than any other), and one less than how far it is
+            auto beyond = [&](uint32_t last, uint32_t* m) {
+                const uint32_t from = ~last;
+                uint32_t part[4];               // (chains side by side)
 #pragma unroll
-                for (int i = 0; i < P; ++i) sum += z[i] > -INFINITY ? expf(z[i] - top) : 0.0f;
-                sum = lanes_sum<L>(sum);
-                inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+                for (int i = 0; i < P; ++i) part[i % 4] = i < 4 ? key[i] + from : min(key[i] + from, part[i % 4]);
+                const uint32_t next = lanes_min<L>(min(min(part[0], part[1]), min(part[2], part[3])));
+                *m = next - from;
+                return next;
+            };
+            uint32_t last = NONE, close = 0, bit = 0;
+            int32_t* const to = chosen + mt * p.k;
+            for (int j = 0; j < p.k; ++j) {
+                if (beyond(last, &last) < apart) close |= bit;
+                bit = bit ? bit << 1 : 1;
+                if (sub == 0) to[j] = (last - 1) & 511;
             }
-        }
-        apart <<= 9;
-        uint32_t last = 0, close = 0;
-        for (int j = 0; j <= p.k; ++j) {
-            // (a key that was taken is last or more: its distance is last or more, all others' is less)
-            uint32_t below = last - 1 - key[0];
-#pragma unroll
-            for (int i = 1; i < P; ++i) below = min(below, last - 1 - key[i]);
-            const uint32_t m = last - 1 - lanes_min<L>(below);
-            if (j > 0 && last - m < apart && m >= 2 * OUT) close |= 1u << (j - 1);
-            if (sub == 0 && j < p.k) chosen[mt * p.k + j] = 511 - (m & 511);
-            last = m;
-        }
-        __syncwarp();
-        if (__any_sync(FULL, close && !bad)) {
-            if (!unsure && have && !bad)
-                for (uint32_t left = close; left; left &= left - 1) {
-                    const int j = __ffs(left) - 1, e = chosen[mt * p.k + j], f = j + 1 < p.k ? chosen[mt * p.k + j + 1] : 511 - (last & 511);
-                    unsure |= !(as_float(row[e]) == as_float(row[f]) && (!by_score || p.bias[e] == p.bias[f]));
-                }
-        }
-        if (__any_sync(FULL, unsure && have)) {
-            // (`top` is every token's largest logit, but for a sigmoid under a bias, which does not need it)
+            uint32_t next;                      // the first that was not chosen
+            if (beyond(last, &next) < apart && next != NONE && next > last) close |= bit;
             __syncwarp();
-            choose_again<T, L, P>(p, tok, have, top, shc[warp], chosen);
+            if (__any_sync(FULL, close && !bad)) {
+                double* const value = scratch + mt * (KM + EXTRA);
+                int32_t* const behind = (int32_t*)(scratch + TOKENS * (KM + EXTRA)) + mt * EXTRA;
+                int32_t* const sorted = (int32_t*)(scratch + TOKENS * (KM + EXTRA + EXTRA / 2)) + mt * KM;
+                const T* const row = (const T*)p.logits + (size_t)tok * p.E;
+                int count = close && have && !bad && !unsure ? p.k : 0;
+                bool more = count && close & bit;
+                while (__any_sync(FULL, more)) {
+                    if (more) {
+                        if (count < p.k + EXTRA) {
+                            if (sub == 0) behind[count - p.k] = (next - 1) & 511;
+                            ++count;
+                        } else {
+                            unsure = true;
+                            more = false;
+                            count = 0;
+                        }
+                    }
+                    uint32_t m;
+                    const uint32_t step = beyond(next, &m);
+                    if (step >= apart || m == NONE || m < next) more = false;
+                    if (more) next = m;
+                }
+                double over = 1.0;
+                if (by_score && p.softmax) {
+                    double sum = 0.0;
+#pragma unroll 2
+                    for (int e = sub; e < p.E; e += L)
+                        if (count && as_float(row[e]) > -INFINITY) sum += exp((double)as_float(row[e]) - (double)top);
+                    over = 1.0 / lanes_sum<L>(sum);
+                }
+                __syncwarp();
+                for (int j = sub; j < count; j += L) {
+                    const int e = j < p.k ? to[j] : behind[j - p.k];
+                    const float x = as_float(row[e]), y = by_score ? p.bias[e] : 0.0f;
+                    double v = x;
+                    if (by_score) v = (p.softmax ? exp(v - (double)top) * over : 1.0 / (1.0 + exp(-v))) + (double)y;
+                    value[j] = x > -INFINITY && y > -INFINITY ? v : -INFINITY;
+                }
+                __syncwarp();
+                for (int j = sub; j < count; j += L) {
+                    const int e = j < p.k ? to[j] : behind[j - p.k];
+                    const double v = value[j];
+                    int before = 0;
+                    for (int i = 0; i < count; ++i) before += value[i] > v || (value[i] == v && (i < p.k ? to[i] : behind[i - p.k]) < e);
+                    if (before < p.k) sorted[before] = e;
+                }
+                __syncwarp();
+                if (count)
+                    for (int j = sub; j < p.k; j += L) to[j] = sorted[j];
+                __syncwarp();
+            }
+            if (__any_sync(FULL, unsure && have)) again |= 1u << round;
+            else weigh<T, L>(p, tok0, chosen, (float*)scratch, sht[warp], hist, top, inv, bad);
         }
-        // weights: a lane per chosen expert
-        if (sub == 0) sht[warp][mt] = make_float4(top, inv, 0.0f, 0.0f);
-        __syncwarp();
-        const int slots = min(TOKENS, p.n - tok0) * p.k;
-        for (int q = lane; q < slots; q += 32) {
-            const int t = q * p.kdiv >> 16, e = chosen[q];
-            const float v = as_float(((const T*)p.logits)[(size_t)(tok0 + t) * p.E + e]);
-            const float4 of = sht[warp][t];
-            float s = p.softmax ? (v > -INFINITY ? expf(v - of.x) * of.y : 0.0f) : sigmoid(v);
-            if (by_score && !(p.bias[e] > -INFINITY)) s = 0.0f;
-            shw[warp][q] = s;
-            p.idx[(size_t)tok0 * p.k + q] = e;
-            if (p.counts) atomicAdd(&hist[e], 1);
-        }
-        __syncwarp();
-        float factor = p.scale;
-        if (p.renorm) {
-            float sum = 0.0f;
-#pragma unroll 4
-            for (int j = 0; j < p.k; ++j) sum += shw[warp][mt * p.k + j];
-            factor = p.scale / (sum + TINY);
-        }
-        if (sub == 0) sht[warp][mt].z = bad ? NAN : factor;
-        __syncwarp();
-        for (int q = lane; q < slots; q += 32) p.w[(size_t)tok0 * p.k + q] = shw[warp][q] * sht[warp][q * p.kdiv >> 16].z;
-        __syncwarp();
+        for (; again; again &= again - 1) route_again<T, L>(p, begin + (__ffs(again) - 1) * stride, scratch, chosen, sht[warp], hist);
     }
     if (p.counts) {
         __syncthreads();
@@ -644,11 +741,12 @@ __global__ void __launch_bounds__(32 * WARPS) route_softmax_bwd_kernel(const Rou
     }
 }
 
-template <typename T, int L, int P> int run_fwd(const RouteP& p, cudaStream_t st)
+template <typename T, int L, int P> int run_fwd(RouteP& p, cudaStream_t st)
 {
-    const int per = WARPS * (32 / L), want = (p.n + per - 1) / per, most = 148 * 8;
-    const bool ordered = p.bias || p.top_groups < p.groups;
-    MGPT_CUDA(launch_pdl(ordered ? route_kernel<T, L, P, true> : route_kernel<T, L, P, false>, want < most ? want : most, 32 * WARPS, 0, st, p));
+    const int per = WARPS * (32 / L), want = (p.n + per - 1) / per, most = 148 * (P > 8 ? 5 : 8), lanes = p.gsize / P;
+    p.group_lanes = p.gsize % P == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
+    void (*const kernel)(RouteP) = p.top_groups < p.groups ? route_kernel<T, L, P, BY_GROUP> : p.bias ? route_kernel<T, L, P, BY_SCORE> : route_kernel<T, L, P, BY_LOGIT>;
+    MGPT_CUDA(launch_pdl(kernel, want < most ? want : most, 32 * WARPS, 0, st, p));
     MGPT_LAUNCHED("route_kernel");
     return 0;
 }
@@ -680,9 +778,12 @@ template <typename T> int run_sigmoid_bwd(const RouteP& p, cudaStream_t st)
 template <typename T> int run_fwd(RouteP& p, cudaStream_t st)
 {
     p.vec = p.E % 4 == 0 && ((uintptr_t)p.logits & (4 * sizeof(T) - 1)) == 0;
-    const int per_lane = p.E <= 256 ? 8 : 16, lanes = p.gsize / per_lane;
-    p.group_lanes = p.gsize % per_lane == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
-    return MGPT_BY_EXPERTS(run_fwd, T);
+    if (p.E > 256) return run_fwd<T, 32, 16>(p, st);
+    if ((int64_t)p.n * p.E > 148 * 32 * 128)
+        return p.E <= 16 ? run_fwd<T, 1, 16>(p, st) : p.E <= 32 ? run_fwd<T, 2, 16>(p, st) : p.E <= 64 ? run_fwd<T, 4, 16>(p, st)
+               : p.E <= 128 ? run_fwd<T, 8, 16>(p, st) : run_fwd<T, 16, 16>(p, st);
+    return p.E <= 8 ? run_fwd<T, 1, 8>(p, st) : p.E <= 16 ? run_fwd<T, 2, 8>(p, st) : p.E <= 32 ? run_fwd<T, 4, 8>(p, st)
+           : p.E <= 64 ? run_fwd<T, 8, 8>(p, st) : p.E <= 128 ? run_fwd<T, 16, 8>(p, st) : run_fwd<T, 32, 8>(p, st);
 }
 template <typename T> int run_bwd(RouteP& p, cudaStream_t st)
 {

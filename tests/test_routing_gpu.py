@@ -122,6 +122,20 @@ def test_scores_closer_than_fp32(E):
         _check(z, 5, score=score, bias=torch.zeros(E, device="cuda"), renormalise=True)
         _check(z, 5, score=score, bias=torch.zeros(E, device="cuda"), groups=E // 2, top_groups=E // 4) if E == 16 else None
         _check(z, 5, score=score)
+    z[:, 3::8] = z[:, 0::8]                                             # equal ones, and a better one behind them
+    for k in (1, 2, 3, 4):
+        _check(z, k)
+        _check(z, k, score="sigmoid", bias=torch.zeros(E, device="cuda"))
+    z[:, :] = 1.0
+    z[:, E - 1] = torch.nextafter(z[:, E - 1], z[:, E - 1] + 1)
+    z[1, E - 1] = 1e9
+    z[2, : E // 2] = -1e9
+    z[3, 5] = math.inf
+    for k in (1, 2, 3, 4):
+        _check(z, k, score="sigmoid")
+        _check(z, k, score="sigmoid", bias=torch.zeros(E, device="cuda"))
+        _check(z[:3], k)
+        _check(z[:3], k, bias=torch.zeros(E, device="cuda"))
     z = torch.linspace(18.0, 30.0, E, device="cuda").repeat(4, 1)       # sigmoids that are 1 in FP32
     _check(z, 5, score="sigmoid", bias=torch.zeros(E, device="cuda"))
     _check(z.flip(1), 5, score="sigmoid")
