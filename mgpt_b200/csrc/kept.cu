@@ -83,7 +83,7 @@ template <typename T> __global__ void __launch_bounds__(THREADS) keep8_kernel(co
             F2 v[E / 2];
             uint32_t w[E / 4];
             widen_piece(u[k], v, T());
-            const uint32_t byte = kept_pack<E>(v, w);
+            const uint32_t byte = kept_pack<T>(u[k], v, w);
             if (at + k * step < end) {
                 store_words<E>(p.v + at + k * step, w);
                 if (threadIdx.x % G == 0) p.e[group + k * group_step] = (uint8_t)byte;
@@ -110,7 +110,11 @@ template <typename T> __global__ void __launch_bounds__(THREADS) restore8_kernel
                 F2 v[E / 2];
                 const F2 unit(kept_unit(byte[k]));
 #pragma unroll
-                for (int j = 0; j < E / 4; ++j) kept_unpack(w[k][j], unit, v[2 * j], v[2 * j + 1]);
+                for (int j = 0; j < E / 4; ++j) {
+                    kept_unpack(w[k][j], v[2 * j], v[2 * j + 1]);
+                    v[2 * j] = v[2 * j] * unit;
+                    v[2 * j + 1] = v[2 * j + 1] * unit;
+                }
                 *reinterpret_cast<uint4*>((T*)p.out + at + k * step) = narrow_piece(v, T());
             }
     });

@@ -18,46 +18,52 @@ __device__ __forceinline__ uint32_t kept_exponent(uint32_t largest)
     const uint32_t e = (largest + 0x10000u) >> 23;
     return largest >= 0x7f800000u ? 255u : min(max(e, 7u), 254u) - 6u;
 }
-__device__ __forceinline__ float kept_units(uint32_t byte) { return __uint_as_float(byte == 255u ? 0u : (254u - byte) << 23); }     // 2^-e
 __device__ __forceinline__ float kept_unit(uint32_t byte) { return __uint_as_float(byte == 255u ? 0x7fffffffu : byte << 23); }     // 2^e, or NaN
-
 __device__ __forceinline__ float at_most(float v, uint32_t top) { return copysignf(fminf(fabsf(v), __uint_as_float(top)), v); }
 
-// N values of one lane (8 or 4), all of a group in 32 / N neighbouring lanes, which all call it (with zeros beyond the row's end):
-// the group's byte, and the values packed.
-template <int N> __device__ __forceinline__ uint32_t kept_pack(const F2 (&v)[N / 2], uint32_t (&packed)[N / 4])
+// The bits of the largest magnitude of a lane's values, as they lie in registers (BF16: two to a word, their maxima side by side until the end).
+__device__ __forceinline__ uint32_t kept_larger(uint32_t a, uint32_t b, bf16) { return __vmaxu2(a, b); }
+__device__ __forceinline__ uint32_t kept_larger(uint32_t a, uint32_t b, float) { return max(a, b); }
+template <typename T> __device__ __forceinline__ uint32_t kept_largest(const uint4& u)
 {
-    uint32_t m = 0;
+    constexpr uint32_t M = sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu;
+    uint32_t m = kept_larger(kept_larger(u.x & M, u.y & M, T()), kept_larger(u.z & M, u.w & M, T()), T());
 #pragma unroll
-    for (int j = 0; j < N / 2; ++j) {
-        const uint32_t a = __float_as_uint(v[j].lo()) & 0x7fffffffu, b = __float_as_uint(v[j].hi()) & 0x7fffffffu;
-        m = max(m, max(a, b));
+    for (int o = KEPT_GROUP * (int)sizeof(T) / 32; o > 0; o >>= 1) m = kept_larger(m, __shfl_xor_sync(0xffffffffu, m, o), T());
+    return sizeof(T) == 2 ? max(m & 0xffff0000u, m << 16) : m;
+}
+
+// 16 bytes of T of one lane, all of a group in neighbouring lanes, which all call it (with zeros beyond the row's end): the group's byte,
+// and the values packed.  v: the same values.
+template <typename T> __device__ __forceinline__ uint32_t kept_pack(const uint4& u, const F2 (&v)[8 / sizeof(T)], uint32_t (&packed)[4 / sizeof(T)])
+{
+    const uint32_t m = kept_largest<T>(u);
+    uint32_t e = max((m + 0x10000u) >> 23, 7u);                     // 6 more than the byte, but for the largest numbers
+    F2 units(__uint_as_float((260u - e) << 23)), magic(12582912.0f);       // 2^-e; 1.5 * 2^23: a sum's last byte is the whole number in two's complement
+    F2 a[8 / sizeof(T)];
+#pragma unroll
+    for (int j = 0; j < 8 / (int)sizeof(T); ++j) a[j] = fma2(v[j], units, magic);
+    if (__builtin_expect(m >= 0x7f7f0000u, 0)) {
+        e = kept_exponent(m) + 6u;
+        if (e == 254u) units = F2(0x1p-121f);
+#pragma unroll
+        for (int j = 0; j < 8 / (int)sizeof(T); ++j) a[j] = F2(at_most(v[j].lo(), 0x7f7e0000u), at_most(v[j].hi(), 0x7f7e0000u)) * units + magic;      // 127 * 2^121
     }
 #pragma unroll
-    for (int o = KEPT_GROUP / N / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const uint32_t byte = kept_exponent(m);
-    const uint32_t top = byte == 248u ? 0x7f7e0000u : 0xffffffffu;      // 127 * 2^121
-    const F2 units(kept_units(byte)), magic(12582912.0f);       // 1.5 * 2^23: the sum's last byte is the whole number in two's complement
-#pragma unroll
-    for (int j = 0; j < N / 4; ++j) {
-        F2 a = fma2(v[2 * j], units, magic), b = fma2(v[2 * j + 1], units, magic);
-        if (__builtin_expect(m > top, 0)) {
-            a = F2(at_most(v[2 * j].lo(), top), at_most(v[2 * j].hi(), top)) * units + magic;
-            b = F2(at_most(v[2 * j + 1].lo(), top), at_most(v[2 * j + 1].hi(), top)) * units + magic;
-        }
-        const uint32_t lo = __byte_perm(__float_as_uint(a.lo()), __float_as_uint(a.hi()), 0x0040);
-        const uint32_t hi = __byte_perm(__float_as_uint(b.lo()), __float_as_uint(b.hi()), 0x0040);
+    for (int j = 0; j < 4 / (int)sizeof(T); ++j) {
+        const uint32_t lo = __byte_perm(__float_as_uint(a[2 * j].lo()), __float_as_uint(a[2 * j].hi()), 0x0040);
+        const uint32_t hi = __byte_perm(__float_as_uint(a[2 * j + 1].lo()), __float_as_uint(a[2 * j + 1].hi()), 0x0040);
         packed[j] = __byte_perm(lo, hi, 0x5410);
     }
-    return byte;
+    return e - 6u;
 }
-// four values of a word
-__device__ __forceinline__ void kept_unpack(uint32_t w, F2 unit, F2& a, F2& b)
+// the four whole numbers of a word
+__device__ __forceinline__ void kept_unpack(uint32_t w, F2& a, F2& b)
 {
     w ^= 0x80808080u;                                           // q + 128 as the last byte of 2^23 + q + 128
     const F2 off(-8388736.0f);
-    a = (F2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7650)), __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7651))) + off) * unit;
-    b = (F2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7652)), __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7653))) + off) * unit;
+    a = F2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7650)), __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7651))) + off;
+    b = F2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7652)), __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7653))) + off;
 }
 
 }  // namespace mgpt

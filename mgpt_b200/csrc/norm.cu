@@ -74,24 +74,33 @@ template <typename T> __device__ __forceinline__ void params(const float* p, int
     }
 }
 
-// a piece of what was kept in 8 bits, RING: as above
-template <typename T, bool RING> __device__ __forceinline__ void take_kept(uint32_t src, const int8_t* mem, uint32_t byte, Piece<T>& o)
+// the whole numbers of a piece that was kept in 8 bits, RING: as above
+template <typename T, bool RING> __device__ __forceinline__ void take_kept(uint32_t src, const int8_t* mem, Piece<T>& o)
 {
-    const F2 unit(kept_unit(byte));
     if constexpr (sizeof(T) == 2) {
         const uint2 u = RING ? taken<uint2>(src) : *reinterpret_cast<const uint2*>(mem);
-        kept_unpack(u.x, unit, o.v[0], o.v[1]);
-        kept_unpack(u.y, unit, o.v[2], o.v[3]);
+        kept_unpack(u.x, o.v[0], o.v[1]);
+        kept_unpack(u.y, o.v[2], o.v[3]);
     } else {
-        kept_unpack(RING ? taken<uint32_t>(src) : *reinterpret_cast<const uint32_t*>(mem), unit, o.v[0], o.v[1]);
+        kept_unpack(RING ? taken<uint32_t>(src) : *reinterpret_cast<const uint32_t*>(mem), o.v[0], o.v[1]);
     }
 }
-// keeps a piece: every lane of a warp calls it, `in` where there is one
-template <typename T> __device__ __forceinline__ void keep(const Piece<T>& v, bool in, int8_t* mem, uint8_t* byte)
+// the 16 bytes of a piece as they are, and keeping it: every lane of a warp calls it, `in` where there is one
+template <typename T, bool RING> __device__ __forceinline__ void take_raw(uint32_t src, const T* mem, uint4& u, Piece<T>& o)
+{
+    u = RING ? taken<uint4>(src) : *reinterpret_cast<const uint4*>(mem);
+    if constexpr (sizeof(T) == 2) {
+        o.v[0] = widen(u.x); o.v[1] = widen(u.y); o.v[2] = widen(u.z); o.v[3] = widen(u.w);
+    } else {
+        o.v[0] = F2(__uint_as_float(u.x), __uint_as_float(u.y));
+        o.v[1] = F2(__uint_as_float(u.z), __uint_as_float(u.w));
+    }
+}
+template <typename T> __device__ __forceinline__ void keep(const uint4& u, const Piece<T>& v, bool in, int8_t* mem, uint8_t* byte)
 {
     constexpr int E = piece<T>();
     uint32_t w[E / 4];
-    const uint32_t e = kept_pack<E>(v.v, w);
+    const uint32_t e = kept_pack<T>(u, v.v, w);
     if (in) {
         if constexpr (E == 8) *reinterpret_cast<uint2*>(mem) = make_uint2(w[0], w[1]);
         else *reinterpret_cast<uint32_t*>(mem) = w[0];
@@ -240,16 +249,18 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 4 : 1) norm_fwd_kernel(c
             const int c = (gt + i * GT) * E;
             const bool in = have && c < p.C;
             Piece<T> h, x;
-            if constexpr (KEEP) {
-#pragma unroll
-                for (int j = 0; j < H; ++j) h.v[j] = x.v[j] = F2(0.0f);
-            }
+            uint4 hr = make_uint4(0, 0, 0, 0), xr = hr;     // (KEEP: what is not there is zeros)
             if (in) {
                 Piece<T> a, g;
                 params<T>(p.post, c, a);
                 params<T>(gate, c, g);
-                take<T, RING>(from + i * vec, (const T*)p.h + o + c, h);
-                take<T, RING>(from + array + i * vec, (const T*)p.x + o + c, x);
+                if constexpr (KEEP) {
+                    take_raw<T, RING>(from + i * vec, (const T*)p.h + o + c, hr, h);
+                    take_raw<T, RING>(from + array + i * vec, (const T*)p.x + o + c, xr, x);
+                } else {
+                    take<T, RING>(from + i * vec, (const T*)p.h + o + c, h);
+                    take<T, RING>(from + array + i * vec, (const T*)p.x + o + c, x);
+                }
 #pragma unroll
                 for (int j = 0; j < H; ++j) {
                     y[i].v[j] = fma2(F2(p.alpha), x.v[j], g.v[j] * a.v[j] * (h.v[j] * F2(r1)));
@@ -259,8 +270,8 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 4 : 1) norm_fwd_kernel(c
             }
             if constexpr (KEEP) {
                 const size_t group = (size_t)tok * kept_groups(p.C) + c / KEPT_GROUP;
-                keep<T>(x, in, p.xv + o + c, p.xe + group);
-                keep<T>(h, in, p.hv + o + c, p.he + group);
+                keep<T>(xr, x, in, p.xv + o + c, p.xe + group);
+                keep<T>(hr, h, in, p.hv + o + c, p.he + group);
             }
         }
         float r2 = 1.0f;
@@ -323,7 +334,8 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
     constexpr uint32_t dy_at = KEPT ? 0 : 2 * array, du_at = dy_at + array;
     const uint32_t mine8 = (uint32_t)__cvta_generic_to_shared(ring) + 2 * array + threadIdx.x * E;
     const int groups_of = kept_groups(p.C);
-    uint32_t nhe[KEPT ? NV : 1], nxe[KEPT ? NV : 1], he[KEPT ? NV : 1], xe[KEPT ? NV : 1];
+    uint32_t nhe[KEPT ? NV : 1], nxe[KEPT ? NV : 1];
+    float hs[KEPT ? NV : 1], xs[KEPT ? NV : 1];            // r1 and alpha in the units of h and x: powers of two, so that products are the same to the bit
     auto exponents = [&](int tok) {
         if constexpr (KEPT) {
 #pragma unroll
@@ -339,8 +351,8 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
     };
     auto take_hx = [&](int i, int slot, size_t at, Piece<T>& h, Piece<T>& x) {
         if constexpr (KEPT) {
-            take_kept<T, RING>(mine8 + slot * stage + i * kvec, p.hv + at, he[i], h);
-            take_kept<T, RING>(mine8 + slot * stage + karray + i * kvec, p.xv + at, xe[i], x);
+            take_kept<T, RING>(mine8 + slot * stage + i * kvec, p.hv + at, h);
+            take_kept<T, RING>(mine8 + slot * stage + karray + i * kvec, p.xv + at, x);
         } else {
             take<T, RING>(mine + slot * stage + i * vec, (const T*)p.h + at, h);
             take<T, RING>(mine + slot * stage + array + i * vec, (const T*)p.x + at, x);
@@ -401,8 +413,8 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
         if constexpr (KEPT) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                he[i] = nhe[i];
-                xe[i] = nxe[i];
+                hs[i] = r1 * kept_unit(nhe[i]);
+                xs[i] = p.alpha * kept_unit(nxe[i]);
             }
         }
         fetch(tok + (STAGES - 1) * GROUPS, slot == 0 ? STAGES - 1 : slot - 1);
@@ -427,7 +439,7 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
                 }
 #pragma unroll
                 for (int j = 0; j < H; ++j) {
-                    const F2 q = gp[i].v[j] * (h.v[j] * F2(r1)), yh = fma2(F2(p.alpha), x.v[j], q) * F2(r2);
+                    const F2 q = gp[i].v[j] * (h.v[j] * F2(KEPT ? hs[i] : r1)), yh = fma2(F2(KEPT ? xs[i] : p.alpha), x.v[j], q) * F2(r2);
                     if (with_u) {
                         const F2 d = du.v[j] * b.v[j];
                         s0 = fma2(d, yh, s0);
@@ -456,9 +468,9 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
                 }
 #pragma unroll
                 for (int j = 0; j < H; ++j) {
-                    const F2 hh = h.v[j] * F2(r1);
+                    const F2 hh = h.v[j] * F2(KEPT ? hs[i] : r1);
                     if (with_u) {
-                        const F2 yh = fma2(F2(p.alpha), x.v[j], gp[i].v[j] * hh) * F2(r2);
+                        const F2 yh = fma2(F2(KEPT ? xs[i] : p.alpha), x.v[j], gp[i].v[j] * hh) * F2(r2);
                         D.v[j] = fma2(F2(r2), fma2(yh, F2(-mA), du.v[j] * b.v[j]), D.v[j]);
                         S2[i].v[j] = fma2(du.v[j], yh, S2[i].v[j]);
                     }

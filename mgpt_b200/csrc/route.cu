@@ -642,101 +642,96 @@ template <typename T> __global__ void __launch_bounds__(32 * WARPS) route_sigmoi
     }
 }
 
-// That of a softmax's: L lanes per token, P experts each, four neighbouring ones at a time (a warp's accesses are runs of memory).
+// That of a softmax's: L lanes per token, at least as many as there are chosen experts, P experts each, four neighbouring ones at a time (a
+// warp's accesses are runs of memory).  The next tokens' logits are on their way while these are worked on.
 template <typename T, int L, int P>
 __global__ void __launch_bounds__(32 * WARPS) route_softmax_bwd_kernel(const RouteP p)
 {
-    constexpr int TOKENS = 32 / L, SLOTS = TOKENS * (8 * L < ROUTE_MAX_K ? 8 * L : ROUTE_MAX_K);
-    __shared__ __align__(16) float shr[WARPS][32 * P];          // [tokens][4 L i + ..]: dg, zeros but for the chosen
-    __shared__ float shg[WARPS][SLOTS], shd[WARPS][SLOTS];
-    __shared__ float4 sht[WARPS][TOKENS];
+    constexpr int TOKENS = 32 / L;
+    __shared__ __align__(16) float shr[WARPS][32 * P];          // [tokens][L * P]: dg, zeros but for the chosen
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % L, mt = lane / L;
+    const int ct = min((int)(lane * p.kdiv >> 16), TOKENS - 1), cj = lane - ct * p.k;      // the token and place of the lane's chosen expert (cj < k)
     float* const rows = shr[warp];
     for (int i = lane; i < 32 * P; i += 32) rows[i] = 0.0f;
     pdl_wait();
-    for (int tok0 = (blockIdx.x * WARPS + warp) * TOKENS; tok0 < p.n; tok0 += gridDim.x * WARPS * TOKENS) {
-        const int tok = tok0 + mt, slots = min(TOKENS, p.n - tok0) * p.k;
-        const bool have = tok < p.n;
+    const int stride = gridDim.x * WARPS * TOKENS;
+    int tok0 = (blockIdx.x * WARPS + warp) * TOKENS;
+    float z[P], dw = 0.0f, v = 0.0f;
+    int e = -1;
+    auto load = [&](int tok0) {
+        const int tok = tok0 + mt;
         const T* const row = (const T*)p.logits + (size_t)tok * p.E;
-        // (asked for before the rows' arithmetic)
-        int e1 = lane < slots ? p.top[(size_t)tok0 * p.k + lane] : -1;
-        const float d1 = lane < slots ? p.dw[(size_t)tok0 * p.k + lane] : 0.0f;
-        float pr[P], top = -INFINITY, sum = 0.0f;
+        e = -1;
+        if (cj < p.k && tok0 + ct < p.n) {
+            e = p.top[(size_t)(tok0 + ct) * p.k + cj];
+            dw = p.dw[(size_t)(tok0 + ct) * p.k + cj];
+        }
 #pragma unroll
         for (int i = 0; i < P; i += 4) {
-            float v[4];
-            load_four(row, have ? (i / 4 * L + sub) * 4 : p.E, p.E, p.vec, -INFINITY, v);
+            float four[4];
+            load_four(row, tok < p.n ? (i / 4 * L + sub) * 4 : p.E, p.E, p.vec, -INFINITY, four);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                pr[i + c] = v[c];
-                top = max_nan(top, v[c]);
-            }
+            for (int c = 0; c < 4; ++c) z[i + c] = four[c];
         }
+    };
+    load(tok0);
+    __syncwarp();
+    for (; tok0 < p.n; tok0 += stride) {
+        const int tok = tok0 + mt, e1 = e;
+        const bool have = tok < p.n, mine = has_gradient(p, e1);
+        const float dw1 = dw;
+        if (mine) v = as_float(((const T*)p.logits)[(size_t)(tok0 + ct) * p.E + e1]);
+        float pr[P], top = z[0], sum = 0.0f;
+#pragma unroll
+        for (int i = 1; i < P; ++i) top = max_nan(top, z[i]);
         top = lanes_max_nan<L>(top);
+        if (top == -INFINITY) top = 0.0f;       // (all out: zeros)
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            pr[i] = pr[i] == -INFINITY ? 0.0f : expf(pr[i] - top);
+            pr[i] = expf(z[i] - top);
             sum += pr[i];
         }
+        load(tok0 + stride);
         sum = lanes_sum<L>(sum);
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        if (sub == 0) sht[warp][mt] = make_float4(top, inv, 0.0f, 0.0f);
-        __syncwarp();
-        for (int q = lane; q < slots; q += 32) {
-            const int t = q * p.kdiv >> 16, e = q == lane ? e1 : p.top[(size_t)tok0 * p.k + q];
-            float g = 0.0f;
-            if (has_gradient(p, e)) {
-                const float v = as_float(((const T*)p.logits)[(size_t)(tok0 + t) * p.E + e]);
-                g = v == -INFINITY ? 0.0f : expf(v - sht[warp][t].x) * sht[warp][t].y;
-            }
-            shg[warp][q] = g;
-            shd[warp][q] = q == lane ? d1 : p.dw[(size_t)tok0 * p.k + q];
-        }
-        __syncwarp();
+        // a lane per chosen expert
+        const float ctop = __shfl_sync(FULL, top, ct * L), cinv = __shfl_sync(FULL, inv, ct * L);
+        const float g = !mine || v == -INFINITY ? 0.0f : expf(v - ctop) * cinv, product = g != 0.0f ? dw1 * g : 0.0f;
         float S = 0.0f, A = 0.0f;
-        if (have)
 #pragma unroll 4
-            for (int j = 0; j < p.k; ++j) {
-                const float g = shg[warp][mt * p.k + j], d = shd[warp][mt * p.k + j];
-                S += g;
-                A += g != 0.0f ? d * g : 0.0f;
-            }
+        for (int j = 0; j < p.k; ++j) {
+            S += __shfl_sync(FULL, g, mt * p.k + j);
+            A += __shfl_sync(FULL, product, mt * p.k + j);
+        }
         const Token of = token_of(p, S, A);
         // sum of dg p: renormalised, scale / S * (A - A * (S - 1e-20) / S)
         const float D = p.renorm ? of.mean * (of.of * TINY) : p.scale * A;
-        if (sub == 0) *reinterpret_cast<float2*>(&sht[warp][mt].z) = make_float2(of.of, of.mean);
-        __syncwarp();
-        for (int q = lane; q < slots; q += 32) {
-            const int t = q * p.kdiv >> 16, e = q == lane ? e1 : p.top[(size_t)tok0 * p.k + q];
-            if (has_gradient(p, e)) atomicAdd(&rows[t * L * P + e], sht[warp][t].z * (shd[warp][q] - sht[warp][t].w));
-        }
+        const float cof = __shfl_sync(FULL, of.of, ct * L), cmean = __shfl_sync(FULL, of.mean, ct * L);
+        if (mine) atomicAdd(&rows[ct * L * P + e1], cof * (dw1 - cmean));       // (one writer each, unless the caller repeats an index)
         __syncwarp();
         T* const out = (T*)p.dz + (size_t)tok * p.E;
 #pragma unroll
         for (int i = 0; i < P; i += 4) {
-            const int e = (i / 4 * L + sub) * 4;
-            float v[4];
-            load4(rows + mt * L * P + e, v);
-            store4(rows + mt * L * P + e, {0.0f, 0.0f, 0.0f, 0.0f});
+            const int at = (i / 4 * L + sub) * 4;
+            float d[4];
+            load4(rows + mt * L * P + at, d);
+            store4(rows + mt * L * P + at, {0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const float pc = pr[i + c] * inv;
-                v[c] = pc == 0.0f ? 0.0f : pc * (v[c] - D);
-            }
-            if (!have || e >= p.E) continue;
+            for (int c = 0; c < 4; ++c) d[c] = pr[i + c] * inv * (d[c] - D);
+            if (!have || at >= p.E) continue;
             if (p.vec) {
-                store4(out + e, v);
-                if (p.dz16) store4(p.dz16 + (size_t)tok * p.E + e, v);
+                store4(out + at, d);
+                if (p.dz16) store4(p.dz16 + (size_t)tok * p.E + at, d);
             } else {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    if (e + c < p.E) store1(out + e + c, v[c]);
-                    if (p.dz16 && e + c < p.E8) p.dz16[(size_t)tok * p.E8 + e + c] = __float2bfloat16(e + c < p.E ? v[c] : 0.0f);
+                    if (at + c < p.E) store1(out + at + c, d[c]);
+                    if (p.dz16 && at + c < p.E8) p.dz16[(size_t)tok * p.E8 + at + c] = __float2bfloat16(at + c < p.E ? d[c] : 0.0f);
                 }
             }
         }
         if (p.dz16 && !p.vec && have)           // (what of the padding lies beyond the last four)
-            for (int e = (p.E + 3) / 4 * 4 + sub; e < p.E8; e += L) p.dz16[(size_t)tok * p.E8 + e] = __float2bfloat16(0.0f);
+            for (int i = (p.E + 3) / 4 * 4 + sub; i < p.E8; i += L) p.dz16[(size_t)tok * p.E8 + i] = __float2bfloat16(0.0f);
         __syncwarp();
     }
 }
@@ -752,10 +747,28 @@ template <typename T, int L, int P> int run_fwd(RouteP& p, cudaStream_t st)
 }
 template <typename T, int L, int P> int run_softmax_bwd(const RouteP& p, cudaStream_t st)
 {
-    const int per = WARPS * (32 / L), want = (p.n + per - 1) / per, most = 148 * 8;
+    const int per = WARPS * (32 / L), want = (p.n + per - 1) / per, most = 148 * 6;
     MGPT_CUDA(launch_pdl(route_softmax_bwd_kernel<T, L, P>, want < most ? want : most, 32 * WARPS, 0, st, p));
     MGPT_LAUNCHED("route_softmax_bwd_kernel");
     return 0;
+}
+template <typename T, int L> int run_softmax_bwd(const RouteP& p, cudaStream_t st)
+{
+    return p.E <= 4 * L ? run_softmax_bwd<T, L, 4>(p, st) : p.E <= 8 * L ? run_softmax_bwd<T, L, 8>(p, st) : run_softmax_bwd<T, L, 16>(p, st);
+}
+// at least as many lanes as chosen experts, and 16 experts per lane at most
+template <typename T> int run_softmax_bwd(const RouteP& p, cudaStream_t st)
+{
+    int lanes = 1;
+    while (lanes < p.k || 16 * lanes < p.E) lanes *= 2;
+    switch (lanes) {
+        case 1: return run_softmax_bwd<T, 1>(p, st);
+        case 2: return run_softmax_bwd<T, 2>(p, st);
+        case 4: return run_softmax_bwd<T, 4>(p, st);
+        case 8: return run_softmax_bwd<T, 8>(p, st);
+        case 16: return run_softmax_bwd<T, 16>(p, st);
+        default: return run_softmax_bwd<T, 32>(p, st);
+    }
 }
 template <typename T> int run_sigmoid_bwd(const RouteP& p, cudaStream_t st)
 {
@@ -766,15 +779,6 @@ template <typename T> int run_sigmoid_bwd(const RouteP& p, cudaStream_t st)
     MGPT_LAUNCHED("route_sigmoid_bwd_kernel");
     return 0;
 }
-// eight experts per lane, and as many lanes as that takes
-#define MGPT_BY_EXPERTS(run, T)                       \
-    (p.E <= 8 ? run<T, 1, 8>(p, st)                   \
-     : p.E <= 16 ? run<T, 2, 8>(p, st)                \
-     : p.E <= 32 ? run<T, 4, 8>(p, st)                \
-     : p.E <= 64 ? run<T, 8, 8>(p, st)                \
-     : p.E <= 128 ? run<T, 16, 8>(p, st)              \
-     : p.E <= 256 ? run<T, 32, 8>(p, st) : run<T, 32, 16>(p, st))
-
 template <typename T> int run_fwd(RouteP& p, cudaStream_t st)
 {
     p.vec = p.E % 4 == 0 && ((uintptr_t)p.logits & (4 * sizeof(T) - 1)) == 0;
@@ -788,7 +792,7 @@ template <typename T> int run_fwd(RouteP& p, cudaStream_t st)
 template <typename T> int run_bwd(RouteP& p, cudaStream_t st)
 {
     p.vec = p.E % 4 == 0 && (((uintptr_t)p.logits | (uintptr_t)p.dz) & (4 * sizeof(T) - 1)) == 0 && (!p.dz16 || p.E8 == p.E);
-    return p.softmax ? MGPT_BY_EXPERTS(run_softmax_bwd, T) : run_sigmoid_bwd<T>(p, st);
+    return p.softmax ? run_softmax_bwd<T>(p, st) : run_sigmoid_bwd<T>(p, st);
 }
 
 int fill(RouteP& p, const mgpt_moe_routing* r, int n, int E, int k)
