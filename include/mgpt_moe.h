@@ -568,7 +568,7 @@ int  mgpt_moe_op_restore8(const int8_t* values, const uint8_t* exponents, int n,
 
 /* mgpt_moe_op_residual_norm that also keeps x and h so, in the same pass, and the backward call that takes them in the
  * tensors' place (`io` is the type of dy, du, dx and dh). The gradients are the formulas' at the kept x and h, with the
- * r1 and r2 of the forward pass. Everything else, the workspace too, as above. */
+ * r1 and r2 of the forward pass. Exponents are 4-byte aligned here. Everything else, the workspace too, as above. */
 int  mgpt_moe_op_residual_norm_keep(const void* x, const void* h, int io, const float* post_scale, const float* gate,
                                     int tokens_per_gate, const float* pre_scale, float alpha, float eps, int n, int C,
                                     void* y, void* u, float* stats, int8_t* x_values, uint8_t* x_exponents,

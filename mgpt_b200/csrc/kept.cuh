@@ -21,23 +21,30 @@ __device__ __forceinline__ uint32_t kept_exponent(uint32_t largest)
 __device__ __forceinline__ float kept_unit(uint32_t byte) { return __uint_as_float(byte == 255u ? 0x7fffffffu : byte << 23); }     // 2^e, or NaN
 __device__ __forceinline__ float at_most(float v, uint32_t top) { return copysignf(fminf(fabsf(v), __uint_as_float(top)), v); }
 
-// The bits of the largest magnitude of a lane's values, as they lie in registers (BF16: two to a word, their maxima side by side until the end).
-__device__ __forceinline__ uint32_t kept_larger(uint32_t a, uint32_t b, bf16) { return __vmaxu2(a, b); }
+// The larger of two magnitudes (NaN: that), BF16: of two pairs of them.
+__device__ __forceinline__ uint32_t kept_larger(uint32_t a, uint32_t b, bf16)
+{
+    uint32_t c;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+    return c;
+}
 __device__ __forceinline__ uint32_t kept_larger(uint32_t a, uint32_t b, float) { return max(a, b); }
+// of 16 bytes, as they lie in registers
 template <typename T> __device__ __forceinline__ uint32_t kept_largest(const uint4& u)
 {
     constexpr uint32_t M = sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu;
-    uint32_t m = kept_larger(kept_larger(u.x & M, u.y & M, T()), kept_larger(u.z & M, u.w & M, T()), T());
+    return kept_larger(kept_larger(u.x & M, u.y & M, T()), kept_larger(u.z & M, u.w & M, T()), T());
+}
+template <typename T> __device__ __forceinline__ uint32_t kept_largest_of_lanes(uint32_t m)
+{
 #pragma unroll
     for (int o = KEPT_GROUP * (int)sizeof(T) / 32; o > 0; o >>= 1) m = kept_larger(m, __shfl_xor_sync(0xffffffffu, m, o), T());
-    return sizeof(T) == 2 ? max(m & 0xffff0000u, m << 16) : m;
+    return m;
 }
 
-// 16 bytes of T of one lane, all of a group in neighbouring lanes, which all call it (with zeros beyond the row's end): the group's byte,
-// and the values packed.  v: the same values.
-template <typename T> __device__ __forceinline__ uint32_t kept_pack(const uint4& u, const F2 (&v)[8 / sizeof(T)], uint32_t (&packed)[4 / sizeof(T)])
+// 16 bytes of T in the units of a group whose largest magnitude has the bits m: the group's byte, and the values packed.
+template <typename T> __device__ __forceinline__ uint32_t kept_round(uint32_t m, const F2 (&v)[8 / sizeof(T)], uint32_t (&packed)[4 / sizeof(T)])
 {
-    const uint32_t m = kept_largest<T>(u);
     uint32_t e = max((m + 0x10000u) >> 23, 7u);                     // 6 more than the byte, but for the largest numbers
     F2 units(__uint_as_float((260u - e) << 23)), magic(12582912.0f);       // 2^-e; 1.5 * 2^23: a sum's last byte is the whole number in two's complement
     F2 a[8 / sizeof(T)];
@@ -56,6 +63,29 @@ template <typename T> __device__ __forceinline__ uint32_t kept_pack(const uint4&
         packed[j] = __byte_perm(lo, hi, 0x5410);
     }
     return e - 6u;
+}
+// 16 bytes of one lane (u, and as numbers v), all of a group in neighbouring lanes, which all call it (with zeros beyond the row's end).
+template <typename T> __device__ __forceinline__ uint32_t kept_pack(const uint4& u, const F2 (&v)[8 / sizeof(T)], uint32_t (&packed)[4 / sizeof(T)])
+{
+    const uint32_t m = kept_largest_of_lanes<T>(kept_largest<T>(u));
+    return kept_round<T>(sizeof(T) == 2 ? max(m & 0xffff0000u, m << 16) : m, v, packed);
+}
+// Two of them, whose groups are not one.  (BF16: both maxima in a word.)
+template <typename T>
+__device__ __forceinline__ void kept_pack_two(const uint4& u, const F2 (&v)[8 / sizeof(T)], const uint4& u2, const F2 (&v2)[8 / sizeof(T)],
+                                              uint32_t (&packed)[4 / sizeof(T)], uint32_t (&packed2)[4 / sizeof(T)], uint32_t& byte, uint32_t& byte2)
+{
+    uint32_t m = kept_largest<T>(u), m2 = kept_largest<T>(u2);
+    if constexpr (sizeof(T) == 2) {
+        m = kept_largest_of_lanes<T>(kept_larger(__byte_perm(m, m2, 0x5410), __byte_perm(m, m2, 0x7632), T()));
+        m2 = m & 0xffff0000u;
+        m <<= 16;
+    } else {
+        m = kept_largest_of_lanes<T>(m);
+        m2 = kept_largest_of_lanes<T>(m2);
+    }
+    byte = kept_round<T>(m, v, packed);
+    byte2 = kept_round<T>(m2, v2, packed2);
 }
 // the four whole numbers of a word
 __device__ __forceinline__ void kept_unpack(uint32_t w, F2& a, F2& b)

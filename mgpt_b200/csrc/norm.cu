@@ -85,7 +85,7 @@ template <typename T, bool RING> __device__ __forceinline__ void take_kept(uint3
         kept_unpack(RING ? taken<uint32_t>(src) : *reinterpret_cast<const uint32_t*>(mem), o.v[0], o.v[1]);
     }
 }
-// the 16 bytes of a piece as they are, and keeping it: every lane of a warp calls it, `in` where there is one
+// the 16 bytes of a piece as they are, and as numbers
 template <typename T, bool RING> __device__ __forceinline__ void take_raw(uint32_t src, const T* mem, uint4& u, Piece<T>& o)
 {
     u = RING ? taken<uint4>(src) : *reinterpret_cast<const uint4*>(mem);
@@ -96,16 +96,10 @@ template <typename T, bool RING> __device__ __forceinline__ void take_raw(uint32
         o.v[1] = F2(__uint_as_float(u.z), __uint_as_float(u.w));
     }
 }
-template <typename T> __device__ __forceinline__ void keep(const uint4& u, const Piece<T>& v, bool in, int8_t* mem, uint8_t* byte)
+template <int N> __device__ __forceinline__ void store_kept(int8_t* p, const uint32_t (&w)[N / 4])
 {
-    constexpr int E = piece<T>();
-    uint32_t w[E / 4];
-    const uint32_t e = kept_pack<T>(u, v.v, w);
-    if (in) {
-        if constexpr (E == 8) *reinterpret_cast<uint2*>(mem) = make_uint2(w[0], w[1]);
-        else *reinterpret_cast<uint32_t*>(mem) = w[0];
-        if (threadIdx.x % (KEPT_GROUP / E) == 0) *byte = (uint8_t)e;
-    }
+    if constexpr (N == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(p) = w[0];
 }
 
 // Sums of K values over the W warps of a token's group; every thread of the group calls it.  Two buffers in turn: who writes one
@@ -176,7 +170,7 @@ constexpr uint32_t ring_bytes(int arrays, int nv, int threads) { return STAGES *
 
 // A group of warps per token, the groups of the grid taking tokens in turn.
 template <typename T, int NV, int W, bool RING, bool KEEP>
-__global__ void __launch_bounds__(threads_of(W), RING ? 4 : 1) norm_fwd_kernel(const NormP p)
+__global__ void __launch_bounds__(threads_of(W), RING ? (KEEP ? 3 : 4) : 1) norm_fwd_kernel(const NormP p)
 {
     extern __shared__ __align__(16) uint8_t ring[];
     constexpr int THREADS = threads_of(W), GT = 32 * W, GROUPS = THREADS / GT, E = piece<T>(), H = E / 2;
@@ -268,10 +262,18 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 4 : 1) norm_fwd_kernel(c
                 }
                 store((T*)p.y + o + c, y[i]);
             }
-            if constexpr (KEEP) {
-                const size_t group = (size_t)tok * kept_groups(p.C) + c / KEPT_GROUP;
-                keep<T>(xr, x, in, p.xv + o + c, p.xe + group);
-                keep<T>(hr, h, in, p.hv + o + c, p.he + group);
+            if constexpr (KEEP) {               // (every lane of a warp)
+                uint32_t xw[E / 4], hw[E / 4], xb, hb;
+                kept_pack_two<T>(xr, x.v, hr, h.v, xw, hw, xb, hb);
+                if (in) {
+                    store_kept<E>(p.xv + o + c, xw);
+                    store_kept<E>(p.hv + o + c, hw);
+                    const size_t group = (size_t)tok * kept_groups(p.C) + (uint32_t)c / KEPT_GROUP;
+                    if (threadIdx.x % (KEPT_GROUP / E) == 0) {
+                        p.xe[group] = (uint8_t)xb;
+                        p.he[group] = (uint8_t)hb;
+                    }
+                }
             }
         }
         float r2 = 1.0f;
@@ -329,26 +331,13 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
     pdl_wait();
     const bool with_u = p.du != nullptr;
     float nr1 = 0.0f, nr2 = 0.0f;                           // of the token that is copied next
-    // A token in the ring: pieces of h, x, dy, du; or of dy, du, then of h and x in 8 bits (whose exponents come as nr1 and nr2 do).
-    constexpr uint32_t kvec = THREADS * E, karray = NV * kvec, stage = KEPT ? 2 * array + 2 * karray : 4 * array;
+    // A token in the ring: pieces of h, x, dy, du; or of dy, du, then of h and x in 8 bits, then the words that their exponents are in.
+    constexpr uint32_t kvec = THREADS * E, karray = NV * kvec, evec = THREADS * 4, earray = NV * evec;
+    constexpr uint32_t stage = KEPT ? 2 * array + 2 * karray + 2 * earray : 4 * array;
     constexpr uint32_t dy_at = KEPT ? 0 : 2 * array, du_at = dy_at + array;
-    const uint32_t mine8 = (uint32_t)__cvta_generic_to_shared(ring) + 2 * array + threadIdx.x * E;
-    const int groups_of = kept_groups(p.C);
-    uint32_t nhe[KEPT ? NV : 1], nxe[KEPT ? NV : 1];
-    float hs[KEPT ? NV : 1], xs[KEPT ? NV : 1];            // r1 and alpha in the units of h and x: powers of two, so that products are the same to the bit
-    auto exponents = [&](int tok) {
-        if constexpr (KEPT) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int c = (gt + i * GT) * E;
-                if (c < p.C) {
-                    const size_t group = (size_t)tok * groups_of + c / KEPT_GROUP;
-                    nhe[i] = p.he[group];
-                    nxe[i] = p.xe[group];
-                }
-            }
-        }
-    };
+    const uint32_t mine8 = mine - threadIdx.x * 16 + 2 * array + threadIdx.x * E, minee = mine - threadIdx.x * 16 + 2 * array + 2 * karray + threadIdx.x * 4;
+    const uint32_t groups_of = kept_groups(p.C), first_group = (uint32_t)(gt * E) / KEPT_GROUP;
+    float hs[KEPT ? NV : 1], xs[KEPT ? NV : 1];             // r1 and alpha in the units of h and x: powers of two, so that products are the same to the bit
     auto take_hx = [&](int i, int slot, size_t at, Piece<T>& h, Piece<T>& x) {
         if constexpr (KEPT) {
             take_kept<T, RING>(mine8 + slot * stage + i * kvec, p.hv + at, h);
@@ -370,6 +359,11 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
                         const uint32_t d8 = mine8 + s * stage + i * kvec;
                         copy_piece8<E>(d8, p.hv + o + c);
                         copy_piece8<E>(d8 + karray, p.xv + o + c);
+                        // (the aligned word that the byte is in, up to the last byte there is)
+                        const size_t group = ((size_t)tok * groups_of + first_group + i * (GT * E / KEPT_GROUP)) & ~(size_t)3;
+                        const uint32_t bytes = (uint32_t)min((size_t)4, (size_t)p.n * groups_of - group), de = minee + s * stage + i * evec;
+                        copy4(de, p.he + group, bytes);
+                        copy4(de + earray, p.xe + group, bytes);
                     } else {
                         copy16(d, (const T*)p.h + o + c);
                         copy16(d + array, (const T*)p.x + o + c);
@@ -401,7 +395,6 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
     if (t0 + group < t1) {
         nr1 = p.stats[t0 + group];
         nr2 = p.stats[p.n + t0 + group];
-        exponents(t0 + group);
     }
     const float inv = 1.0f / (float)p.C;
     int slot = 0;
@@ -410,21 +403,31 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
         const bool have = tok < t1;
         const size_t o = (size_t)tok * p.C;
         const float r1 = nr1, r2 = nr2;
-        if constexpr (KEPT) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                hs[i] = r1 * kept_unit(nhe[i]);
-                xs[i] = p.alpha * kept_unit(nxe[i]);
-            }
-        }
         fetch(tok + (STAGES - 1) * GROUPS, slot == 0 ? STAGES - 1 : slot - 1);
         if (tok + GROUPS < t1) {
             nr1 = p.stats[tok + GROUPS];
             nr2 = p.stats[p.n + tok + GROUPS];
-            exponents(tok + GROUPS);
         }
         copy_wait<STAGES - 1>();
         const uint32_t from = mine + slot * stage;
+        if constexpr (KEPT) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const size_t group = (size_t)tok * groups_of + first_group + i * (GT * E / KEPT_GROUP);
+                uint32_t hb = 127, xb = 127;
+                if (have && (gt + i * GT) * E < p.C) {
+                    if constexpr (RING) {
+                        hb = taken<uint32_t>(minee + slot * stage + i * evec) >> ((uint32_t)group % 4 * 8) & 255;
+                        xb = taken<uint32_t>(minee + slot * stage + earray + i * evec) >> ((uint32_t)group % 4 * 8) & 255;
+                    } else {
+                        hb = p.he[group];
+                        xb = p.xe[group];
+                    }
+                }
+                hs[i] = r1 * kept_unit(hb);
+                xs[i] = p.alpha * kept_unit(xb);
+            }
+        }
         F2 s0(0.0f), s1(0.0f), s2(0.0f);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -600,7 +603,7 @@ template <typename T, int NV, int W, bool RING, bool KEEP> int run_fwd(const Nor
 {
     constexpr int threads = threads_of(W), groups = threads / (32 * W);
     constexpr uint32_t smem = RING ? ring_bytes(2, NV, threads) : 0;
-    const int most = 148 * FWD_CTAS, want = (p.n + groups - 1) / groups;
+    const int most = 148 * (KEEP ? 3 : FWD_CTAS), want = (p.n + groups - 1) / groups;
     static bool done[64];
     MGPT_TRY(opt_in(norm_fwd_kernel<T, NV, W, RING, KEEP>, smem, done));
     MGPT_CUDA(launch_pdl(norm_fwd_kernel<T, NV, W, RING, KEEP>, want < most ? want : most, threads, smem, st, p));
@@ -614,7 +617,7 @@ template <typename T, int NV, int W, bool RING> int run_fwd(const NormP& p, cuda
 template <typename T, int NV, int W, bool RING, bool KEPT> int run_bwd(const NormP& p, int units, cudaStream_t st)
 {
     // (the ring is more than the sums at the end, 4 NV piece<T>() bytes per thread where there are groups)
-    constexpr uint32_t smem = !RING ? 0 : KEPT ? ring_bytes(2, NV, threads_of(W)) + STAGES * 2 * NV * threads_of(W) * piece<T>() : ring_bytes(4, NV, threads_of(W));
+    constexpr uint32_t smem = !RING ? 0 : KEPT ? ring_bytes(2, NV, threads_of(W)) + STAGES * 2 * NV * threads_of(W) * (piece<T>() + 4) : ring_bytes(4, NV, threads_of(W));
     static bool done[64];
     MGPT_TRY(opt_in(norm_bwd_kernel<T, NV, W, RING, KEPT>, smem, done));
     MGPT_CUDA(launch_pdl(norm_bwd_kernel<T, NV, W, RING, KEPT>, units, threads_of(W), smem, st, p));
@@ -660,7 +663,9 @@ int check_kept(const Kept& k)
 {
     if (!k.xv || !k.hv || !k.xe || !k.he) return fail(MGPT_MOE_EINVAL, "null argument");
     MGPT_TRY(check_aligned(k.xv, "x_values", 8));
-    return check_aligned(k.hv, "h_values", 8);
+    MGPT_TRY(check_aligned(k.hv, "h_values", 8));
+    MGPT_TRY(check_aligned(k.xe, "x_exponents", 4));
+    return check_aligned(k.he, "h_exponents", 4);
 }
 
 int forward(const void* x, const void* h, int io, const float* post_scale, const float* gate, int tokens_per_gate, const float* pre_scale,

@@ -31,6 +31,8 @@ __device__ __forceinline__ uint32_t narrow(F2 v)
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void copy8(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
+// the first `bytes` (0 to 4) of a word, zeros behind them
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, uint32_t bytes) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory"); }
 template <int BYTES> __device__ __forceinline__ void copy_piece8(uint32_t dst, const void* src)
 {
     static_assert(BYTES == 8 || BYTES == 4, "");

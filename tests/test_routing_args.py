@@ -60,13 +60,13 @@ def test_keep_and_restore_refuse(lib, bad):  # noqa: F811
     assert lib.mgpt_moe_op_restore8(a["v"], a["e"], a["n"], a["C"], a["x"], a["io"], None) == EINVAL
 
 
-@pytest.mark.parametrize("bad", [dict(x=None), dict(h=P + 8), dict(xv=None), dict(hv=None), dict(xe=None), dict(he=None), dict(xv=P + 4), dict(hv=P + 4), dict(C=12), dict(io=3), dict(u=None)])
+@pytest.mark.parametrize("bad", [dict(x=None), dict(h=P + 8), dict(xv=None), dict(hv=None), dict(xe=None), dict(he=None), dict(xv=P + 4), dict(hv=P + 4), dict(xe=P + 2), dict(he=P + 1), dict(C=12), dict(io=3), dict(u=None)])
 def test_residual_norm_keep_refuses(lib, bad):  # noqa: F811
     a = dict(x=P, h=P, io=1, C=64, u=P, xv=P, xe=P, hv=P, he=P) | bad
     assert lib.mgpt_moe_op_residual_norm_keep(a["x"], a["h"], a["io"], P, P, 0, P, 1.0, 1e-5, 4, a["C"], P, a["u"], P, a["xv"], a["xe"], a["hv"], a["he"], None) == EINVAL
 
 
-@pytest.mark.parametrize("bad", [dict(xv=None), dict(hv=None), dict(xe=None), dict(he=None), dict(xv=P + 4), dict(hv=P + 4), dict(C=12), dict(dy=None), dict(du=None), dict(dx=None), dict(ws=None)])
+@pytest.mark.parametrize("bad", [dict(xv=None), dict(hv=None), dict(xe=None), dict(he=None), dict(xv=P + 4), dict(hv=P + 4), dict(xe=P + 1), dict(he=P + 2), dict(C=12), dict(dy=None), dict(du=None), dict(dx=None), dict(ws=None)])
 def test_residual_norm_backward_kept_refuses(lib, bad):  # noqa: F811
     a = dict(xv=P, xe=P, hv=P, he=P, C=64, dy=P, du=P, dx=P, ws=P) | bad
     assert lib.mgpt_moe_op_residual_norm_backward_kept(a["xv"], a["xe"], a["hv"], a["he"], 1, P, P, 0, P, 1.0, 4, a["C"], P, a["dy"], a["du"], a["dx"], P, P, P, P, a["ws"], 1 << 30, None) == EINVAL
