@@ -7,6 +7,7 @@ experts, the k largest, renormalised weights; and the gradient.
 from __future__ import annotations
 
 import ctypes as ct
+import functools
 
 import torch
 
@@ -15,19 +16,29 @@ from ._lib import MoeError
 from .training import _DTYPES, _EITHER, _F32, _I32, _INT_MAX, _check, _device, _need, _optional, _stream
 
 
-def _routing(E, score, bias, groups, top_groups, group_top, renormalise, scale, device):
+@functools.lru_cache(maxsize=64)
+def _numbers(score, groups, top_groups, group_top, renormalise, scale):
+    """The argument's bytes without the bias (a copy is quicker made than a new one filled)."""
     _need(score in _lib.SCORES, f"routing: score is 'softmax' or 'sigmoid', got {score!r}")
     numbers = (groups, groups if top_groups is None else top_groups, group_top)
     _need(all(-_INT_MAX <= v <= _INT_MAX for v in numbers), "routing: sizes out of range")
-    return _lib.Routing(_lib.SCORES[score], *numbers, int(bool(renormalise)), scale, _optional(bias, "bias", (E,), _F32, device))
+    return bytes(_lib.Routing(_lib.SCORES[score], *numbers, int(bool(renormalise)), scale, None))
+
+
+def _routing(E, score, bias, groups, top_groups, group_top, renormalise, scale, device):
+    r = _lib.Routing.from_buffer_copy(_numbers(score, groups, top_groups, group_top, renormalise, scale))
+    if bias is not None:
+        r.bias = _check(bias, "bias", (E,), _F32, device)
+    return r
 
 
 def _logits(logits):
     device, shape = _device(logits), logits.shape
     if not shape or not shape[-1] or logits.dtype not in _DTYPES:
         raise MoeError(f"routing: logits are [..., E] of FP32 or BF16, got {tuple(shape)} of {logits.dtype}")
-    n, E = shape[:-1].numel(), shape[-1]
-    _need(max(n, E) <= _INT_MAX, "routing: sizes out of range")
+    E = shape[-1]
+    n = shape.numel() // E
+    _need(n <= _INT_MAX >= E, "routing: sizes out of range")
     return device, n, E, _check(logits, "logits", shape, _EITHER, device)
 
 
@@ -52,7 +63,8 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: tor
     cp = _optional(counts, "counts", (E,), _I32, device)
     shape = logits.shape[:-1] + (top_k,)
     _need(top_k <= E, "routing: top_k is more than the experts")
-    top_idx, weights = torch.empty(shape, dtype=torch.int32, device=device), torch.empty(shape, dtype=torch.float32, device=device)
+    top_idx = torch.empty(shape, dtype=torch.int32, device=device)
+    weights = torch.empty_like(top_idx, dtype=torch.float32)
     _lib.check(lib.mgpt_moe_op_route(lp, _DTYPES[logits.dtype], n, E, top_k, ct.byref(r), top_idx.data_ptr(), weights.data_ptr(), cp, _stream(device)))
     return top_idx, weights
 

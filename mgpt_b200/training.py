@@ -151,37 +151,56 @@ KEPT_GROUP = 32                 # channels that share an exponent
 class Kept8:
     """Activations ``[..., C]`` in 8 bits: ``values`` (int8 ``[..., C]``) in units of ``2**(exponents - 127)`` (uint8
     ``[..., ceil(C/32)]``: one for 32 consecutive channels).  ``dtype`` is that of the tensor that was kept."""
-    __slots__ = ("values", "exponents", "dtype")
+    __slots__ = ("shape", "dtype", "_values", "_exponents", "_buffer")
 
     def __init__(self, values: torch.Tensor, exponents: torch.Tensor, dtype: torch.dtype):
-        self.values, self.exponents, self.dtype = values, exponents, dtype
+        self.shape, self.dtype, self._values, self._exponents, self._buffer = values.shape, dtype, values, exponents, None
 
     @property
-    def shape(self):
-        return self.values.shape
+    def values(self) -> torch.Tensor:
+        if self._values is None:
+            self._values = self._buffer[:self.shape.numel()].view(self.shape)
+        return self._values
+
+    @property
+    def exponents(self) -> torch.Tensor:
+        if self._exponents is None:
+            self._exponents = self._buffer[self.shape.numel():].view(torch.uint8).view(self.shape[:-1] + (-(-self.shape[-1] // KEPT_GROUP),))
+        return self._exponents
 
     @property
     def nbytes(self) -> int:
-        return self.values.numel() + self.exponents.numel()
+        n = self.shape.numel()
+        return n + n // self.shape[-1] * -(-self.shape[-1] // KEPT_GROUP)
 
 
-def _kept_size(shape, what):
+def _kept_size(t, what):
+    """Rows and channels of a tensor [..., C] that is kept."""
+    shape = t.shape
     C = shape[-1] if shape else 0
     if C <= 0 or C % 8:
         raise MoeError(f"{what}: expected [..., C], C a multiple of 8, got {tuple(shape)}")
-    n = shape[:-1].numel()
-    _need(max(n, C) <= _INT_MAX, f"{what}: sizes out of range")
+    n = shape.numel() // C
+    _need(n <= _INT_MAX >= C, f"{what}: sizes out of range")
     return n, C
 
 
-def _kept_empty(x: torch.Tensor) -> Kept8:
-    groups = -(-x.shape[-1] // KEPT_GROUP)
-    return Kept8(torch.empty_like(x, dtype=torch.int8), torch.empty(x.shape[:-1] + (groups,), dtype=torch.uint8, device=x.device), x.dtype)
+def _kept_empty(x, n, C):
+    """Room for x ([n, C]) in 8 bits, in one piece: the values, then the exponents; and the addresses of both."""
+    kept = Kept8.__new__(Kept8)
+    kept.shape, kept.dtype, kept._values, kept._exponents = x.shape, x.dtype, None, None
+    kept._buffer = buffer = torch.empty(n * (C + -(-C // KEPT_GROUP)), dtype=torch.int8, device=x.device)
+    at = buffer.data_ptr()
+    return kept, at, at + n * C
 
 
 def _check_kept(kept, name, shape, device):
     if not isinstance(kept, Kept8):
         raise MoeError(f"{name}: expected a Kept8, got {type(kept).__name__}")
+    buffer = kept._buffer
+    if buffer is not None and kept.shape == shape and buffer.device == device:
+        at = buffer.data_ptr()
+        return at, at + shape.numel()
     groups = -(-shape[-1] // KEPT_GROUP)
     return (_check(kept.values, f"{name}.values", shape, _I8, device),
             _check(kept.exponents, f"{name}.exponents", shape[:-1] + (groups,), _U8, device))
@@ -193,10 +212,10 @@ def keep8(x: torch.Tensor) -> Kept8:
     half a unit at most, 1/128 of the largest.  A group with a NaN or an infinity comes back as NaN."""
     lib = _lib.load()
     device = _device(x)
-    n, C = _kept_size(x.shape, "keep8")
+    n, C = _kept_size(x, "keep8")
     xp = _check(x, "x", x.shape, _EITHER, device)
-    kept = _kept_empty(x)
-    _lib.check(lib.mgpt_moe_op_keep8(xp, _DTYPES[x.dtype], n, C, kept.values.data_ptr(), kept.exponents.data_ptr(), _stream(device)))
+    kept, values, exponents = _kept_empty(x, n, C)
+    _lib.check(lib.mgpt_moe_op_keep8(xp, _DTYPES[x.dtype], n, C, values, exponents, _stream(device)))
     return kept
 
 
@@ -205,13 +224,13 @@ def restore8(kept: Kept8, dtype: torch.dtype = None) -> torch.Tensor:
     lib = _lib.load()
     if not isinstance(kept, Kept8):
         raise MoeError(f"restore8: expected a Kept8, got {type(kept).__name__}")
-    device, dtype = _device(kept.values), kept.dtype if dtype is None else dtype
-    n, C = _kept_size(kept.shape, "restore8")
+    device, dtype = _device(kept._values if kept._buffer is None else kept._buffer), kept.dtype if dtype is None else dtype
+    n, C = _kept_size(kept, "restore8")
     if dtype not in _DTYPES:
         raise MoeError(f"restore8: unsupported dtype {dtype}")
-    vp, ep = _check_kept(kept, "kept", kept.shape, device)
-    x = torch.empty_like(kept.values, dtype=dtype)
-    _lib.check(lib.mgpt_moe_op_restore8(vp, ep, n, C, x.data_ptr(), _DTYPES[dtype], _stream(device)))
+    values, exponents = _check_kept(kept, "kept", kept.shape, device)
+    x = torch.empty(kept.shape, dtype=dtype, device=device)
+    _lib.check(lib.mgpt_moe_op_restore8(values, exponents, n, C, x.data_ptr(), _DTYPES[dtype], _stream(device)))
     return x
 
 
@@ -259,9 +278,8 @@ def residual_norm(x: torch.Tensor, h: torch.Tensor, *, post_scale=None, gate=Non
     if not keep:
         _lib.check(lib.mgpt_moe_op_residual_norm(*args, _stream(device)))
         return y, u, stats
-    x8, h8 = _kept_empty(x), _kept_empty(h)
-    _lib.check(lib.mgpt_moe_op_residual_norm_keep(*args, x8.values.data_ptr(), x8.exponents.data_ptr(), h8.values.data_ptr(), h8.exponents.data_ptr(),
-                                                  _stream(device)))
+    (x8, xv, xe), (h8, hv, he) = _kept_empty(x, n, C), _kept_empty(h, n, C)
+    _lib.check(lib.mgpt_moe_op_residual_norm_keep(*args, xv, xe, hv, he, _stream(device)))
     return y, u, stats, (x8, h8)
 
 
