@@ -119,16 +119,22 @@ __device__ __forceinline__ void load4(const float* p, float (&v)[4])
     const float4 a = *reinterpret_cast<const float4*>(p);
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
 }
-__device__ __forceinline__ void load4(const bf16* p, float (&v)[4])
+// from global memory, here and not where the values are needed first
+__device__ __forceinline__ void fetch4(const float* p, float (&v)[4])
 {
-    const uint2 a = *reinterpret_cast<const uint2*>(p);
+    asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "l"(p));
+}
+__device__ __forceinline__ void fetch4(const bf16* p, float (&v)[4])
+{
+    uint2 a;
+    asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(a.x), "=r"(a.y) : "l"(p));
     v[0] = __uint_as_float(a.x << 16); v[1] = __uint_as_float(a.x & 0xffff0000u);
     v[2] = __uint_as_float(a.y << 16); v[3] = __uint_as_float(a.y & 0xffff0000u);
 }
 template <typename T> __device__ __forceinline__ void load_four(const T* row, int e, int E, bool vec, float none, float (&v)[4])
 {
     if (vec) {
-        if (e < E) load4(row + e, v);
+        if (e < E) fetch4(row + e, v);
         else v[0] = v[1] = v[2] = v[3] = none;
     } else {
 #pragma unroll
@@ -313,6 +319,48 @@ __device__ __forceinline__ float near_over(float v)
     return r;
 }
 
+// Whether a lane's group stays: known (`stays`), or `open`, and then by exact values of its experts that may be among its largest, those whose
+// score is near `least` or above.  Lanes of groups (route_kernel).
+template <typename T, int L, int P>
+__device__ __noinline__ bool settle_group(const RouteP& p, int tok, bool have, float top, float least, bool open, bool stays)
+{
+    const int lane = threadIdx.x & 31, sub = lane % L, mt = lane / L, e0 = sub * P;
+    const T* const row = (const T*)p.logits + (size_t)tok * p.E;
+    double over = 1.0, d1 = -INFINITY, d2 = -INFINITY;
+    open &= have;
+    if (p.softmax) {
+        double sum = 0.0;
+#pragma unroll 2
+        for (int e = sub; e < p.E; e += L)
+            if (have && as_float(row[e]) > -INFINITY) sum += exp((double)as_float(row[e]) - (double)top);
+        over = 1.0 / lanes_sum<L>(sum);
+    }
+    if (open)
+        for (int i = 0; i < P; ++i) {
+            const float z = as_float(row[e0 + i]), b = p.bias ? p.bias[e0 + i] : 0.0f;
+            const float c = (p.softmax ? near_exp(z - top) * (float)over : near_over(1.0f + near_exp(-z))) + b;
+            if (!(z > -INFINITY) || !(c >= least)) continue;
+            const double v = (p.softmax ? exp((double)z - (double)top) * over : 1.0 / (1.0 + exp(-(double)z))) + (double)b;
+            d2 = v > d1 ? d1 : v > d2 ? v : d2;
+            d1 = v > d1 ? v : d1;
+        }
+    for (int o = p.group_lanes / 2; o > 0; o >>= 1) {
+        const double n1 = __shfl_xor_sync(FULL, d1, o), n2 = __shfl_xor_sync(FULL, d2, o);
+        const double low = n1 > d1 ? d1 : n1;
+        d1 = n1 > d1 ? n1 : d1;
+        d2 = n2 > d2 ? n2 : d2;
+        d2 = low > d2 ? low : d2;
+    }
+    if (p.group_top == 2 && d2 > -INFINITY) d1 += d2;
+    int before = 0;
+    for (int g = 0; g < p.groups; ++g) {
+        const int from = mt * L + g * p.group_lanes, state = __shfl_sync(FULL, stays ? 2 : open ? 1 : 0, from);
+        const double d = __shfl_sync(FULL, d1, from);
+        before += state == 2 || (state == 1 && (d > d1 || (d == d1 && g * p.group_lanes < sub - sub % p.group_lanes)));
+    }
+    return open ? before < p.top_groups : stays;
+}
+
 // L lanes per token, P experts each; 32 / L tokens per warp.
 //
 // The rounds of the choice: a score becomes the number of steps of R / 2^23 that it is below a bound on all of them (23 bits; further
@@ -360,6 +408,18 @@ __global__ void __launch_bounds__(32 * WARPS, P > 8 ? 5 : 8) route_kernel(const 
         if (!(bhi >= blo)) bhi = blo = 0.0f;
     }
     const float bmax = fmaxf(fabsf(bhi), fabsf(blo)), rounding = 6e-8f * (1.0f + bmax);       // (of a score with its bias)
+    // Steps of scores.  How far a score may be off (base).  exp: (|argument| + 2) 2^-23 of itself.  A softmax's term: that, 0.37 * 2^-23 at
+    // most, and its share of the sum's error: as much in the mean (6.3 + 2) and 21 roundings; a sigmoid: (0.23 + 0.5) 2^-23, and
+    // 2^-24 and 2^-22 for the sum and the quotient.  A softmax's largest term, and so all of this, is its token's.
+    float base, bound, S;
+    uint32_t apart = 1u << 9;
+    auto steps = [&](float most) {
+        base = p.softmax ? fmaf(2.6e-6f, most, 8e-8f) : 4e-7f;
+        bound = most + bhi + 4.0f * (base + rounding);
+        S = __fdividef(8388600.0f, fminf(bound - blo, 4.0f));
+        if (by_score) apart = (uint32_t)fminf(2.0f * S * (base + rounding) + 4.0f, 4e6f) << 9;      // (and two roundings to steps)
+    };
+    steps(1.0f);
     int32_t* const chosen = shi[warp];
     const int stride = gridDim.x * WARPS * TOKENS;
     float z[P];
@@ -388,7 +448,8 @@ __global__ void __launch_bounds__(32 * WARPS, P > 8 ? 5 : 8) route_kernel(const 
             bool unsure = HOW != BY_LOGIT && top == INFINITY;
             if (!by_score || p.softmax) top = lanes_max_nan<L>(top);
             float inv = 1.0f;                   // (what the weights are divided by has exp(0) in it, where they are all there is)
-            uint32_t key[P], apart = 1;
+            uint32_t key[P];
+            bool aside = false;                 // the lane's experts are not in a group that stays
             if constexpr (HOW != BY_LOGIT) {
                 float c[P];                     // (NaN: out.  A logit of infinity has been seen to above)
                 if (p.softmax) {
@@ -406,11 +467,8 @@ __global__ void __launch_bounds__(32 * WARPS, P > 8 ? 5 : 8) route_kernel(const 
 #pragma unroll
                     for (int i = 0; i < P; ++i) c[i] = near_over(1.0f + near_exp(-z[i])) + fmaf(z[i], 0.0f, b[i]);
                 }
-                // How far a score may be off.  exp: (|argument| + 2) 2^-23 of itself.  A softmax's term: that, 0.37 * 2^-23 at most, and its
-                // share of the sum's error: as much in the mean (6.3 + 2) and 21 roundings; a sigmoid: (0.23 + 0.5) 2^-23, and
-                // 2^-24 and 2^-22 for the sum and the quotient.
-                const float most = p.softmax ? inv : 1.0f, base = p.softmax ? fmaf(2.6e-6f, inv, 8e-8f) : 4e-7f;
-                uint32_t outside = 0;           // bit i: not in a group that stays
+                if (p.softmax) steps(inv);
+                uint32_t outside = 0;           // bit i: not in a group that stays, where groups are not runs of lanes
                 if constexpr (HOW == BY_GROUP) {
                     // (a group's score: twice that, and three roundings of twice the size)
                     const float margin = 4.0f * base + 9.0f * rounding;
@@ -418,7 +476,7 @@ __global__ void __launch_bounds__(32 * WARPS, P > 8 ? 5 : 8) route_kernel(const 
                         float m1 = -INFINITY, m2 = -INFINITY;
 #pragma unroll
                         for (int i = 0; i < P; ++i) {
-                            const float v = c[i] > -INFINITY ? c[i] : -INFINITY;
+                            const float v = fmaxf(c[i], -INFINITY);     // (of a NaN: the other)
                             m2 = fmaxf(m2, fminf(m1, v));
                             m1 = fmaxf(m1, v);
                         }
@@ -427,6 +485,7 @@ __global__ void __launch_bounds__(32 * WARPS, P > 8 ? 5 : 8) route_kernel(const 
                             m2 = fmaxf(fmaxf(m2, n2), fminf(m1, n1));
                             m1 = fmaxf(m1, n1);
                         }
+                        const float least = p.group_top == 2 ? m2 : m1;
                         if (p.group_top == 2 && m2 > -INFINITY) m1 += m2;
                         // the groups that may be ahead of this one (it is among them), and those that are
                         int may = -1, are = 0;
@@ -435,10 +494,15 @@ __global__ void __launch_bounds__(32 * WARPS, P > 8 ? 5 : 8) route_kernel(const 
                             may += !(d <= -margin);
                             are += d > margin;
                         }
-                        if (may >= p.top_groups) {
-                            outside = FULL;
-                            unsure |= e0 < p.E && are < p.top_groups;
+                        bool stays = may < p.top_groups;
+                        const bool open = e0 < p.E && !stays && are < p.top_groups;
+                        if (__builtin_expect(__any_sync(FULL, open && have && !bad && margin < 1e-3f), 0)) {
+                            stays = settle_group<T, L, P>(p, tok, have, top, least - margin, open && !bad, stays);
+                            unsure |= open && bad;
+                        } else {
+                            unsure |= open;
                         }
+                        aside = !stays;
                     } else {
                         float* const cs = (float*)scratch;
                         __syncwarp();
@@ -454,15 +518,13 @@ __global__ void __launch_bounds__(32 * WARPS, P > 8 ? 5 : 8) route_kernel(const 
                     }
                 }
                 if (by_score) {
-                    const float bound = most + bhi + 4.0f * (base + rounding), R = fminf(bound - blo, 4.0f), S = 8388600.0f / R;
-                    apart = (uint32_t)fminf(2.0f * S * (base + rounding) + 4.0f, 4e6f);      // (and two roundings to steps)
 #pragma unroll
                     for (int i = 0; i < P; ++i) key[i] = (min(__float_as_uint(fmaf(bound - c[i], S, 8388608.0f)), LAST) << 9) + (expert(i) + 1);
                 } else {
 #pragma unroll
                     for (int i = 0; i < P; ++i) key[i] = (min(__float_as_uint(fmaf(top - z[i], 524288.0f, 8388608.0f)), LAST) << 9) + (expert(i) + 1);
                 }
-                if (HOW == BY_GROUP) {
+                if (HOW == BY_GROUP && !p.group_lanes) {
 #pragma unroll
                     for (int i = 0; i < P; ++i)
                         if (outside >> i & 1) key[i] = NONE;
@@ -486,14 +548,15 @@ __global__ void __launch_bounds__(32 * WARPS, P > 8 ? 5 : 8) route_kernel(const 
                     if (expert(i) >= p.E) key[i] = NONE;
             }
             load(tok + stride);                 // (what the next round needs, on its way meanwhile)
-            apart <<= 9;
             // the least key above `last` (a key that was taken is further, modulo 2^32, than any other), and one less than how far it is
             auto beyond = [&](uint32_t last, uint32_t* m) {
                 const uint32_t from = ~last;
                 uint32_t part[4];               // (chains side by side)
 #pragma unroll
                 for (int i = 0; i < P; ++i) part[i % 4] = i < 4 ? key[i] + from : min(key[i] + from, part[i % 4]);
-                const uint32_t next = lanes_min<L>(min(min(part[0], part[1]), min(part[2], part[3])));
+                uint32_t next = min(min(part[0], part[1]), min(part[2], part[3]));
+                if (HOW == BY_GROUP && aside) next = NONE + from;
+                next = lanes_min<L>(next);
                 *m = next - from;
                 return next;
             };
@@ -507,7 +570,7 @@ __global__ void __launch_bounds__(32 * WARPS, P > 8 ? 5 : 8) route_kernel(const 
             uint32_t next;                      // the first that was not chosen
             if (beyond(last, &next) < apart && next != NONE && next > last) close |= bit;
             __syncwarp();
-            if (__any_sync(FULL, close && !bad)) {
+            if (__builtin_expect(__any_sync(FULL, close && !bad), 0)) {
                 double* const value = scratch + mt * (KM + EXTRA);
                 int32_t* const behind = (int32_t*)(scratch + TOKENS * (KM + EXTRA)) + mt * EXTRA;
                 int32_t* const sorted = (int32_t*)(scratch + TOKENS * (KM + EXTRA + EXTRA / 2)) + mt * KM;
