@@ -1,6 +1,6 @@
 """A small language model trained with the layer and the operators beside it: a whole training step without attention.
 
-    python examples/train_lm.py [--steps 60]
+    python examples/train_lm.py [--steps 60] [--routing sigmoid] [--kept-bits 8]
 
 Each block is the Mixture-of-Experts layer between two norms, with a gate per channel on the residual stream:
 
@@ -11,6 +11,9 @@ The embedding is the head as well.  What a step consists of:
     embedding rows -> [MoELayer.forward, residual_norm] x blocks -> head_loss
     head_loss_backward -> [residual_norm_backward, MoELayer.backward] x blocks -> embedding rows' gradients
     AdamW over every tensor at once, moments in 8 bits
+
+With ``--routing`` the layers choose their experts by softmax or sigmoid scores with renormalised weights, under a bias that is moved towards
+equal loads after every step; with ``--kept-bits 8`` what the norms keep for their backward pass is in 8 bits.
 
 The data are sequences in which a token fixes the next one nine times out of ten; the first tokens of each sequence carry no loss.
 """
@@ -25,17 +28,20 @@ from mgpt_b200 import AdamW, MoELayer, check_status, head_loss, head_loss_backwa
 
 
 class Model:
-    def __init__(self, vocab=1000, dim=128, hidden=256, experts=8, top_k=2, blocks=2, alpha=1.0, seed=0, state_bits=8):
+    def __init__(self, vocab=1000, dim=128, hidden=256, experts=8, top_k=2, blocks=2, alpha=1.0, seed=0, state_bits=8, routing=None, kept_bits=16):
         g = torch.Generator().manual_seed(seed)
-        self.alpha, self.dim = alpha, dim
+        self.alpha, self.dim, self.keep = alpha, dim, kept_bits == 8
         self.embed = (torch.randn(vocab, dim, generator=g) * 0.1).cuda()             # the masters are FP32
         self.head = self.embed.bfloat16()                                            # the copy that the products read
         self.d_embed = torch.zeros_like(self.embed)
-        self.moe, self.small, self.d_small = [], [], []
+        self.moe, self.bias, self.small, self.d_small = [], [], [], []
         for _ in range(blocks):
             layer = MoELayer(dim, hidden, experts, top_k)
             layer.load_parameters([torch.randn(p.shape, generator=g).numpy() * (p.shape[0] ** -0.5 if p.shape[0] > 1 else 0.0) for p in layer.get_parameters()])
             self.moe.append(layer)
+            self.bias.append(torch.zeros(experts).cuda() if routing else None)
+            if routing:
+                layer.set_routing(routing, bias=self.bias[-1], renormalise=True)
             self.small.append(dict(pre=torch.ones(dim).cuda(), post=torch.ones(dim).cuda(), gate=torch.full((1, dim), 0.5).cuda()))
         self.final = torch.ones(dim).cuda()                                          # scale of the norm in front of the head
         self.d_small = [{k: torch.zeros_like(v) for k, v in s.items()} for s in self.small]
@@ -64,8 +70,8 @@ class Model:
         kept = []
         for i, moe in enumerate(self.moe):
             h = moe.forward(u)
-            y, v, stats = residual_norm(x, h, **self.norm_args(i))
-            kept.append((x, h, stats))
+            y, v, stats, *kept8 = residual_norm(x, h, keep=self.keep, **self.norm_args(i))
+            kept.append((*(kept8[0] if self.keep else (x, h)), stats))
             x, u = y, v
         targets = targets.reshape(-1)
         loss, lse = head_loss(u, self.head, targets)
@@ -83,8 +89,11 @@ class Model:
         self.d_embed.index_add_(0, rows.long(), dx0.float())
         self.t += 1
         self.optimiser.step(self.t, lr=lr)
-        for m in self.moe:
+        for m, bias in zip(self.moe, self.bias):
             m.sync_weights()                                                         # the layer's own BF16 copies
+            if bias is not None and lr:                                              # experts with more tokens than the mean are asked less
+                counts = m.workspace_view("counts", torch.int32, (m.E,)).float()
+                bias += 1e-3 * torch.sign(counts.mean() - counts)
         return (loss * share).sum()
 
 
@@ -101,8 +110,8 @@ def batch(n, length, vocab, seed):
     return t[:, :-1].int().cuda(), targets.int().cuda()
 
 
-def train(steps=60, vocab=1000, seed=0, state_bits=8, report=None):
-    model = Model(vocab=vocab, seed=seed, state_bits=state_bits)
+def train(steps=60, vocab=1000, seed=0, state_bits=8, report=None, **how):
+    model = Model(vocab=vocab, seed=seed, state_bits=state_bits, **how)
     losses = []
     for i in range(steps):
         losses.append(model.step(*batch(32, 64, vocab, 100 + i)))
@@ -118,5 +127,7 @@ if __name__ == "__main__":
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
     ap.add_argument("--steps", type=int, default=60)
     ap.add_argument("--state-bits", type=int, default=8, choices=(8, 32))
+    ap.add_argument("--routing", choices=("softmax", "sigmoid"))
+    ap.add_argument("--kept-bits", type=int, default=16, choices=(8, 16))
     args = ap.parse_args()
-    train(args.steps, state_bits=args.state_bits, report=10)
+    train(args.steps, state_bits=args.state_bits, report=10, routing=args.routing, kept_bits=args.kept_bits)

@@ -883,24 +883,26 @@ int fill(RouteP& p, const mgpt_moe_routing* r, int n, int E, int k)
     return 0;
 }
 
-// Column sums of dz, in a fixed order: blocks of rows, then the blocks.  (The layer's router bias; d_bias is added to.)
-__global__ void __launch_bounds__(256) route_bias_kernel(const float* dz, int n, int E, int rows, float* part)
+// Column sums of blocks of rows of [n, E], in a fixed order: 256 / E' threads to a column, E' the power of two that E fits.  (The layer's router
+// bias: first its blocks of rows, then those sums; the last are added to what is there.)
+__global__ void __launch_bounds__(256) route_columns_kernel(const float* from, int n, int E, int rows, float* to, bool add)
 {
     pdl_wait();
+    __shared__ float sums[256];
+    int cols = 1;
+    while (cols < E) cols *= 2;
+    const int e = threadIdx.x % cols, group = threadIdx.x / cols, groups = 256 / cols;
     const int r0 = blockIdx.x * rows, r1 = min(r0 + rows, n);
-    for (int e = threadIdx.x; e < E; e += 256) {
-        float s = 0.0f;
-        for (int r = r0; r < r1; ++r) s += dz[(size_t)r * E + e];
-        part[(size_t)blockIdx.x * E + e] = s;
-    }
-}
-__global__ void __launch_bounds__(256) route_bias_join_kernel(const float* part, int parts, int E, float* d_bias)
-{
-    pdl_wait();
-    for (int e = threadIdx.x; e < E; e += 256) {
-        float s = 0.0f;
-        for (int i = 0; i < parts; ++i) s += part[(size_t)i * E + e];
-        d_bias[e] += s;
+    float s = 0.0f;
+    if (e < E)
+#pragma unroll 8
+        for (int r = r0 + group; r < r1; r += groups) s += from[(size_t)r * E + e];
+    sums[threadIdx.x] = s;
+    __syncthreads();
+    if (group == 0 && e < E) {
+        for (int g = 1; g < groups; ++g) s += sums[g * cols + e];
+        float* const out = to + (size_t)blockIdx.x * E + e;
+        *out = add ? *out + s : s;
     }
 }
 
@@ -953,10 +955,10 @@ int launch_routed_bwd(mgpt_moe_layer* L, const Workspace& w, char* ws, bf16* dl1
     while ((p.n + rows - 1) / rows > 256 || (p.n + rows - 1) / rows > d.C) rows *= 2;
     const int parts = (p.n + rows - 1) / rows;
     float* const part = (float*)(ws + w.rw_part);
-    MGPT_CUDA(launch_pdl(route_bias_kernel, parts, 256, 0, st, (const float*)p.dz, p.n, d.E, rows, part));
-    MGPT_LAUNCHED("route_bias_kernel");
-    MGPT_CUDA(launch_pdl(route_bias_join_kernel, 1, 256, 0, st, part, parts, d.E, d_bias));
-    MGPT_LAUNCHED("route_bias_join_kernel");
+    MGPT_CUDA(launch_pdl(route_columns_kernel, parts, 256, 0, st, (const float*)p.dz, p.n, d.E, rows, part, false));
+    MGPT_LAUNCHED("route_columns_kernel");
+    MGPT_CUDA(launch_pdl(route_columns_kernel, 1, 256, 0, st, (const float*)part, parts, d.E, parts, d_bias, true));
+    MGPT_LAUNCHED("route_columns_kernel");
     return 0;
 }
 
