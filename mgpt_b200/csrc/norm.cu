@@ -20,6 +20,12 @@
 // issue slots.  Before: loads
 // into registers, four pieces per thread, 193 and 316; the ring with the number of warps at run time 116 and 190; FP32 in two
 // pieces of 32 bytes side by side, half a sector per access, 137 and 227.  A third token in the ring costs more blocks than it hides.
+//
+// KEEP, KEPT: x and h in 8 bits (kept.cuh), written beside y and u, read in their place by the backward pass.  32768 x 2048 BF16: forward 136 us (5.0 TB/s
+// of 675 MB), backward 178 (3.8 TB/s; 151 from tensors).  Both are bound by what a value costs in instructions (a group's maximum over lanes and
+// three byte permutations per four values; unpacking twice), at 58 to 61 % of the issue slots.  The units of a power of two are folded into r1 and
+// alpha; exponents come through the ring as the words they are in (loaded into registers a token ahead: 188 us); the maxima of x and h share a
+// word and a block's registers leave three blocks per SM (four: spills, 149 us); one piece per thread in the backward pass: 202.
 #include "kept.cuh"
 
 namespace mgpt {
@@ -331,12 +337,24 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
     pdl_wait();
     const bool with_u = p.du != nullptr;
     float nr1 = 0.0f, nr2 = 0.0f;                           // of the token that is copied next
-    // A token in the ring: pieces of h, x, dy, du; or of dy, du, then of h and x in 8 bits, then the words that their exponents are in.
+    // A token in the ring: pieces of h, x, dy, du; or of dy, du, then of h and x in 8 bits, then (BF16, which has no registers left for
+    // them) the words that their exponents are in.
+    constexpr bool EXPONENTS = KEPT && RING && sizeof(T) == 2;
     constexpr uint32_t kvec = THREADS * E, karray = NV * kvec, evec = THREADS * 4, earray = NV * evec;
-    constexpr uint32_t stage = KEPT ? 2 * array + 2 * karray + 2 * earray : 4 * array;
+    constexpr uint32_t stage = KEPT ? 2 * array + 2 * karray + (EXPONENTS ? 2 * earray : 0) : 4 * array;
     constexpr uint32_t dy_at = KEPT ? 0 : 2 * array, du_at = dy_at + array;
     const uint32_t mine8 = mine - threadIdx.x * 16 + 2 * array + threadIdx.x * E, minee = mine - threadIdx.x * 16 + 2 * array + 2 * karray + threadIdx.x * 4;
     const uint32_t groups_of = kept_groups(p.C), first_group = (uint32_t)(gt * E) / KEPT_GROUP;
+    uint32_t nhb[KEPT ? NV : 1], nxb[KEPT ? NV : 1];        // exponents of the token that is copied next, as nr1 and nr2
+    auto exponents = [&](int tok, uint32_t (&hb)[KEPT ? NV : 1], uint32_t (&xb)[KEPT ? NV : 1]) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if ((gt + i * GT) * E < p.C) {
+                const size_t group = (size_t)tok * groups_of + first_group + i * (GT * E / KEPT_GROUP);
+                hb[i] = p.he[group];
+                xb[i] = p.xe[group];
+            }
+    };
     float hs[KEPT ? NV : 1], xs[KEPT ? NV : 1];             // r1 and alpha in the units of h and x: powers of two, so that products are the same to the bit
     auto take_hx = [&](int i, int slot, size_t at, Piece<T>& h, Piece<T>& x) {
         if constexpr (KEPT) {
@@ -359,11 +377,12 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
                         const uint32_t d8 = mine8 + s * stage + i * kvec;
                         copy_piece8<E>(d8, p.hv + o + c);
                         copy_piece8<E>(d8 + karray, p.xv + o + c);
-                        // (the aligned word that the byte is in, up to the last byte there is)
-                        const size_t group = ((size_t)tok * groups_of + first_group + i * (GT * E / KEPT_GROUP)) & ~(size_t)3;
-                        const uint32_t bytes = (uint32_t)min((size_t)4, (size_t)p.n * groups_of - group), de = minee + s * stage + i * evec;
-                        copy4(de, p.he + group, bytes);
-                        copy4(de + earray, p.xe + group, bytes);
+                        if constexpr (EXPONENTS) {      // (the aligned word that the byte is in, up to the last byte there is)
+                            const size_t group = ((size_t)tok * groups_of + first_group + i * (GT * E / KEPT_GROUP)) & ~(size_t)3;
+                            const uint32_t bytes = (uint32_t)min((size_t)4, (size_t)p.n * groups_of - group), de = minee + s * stage + i * evec;
+                            copy4(de, p.he + group, bytes);
+                            copy4(de + earray, p.xe + group, bytes);
+                        }
                     } else {
                         copy16(d, (const T*)p.h + o + c);
                         copy16(d + array, (const T*)p.x + o + c);
@@ -395,6 +414,7 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
     if (t0 + group < t1) {
         nr1 = p.stats[t0 + group];
         nr2 = p.stats[p.n + t0 + group];
+        if constexpr (KEPT && !EXPONENTS) exponents(t0 + group, nhb, nxb);
     }
     const float inv = 1.0f / (float)p.C;
     int slot = 0;
@@ -403,27 +423,26 @@ __global__ void __launch_bounds__(threads_of(W), RING ? 2 : 1) norm_bwd_kernel(c
         const bool have = tok < t1;
         const size_t o = (size_t)tok * p.C;
         const float r1 = nr1, r2 = nr2;
+        if constexpr (KEPT && !EXPONENTS) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                hs[i] = r1 * kept_unit(nhb[i]);
+                xs[i] = p.alpha * kept_unit(nxb[i]);
+            }
+        }
         fetch(tok + (STAGES - 1) * GROUPS, slot == 0 ? STAGES - 1 : slot - 1);
         if (tok + GROUPS < t1) {
             nr1 = p.stats[tok + GROUPS];
             nr2 = p.stats[p.n + tok + GROUPS];
+            if constexpr (KEPT && !EXPONENTS) exponents(tok + GROUPS, nhb, nxb);
         }
         copy_wait<STAGES - 1>();
         const uint32_t from = mine + slot * stage;
-        if constexpr (KEPT) {
+        if constexpr (EXPONENTS) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const size_t group = (size_t)tok * groups_of + first_group + i * (GT * E / KEPT_GROUP);
-                uint32_t hb = 127, xb = 127;
-                if (have && (gt + i * GT) * E < p.C) {
-                    if constexpr (RING) {
-                        hb = taken<uint32_t>(minee + slot * stage + i * evec) >> ((uint32_t)group % 4 * 8) & 255;
-                        xb = taken<uint32_t>(minee + slot * stage + earray + i * evec) >> ((uint32_t)group % 4 * 8) & 255;
-                    } else {
-                        hb = p.he[group];
-                        xb = p.xe[group];
-                    }
-                }
+                const uint32_t shift = ((uint32_t)tok * groups_of + first_group + i * (GT * E / KEPT_GROUP)) % 4 * 8;
+                const uint32_t hb = taken<uint32_t>(minee + slot * stage + i * evec) >> shift & 255, xb = taken<uint32_t>(minee + slot * stage + earray + i * evec) >> shift & 255;
                 hs[i] = r1 * kept_unit(hb);
                 xs[i] = p.alpha * kept_unit(xb);
             }
@@ -617,7 +636,7 @@ template <typename T, int NV, int W, bool RING> int run_fwd(const NormP& p, cuda
 template <typename T, int NV, int W, bool RING, bool KEPT> int run_bwd(const NormP& p, int units, cudaStream_t st)
 {
     // (the ring is more than the sums at the end, 4 NV piece<T>() bytes per thread where there are groups)
-    constexpr uint32_t smem = !RING ? 0 : KEPT ? ring_bytes(2, NV, threads_of(W)) + STAGES * 2 * NV * threads_of(W) * (piece<T>() + 4) : ring_bytes(4, NV, threads_of(W));
+    constexpr uint32_t smem = !RING ? 0 : KEPT ? ring_bytes(2, NV, threads_of(W)) + STAGES * 2 * NV * threads_of(W) * (piece<T>() + (sizeof(T) == 2 ? 4 : 0)) : ring_bytes(4, NV, threads_of(W));
     static bool done[64];
     MGPT_TRY(opt_in(norm_bwd_kernel<T, NV, W, RING, KEPT>, smem, done));
     MGPT_CUDA(launch_pdl(norm_bwd_kernel<T, NV, W, RING, KEPT>, units, threads_of(W), smem, st, p));

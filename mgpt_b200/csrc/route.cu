@@ -11,7 +11,16 @@
 // The reference has clamped softmax and top-k only (utils/Tensor.cpp:850-909).
 //
 // What is chosen is what exact arithmetic chooses (up to FP64's rounding): scores are formed in FP32 with a known bound on their
-// error, and a token in which some comparison that decides is closer than that is gone through again in FP64 by its warp.
+// error, and what is closer than that is settled by exact values: of the few experts concerned, of a group's largest, or (a logit of
+// infinity, biases of very different size, long runs of equals) of all.  What is chosen does not depend on which way that goes.
+//
+// Bytes: the logits once, the weights and indices; backward the gradients' bytes, for a softmax the logits too.  Forward is bound by the
+// integer pipe (minima and comparisons run at half the rate of additions): about 180 instructions per token of 128 experts and 8
+// chosen, 690 per token of 256 in groups.  us in a graph on a B200, FP32 logits: 8 x 256 in
+// groups 4.3, 32768 x 64, 4 chosen 8.5, 32768 x 256 in groups, 8 chosen 35 (floor 5.3), 131072 x 128, 8 chosen 36 (floor 12); backward
+// of the last two 7.9 (sigmoid; 4.3 TB/s) and 29 (softmax; 4.6 TB/s).  Of the forward call 2 us are the counts' atomics, where counts are asked for.
+// Not kept: the eight least by sorting and merging lists (38 against 36 us, 39 against 35: more minima), two warps per block (44 against 38),
+// six to eight blocks per SM (37 to 41 against 36).
 #include "common.cuh"
 
 namespace mgpt {
@@ -799,6 +808,7 @@ __global__ void __launch_bounds__(32 * WARPS) route_softmax_bwd_kernel(const Rou
     }
 }
 
+bool many(const RouteP& p) { return (int64_t)p.n * p.E > 148 * 2048; }
 template <typename T, int L, int P> int run_fwd(RouteP& p, cudaStream_t st)
 {
     const int per = WARPS * (32 / L), want = (p.n + per - 1) / per, most = 148 * (P > 8 ? 5 : 8), lanes = p.gsize / P;
@@ -819,11 +829,11 @@ template <typename T, int L> int run_softmax_bwd(const RouteP& p, cudaStream_t s
 {
     return p.E <= 4 * L ? run_softmax_bwd<T, L, 4>(p, st) : p.E <= 8 * L ? run_softmax_bwd<T, L, 8>(p, st) : run_softmax_bwd<T, L, 16>(p, st);
 }
-// at least as many lanes as chosen experts, and 16 experts per lane at most
+// at least as many lanes as chosen experts (one each), and 16 experts per lane at most (few tokens: 8, as above; 1021 x 155: 2.8 us against 3.5)
 template <typename T> int run_softmax_bwd(const RouteP& p, cudaStream_t st)
 {
     int lanes = 1;
-    while (lanes < p.k || 16 * lanes < p.E) lanes *= 2;
+    while (lanes < p.k || 16 * lanes < p.E || (lanes < 32 && 8 * lanes < p.E && !many(p))) lanes *= 2;
     switch (lanes) {
         case 1: return run_softmax_bwd<T, 1>(p, st);
         case 2: return run_softmax_bwd<T, 2>(p, st);
@@ -845,8 +855,11 @@ template <typename T> int run_sigmoid_bwd(const RouteP& p, cudaStream_t st)
 template <typename T> int run_fwd(RouteP& p, cudaStream_t st)
 {
     p.vec = p.E % 4 == 0 && ((uintptr_t)p.logits & (4 * sizeof(T) - 1)) == 0;
+    // Sixteen experts per lane where that leaves an SM two thousand logits and more: what a round costs beside its minima is shared by more tokens
+    // (131072 x 128: 39 us against 55 with eight, 4096 x 128: 3.5 against 5.1).  Fewer: eight, whose chains are shorter (64 x 256 in groups: 4.1
+    // against 5.0).
     if (p.E > 256) return run_fwd<T, 32, 16>(p, st);
-    if ((int64_t)p.n * p.E > 148 * 32 * 128)
+    if (many(p))
         return p.E <= 16 ? run_fwd<T, 1, 16>(p, st) : p.E <= 32 ? run_fwd<T, 2, 16>(p, st) : p.E <= 64 ? run_fwd<T, 4, 16>(p, st)
                : p.E <= 128 ? run_fwd<T, 8, 16>(p, st) : run_fwd<T, 16, 16>(p, st);
     return p.E <= 8 ? run_fwd<T, 1, 8>(p, st) : p.E <= 16 ? run_fwd<T, 2, 8>(p, st) : p.E <= 32 ? run_fwd<T, 4, 8>(p, st)
