@@ -13,7 +13,7 @@ import torch
 
 from . import _lib
 from ._lib import MoeError
-from .training import _DTYPES, _EITHER, _F32, _I32, _INT_MAX, _check, _device, _need, _optional, _stream
+from .training import _DTYPES, _EITHER, _F32, _I32, _INT_MAX, _check, _device, _need, _stream
 
 
 @functools.lru_cache(maxsize=64)
@@ -58,11 +58,10 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: tor
     adjusted by (``bias += rate * sign(counts.mean() - counts)``)."""
     lib = _lib.load()
     device, n, E, lp = _logits(logits)
-    _need(0 < top_k <= _INT_MAX, "routing: top_k must be positive")
+    _need(0 < top_k <= E, "routing: top_k is 1 to the number of experts")
     r = _routing(E, score, bias, groups, top_groups, group_top, renormalise, scale, device)
-    cp = _optional(counts, "counts", (E,), _I32, device)
+    cp = None if counts is None else _check(counts, "counts", (E,), _I32, device)
     shape = logits.shape[:-1] + (top_k,)
-    _need(top_k <= E, "routing: top_k is more than the experts")
     top_idx = torch.empty(shape, dtype=torch.int32, device=device)
     weights = torch.empty_like(top_idx, dtype=torch.float32)
     _lib.check(lib.mgpt_moe_op_route(lp, _DTYPES[logits.dtype], n, E, top_k, ct.byref(r), top_idx.data_ptr(), weights.data_ptr(), cp, _stream(device)))

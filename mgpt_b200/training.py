@@ -151,7 +151,7 @@ KEPT_GROUP = 32                 # channels that share an exponent
 class Kept8:
     """Activations ``[..., C]`` in 8 bits: ``values`` (int8 ``[..., C]``) in units of ``2**(exponents - 127)`` (uint8
     ``[..., ceil(C/32)]``: one for 32 consecutive channels).  ``dtype`` is that of the tensor that was kept."""
-    __slots__ = ("shape", "dtype", "_values", "_exponents", "_buffer")
+    __slots__ = ("shape", "dtype", "_values", "_exponents", "_buffer", "_at")
 
     def __init__(self, values: torch.Tensor, exponents: torch.Tensor, dtype: torch.dtype):
         self.shape, self.dtype, self._values, self._exponents, self._buffer = values.shape, dtype, values, exponents, None
@@ -159,13 +159,15 @@ class Kept8:
     @property
     def values(self) -> torch.Tensor:
         if self._values is None:
-            self._values = self._buffer[:self.shape.numel()].view(self.shape)
+            self._values = self._buffer[self._at:self._at + self.shape.numel()].view(self.shape)
         return self._values
 
     @property
     def exponents(self) -> torch.Tensor:
         if self._exponents is None:
-            self._exponents = self._buffer[self.shape.numel():].view(torch.uint8).view(self.shape[:-1] + (-(-self.shape[-1] // KEPT_GROUP),))
+            groups = self.shape[:-1] + (-(-self.shape[-1] // KEPT_GROUP),)
+            at = self._at + self.shape.numel()
+            self._exponents = self._buffer[at:at + groups.numel()].view(torch.uint8).view(groups)
         return self._exponents
 
     @property
@@ -185,13 +187,19 @@ def _kept_size(t, what):
     return n, C
 
 
-def _kept_empty(x, n, C):
-    """Room for x ([n, C]) in 8 bits, in one piece: the values, then the exponents; and the addresses of both."""
-    kept = Kept8.__new__(Kept8)
-    kept.shape, kept.dtype, kept._values, kept._exponents = x.shape, x.dtype, None, None
-    kept._buffer = buffer = torch.empty(n * (C + -(-C // KEPT_GROUP)), dtype=torch.int8, device=x.device)
-    at = buffer.data_ptr()
-    return kept, at, at + n * C
+def _kept_empty(x, n, C, count):
+    """Room for ``count`` tensors like x ([n, C]) in 8 bits in one allocation: each its values, then its exponents, on boundaries of 16
+    bytes.  Returns them and the addresses of their values and exponents."""
+    size = n * (C + -(-C // KEPT_GROUP))
+    step = size + -size % 16
+    buffer = torch.empty(step * count, dtype=torch.int8, device=x.device)
+    start, shape, dtype, made, addresses = buffer.data_ptr(), x.shape, x.dtype, [], []
+    for at in range(0, step * count, step) if n else (0,) * count:
+        kept = Kept8.__new__(Kept8)
+        kept.shape, kept.dtype, kept._values, kept._exponents, kept._buffer, kept._at = shape, dtype, None, None, buffer, at
+        made.append(kept)
+        addresses += (start + at, start + at + n * C)
+    return made, addresses
 
 
 def _check_kept(kept, name, shape, device):
@@ -199,7 +207,7 @@ def _check_kept(kept, name, shape, device):
         raise MoeError(f"{name}: expected a Kept8, got {type(kept).__name__}")
     buffer = kept._buffer
     if buffer is not None and kept.shape == shape and buffer.device == device:
-        at = buffer.data_ptr()
+        at = buffer.data_ptr() + kept._at
         return at, at + shape.numel()
     groups = -(-shape[-1] // KEPT_GROUP)
     return (_check(kept.values, f"{name}.values", shape, _I8, device),
@@ -214,8 +222,8 @@ def keep8(x: torch.Tensor) -> Kept8:
     device = _device(x)
     n, C = _kept_size(x, "keep8")
     xp = _check(x, "x", x.shape, _EITHER, device)
-    kept, values, exponents = _kept_empty(x, n, C)
-    _lib.check(lib.mgpt_moe_op_keep8(xp, _DTYPES[x.dtype], n, C, values, exponents, _stream(device)))
+    (kept,), addresses = _kept_empty(x, n, C, 1)
+    _lib.check(lib.mgpt_moe_op_keep8(xp, _DTYPES[x.dtype], n, C, *addresses, _stream(device)))
     return kept
 
 
@@ -268,7 +276,7 @@ def residual_norm(x: torch.Tensor, h: torch.Tensor, *, post_scale=None, gate=Non
     ``gate`` it is 1, without ``pre_scale`` there is no u (None).  ``gate``: FP32 ``[rows, C]``, a row for every
     ``tokens_per_gate`` consecutive tokens (0: one row, which may be given as ``[C]``).  Returns ``(y, u, stats)``; ``stats`` is
     what :func:`residual_norm_backward` needs.  With ``keep``: ``(y, u, stats, (x8, h8))``, x and h in 8 bits as :func:`keep8` keeps
-    them, from the same pass."""
+    them, from the same pass and in one allocation."""
     lib = _lib.load()
     device, n, C, _, tokens_per_gate, xp, hp, post, gp, pre = _norm_args(x, h, post_scale, gate, pre_scale, tokens_per_gate)
     y = torch.empty_like(x)
@@ -278,9 +286,9 @@ def residual_norm(x: torch.Tensor, h: torch.Tensor, *, post_scale=None, gate=Non
     if not keep:
         _lib.check(lib.mgpt_moe_op_residual_norm(*args, _stream(device)))
         return y, u, stats
-    (x8, xv, xe), (h8, hv, he) = _kept_empty(x, n, C), _kept_empty(h, n, C)
-    _lib.check(lib.mgpt_moe_op_residual_norm_keep(*args, xv, xe, hv, he, _stream(device)))
-    return y, u, stats, (x8, h8)
+    kept, addresses = _kept_empty(x, n, C, 2)
+    _lib.check(lib.mgpt_moe_op_residual_norm_keep(*args, *addresses, _stream(device)))
+    return y, u, stats, tuple(kept)
 
 
 def residual_norm_backward(x, h, stats: torch.Tensor, dy: torch.Tensor, du: torch.Tensor = None, *, post_scale=None,
