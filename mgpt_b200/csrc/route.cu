@@ -159,7 +159,12 @@ __device__ __forceinline__ void store4(bf16* p, const float (&v)[4])
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store1(bf16* p, float v) { *p = __float2bfloat16(v); }
 
-__device__ __forceinline__ float sigmoid(float z) { return 1.0f / (1.0f + expf(-z)); }
+// (of numbers far below zero too: neither exponential is infinite)
+__device__ __forceinline__ float sigmoid(float z)
+{
+    const float e = expf(-fabsf(z));
+    return (z < 0.0f ? e : 1.0f) / (1.0f + e);
+}
 
 // The groups that stay, a bit each, of a token's scores c (minus infinity: out): its lanes call it.  *close: the last that stays and the first
 // that does not differ by `margin` or less.  The warp's shared memory: c [tokens][E], then room for [tokens][groups].
