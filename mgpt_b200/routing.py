@@ -61,8 +61,7 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: tor
     _need(0 < top_k <= E, "routing: top_k is 1 to the number of experts")
     r = _routing(E, score, bias, groups, top_groups, group_top, renormalise, scale, device)
     cp = None if counts is None else _check(counts, "counts", (E,), _I32, device)
-    shape = logits.shape[:-1] + (top_k,)
-    top_idx = torch.empty(shape, dtype=torch.int32, device=device)
+    top_idx = torch.empty(*logits.shape[:-1], top_k, dtype=torch.int32, device=device)
     weights = torch.empty_like(top_idx, dtype=torch.float32)
     _lib.check(lib.mgpt_moe_op_route(lp, _DTYPES[logits.dtype], n, E, top_k, ct.byref(r), top_idx.data_ptr(), weights.data_ptr(), cp, _stream(device)))
     return top_idx, weights

@@ -187,19 +187,15 @@ def _kept_size(t, what):
     return n, C
 
 
-def _kept_empty(x, n, C, count):
-    """Room for ``count`` tensors like x ([n, C]) in 8 bits in one allocation: each its values, then its exponents, on boundaries of 16
-    bytes.  Returns them and the addresses of their values and exponents."""
-    size = n * (C + -(-C // KEPT_GROUP))
-    step = size + -size % 16
-    buffer = torch.empty(step * count, dtype=torch.int8, device=x.device)
-    start, shape, dtype, made, addresses = buffer.data_ptr(), x.shape, x.dtype, [], []
-    for at in range(0, step * count, step) if n else (0,) * count:
-        kept = Kept8.__new__(Kept8)
-        kept.shape, kept.dtype, kept._values, kept._exponents, kept._buffer, kept._at = shape, dtype, None, None, buffer, at
-        made.append(kept)
-        addresses += (start + at, start + at + n * C)
-    return made, addresses
+def _kept_in(buffer, at, x):
+    kept = Kept8.__new__(Kept8)
+    kept.shape, kept.dtype, kept._values, kept._exponents, kept._buffer, kept._at = x.shape, x.dtype, None, None, buffer, at
+    return kept
+
+
+def _kept_bytes(n, C):
+    """Of [n, C] in 8 bits: the values, then the exponents, up to a boundary of 16 bytes."""
+    return (n * (C + -(-C // KEPT_GROUP)) + 15) // 16 * 16
 
 
 def _check_kept(kept, name, shape, device):
@@ -222,9 +218,10 @@ def keep8(x: torch.Tensor) -> Kept8:
     device = _device(x)
     n, C = _kept_size(x, "keep8")
     xp = _check(x, "x", x.shape, _EITHER, device)
-    (kept,), addresses = _kept_empty(x, n, C, 1)
-    _lib.check(lib.mgpt_moe_op_keep8(xp, _DTYPES[x.dtype], n, C, *addresses, _stream(device)))
-    return kept
+    buffer = torch.empty(_kept_bytes(n, C), dtype=torch.int8, device=device)
+    at = buffer.data_ptr()
+    _lib.check(lib.mgpt_moe_op_keep8(xp, _DTYPES[x.dtype], n, C, at, at + n * C, _stream(device)))
+    return _kept_in(buffer, 0, x)
 
 
 def restore8(kept: Kept8, dtype: torch.dtype = None) -> torch.Tensor:
@@ -237,7 +234,7 @@ def restore8(kept: Kept8, dtype: torch.dtype = None) -> torch.Tensor:
     if dtype not in _DTYPES:
         raise MoeError(f"restore8: unsupported dtype {dtype}")
     values, exponents = _check_kept(kept, "kept", kept.shape, device)
-    x = torch.empty(kept.shape, dtype=dtype, device=device)
+    x = torch.empty(*kept.shape, dtype=dtype, device=device)      # (as numbers: half the time of a shape)
     _lib.check(lib.mgpt_moe_op_restore8(values, exponents, n, C, x.data_ptr(), _DTYPES[dtype], _stream(device)))
     return x
 
@@ -258,15 +255,14 @@ def _norm_args(x, h, post_scale, gate, pre_scale, tokens_per_gate, like=None):
         tokens_per_gate = min(tokens_per_gate, n)       # (C's int does not hold every number that means one row)
     else:
         rows = 1
-    if gate is not None and rows == 1 and gate.dim() == 1 and gate.numel() == C:
-        gate = gate.view(1, C)
     types, cols = (dtype,), (C,)
+    gates = cols if gate is not None and rows == 1 and gate.dim() == 1 else (rows, C)
     if kept:
         xp, hp = _check_kept(x, "x", shape, device), _check_kept(h, "h", shape, device)
     else:
         xp, hp = _check(x, "x", shape, types, device), _check(h, "h", shape, types, device)
     return (device, n, C, rows, tokens_per_gate, xp, hp, _optional(post_scale, "post_scale", cols, _F32, device),
-            _optional(gate, "gate", (rows, C), _F32, device), _optional(pre_scale, "pre_scale", cols, _F32, device))
+            _optional(gate, "gate", gates, _F32, device), _optional(pre_scale, "pre_scale", cols, _F32, device))
 
 
 def residual_norm(x: torch.Tensor, h: torch.Tensor, *, post_scale=None, gate=None, pre_scale=None, alpha: float = 1.0, eps: float = 1e-5,
@@ -281,14 +277,16 @@ def residual_norm(x: torch.Tensor, h: torch.Tensor, *, post_scale=None, gate=Non
     device, n, C, _, tokens_per_gate, xp, hp, post, gp, pre = _norm_args(x, h, post_scale, gate, pre_scale, tokens_per_gate)
     y = torch.empty_like(x)
     u = torch.empty_like(x) if pre_scale is not None else None
-    stats = torch.empty((2, n), dtype=torch.float32, device=device)
+    stats = torch.empty(2, n, dtype=torch.float32, device=device)
     args = (xp, hp, _DTYPES[x.dtype], post, gp, tokens_per_gate, pre, alpha, eps, n, C, y.data_ptr(), None if u is None else u.data_ptr(), stats.data_ptr())
     if not keep:
         _lib.check(lib.mgpt_moe_op_residual_norm(*args, _stream(device)))
         return y, u, stats
-    kept, addresses = _kept_empty(x, n, C, 2)
-    _lib.check(lib.mgpt_moe_op_residual_norm_keep(*args, *addresses, _stream(device)))
-    return y, u, stats, tuple(kept)
+    size = _kept_bytes(n, C)
+    buffer = torch.empty(2 * size, dtype=torch.int8, device=device)
+    at = buffer.data_ptr()
+    _lib.check(lib.mgpt_moe_op_residual_norm_keep(*args, at, at + n * C, at + size, at + size + n * C, _stream(device)))
+    return y, u, stats, (_kept_in(buffer, 0, x), _kept_in(buffer, size, h))
 
 
 def residual_norm_backward(x, h, stats: torch.Tensor, dy: torch.Tensor, du: torch.Tensor = None, *, post_scale=None,
@@ -304,9 +302,8 @@ def residual_norm_backward(x, h, stats: torch.Tensor, dy: torch.Tensor, du: torc
     f32 = _F32
     sp = _check(stats, "stats", (2, n), f32, device)
     dyp, dup = _check(dy, "dy", x.shape, (dy.dtype if kept else x.dtype,), device), _optional(du, "du", x.shape, (dy.dtype,), device)
-    if d_gate is not None and d_gate.dim() == 1 and rows == 1 and d_gate.numel() == C:
-        d_gate = d_gate.view(1, C)
-    dpost, dgate, dpre = (_optional(d_post_scale, "d_post_scale", (C,), f32, device), _optional(d_gate, "d_gate", (rows, C), f32, device),
+    gates = (C,) if d_gate is not None and rows == 1 and d_gate.dim() == 1 else (rows, C)
+    dpost, dgate, dpre = (_optional(d_post_scale, "d_post_scale", (C,), f32, device), _optional(d_gate, "d_gate", gates, f32, device),
                           _optional(d_pre_scale, "d_pre_scale", (C,), f32, device))
     dx, dh = torch.empty_like(dy), torch.empty_like(dy)
     size = lib.mgpt_moe_op_residual_norm_backward_workspace_bytes(n, C, tokens_per_gate)
