@@ -105,6 +105,12 @@ class CudaStages:
     def _stream():
         return ct.c_void_p(torch.cuda.current_stream().cuda_stream)
 
+    def set_routing(self, score=None, **how):
+        """Arguments of ``MoELayer.set_routing``, for the routing side."""
+        from .routing import _set
+        _set(self.lib, self.home, self.E, self.device, score, **how)
+        self._routing_bias = how.get("bias")        # (read by every call)
+
     def adamw_step(self, t, lr=3e-4, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01):
         """One fused AdamW step (BF16 copies refreshed in the same pass) over the router replica and this
         rank's experts; moment buffers ``opt_m`` / ``opt_v`` (router first, then the experts) are created on first use."""
@@ -413,6 +419,11 @@ class ExpertParallelMoE:
         """Optimiser step over the router replica and this rank's experts (sum the router gradients over the
         group first with ``allreduce_router_grads()`` if the replicas are to stay identical)."""
         self.stages.adamw_step(t, **hyper)
+
+    def set_routing(self, score=None, **how):
+        """As :meth:`mgpt_b200.MoELayer.set_routing`.  A bias is each rank's own: ranks that are to route alike need the same one, moved
+        by counts that are summed over the group."""
+        self.stages.set_routing(score, **how)
 
     def allreduce_router_grads(self):
         """Sum the router gradients over the group so that the replicas stay identical."""

@@ -17,7 +17,7 @@ import torch
 
 from . import _lib
 from ._lib import BF16, FP32, IO_BF16, IO_F32, MoeError  # noqa: F401
-from .routing import _routing
+from .routing import _set
 
 
 class MoELayer:
@@ -95,13 +95,8 @@ class MoELayer:
         """Has the layer choose and weigh its experts as :func:`mgpt_b200.route` does, from its own router's logits, in every forward and
         backward that follows; without arguments: as the reference does.  ``bias`` (FP32 ``[E]``) is kept and read by every call, so
         that changing it in place is enough.  There is no load-balance term then."""
-        if score is None:
-            _lib.check(self.lib.mgpt_moe_set_routing(self._h, None))
-            self._routing_bias = None
-            return
-        r = _routing(self.E, score, bias, groups, top_groups, group_top, renormalise, scale, self.device)
-        _lib.check(self.lib.mgpt_moe_set_routing(self._h, ct.byref(r)))
-        self._routing_bias = bias
+        _set(self.lib, self._h, self.E, self.device, score, bias, groups, top_groups, group_top, renormalise, scale)
+        self._routing_bias = bias if score is not None else None
 
     # -- optimiser -----------------------------------------------------------
     def adamw_step(self, t: int, lr: float = 3e-4, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8,

@@ -32,6 +32,15 @@ def _routing(E, score, bias, groups, top_groups, group_top, renormalise, scale, 
     return r
 
 
+def _set(lib, handle, E, device, score, bias=None, groups=1, top_groups=None, group_top=2, renormalise=False, scale=1.0):
+    """Has the layer behind the handle route so (score None: as the reference does)."""
+    if score is None:
+        _lib.check(lib.mgpt_moe_set_routing(handle, None))
+    else:
+        r = _routing(E, score, bias, groups, top_groups, group_top, renormalise, scale, device)
+        _lib.check(lib.mgpt_moe_set_routing(handle, ct.byref(r)))
+
+
 def _logits(logits):
     device, shape = _device(logits), logits.shape
     if not shape or not shape[-1] or logits.dtype not in _DTYPES:

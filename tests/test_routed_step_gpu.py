@@ -141,6 +141,30 @@ def test_the_layer_cut_at_its_exchange_points(mode, dtype):
         assert _rel(side.get_parameters()[i].grad, whole.get_parameters()[i].grad.double()) < bar
 
 
+@pytest.mark.parametrize("chunks", [1, 2])
+@pytest.mark.parametrize("mode,dtype", [("fp32", torch.float32), ("bf16", torch.bfloat16)])
+def test_the_expert_parallel_layer_with_one_rank(mode, dtype, chunks):
+    from mgpt_b200.ep import ExpertParallelMoE
+    n, C, H, E, k = 333, 64, 128, 8, 3
+    bias = torch.randn(E, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)) * 0.1
+    how = dict(bias=bias, groups=4, top_groups=2, renormalise=True, scale=1.5)
+    whole = _layer(C, H, E, k, mode)
+    ep = ExpertParallelMoE(C, H, E, k, mode=mode, n_chunks=chunks)
+    ep.load_parameters([p.detach() for p in whole.get_parameters()])
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, dy = (torch.randn(n, C, device="cuda", generator=g).to(dtype) for _ in range(2))
+    bar = 1e-5 if mode == "fp32" else 1e-2
+    for score in ("sigmoid", "softmax", None):
+        for layer in (whole, ep):
+            layer.set_routing(score, **(how if score else {}))
+            layer.zero_grad()
+        y, y2 = whole.forward(x), ep.forward(x)
+        dx, dx2 = whole.backward(dy), ep.backward(dy)
+        assert _rel(y2, y.double()) < bar and _rel(dx2, dx.double()) < bar
+        for p, q in zip(whole.get_parameters(), ep.get_parameters()):
+            assert _rel(q.grad, p.grad.double()) < bar
+
+
 @pytest.mark.parametrize("mode,dtype", [("fp32", torch.float32), ("bf16", torch.bfloat16)])
 def test_the_blocks_glue(mode, dtype):
     n, C, H, E, k = 150, 64, 128, 8, 2
