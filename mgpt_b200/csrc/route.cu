@@ -381,8 +381,8 @@ __device__ __noinline__ bool settle_group(const RouteP& p, int tok, bool have, f
 // than R: the last step, and so is what is out), with e + 1 added below: keys are unlike each other, equal scores go by index, and a round
 // is the least key above the last round's: an addition and a minimum per expert, one reduction, nothing to cross out.  Two
 // keys in a row that are further apart than the scores may be wrong are in the right order.  Where some are not, what was chosen and
-// what is not far enough behind it are put in order by their exact values (FP64; the logits themselves where they decide).  Groups
-// whose scores are too close send the token to route_again.
+// what is not far enough behind it are put in order by their exact values (FP64; the logits themselves where they decide).  Of groups
+// whose scores are too close settle_group decides; a token that is none of this (see `unsure`) is left to route_again.
 enum { BY_LOGIT, BY_SCORE, BY_GROUP };          // no bias and no choice of groups; a bias; groups
 template <typename T, int L, int P, int HOW>
 __global__ void __launch_bounds__(32 * WARPS, P > 8 ? 5 : 8) route_kernel(const RouteP p)
