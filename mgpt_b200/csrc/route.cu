@@ -18,7 +18,7 @@
 // integer pipe (minima and comparisons run at half the rate of additions): about 180 instructions per token of 128 experts and 8
 // chosen, 690 per token of 256 in groups.  us in a graph on a B200, FP32 logits: 8 x 256 in
 // groups 4.3, 32768 x 64, 4 chosen 8.5, 32768 x 256 in groups, 8 chosen 35 (floor 5.3), 131072 x 128, 8 chosen 36 (floor 12); backward
-// of the last two 7.9 (sigmoid; 4.3 TB/s) and 29 (softmax; 4.6 TB/s).  Of the forward call 2 us are the counts' atomics, where counts are asked for.
+// of the last two 7.9 (sigmoid; 4.3 TB/s) and 27 (softmax; 5.0 TB/s; with six blocks per SM 29).  Of the forward call 2 us are the counts' atomics, where counts are asked for.
 // Not kept: the eight least by sorting and merging lists (38 against 36 us, 39 against 35: more minima), two warps per block (44 against 38),
 // six to eight blocks per SM (37 to 41 against 36).
 #include "common.cuh"
@@ -722,7 +722,7 @@ template <typename T> __global__ void __launch_bounds__(32 * WARPS) route_sigmoi
 // That of a softmax's: L lanes per token, at least as many as there are chosen experts, P experts each, four neighbouring ones at a time (a
 // warp's accesses are runs of memory).  The next tokens' logits are on their way while these are worked on.
 template <typename T, int L, int P>
-__global__ void __launch_bounds__(32 * WARPS) route_softmax_bwd_kernel(const RouteP p)
+__global__ void __launch_bounds__(32 * WARPS, 8) route_softmax_bwd_kernel(const RouteP p)
 {
     constexpr int TOKENS = 32 / L;
     __shared__ __align__(16) float shr[WARPS][32 * P];          // [tokens][L * P]: dg, zeros but for the chosen
@@ -825,7 +825,7 @@ template <typename T, int L, int P> int run_fwd(RouteP& p, cudaStream_t st)
 }
 template <typename T, int L, int P> int run_softmax_bwd(const RouteP& p, cudaStream_t st)
 {
-    const int per = WARPS * (32 / L), want = (p.n + per - 1) / per, most = 148 * 6;
+    const int per = WARPS * (32 / L), want = (p.n + per - 1) / per, most = 148 * 8;
     MGPT_CUDA(launch_pdl(route_softmax_bwd_kernel<T, L, P>, want < most ? want : most, 32 * WARPS, 0, st, p));
     MGPT_LAUNCHED("route_softmax_bwd_kernel");
     return 0;
