@@ -5,9 +5,10 @@
 //   chosen are their k largest c in falling order, equal ones by index; without a bias the order is that of z itself
 //   w_j = scale * s_j / (sum of the chosen s + 1e-20)   or   scale * s_j
 //
-// Gradient, with S the sum of the chosen s plus 1e-20 and A = sum dw_j s_j:
-//   dg_j = scale / S * (dw_j - A / S)   or   scale * dw_j
+// Gradient, with S the sum of the chosen s plus 1e-20, A = sum dw_j s_j and T_j = sum_i s_i (dw_j - dw_i):
+//   dg_j = scale / S * (dw_j - A / S) = scale / S * (T_j + 1e-20 dw_j) / S   or   scale * dw_j
 //   sigmoid: dz_e = dg_j s_j (1 - s_j) for the chosen, 0 elsewhere;   softmax: dz_e = p_e ([chosen] dg_j - sum_j dg_j p_j)
+// (dw_j - A / S as it stands has no digits left where one expert has nearly all of S; of a single chosen expert it is rounding and nothing else.)
 // The reference has clamped softmax and top-k only (utils/Tensor.cpp:850-909).
 //
 // What is chosen is what exact arithmetic chooses (up to FP64's rounding): scores are formed in FP32 with a known bound on their
@@ -648,15 +649,6 @@ __global__ void __launch_bounds__(32 * WARPS, P > 8 ? 5 : 8) route_kernel(const 
     }
 }
 
-// dg of a chosen expert: the sums of its token's weights, scale / S and A / S
-struct Token {
-    float of, mean;
-};
-__device__ __forceinline__ Token token_of(const RouteP& p, float S, float A)
-{
-    const float over = 1.0f / (S + TINY);
-    return p.renorm ? Token{p.scale * over, A * over} : Token{p.scale, 0.0f};
-}
 __device__ __forceinline__ bool has_gradient(const RouteP& p, int e) { return e >= 0 && e < p.E && !(p.bias && !(p.bias[e] > -INFINITY)); }
 
 // The gradient of a sigmoid's logits: zeros but for the chosen.  A lane per chosen expert, as many tokens per warp as that gives (at most
@@ -686,16 +678,20 @@ template <typename T> __global__ void __launch_bounds__(32 * WARPS) route_sigmoi
                 e = -1;
             }
         }
-        float S = 0.0f, A = 0.0f;
+        float share = g;                        // with its factor, dg of the weight
         if (p.renorm) {
-            const float product = g != 0.0f ? dw * g : 0.0f;
+            const float known = g != 0.0f ? dw : 0.0f;
+            float S = 0.0f, diff = 0.0f;
             for (int j = 0; j < p.k; ++j) {
-                S += __shfl_sync(FULL, g, (first + j) & 31);
-                A += __shfl_sync(FULL, product, (first + j) & 31);
+                const float gj = __shfl_sync(FULL, g, (first + j) & 31);
+                S += gj;
+                diff = fmaf(gj, dw - __shfl_sync(FULL, known, (first + j) & 31), diff);
             }
+            const float over = 1.0f / (S + TINY);
+            share *= over;
+            dw = fmaf(TINY, dw, diff) * over;
         }
-        const Token of = token_of(p, S, A);
-        if (e >= 0 && g != 0.0f) atomicAdd(&rows[mt * p.E + e], of.of * (dw - of.mean) * g * rest);       // (one writer each, unless the caller repeats an index)
+        if (e >= 0 && g != 0.0f) atomicAdd(&rows[mt * p.E + e], p.scale * dw * share * rest);       // (one writer each, unless the caller repeats an index)
         __syncwarp();
         T* const out = (T*)p.dz + tok0 * p.E;
         const int count = tokens * p.E;
@@ -773,18 +769,19 @@ __global__ void __launch_bounds__(32 * WARPS, 8) route_softmax_bwd_kernel(const 
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         // a lane per chosen expert
         const float ctop = __shfl_sync(FULL, top, ct * L), cinv = __shfl_sync(FULL, inv, ct * L);
-        const float g = !mine || v == -INFINITY ? 0.0f : expf(v - ctop) * cinv, product = g != 0.0f ? dw1 * g : 0.0f;
-        float S = 0.0f, A = 0.0f;
-#pragma unroll 4
+        const float g = !mine || v == -INFINITY ? 0.0f : expf(v - ctop) * cinv, known = g != 0.0f ? dw1 : 0.0f;
+        float S = 0.0f, A = 0.0f, diff = 0.0f;
+#pragma unroll 1            // (unrolled: spills, 31 us against 27.6 at 131072 x 128)
         for (int j = 0; j < p.k; ++j) {
-            S += __shfl_sync(FULL, g, mt * p.k + j);
-            A += __shfl_sync(FULL, product, mt * p.k + j);
+            const float gj = __shfl_sync(FULL, g, ct * p.k + j), dj = __shfl_sync(FULL, known, ct * p.k + j);
+            S += gj;
+            A = fmaf(gj, dj, A);
+            diff = fmaf(gj, dw1 - dj, diff);
         }
-        const Token of = token_of(p, S, A);
+        const float over = 1.0f / (S + TINY);
         // sum of dg p: renormalised, scale / S * (A - A * (S - 1e-20) / S)
-        const float D = p.renorm ? of.mean * (of.of * TINY) : p.scale * A;
-        const float cof = __shfl_sync(FULL, of.of, ct * L), cmean = __shfl_sync(FULL, of.mean, ct * L);
-        if (mine) atomicAdd(&rows[ct * L * P + e1], cof * (dw1 - cmean));       // (one writer each, unless the caller repeats an index)
+        const float D = __shfl_sync(FULL, p.renorm ? A * over * (p.scale * over * TINY) : p.scale * A, mt * p.k);
+        if (mine) atomicAdd(&rows[ct * L * P + e1], p.renorm ? p.scale * over * (fmaf(TINY, dw1, diff) * over) : p.scale * dw1);       // (one writer each, unless the caller repeats an index)
         __syncwarp();
         T* const out = (T*)p.dz + (size_t)tok * p.E;
 #pragma unroll
