@@ -7,8 +7,9 @@
 //
 // Gradient, with S the sum of the chosen s plus 1e-20, A = sum dw_j s_j and T_j = sum_i s_i (dw_j - dw_i):
 //   dg_j = scale / S * (dw_j - A / S) = scale / S * (T_j + 1e-20 dw_j) / S   or   scale * dw_j
-//   sigmoid: dz_e = dg_j s_j (1 - s_j) for the chosen, 0 elsewhere;   softmax: dz_e = p_e ([chosen] dg_j - sum_j dg_j p_j)
-// (dw_j - A / S as it stands has no digits left where one expert has nearly all of S; of a single chosen expert it is rounding and nothing else.)
+//   sigmoid: dz_e = dg_j s_j (1 - s_j) for the chosen, 0 elsewhere;   softmax: dz_e = p_e ([chosen] dg_j - sum_j dg_j p_j),
+//   of weights as they are scale p_e (T_j + dw_j * the sum of the p that were not chosen) for the chosen, -scale p_e A elsewhere
+// (dw_j - A / S and dw_j - A as they stand have no digits left where one expert has nearly all of S; of a single chosen expert they are rounding.)
 // The reference has clamped softmax and top-k only (utils/Tensor.cpp:850-909).
 //
 // What is chosen is what exact arithmetic chooses (up to FP64's rounding): scores are formed in FP32 with a known bound on their
@@ -717,15 +718,18 @@ template <typename T> __global__ void __launch_bounds__(32 * WARPS) route_sigmoi
 
 // That of a softmax's: L lanes per token, at least as many as there are chosen experts, P experts each, four neighbouring ones at a time (a
 // warp's accesses are runs of memory).  The next tokens' logits are on their way while these are worked on.
-template <typename T, int L, int P>
+template <typename T, int L, int P, bool RENORM>
 __global__ void __launch_bounds__(32 * WARPS, 8) route_softmax_bwd_kernel(const RouteP p)
 {
     constexpr int TOKENS = 32 / L;
     __shared__ __align__(16) float shr[WARPS][32 * P];          // [tokens][L * P]: dg, zeros but for the chosen
+    __shared__ uint32_t shb[RENORM ? 1 : WARPS][32];            // bits of a lane's experts that were chosen, for weights as they are
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % L, mt = lane / L;
     const int ct = min((int)(lane * p.kdiv >> 16), TOKENS - 1), cj = lane - ct * p.k;      // the token and place of the lane's chosen expert (cj < k)
     float* const rows = shr[warp];
+    uint32_t* const bits = shb[RENORM ? 0 : warp];
     for (int i = lane; i < 32 * P; i += 32) rows[i] = 0.0f;
+    if (!RENORM) bits[lane] = 0;
     pdl_wait();
     const int stride = gridDim.x * WARPS * TOKENS;
     int tok0 = (blockIdx.x * WARPS + warp) * TOKENS;
@@ -751,8 +755,9 @@ __global__ void __launch_bounds__(32 * WARPS, 8) route_softmax_bwd_kernel(const 
     __syncwarp();
     for (; tok0 < p.n; tok0 += stride) {
         const int tok = tok0 + mt, e1 = e;
-        const bool have = tok < p.n, mine = has_gradient(p, e1);
-        const float dw1 = dw;
+        const bool have = tok < p.n;
+        bool mine = has_gradient(p, e1);
+        float dw1 = dw, rest = 0.0f;
         if (mine) v = as_float(((const T*)p.logits)[(size_t)(tok0 + ct) * p.E + e1]);
         float pr[P], top = z[0], sum = 0.0f;
 #pragma unroll
@@ -767,6 +772,23 @@ __global__ void __launch_bounds__(32 * WARPS, 8) route_softmax_bwd_kernel(const 
         load(tok0 + stride);
         sum = lanes_sum<L>(sum);
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        if constexpr (!RENORM) {
+            // what was not chosen, and the entries that repeat an expert together, in the place of one of them
+            bool one = false;
+            if (mine) {
+                const uint32_t bit = 1u << (e1 / (4 * L) * 4 + e1 % 4);
+                atomicAdd(&rows[ct * L * P + e1], dw1);
+                one = !(atomicOr(&bits[ct * L + e1 / 4 % L], bit) & bit);
+            }
+            __syncwarp();
+            const uint32_t chosen = bits[lane];
+            bits[lane] = 0;
+#pragma unroll
+            for (int i = 0; i < P; ++i) rest += chosen >> i & 1 ? 0.0f : pr[i];
+            rest = lanes_sum<L>(rest) * inv;
+            if (mine) dw1 = rows[ct * L * P + e1];
+            mine = one;
+        }
         // a lane per chosen expert
         const float ctop = __shfl_sync(FULL, top, ct * L), cinv = __shfl_sync(FULL, inv, ct * L);
         const float g = !mine || v == -INFINITY ? 0.0f : expf(v - ctop) * cinv, known = g != 0.0f ? dw1 : 0.0f;
@@ -780,8 +802,18 @@ __global__ void __launch_bounds__(32 * WARPS, 8) route_softmax_bwd_kernel(const 
         }
         const float over = 1.0f / (S + TINY);
         // sum of dg p: renormalised, scale / S * (A - A * (S - 1e-20) / S)
-        const float D = __shfl_sync(FULL, p.renorm ? A * over * (p.scale * over * TINY) : p.scale * A, mt * p.k);
-        if (mine) atomicAdd(&rows[ct * L * P + e1], p.renorm ? p.scale * over * (fmaf(TINY, dw1, diff) * over) : p.scale * dw1);       // (one writer each, unless the caller repeats an index)
+        float D = __shfl_sync(FULL, RENORM ? A * over * (p.scale * over * TINY) : p.scale * A, mt * p.k);
+        if constexpr (RENORM) {
+            if (mine) atomicAdd(&rows[ct * L * P + e1], p.scale * over * (fmaf(TINY, dw1, diff) * over));       // (one writer each, unless the caller repeats an index)
+        } else {
+            const float crest = __shfl_sync(FULL, rest, ct * L);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < P; i += 4) store4(rows + mt * L * P + (i / 4 * L + sub) * 4, {-D, -D, -D, -D});
+            D = 0.0f;
+            __syncwarp();
+            if (mine) rows[ct * L * P + e1] = p.scale * fmaf(dw1, crest, diff);
+        }
         __syncwarp();
         T* const out = (T*)p.dz + (size_t)tok * p.E;
 #pragma unroll
@@ -823,7 +855,7 @@ template <typename T, int L, int P> int run_fwd(RouteP& p, cudaStream_t st)
 template <typename T, int L, int P> int run_softmax_bwd(const RouteP& p, cudaStream_t st)
 {
     const int per = WARPS * (32 / L), want = (p.n + per - 1) / per, most = 148 * 8;
-    MGPT_CUDA(launch_pdl(route_softmax_bwd_kernel<T, L, P>, want < most ? want : most, 32 * WARPS, 0, st, p));
+    MGPT_CUDA(launch_pdl(p.renorm ? route_softmax_bwd_kernel<T, L, P, true> : route_softmax_bwd_kernel<T, L, P, false>, want < most ? want : most, 32 * WARPS, 0, st, p));
     MGPT_LAUNCHED("route_softmax_bwd_kernel");
     return 0;
 }

@@ -61,7 +61,8 @@ def _dw(n, k, seed=5):
 
 SCORES = ["softmax", "sigmoid"]
 TYPES = [torch.float32, torch.bfloat16]
-WAYS = [True]                                                           # renormalised
+# renormalised or not
+WAYS = [True, False]
 
 
 @pytest.mark.parametrize("score", SCORES)
@@ -146,6 +147,16 @@ def test_repeated_experts():
     dw = torch.tensor([[1.0, 0.5, 2.0, 7.0]], device="cuda").expand(3, 4).contiguous()
     p = torch.softmax(z.double(), 1)
     p5, p1 = p[:, 5:6], p[:, 1:2]
+    got = mgpt_b200.route_backward(z, idx, dw).double()
+    rest = p.clone()
+    rest[:, 5] = rest[:, 1] = 0.0
+    rest = rest.sum(1, keepdim=True)
+    A = 1.5 * p5 + 2.0 * p1
+    want = -p * A
+    want[:, 5:6], want[:, 1:2] = p5 * (p1 * (1.5 - 2.0) + 1.5 * rest), p1 * (p5 * (2.0 - 1.5) + 2.0 * rest)
+    size = p * A
+    size[:, 5:6], size[:, 1:2] = p5 * (p1 * 0.5 + 1.5 * rest), p1 * (p5 * 0.5 + 2.0 * rest)
+    assert ((got - want).abs() <= (64 + 4 * 24) * U * size).all()
     got = mgpt_b200.route_backward(z, idx, dw, renormalise=True).double()
     S = 2.0 * p5 + p1
     want, size = torch.zeros_like(p), torch.full_like(p, 1e-19)
