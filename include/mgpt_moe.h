@@ -320,7 +320,7 @@ int  mgpt_moe_op_router(const void* x, int io_dtype, const float* Wr, const floa
  *   order, equal ones by index (without a bias: the k largest z);   w = scale * s / (sum of the chosen s + 1e-20), or scale * s
  * The choice is that of exact arithmetic (comparisons too close for FP32 are made in FP64). An expert whose logit or bias is -inf or NaN
  * is out: chosen, by index and with weight 0, only where fewer than k others are left. A NaN among a token's logits (softmax: or
- * +inf) makes its weights NaN. top_idx always holds k different numbers of [0, E), in the form mgpt_moe_op_plan takes.
+ * +inf) makes its weights NaN; its experts are chosen as ever (softmax: m logits of +inf have the scores 1/m, the others 0). top_idx always holds k different numbers of [0, E), in the form mgpt_moe_op_plan takes.
  * counts (may be NULL): int32 [E], added to: how many tokens chose an expert (what a bias is adjusted by). E up to 512, k up to 32. */
 int  mgpt_moe_op_route(const void* logits, int io, int n, int E, int k, const mgpt_moe_routing* routing,
                        int32_t* top_idx, float* weights, int32_t* counts, mgpt_stream_t stream);

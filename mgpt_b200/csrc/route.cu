@@ -14,7 +14,7 @@
 //
 // What is chosen is what exact arithmetic chooses (up to FP64's rounding): scores are formed in FP32 with a known bound on their
 // error, and what is closer than that is settled by exact values: of the few experts concerned, of a group's largest, or (a logit of
-// infinity, biases of very different size, long runs of equals) of all.  What is chosen does not depend on which way that goes.
+// infinity or a NaN, biases of very different size, long runs of equals) of all.  What is chosen does not depend on which way that goes.
 //
 // Bytes: the logits once, the weights and indices; backward the gradients' bytes, for a softmax the logits too.  Forward is bound by the
 // integer pipe (minima and comparisons run at half the rate of additions): about 180 instructions per token of 128 experts and 8
@@ -264,19 +264,24 @@ __device__ __noinline__ void route_again(const RouteP& p, int tok0, double* c, i
     const bool have = tok < p.n;
     const T* const row = (const T*)p.logits + (size_t)tok * p.E;
     double* const mine = c + mt * p.E;
-    float top = -INFINITY;
+    float top = -INFINITY;                      // of the numbers
+    bool bad = false;
     uint32_t taken = 0;                         // bits of the lane's experts i * L + sub
 #pragma unroll 4
-    for (int e = sub; e < p.E; e += L) top = max_nan(top, have ? as_float(row[e]) : -INFINITY);
-    top = lanes_max_nan<L>(top);
-    const bool bad = top != top || (p.softmax && top == INFINITY);
+    for (int e = sub; e < p.E; e += L) {
+        const float z = have ? as_float(row[e]) : -INFINITY;
+        bad |= z != z;
+        top = fmaxf(top, z);
+    }
+    top = lanes_max<L>(top);
+    bad = (__ballot_sync(FULL, bad) & lanes_of<L>(mt)) || (p.softmax && top == INFINITY);
     double inv = 1.0;
     if (p.softmax) {
         double sum = 0.0;
 #pragma unroll 2
         for (int e = sub; e < p.E; e += L) {
             const float z = have ? as_float(row[e]) : -INFINITY;
-            const double s = z > -INFINITY ? exp((double)z - (double)top) : 0.0;
+            const double s = z == top && z > -INFINITY ? 1.0 : z > -INFINITY ? exp((double)z - (double)top) : 0.0;      // (+inf less itself is no number)
             mine[e] = s;
             sum += s;
         }
@@ -460,8 +465,14 @@ __global__ void __launch_bounds__(32 * WARPS, P > 8 ? 5 : 8) route_kernel(const 
 #pragma unroll
             for (int i = 1; i < P; ++i) top = max_nan(top, z[i]);
             // a NaN (softmax: or infinity) among the logits
-            const bool bad = __ballot_sync(FULL, top != top || (p.softmax && top == INFINITY)) & lanes_of<L>(mt);
-            bool unsure = HOW != BY_LOGIT && top == INFINITY;
+            const unsigned none = __ballot_sync(FULL, top != top || (p.softmax && top == INFINITY));
+            if (HOW == BY_LOGIT && __builtin_expect(none, 0)) {      // (32768 x 256 in groups: 38 us in place of 34.7)
+                again |= 1u << round;
+                load(tok + stride);
+                continue;
+            }
+            const bool bad = HOW != BY_LOGIT && none & lanes_of<L>(mt);
+            bool unsure = bad || (HOW != BY_LOGIT && top == INFINITY);
             if (!by_score || p.softmax) top = lanes_max_nan<L>(top);
             float inv = 1.0f;                   // (what the weights are divided by has exp(0) in it, where they are all there is)
             uint32_t key[P];
@@ -512,12 +523,8 @@ __global__ void __launch_bounds__(32 * WARPS, P > 8 ? 5 : 8) route_kernel(const 
                         }
                         bool stays = may < p.top_groups;
                         const bool open = e0 < p.E && !stays && are < p.top_groups;
-                        if (__builtin_expect(__any_sync(FULL, open && have && !bad && margin < 1e-3f), 0)) {
-                            stays = settle_group<T, L, P>(p, tok, have, top, least - margin, open && !bad, stays);
-                            unsure |= open && bad;
-                        } else {
-                            unsure |= open;
-                        }
+                        if (__builtin_expect(__any_sync(FULL, open && have && !bad && margin < 1e-3f), 0)) stays = settle_group<T, L, P>(p, tok, have, top, least - margin, open && !bad, stays);
+                        else unsure |= open;
                         aside = !stays;
                     } else {
                         float* const cs = (float*)scratch;
@@ -586,12 +593,12 @@ __global__ void __launch_bounds__(32 * WARPS, P > 8 ? 5 : 8) route_kernel(const 
             uint32_t next;                      // the first that was not chosen
             if (beyond(last, &next) < apart && next != NONE && next > last) close |= bit;
             __syncwarp();
-            if (__builtin_expect(__any_sync(FULL, close && !bad), 0)) {
+            if (__builtin_expect(__any_sync(FULL, close && !unsure), 0)) {
                 double* const value = scratch + mt * (KM + EXTRA);
                 int32_t* const behind = (int32_t*)(scratch + TOKENS * (KM + EXTRA)) + mt * EXTRA;
                 int32_t* const sorted = (int32_t*)(scratch + TOKENS * (KM + EXTRA + EXTRA / 2)) + mt * KM;
                 const T* const row = (const T*)p.logits + (size_t)tok * p.E;
-                int count = close && have && !bad && !unsure ? p.k : 0;
+                int count = close && have && !unsure ? p.k : 0;
                 bool more = count && close & bit;
                 while (__any_sync(FULL, more)) {
                     if (more) {
@@ -639,7 +646,7 @@ __global__ void __launch_bounds__(32 * WARPS, P > 8 ? 5 : 8) route_kernel(const 
                 __syncwarp();
             }
             if (__any_sync(FULL, unsure && have)) again |= 1u << round;
-            else weigh<T, L>(p, tok0, chosen, (float*)scratch, sht[warp], hist, top, inv, bad);
+            else weigh<T, L>(p, tok0, chosen, (float*)scratch, sht[warp], hist, top, inv, false);
         }
         for (; again; again &= again - 1) route_again<T, L>(p, begin + (__ffs(again) - 1) * stride, scratch, chosen, sht[warp], hist);
     }

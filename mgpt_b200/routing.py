@@ -62,7 +62,8 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: tor
     over the sum of the chosen s (plus 1e-20).  The choice is that of exact arithmetic on the logits given.
 
     An expert whose logit or bias is -inf or NaN is out: it is chosen only where fewer than ``top_k`` others are left, by index and with
-    weight 0.  A NaN among a token's logits (softmax: or +inf) makes its weights NaN.  The indices of a token always differ and
+    weight 0.  A NaN among a token's logits (softmax: or +inf) makes its weights NaN; its experts are chosen as ever (softmax: m logits
+    of +inf have the scores 1/m, the others 0).  The indices of a token always differ and
     always lie in ``[0, E)``.  ``counts``: int32 ``[E]``, added to: the tokens that chose each expert, which is what a bias is
     adjusted by (``bias += rate * sign(counts.mean() - counts)``)."""
     lib = _lib.load()
