@@ -586,6 +586,7 @@ static int forward_impl(mgpt_moe_layer* L, const void* x, void* y, int n_tokens,
     L->last_io = io;
     L->last_ws = workspace;
     L->last_stream = st;
+    L->plan_outdated = false;
     L->fwd_done = !inference;        // nothing was kept: backward cannot follow an inference forward
     L->last_inference = inference;
     return 0;

@@ -250,6 +250,7 @@ struct mgpt_moe_layer {
     // mgpt_moe_set_routing: how experts are chosen, where it is not by clamped softmax and top-k
     bool routed = false;
     mgpt_moe_routing routing = {};
+    bool plan_outdated = false;              // it was called after the last mgpt_moe_route_plan or forward
 
     // optional per-stage timing
     bool profiling = false;

@@ -1029,6 +1029,7 @@ int mgpt_moe_set_routing(mgpt_moe_layer* L, const mgpt_moe_routing* r)
     L->routed = r != nullptr;
     if (r) L->routing = *r;
     L->fwd_done = false;        // a backward would take the other routing's gradient
+    L->plan_outdated = true;
     return 0;
 }
 

@@ -85,6 +85,7 @@ int mgpt_moe_route_plan(mgpt_moe_layer* L, const void* x, int n_tokens, int io, 
     L->last_io = io;
     L->last_ws = workspace;
     L->last_stream = st;
+    L->plan_outdated = false;
     return 0;
 }
 
@@ -94,6 +95,7 @@ int mgpt_moe_route_rows(mgpt_moe_layer* L, const void* x, int io, void* workspac
 {
     MGPT_TRY(check_route_layer(L, io));
     if (workspace != L->last_ws || io != L->last_io) return fail(MGPT_MOE_ESTATE, "route_rows follows route_plan on the same workspace");
+    if (L->plan_outdated) return fail(MGPT_MOE_ESTATE, "route_rows: the routing was set after route_plan");
     const int n_tokens = L->last_n;
     if (n_tokens > 0 && (!x || !send_rows)) return fail(MGPT_MOE_EINVAL, "bad token buffer");
     if (n_tokens > 0) MGPT_TRY(check_aligned(send_rows, "send_rows"));

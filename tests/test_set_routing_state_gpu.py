@@ -1,0 +1,47 @@
+"""mgpt_moe_set_routing between two calls that belong together: what was computed under the other setting is refused, or stays what it was."""
+import pytest
+import torch
+
+from mgpt_b200 import MoELayer, MoeError, _lib
+
+pytestmark = pytest.mark.gpu
+
+
+def _layer(C=64, H=64, E=8, k=2, mode="bf16", seed=0):
+    g = torch.Generator().manual_seed(seed)
+    layer = MoELayer(C, H, E, k, mode=mode)
+    layer.load_parameters([(torch.randn(p.shape, generator=g) * (p.shape[0] ** -0.5 if p.shape[0] > 1 else 0.1)).numpy() for p in layer.get_parameters()])
+    return layer
+
+
+def _x(n, C, seed=1):
+    return torch.randn(n, C, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)).bfloat16()
+
+
+@pytest.mark.parametrize("first,then", [((), ("sigmoid",)), (("sigmoid",), ()), (("sigmoid",), ("softmax",))])
+def test_stage_calls_do_not_mix_settings(first, then):
+    layer, x = _layer(), _x(100, 64)
+    lib, h, stream = layer.lib, layer._h, layer._stream()
+    ws = torch.empty(int(lib.mgpt_moe_stage_workspace_bytes(h, 100, 1)), dtype=torch.uint8, device="cuda")
+    rows = torch.zeros(100 * 2 + 8 * 128, 64, dtype=torch.bfloat16, device="cuda")
+
+    def plan():
+        _lib.check(lib.mgpt_moe_route_plan(h, x.data_ptr(), 100, _lib.IO_BF16, ws.data_ptr(), ws.numel(), stream))
+
+    def call(f, *args):
+        _lib.check(f(h, *args, ws.data_ptr(), ws.numel(), stream))
+
+    layer.set_routing(*first)
+    plan()
+    layer.set_routing(*then)
+    with pytest.raises(MoeError, match="set after route_plan"):
+        _lib.check(lib.mgpt_moe_route_rows(h, x.data_ptr(), _lib.IO_BF16, ws.data_ptr(), ws.numel(), rows.data_ptr(), stream))
+    with pytest.raises(MoeError):
+        call(lib.mgpt_moe_route_backward, x.data_ptr(), rows.data_ptr(), torch.empty_like(x).data_ptr(), _lib.IO_BF16)
+    plan()
+    _lib.check(lib.mgpt_moe_route_rows(h, x.data_ptr(), _lib.IO_BF16, ws.data_ptr(), ws.numel(), rows.data_ptr(), stream))
+    y = torch.empty_like(x)
+    call(lib.mgpt_moe_combine, rows.data_ptr(), y.data_ptr(), _lib.IO_BF16)
+    layer.set_routing(*first)
+    with pytest.raises(MoeError):
+        call(lib.mgpt_moe_combine_backward, rows.data_ptr(), x.data_ptr(), _lib.IO_BF16, rows.data_ptr())
