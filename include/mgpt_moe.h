@@ -210,7 +210,7 @@ int  mgpt_moe_block_backward(mgpt_moe_layer* layer, const void* x1, const float*
  * before that block's backward, the arena rewound in between). The same tokens route
  * the same way, so the second run can skip router and plan: after the first forward
  * save_routing copies the routing results and the plan (routing_bytes(n_tokens) bytes:
- * probabilities, top-k, counts, offsets, tile list, row permutation) into memory the
+ * probabilities -- under mgpt_moe_set_routing logits --, top-k, counts, offsets, tile list, row permutation) into memory the
  * caller keeps outside the arena; forward_with_routing takes them back instead of
  * recomputing them and then runs dispatch, the expert products and combine as
  * mgpt_moe_forward does. Backward follows it as usual. The caller guarantees that x,

@@ -387,7 +387,7 @@ int mgpt_moe_workspace_view(const mgpt_moe_layer* L, int n_tokens, const char* n
     const Dims& d = L->d;
     const size_t N = n_tokens, E = d.E, k = d.k, C = d.C, H = d.H, rc = w.row_cap, ab = w.act_bytes;
     struct { const char* n; size_t o, b; } tab[] = {
-        {"logits", L->routed ? w.probs : w.logits, N * E * 4}, {"probs", L->routed ? w.logits : w.probs, N * E * 4}, {"top_idx", w.top_idx, N * k * 4},
+        {"logits", w.logits, N * E * 4}, {"probs", w.probs, N * E * 4}, {"top_idx", w.top_idx, N * k * 4},
         {"top_p", w.top_p, N * k * 4}, {"counts", w.counts, E * 4}, {"offsets", w.offsets, E * 4},
         {"padded_offsets", w.padded_offsets, (E + 1) * 4}, {"tile_expert", w.tile_expert, (size_t)w.max_tiles * 4},
         {"n_tiles", w.n_tiles, 4}, {"status", w.status, 4}, {"map", w.map, N * k * 4}, {"pos", w.pos, N * k * 4},
@@ -467,9 +467,16 @@ int mgpt_moe_selftest_bounded_wait(mgpt_moe_layer* L, mgpt_stream_t stream)
 
 // Routing results and plan of one forward: the workspace bytes from probs up to (not including) the plan's
 // scratch -- probs, top_idx, top_p, counts, offsets, padded_offsets, tile_expert, n_tiles, status, map, pos, row_src,
-// groups, n_groups.
+// groups, n_groups.  Under mgpt_moe_set_routing backward needs the logits and not the probabilities, which they take the place of.
 static size_t routing_begin(const Workspace& w) { return w.probs; }
 static size_t routing_end(const Workspace& w) { return w.blk_cnt; }
+static int copy_routing(const mgpt_moe_layer* L, const Workspace& w, char* ws, char* state, bool save, cudaStream_t st)
+{
+    const size_t first = w.top_idx - w.probs;       // (as many bytes of logits)
+    char *const a = ws + (L->routed ? w.logits : w.probs), *const b = ws + w.top_idx;
+    return save ? copy_on_device(state, a, first, state + first, b, routing_end(w) - w.top_idx, st)
+                : copy_on_device(a, state, first, b, state + first, routing_end(w) - w.top_idx, st);
+}
 
 size_t mgpt_moe_routing_bytes(const mgpt_moe_layer* L, int n_tokens)
 {
@@ -484,7 +491,7 @@ int mgpt_moe_save_routing(mgpt_moe_layer* L, void* dst, mgpt_stream_t stream)
     if (!L->fwd_done) return fail(MGPT_MOE_ESTATE, "save_routing without a forward");
     const Workspace w = make_workspace(L->d, L->last_n);
     MGPT_CUDA(cudaSetDevice(L->device));
-    return copy_on_device(dst, (const char*)L->last_ws + routing_begin(w), routing_end(w) - routing_begin(w), (cudaStream_t)stream);
+    return copy_routing(L, w, (char*)L->last_ws, (char*)dst, true, (cudaStream_t)stream);
 }
 
 static int forward_impl(mgpt_moe_layer* L, const void* x, void* y, int n_tokens, int io, void* workspace,
@@ -543,9 +550,9 @@ static int forward_impl(mgpt_moe_layer* L, const void* x, void* y, int n_tokens,
     for (int s = 0; s < ST_COUNT; ++s) L->ev_used[s] = false;
     if (routing) {
         // recompute of a forward whose routing was saved: the same tokens route the same way, so router and plan
-        // are replaced by one copy (the logits are not part of the saved state and stay undefined)
+        // are replaced by one copy (of logits and probabilities what is not part of the saved state stays undefined)
         L->stage_begin(ST_PLAN, st);
-        MGPT_TRY(copy_on_device(ws + routing_begin(w), routing, routing_end(w) - routing_begin(w), st));
+        MGPT_TRY(copy_routing(L, w, ws, (char*)const_cast<void*>(routing), false, st));
         L->stage_end(ST_PLAN, st);
     } else {
         bool planned = false;

@@ -969,24 +969,20 @@ int check_routing(const mgpt_moe_routing* r, int E, int k)
     return fill(p, r, 0, E, k);
 }
 
-// The router's product, then this routing over its own.  (The logits lie where the probabilities do without one: what
-// a saved routing holds has to be enough for backward.)
+// The router's product, then this routing over its own.
 int launch_routed(mgpt_moe_layer* L, const Workspace& w, char* ws, const void* x, int io, cudaStream_t st)
 {
     const Dims& d = L->d;
-    Workspace r = w;
-    r.logits = w.probs;
-    r.probs = w.logits;
     int32_t* const idx = (int32_t*)(ws + w.top_idx);
     float* const weights = (float*)(ws + w.top_p);
     if (tc_router_usable(L, x, io, w.n_tokens))
-        MGPT_TRY(tc_router_fwd(L, r, ws, x, st));
+        MGPT_TRY(tc_router_fwd(L, w, ws, x, st));
     else
-        MGPT_TRY(launch_router_fwd(x, io, L->p_data[0], L->p_data[1], w.n_tokens, d.C, d.E, d.k, (float*)(ws + r.logits), (float*)(ws + r.probs),
+        MGPT_TRY(launch_router_fwd(x, io, L->p_data[0], L->p_data[1], w.n_tokens, d.C, d.E, d.k, (float*)(ws + w.logits), (float*)(ws + w.probs),
                                    idx, weights, st, nullptr, nullptr, L->d_status));
     RouteP p = {};
     MGPT_TRY(fill(p, &L->routing, w.n_tokens, d.E, d.k));
-    p.logits = ws + r.logits; p.idx = idx; p.w = weights;
+    p.logits = ws + w.logits; p.idx = idx; p.w = weights;
     return run_fwd<float>(p, st);
 }
 
@@ -996,7 +992,7 @@ int launch_routed_bwd(mgpt_moe_layer* L, const Workspace& w, char* ws, bf16* dl1
     const Dims& d = L->d;
     RouteP p = {};
     MGPT_TRY(fill(p, &L->routing, w.n_tokens, d.E, d.k));
-    p.logits = ws + w.probs;
+    p.logits = ws + w.logits;
     p.top = (const int32_t*)(ws + w.top_idx);
     p.dw = (const float*)(ws + w.d_top_p);
     p.dz = ws + w.dlogits;

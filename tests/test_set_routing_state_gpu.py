@@ -45,3 +45,47 @@ def test_stage_calls_do_not_mix_settings(first, then):
     layer.set_routing(*first)
     with pytest.raises(MoeError):
         call(lib.mgpt_moe_combine_backward, rows.data_ptr(), x.data_ptr(), _lib.IO_BF16, rows.data_ptr())
+
+
+@pytest.mark.parametrize("mode", ["fp32", "bf16"])
+def test_views_are_of_the_forward_that_filled_them(mode):
+    layer, x = _layer(mode=mode), _x(100, 64)
+    x = x.float() if mode == "fp32" else x
+
+    def views():
+        return [layer.workspace_view(name, torch.float32, (100, 8)).clone() for name in ("logits", "probs")]
+
+    layer.forward(x)
+    logits, probs = views()
+    want = x.double() @ layer.get_parameters()[0].double() + layer.get_parameters()[1].double()
+    assert (logits - want).abs().max() < 1e-4 and (probs - torch.softmax(want, 1)).abs().max() < 1e-4
+    layer.set_routing("sigmoid")
+    assert torch.equal(views()[0], logits) and torch.equal(views()[1], probs)
+    layer.forward(x)                                                    # the router's product and its own softmax are the same
+    assert torch.equal(views()[0], logits) and torch.equal(views()[1], probs)
+    saved = layer.save_routing()
+    layer._ws.zero_()
+    layer.recompute_into(x, torch.empty_like(x), saved)                 # brings the logits back, which backward reads
+    assert torch.equal(views()[0], logits)
+    layer.set_routing()
+    assert torch.equal(views()[0], logits)
+
+
+def test_saved_routing_in_memory_of_any_alignment():
+    layer, x = _layer(), _x(100, 64)
+    lib, h, stream = layer.lib, layer._h, layer._stream()
+    size = int(lib.mgpt_moe_routing_bytes(h, 100))
+    for how in ((), ("sigmoid",)):
+        layer.set_routing(*how)
+        y = layer.forward(x).clone()
+        dx = layer.backward(x).clone()
+        for at in (0, 4, 1):
+            buffer = torch.zeros(size + 16, dtype=torch.uint8, device="cuda")
+            layer.forward(x)
+            _lib.check(lib.mgpt_moe_save_routing(h, buffer.data_ptr() + at, stream))
+            layer._ws.zero_()
+            again = torch.empty_like(x)
+            _lib.check(lib.mgpt_moe_forward_with_routing(h, x.data_ptr(), again.data_ptr(), 100, _lib.IO_BF16, layer._ws.data_ptr(), layer._ws.numel(),
+                                                         buffer.data_ptr() + at, stream))
+            assert torch.equal(again, y) and torch.equal(layer.backward(x), dx)
+            layer.check_status()
