@@ -544,7 +544,7 @@ static int forward_impl(mgpt_moe_layer* L, const void* x, void* y, int n_tokens,
     cudaStream_t st = (cudaStream_t)stream;
     char* ws = (char*)workspace;
     const Dims& d = L->d;
-    L->fwd_done = false;
+    L->fwd_done = L->counts_left = false;
     L->ext_Xg = L->ext_Yg = L->ext_dYg = L->ext_dXg = nullptr;      // whole-layer calls keep every buffer in the workspace
     L->n_seg = 0;
     for (int s = 0; s < ST_COUNT; ++s) L->ev_used[s] = false;
@@ -640,7 +640,7 @@ int mgpt_moe_backward(mgpt_moe_layer* L, const void* x, const void* dy, void* dx
 int mgpt_moe_expert_counts(mgpt_moe_layer* L, int32_t* host_counts)
 {
     if (!L || !host_counts) return fail(MGPT_MOE_EINVAL, "null argument");
-    if (!L->fwd_done && !L->last_inference) return fail(MGPT_MOE_ESTATE, "no forward has run");
+    if (!L->fwd_done && !L->last_inference && !L->counts_left) return fail(MGPT_MOE_ESTATE, "no forward has run");
     MGPT_CUDA(cudaSetDevice(L->device));
     const Workspace w = make_workspace(L->d, L->last_n, L->last_inference ? 3 : 0);
     MGPT_CUDA(cudaMemcpyAsync(host_counts, (char*)L->last_ws + w.counts, (size_t)L->d.E * sizeof(int32_t),

@@ -251,6 +251,7 @@ struct mgpt_moe_layer {
     bool routed = false;
     mgpt_moe_routing routing = {};
     bool plan_outdated = false;              // it was called after the last mgpt_moe_route_plan or forward
+    bool counts_left = false;                // and after a forward, whose counts stay readable
 
     // optional per-stage timing
     bool profiling = false;

@@ -1024,6 +1024,7 @@ int mgpt_moe_set_routing(mgpt_moe_layer* L, const mgpt_moe_routing* r)
     if (r) MGPT_TRY(check_routing(r, L->d.E, L->d.k));
     L->routed = r != nullptr;
     if (r) L->routing = *r;
+    L->counts_left |= L->fwd_done;
     L->fwd_done = false;        // a backward would take the other routing's gradient
     L->plan_outdated = true;
     return 0;

@@ -70,7 +70,7 @@ int mgpt_moe_route_plan(mgpt_moe_layer* L, const void* x, int n_tokens, int io, 
     cudaStream_t st = (cudaStream_t)stream;
     char* ws = (char*)workspace;
     const Dims& d = L->d;
-    L->fwd_done = false;
+    L->fwd_done = L->counts_left = false;
     if (n_tokens > 0) {
         if (L->routed)
             MGPT_TRY(launch_routed(L, w, ws, x, io, st));
@@ -183,7 +183,7 @@ int mgpt_moe_experts_forward(mgpt_moe_layer* L, const void* rows, const int32_t*
     cudaStream_t st = (cudaStream_t)stream;
     char* ws = (char*)workspace;
     const Dims& d = L->d;
-    L->fwd_done = false;
+    L->fwd_done = L->counts_left = false;
     for (int s = 0; s < ST_COUNT; ++s) L->ev_used[s] = false;
     L->ext_Xg = const_cast<void*>(rows);
     L->ext_Yg = out_rows;

@@ -89,3 +89,20 @@ def test_saved_routing_in_memory_of_any_alignment():
                                                          buffer.data_ptr() + at, stream))
             assert torch.equal(again, y) and torch.equal(layer.backward(x), dx)
             layer.check_status()
+
+
+def test_counts_of_the_last_forward_stay_readable():
+    layer, x = _layer(), _x(100, 64)
+    layer.set_routing("sigmoid")
+    with pytest.raises(MoeError):                                       # there has been none
+        layer.get_expert_counts()
+    layer.forward(x)
+    counts = layer.get_expert_counts()
+    assert sum(counts) == 200
+    for how in (("softmax",), (), ("sigmoid",)):
+        layer.set_routing(*how)
+        assert layer.get_expert_counts() == counts
+    layer.forward_inference(x[:50].contiguous())
+    counts = layer.get_expert_counts()
+    layer.set_routing()
+    assert sum(counts) == 100 and layer.get_expert_counts() == counts
