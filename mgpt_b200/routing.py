@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as ct
 import functools
+from operator import index
 
 import torch
 
@@ -17,16 +18,22 @@ from .training import _DTYPES, _EITHER, _F32, _I32, _INT_MAX, _check, _device, _
 
 
 @functools.lru_cache(maxsize=64)
-def _numbers(score, groups, top_groups, group_top, renormalise, scale):
-    """The argument's bytes without the bias (a copy is quicker made than a new one filled)."""
+def _numbers(score, groups, top_groups, group_top, renormalise):
+    """The argument's bytes without scale and bias (a copy is quicker made than a new one filled), from plain numbers."""
     _need(score in _lib.SCORES, f"routing: score is 'softmax' or 'sigmoid', got {score!r}")
-    numbers = (groups, groups if top_groups is None else top_groups, group_top)
+    numbers = (groups, top_groups, group_top)
     _need(all(-_INT_MAX <= v <= _INT_MAX for v in numbers), "routing: sizes out of range")
-    return bytes(_lib.Routing(_lib.SCORES[score], *numbers, int(bool(renormalise)), scale, None))
+    return bytes(_lib.Routing(_lib.SCORES[score], *numbers, int(renormalise), 0.0, None))
 
 
 def _routing(E, score, bias, groups, top_groups, group_top, renormalise, scale, device):
-    r = _lib.Routing.from_buffer_copy(_numbers(score, groups, top_groups, group_top, renormalise, scale))
+    try:                        # (the cache must not see what can change, such as a tensor of one number)
+        groups, group_top, scale, renormalise = index(groups), index(group_top), float(scale), bool(renormalise)
+        top_groups = groups if top_groups is None else index(top_groups)
+    except (TypeError, ValueError, OverflowError, RuntimeError) as e:
+        raise MoeError(f"routing: {e}") from None
+    r = _lib.Routing.from_buffer_copy(_numbers(str(score), groups, top_groups, group_top, renormalise))
+    r.scale = scale
     if bias is not None:
         r.bias = _check(bias, "bias", (E,), _F32, device)
     return r
@@ -68,6 +75,10 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: tor
     adjusted by (``bias += rate * sign(counts.mean() - counts)``)."""
     lib = _lib.load()
     device, n, E, lp = _logits(logits)
+    try:
+        top_k = index(top_k)
+    except TypeError as e:
+        raise MoeError(f"routing: top_k: {e}") from None
     _need(0 < top_k <= E, "routing: top_k is 1 to the number of experts")
     r = _routing(E, score, bias, groups, top_groups, group_top, renormalise, scale, device)
     cp = None if counts is None else _check(counts, "counts", (E,), _I32, device)
