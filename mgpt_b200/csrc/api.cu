@@ -430,6 +430,7 @@ static std::string describe_status(int32_t bits)
     if (bits & ST_ACC_WAIT) m += " an accumulator wait ran out;";
     if (bits & ST_SCHED_WAIT) m += " the work-item queue stalled (bounded wait ran out);";
     if (bits & ST_BAD_EXPERT) m += " an expert id outside [0, num_experts) was skipped;";
+    if (bits & ST_OTHER_ROUTING) m += " a saved routing was taken under another setting (set_routing) than it was saved under;";
     m += " outputs and gradients of the affected step are incomplete";
     return m;
 }
@@ -474,8 +475,10 @@ static int copy_routing(const mgpt_moe_layer* L, const Workspace& w, char* ws, c
 {
     const size_t first = w.top_idx - w.probs;       // (as many bytes of logits)
     char *const a = ws + (L->routed ? w.logits : w.probs), *const b = ws + w.top_idx;
-    return save ? copy_on_device(state, a, first, state + first, b, routing_end(w) - w.top_idx, st)
-                : copy_on_device(a, state, first, b, state + first, routing_end(w) - w.top_idx, st);
+    // (behind the status word, in what fills its buffer up)
+    const CopyTag tag = {w.status - w.top_idx, routing_tag(L), save ? nullptr : L->d_status, ST_OTHER_ROUTING};
+    return save ? copy_on_device(state, a, first, state + first, b, routing_end(w) - w.top_idx, tag, st)
+                : copy_on_device(a, state, first, b, state + first, routing_end(w) - w.top_idx, tag, st);
 }
 
 size_t mgpt_moe_routing_bytes(const mgpt_moe_layer* L, int n_tokens)

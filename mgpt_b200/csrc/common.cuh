@@ -30,6 +30,7 @@ enum StatusBits {
     ST_ACC_WAIT = 8,          //   ... an accumulator was never completed / released
     ST_SCHED_WAIT = 16,       //   ... the work-item queue stalled
     ST_BAD_EXPERT = 32,       // an expert id outside [0, E) was met by the dispatch plan and skipped
+    ST_OTHER_ROUTING = 64,    // a saved routing was taken under another mgpt_moe_set_routing than it was saved under
 };
 
 enum Stage {
@@ -294,12 +295,20 @@ int launch_router_bwd(mgpt_moe_layer* L, const Workspace& w, char* ws, const voi
                       void* dx, cudaStream_t st, const void* dXg_rows = nullptr, const int32_t* pos_rows = nullptr);
 
 // route.cu
+uint32_t routing_tag(const mgpt_moe_layer* L);
 int launch_routed(mgpt_moe_layer* L, const Workspace& w, char* ws, const void* x, int io, cudaStream_t st);
 int launch_routed_bwd(mgpt_moe_layer* L, const Workspace& w, char* ws, bf16* dl16, int E8, float* d_bias, cudaStream_t st);
 
 // plan.cu
 struct PlanArgs plan_args(const Dims& d, const Workspace& w, char* ws, int32_t* sticky);      // plan_block.cuh
-int copy_on_device(void* dst, const void* src, size_t bytes, void* dst2, const void* src2, size_t bytes2, cudaStream_t st);
+// A word that a copy leaves beside the data (save), or finds there: bit `bits` of *status where it is another one.
+struct CopyTag {
+    size_t at;          // its place in the second run, bytes; a second word of 16
+    uint32_t value;
+    int32_t* status;    // null: save
+    int bits;
+};
+int copy_on_device(void* dst, const void* src, size_t bytes, void* dst2, const void* src2, size_t bytes2, const CopyTag& tag, cudaStream_t st);
 int launch_plan(const Dims& d, const Workspace& w, char* ws, cudaStream_t st, int32_t* sticky);
 int launch_dispatch(const Dims& d, const Workspace& w, char* ws, const void* x, int io, bool zero_pad, cudaStream_t st);
 int launch_combine_fwd(const Dims& d, const Workspace& w, char* ws, void* y, int io, cudaStream_t st,

@@ -25,6 +25,8 @@
 // six to eight blocks per SM (37 to 41 against 36).
 #include "common.cuh"
 
+#include <cstring>
+
 namespace mgpt {
 
 namespace {
@@ -967,6 +969,18 @@ int check_routing(const mgpt_moe_routing* r, int E, int k)
 {
     RouteP p = {};
     return fill(p, r, 0, E, k);
+}
+
+// What tells settings apart: 0 for the reference's, else a hash of all but the bias's address.
+uint32_t routing_tag(const mgpt_moe_layer* L)
+{
+    if (!L->routed) return 0;
+    const mgpt_moe_routing& r = L->routing;
+    uint32_t bits, h = 2166136261u;             // FNV-1a
+    memcpy(&bits, &r.scale, 4);
+    for (uint32_t v : {(uint32_t)r.score, (uint32_t)r.groups, (uint32_t)r.top_groups, (uint32_t)r.group_top, (uint32_t)(r.renormalise != 0), bits, (uint32_t)(r.bias != nullptr)})
+        for (int i = 0; i < 32; i += 8) h = (h ^ (v >> i & 255)) * 16777619u;
+    return h ? h : 1;
 }
 
 // The router's product, then this routing over its own.

@@ -106,3 +106,32 @@ def test_counts_of_the_last_forward_stay_readable():
     counts = layer.get_expert_counts()
     layer.set_routing()
     assert sum(counts) == 100 and layer.get_expert_counts() == counts
+
+
+@pytest.mark.parametrize("at", [0, 4])
+def test_a_saved_routing_of_another_setting_is_reported(at):
+    layer, x = _layer(), _x(100, 64)
+    lib, h, stream = layer.lib, layer._h, layer._stream()
+    size = int(lib.mgpt_moe_routing_bytes(h, 100))
+    bias = torch.zeros(8, device="cuda")
+    settings = [{}, dict(score="sigmoid"), dict(score="softmax"), dict(score="sigmoid", renormalise=True), dict(score="sigmoid", scale=2.0), dict(score="sigmoid", bias=bias),
+                dict(score="sigmoid", groups=4, top_groups=2), dict(score="sigmoid", groups=4, top_groups=2, group_top=1)]
+    saved = []
+    for how in settings:
+        layer.set_routing(**how)
+        layer.forward(x)
+        saved.append(torch.zeros(size + 16, dtype=torch.uint8, device="cuda"))
+        _lib.check(lib.mgpt_moe_save_routing(h, saved[-1].data_ptr() + at, stream))
+    y = torch.empty_like(x)
+    for i, how in enumerate(settings):
+        layer.set_routing(**how)
+        for j, state in enumerate(saved):
+            _lib.check(lib.mgpt_moe_forward_with_routing(h, x.data_ptr(), y.data_ptr(), 100, _lib.IO_BF16, layer._ws.data_ptr(), layer._ws.numel(), state.data_ptr() + at, stream))
+            if i == j:
+                layer.check_status()
+            else:
+                with pytest.raises(MoeError, match="saved routing"):
+                    layer.check_status()
+    layer.set_routing("sigmoid", bias=bias.clone())                     # another tensor, the same setting
+    layer.recompute_into(x, y, saved[5][at:at + size] if at % 16 else saved[5][:size])
+    layer.check_status()
