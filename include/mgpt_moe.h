@@ -284,9 +284,11 @@ int  mgpt_moe_set_sm_budget(mgpt_moe_layer* layer, int n_sms);
  * Every forward and backward of the layer and the routing-side stage calls follow it: the logits are the layer's own router's
  * (x Wr + br), the gradient goes through the weights to Wr, br and x, and there is no load-balance term (lb_alpha): the
  * bias balances. `bias` stays the caller's and is read on the device by every call. A saved routing belongs to the setting it was
- * saved under (under another one mgpt_moe_check_status reports it), and neither backward nor mgpt_moe_route_rows can follow a forward or mgpt_moe_route_plan of before the call. With a routing set, the workspace view "probs" has what
- * the router left there (its clamped softmax), top_p the weights. Logits of calls beyond n_tokens * embed_dim * num_experts = 4e8 agree with
- * exact ones to a few 1e-6 (tensor cores), and experts are chosen from them. */
+ * saved under (under another one mgpt_moe_check_status reports it), and neither backward nor mgpt_moe_route_rows can follow a
+ * forward or mgpt_moe_route_plan of before the call. With a routing set, the workspace view "probs" has what the router left there
+ * (its clamped softmax), top_p the weights. Experts are chosen from the logits that the router computes. In calls with BF16 tokens beyond
+ * n_tokens * embed_dim * num_experts = 4e8 those come from the tensor cores and from Wr in two BF16 pieces: off by
+ * (1.5 * embed_dim * 2^-24 + 2^-16) * |x| * max |Wr[:,e]| (lengths of a token and of a column) at most, in the mean far less. */
 #define MGPT_MOE_SCORE_SOFTMAX 0
 #define MGPT_MOE_SCORE_SIGMOID 1
 typedef struct {
