@@ -562,9 +562,10 @@ int  mgpt_moe_op_residual_norm_backward(const void* x, const void* h, int io, co
 
 /* Activations kept for a backward pass in 8 bits: values int8 [n, C], exponents uint8 [n, ceil(C/32)], a byte b for 32 consecutive
  * channels of a row (the last of a row may be fewer), whose values are in units of 2^(b-127): the least power of two, 2^-126 at
- * least, in which the largest of them rounds to 127 or less. Rounding is to nearest, ties to even: off by half a unit at most, 1/127
- * of the group's largest value (b is 248 at most: values from 3.39e38 on are kept as 127 units). b = 255: a value was NaN or infinite, and all of the group come back as NaN. x: [n, C] of `io`, C a
- * multiple of 8, 16-byte aligned; values 8-byte aligned. restore8 gives values * 2^(b-127), exact in either type. */
+ * least, in which the largest of them rounds to 127 or less. Rounding is to nearest, ties to even: off by half a unit at most, which is
+ * 1/127 of the group's largest value where that is 2^-120 or more (in groups of smaller ones the unit stays 2^-126; b is 248 at most: values
+ * from 3.39e38 on are kept as 127 units, up to a whole one off). b = 255: a value was NaN or infinite, and all of the group come back
+ * as NaN. x: [n, C] of `io`, C a multiple of 8, 16-byte aligned; values 8-byte aligned. restore8 gives values * 2^(b-127), exact in either type. */
 int  mgpt_moe_op_keep8(const void* x, int io, int n, int C, int8_t* values, uint8_t* exponents, mgpt_stream_t stream);
 int  mgpt_moe_op_restore8(const int8_t* values, const uint8_t* exponents, int n, int C, void* x, int io, mgpt_stream_t stream);
 

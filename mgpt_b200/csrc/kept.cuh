@@ -1,8 +1,9 @@
 // Activations kept in 8 bits: 32 channels of a row (the last of a row may be fewer) in units of a power of two 2^e, the least with
 // -126 <= e <= 121 in which the largest rounds to at most 127; the byte e + 127 beside them, 255 where a value is not finite (they come back as NaN).
-// x / 2^e is exact, so that rounding to the nearest whole number (ties to even) is the only one: half a unit at most, 1/127
-// of the group's largest.  (From 127.5 * 2^121 = 3.39e38 on, 128 * 2^121 being no number: 127 units.)  A value of 7 bits and a sign
-// times a power of two is exact in BF16.
+// x / 2^e is exact, so that rounding to the nearest whole number (ties to even) is the only one: half a unit at most, which is 1/127
+// of the group's largest where that is 2^-120 or more; below, the unit stays 2^-126 (2^-127 and less comes back as 0).  (From
+// 127.5 * 2^121 = 3.39e38 on, 128 * 2^121 being no number: 127 units, up to a whole one off.)  A value of 7 bits and a sign times a power of
+// two is exact in BF16.
 #pragma once
 
 #include "pairs.cuh"

@@ -46,7 +46,7 @@ struct RouteP {
     int gsize;          // experts per group
     int group_lanes;    // lanes that hold a group, where that is a power of two of whole lanes (route_kernel), else 0
     uint32_t gdiv;      // 2^20 / gsize, rounded up: e * gdiv >> 20 is e / gsize for e < 512
-    uint32_t kdiv;      // 2^16 / k, rounded up: q * kdiv >> 16 is q / k for q < 256
+    uint32_t kdiv;      // 2^16 / k, rounded up: q * kdiv >> 16 is q / k for q < 512, as many as a warp's tokens have (q * (k - 1) < 2^16)
     int32_t* idx;
     float* w;
     int32_t* counts;

@@ -213,7 +213,8 @@ def _check_kept(kept, name, shape, device):
 def keep8(x: torch.Tensor) -> Kept8:
     """``x`` (``[..., C]``, FP32 or BF16, C a multiple of 8) in 8 bits, for a backward pass: 1 1/32 bytes per value.  32 consecutive
     channels share a power of two as their unit, the least in which the largest of them rounds to 127 or less: a value is off by
-    half a unit at most, 1/127 of the largest.  A group with a NaN or an infinity comes back as NaN."""
+    half a unit at most, 1/127 of the largest.  (In groups of values below 2^-120 half of 2^-126, the smallest unit; the largest FP32
+    numbers up to a unit.)  A group with a NaN or an infinity comes back as NaN."""
     lib = _lib.load()
     device = _device(x)
     n, C = _kept_size(x, "keep8")
