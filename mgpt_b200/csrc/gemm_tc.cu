@@ -1744,10 +1744,11 @@ int prepare(mgpt_moe_layer* L, const Workspace& w, char* ws)
     const void *xg = buf_Xg(L, w, ws), *yg = buf_Yg(L, w, ws), *dyg = buf_dYg(L, w, ws), *dxg = buf_dXg(L, w, ws);
     if (s->ws == ws && s->n_tokens == w.n_tokens && s->xg == xg && s->yg == yg && s->dyg == dyg && s->dxg == dxg) return 0;
     const Dims& d = L->d;
-    const uint64_t rc = w.row_cap, C = d.C, H = d.H, E = d.E;
-    MGPT_TRY(make_map(&s->Xg, xg, rc, C, 128));
+    // row_cap rows in the workspace; of a caller's buffers (the expert side) the rows that the call has, and not one more
+    const uint64_t rc = w.row_cap, C = d.C, H = d.H, E = d.E, rows = L->ext_Xg ? (uint64_t)w.n_tokens : rc;
+    MGPT_TRY(make_map(&s->Xg, xg, rows, C, 128));
     MGPT_TRY(make_map(&s->Hh, ws + w.Hh, rc, H, 128));
-    MGPT_TRY(make_map(&s->dYg, dyg, rc, C, 128));
+    MGPT_TRY(make_map(&s->dYg, dyg, rows, C, 128));
     MGPT_TRY(make_map(&s->dG, ws + w.dG, rc, H, 128));
     MGPT_TRY(make_map(&s->dU, ws + w.dU, rc, H, 128));
     // tile-major weight copies, 16 KiB (8192 elements) per block
@@ -1758,27 +1759,27 @@ int prepare(mgpt_moe_layer* L, const Workspace& w, char* ws)
     MGPT_TRY(make_map_weights(&s->Wg_h, L->sWgT, eCH / BLK, BLK, 0, 0, 64, BN / 64, 1));
     MGPT_TRY(make_map_weights(&s->Wu_h, L->sWuT, eCH / BLK, BLK, 0, 0, 64, BN / 64, 1));
     MGPT_TRY(make_map_weights(&s->Wd_h, L->sWdT, eHC / BLK, BLK, 0, 0, 64, BN / 64, 1));
-    MGPT_TRY(make_map(&s->Xg_t, xg, rc, C, 64));
+    MGPT_TRY(make_map(&s->Xg_t, xg, rows, C, 64));
     MGPT_TRY(make_map(&s->Hh_t, ws + w.Hh, rc, H, 64));
-    MGPT_TRY(make_map(&s->dYg_t, dyg, rc, C, 64));
+    MGPT_TRY(make_map(&s->dYg_t, dyg, rows, C, 64));
     MGPT_TRY(make_map(&s->dG_t, ws + w.dG, rc, H, 64));
     MGPT_TRY(make_map(&s->dU_t, ws + w.dU, rc, H, 64));
     s->c_blocks = C % 64 == 0;
     if (s->c_blocks) {
-        MGPT_TRY(make_map_blocks(&s->Xg_b4, xg, rc, C, 64, BN / 64));
-        MGPT_TRY(make_map_blocks(&s->dYg_b4, dyg, rc, C, 64, BN / 64));
-        MGPT_TRY(make_map_blocks(&s->Xg_b2, xg, rc, C, 64, BM / 64));
-        MGPT_TRY(make_map_blocks(&s->dYg_b2, dyg, rc, C, 64, BM / 64));
+        MGPT_TRY(make_map_blocks(&s->Xg_b4, xg, rows, C, 64, BN / 64));
+        MGPT_TRY(make_map_blocks(&s->dYg_b4, dyg, rows, C, 64, BN / 64));
+        MGPT_TRY(make_map_blocks(&s->Xg_b2, xg, rows, C, 64, BM / 64));
+        MGPT_TRY(make_map_blocks(&s->dYg_b2, dyg, rows, C, 64, BM / 64));
     }
     // (the last block may reach up to 112 bytes past the buffer: other buffers of the workspace follow all three)
     MGPT_TRY(make_map_blocks(&s->dG_b2, ws + w.dG, rc, H, 64, BM / 64));
     MGPT_TRY(make_map_blocks(&s->dU_b2, ws + w.dU, rc, H, 64, BM / 64));
     MGPT_TRY(make_map_blocks(&s->Hh_b2, ws + w.Hh, rc, H, 64, BM / 64));
     MGPT_TRY(make_map(&s->Hh_s, ws + w.Hh, rc, H, 32));
-    MGPT_TRY(make_map(&s->Yg_s, yg, rc, C, 32));
+    MGPT_TRY(make_map(&s->Yg_s, yg, rows, C, 32));
     MGPT_TRY(make_map(&s->dG_s, ws + w.dG, rc, H, 32));
     MGPT_TRY(make_map(&s->dU_s, ws + w.dU, rc, H, 32));
-    MGPT_TRY(make_map(&s->dXg_s, dxg, rc, C, 32));
+    MGPT_TRY(make_map(&s->dXg_s, dxg, rows, C, 32));
     s->ws = ws;
     s->n_tokens = w.n_tokens;
     s->xg = xg; s->yg = yg; s->dyg = dyg; s->dxg = dxg;
