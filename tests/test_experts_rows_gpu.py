@@ -1,4 +1,4 @@
-"""The expert side touches the rows of a call and no others: behind them lie NaN in what it reads and a pattern in what it writes."""
+"""The expert side touches the rows of a call and no others: behind them lie NaN in what it reads and a pattern in what it writes, or no memory at all."""
 import math
 
 import pytest
@@ -8,16 +8,18 @@ from mgpt_b200 import MoELayer, _lib
 
 pytestmark = pytest.mark.gpu
 BEHIND = 1024                           # rows
+MAPPED = 14 << 20                       # bytes
 
 
 def _rel(got, want):
     return float((got.double() - want).norm() / want.norm().clamp(min=1e-12))
 
 
+@pytest.mark.parametrize("at_the_end", [False, True])
 @pytest.mark.parametrize("mode,gemm_impl", [("fp32", 0), ("bf16", 0), ("bf16", 1)])
 @pytest.mark.parametrize("C,H,counts", [(64, 128, [[128, 152, 72, 45]]), (64, 128, [[143, 141, 117, 201]]), (72, 136, [[1, 0, 300, 128]]), (128, 320, [[5, 7], [0, 260], [129, 1]]),
                                         (320, 328, [[700, 520]])])
-def test_rows(mode, gemm_impl, C, H, counts):
+def test_rows(mode, gemm_impl, C, H, counts, at_the_end):
     E, n_src = len(counts[0]), len(counts)
     g = torch.Generator(device="cuda").manual_seed(C + H)
     layer = MoELayer(C, H, E, 1, mode=mode, gemm_impl=gemm_impl)
@@ -34,7 +36,10 @@ def test_rows(mode, gemm_impl, C, H, counts):
     real, expert = torch.tensor(real, device="cuda"), torch.tensor(expert, device="cuda")
 
     def rows(fill):
-        return torch.full((n + BEHIND, C), fill, device="cuda").to(dtype)
+        if not at_the_end:
+            return torch.full((n + BEHIND, C), fill, device="cuda").to(dtype)
+        whole = torch.empty(MAPPED, dtype=torch.uint8, device="cuda")       # (an allocation of its own, of whole pages)
+        return whole[MAPPED - n * C * dtype.itemsize:].view(dtype).view(n, C)
 
     x, dy, out, dx = rows(math.nan), rows(math.nan), rows(-7.0), rows(-7.0)
     for t in (x, dy):
