@@ -22,8 +22,8 @@
 // pieces of 32 bytes side by side, half a sector per access, 137 and 227.  A third token in the ring costs more blocks than it hides.
 //
 // KEEP, KEPT: x and h in 8 bits (kept.cuh), written beside y and u, read in their place by the backward pass.  32768 x 2048 BF16: forward 136 us (5.0 TB/s
-// of 675 MB), backward 178 (3.8 TB/s; 151 from tensors).  Both are bound by what a value costs in instructions (a group's maximum over lanes and
-// three byte permutations per four values; unpacking twice), at 58 to 61 % of the issue slots.  The units of a power of two are folded into r1 and
+// of 675 MB), backward 178 (3.8 TB/s; 151 from tensors).  Neither reaches a limit: a value costs more instructions (a group's maximum over lanes and
+// three byte permutations per four values; unpacking twice), which take 57 to 61 % of the issue slots, with 24 to 35 % of the warps to wait in.  The units of a power of two are folded into r1 and
 // alpha; exponents come through the ring as the words they are in (loaded into registers a token ahead: 188 us); the maxima of x and h share a
 // word and a block's registers leave three blocks per SM (four: spills, 149 us); one piece per thread in the backward pass: 202.
 #include "kept.cuh"

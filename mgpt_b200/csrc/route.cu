@@ -16,11 +16,14 @@
 // error, and what is closer than that is settled by exact values: of the few experts concerned, of a group's largest, or (a logit of
 // infinity or a NaN, biases of very different size, long runs of equals) of all.  What is chosen does not depend on which way that goes.
 //
-// Bytes: the logits once, the weights and indices; backward the gradients' bytes, for a softmax the logits too.  Forward is bound by the
-// integer pipe (minima and comparisons run at half the rate of additions): about 180 instructions per token of 128 experts and 8
-// chosen, 690 per token of 256 in groups.  us in a graph on a B200, FP32 logits: 8 x 256 in
-// groups 4.3, 32768 x 64, 4 chosen 8.5, 32768 x 256 in groups, 8 chosen 35 (floor 5.3), 131072 x 128, 8 chosen 36 (floor 12); backward
-// of the last two 7.9 (sigmoid; 4.3 TB/s) and 27 (softmax; 5.0 TB/s; with six blocks per SM 29).  Of the forward call 2 us are the counts' atomics, where counts are asked for.
+// Bytes: the logits once, the weights and indices; backward the gradients' bytes, for a softmax the logits too.  Forward reaches no limit of the
+// chip: about 180 instructions per token of 128 experts and 8 chosen, 690 per token of 256 in groups, at 52 to 58 % of the issue slots and 49 to 54 %
+// of the integer pipe (minima and comparisons, at half the rate of additions), with 28 to 30 % of the warps: the rounds' reductions wait for one
+// another.  us in a graph on a B200, FP32 logits: 8 x 256 in groups 4.4, 32768 x 64, 4 chosen 8.6, 32768 x 256 in groups, 8 chosen 35 (floor
+// 5.3), 131072 x 128, 8 chosen 37 (floor 12).  Of equal logits, which BF16 has among the first k + 1 in 10 % of the tokens at 64 experts and a third at
+// 128 and 256, the order is settled like that of close ones: 32768 x 64 10.5 us in BF16 against 7.3 in FP32 (without counts), 131072 x 128 64 against
+// 37.  Backward: 32768 x 256 (sigmoid) 7.9 (4.3 TB/s), 131072 x 128 (softmax) 27.5 (4.9 TB/s; with six blocks per SM 29), of weights as they are
+// 30.  Of the forward call 2 us are the counts' atomics, where counts are asked for.
 // Not kept: the eight least by sorting and merging lists (38 against 36 us, 39 against 35: more minima), two warps per block (44 against 38),
 // six to eight blocks per SM (37 to 41 against 36).
 #include "common.cuh"
